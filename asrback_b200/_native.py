@@ -25,6 +25,7 @@ ERR_WORKSPACE = 3
 STATUS_POSITION = 1
 STATUS_TIMEOUT = 2
 STATUS_SEGMENT = 4
+STATUS_TREE = 8
 
 ABI_MAJOR = 1
 
@@ -136,6 +137,59 @@ SIGNATURES: dict[str, tuple[list, object]] = {
          _c_p, _c_size, _c_p, _c_p],
         _c_int,
     ),
+    "asrback_draft_tree": (
+        [_c_int, _c_int, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
+        _c_int,
+    ),
+    "asrback_tree_counter_bytes": ([_c_int] * 5, _c_size),
+    "asrback_tree_workspace_bytes": ([_c_int] * 8, _c_size),
+    "asrback_tree_attention": (
+        [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_p, _c_i64, _c_i64, _c_i64,
+         _c_p, _c_i64, _c_i64, _c_i64,
+         _c_p, _c_i64, _c_i64, _c_i64,
+         _c_p, _c_p, _c_f,
+         _c_p, _c_p, _c_i64, _c_int,
+         _c_p,
+         _c_p, _c_p, _c_p, _c_p,
+         _c_p, _c_p,
+         _c_i64, _c_i64, _c_i64,
+         _c_p, _c_i64, _c_i64, _c_i64,
+         _c_p, _c_i64, _c_i64,
+         _c_f, _c_p, _c_size, _c_p, _c_size,
+         _c_p, _c_p],
+        _c_int,
+    ),
+    "asrback_accept_tree": (
+        [_c_int, _c_int, _c_p, _c_i64, _c_p,
+         _c_p, _c_i64, _c_p, _c_i64,
+         _c_p, _c_i64,
+         _c_p, _c_i64, _c_p, _c_p,
+         _c_p, _c_p,
+         _c_p, _c_i64, _c_i64,
+         _c_p, _c_p, _c_int,
+         _c_p, _c_p, _c_p, _c_p, _c_p],
+        _c_int,
+    ),
+    "asrback_commit_tree": (
+        [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_p, _c_p,
+         _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_p, _c_i64, _c_i64, _c_i64,
+         _c_p, _c_p, _c_p,
+         _c_p, _c_p],
+        _c_int,
+    ),
+    "asrback_evict": (
+        [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_p, _c_p,
+         _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_p, _c_i64, _c_i64, _c_i64,
+         _c_p, _c_int, _c_int, _c_int,
+         _c_p, _c_p, _c_p, _c_p],
+        _c_int,
+    ),
+    "asrback_stream_capture_id": ([_c_p], ctypes.c_uint64),
     "asrback_selftest_bounded_wait": ([_c_i64, _c_p, _c_p], _c_int),
 }
 

@@ -22,12 +22,20 @@ Reference call sites (asrback project paths):
 - :func:`whisper_cross_kv_projection`: ``set_encoder_output``,
   ``whisper.py:313-319`` (``project_key_value``, ``:88-91``, and the copy into
   the cross-attention cache), one decoder layer per call.
+
+Without a counterpart in the reference, for speculative decoding and bounded
+caches: :func:`draft_tree` plans the trees of drafted tokens of a step, and
+:func:`qwen3_attention_tree` and :func:`whisper_self_attention_tree` run a
+layer's attention for all their nodes, optionally keeping the attention weight
+that every key gathers (:mod:`asrback_b200.cache` evicts by it).
 """
 
 from __future__ import annotations
 
 import math
 import threading
+from contextlib import nullcontext
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
@@ -41,6 +49,12 @@ __all__ = [
     "whisper_encoder_attention",
     "whisper_cross_kv_projection",
     "varlen_attention",
+    "DraftTree",
+    "draft_tree",
+    "qwen3_attention_tree",
+    "whisper_self_attention_tree",
+    "MAX_NODES",
+    "MAX_WEIGHT_ROWS",
     "reserve_workspace",
     "read_status",
     "DeviceStatusError",
@@ -470,3 +484,215 @@ def varlen_attention(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, longest: i
         state.status.data_ptr(), _stream(q.device),
     )
     return out
+
+
+MAX_NODES = 64  # of a draft tree
+MAX_WEIGHT_ROWS = 16  # nodes x heads / kv_heads of a call with weights
+
+
+class DraftTree(NamedTuple):
+    """Trees of drafted tokens, one per row, as :func:`draft_tree` plans them
+    (all tensors on the device): ``parents`` (B, N) int32, ``counts`` (B,)
+    int32 live nodes, ``ancestors`` (B, N) int64 (bit ``j``: node ``j`` is the
+    node itself or above it; 0: padding) and ``depths`` (B, N) int32."""
+
+    parents: Tensor
+    counts: Tensor
+    ancestors: Tensor
+    depths: Tensor
+
+
+# Zeroed counters of the tree kernels, one buffer per stream, and one more per
+# graph capture on it: calls that may run at the same time never share them.
+# The kernels leave them at zero. A capture's buffer is zeroed by the graph
+# itself, on every replay.
+_counters: dict[tuple[int, int, bool], tuple[int, Tensor]] = {}
+_MIN_COUNTER_BYTES = 1 << 16
+
+
+def _counters_for(device: torch.device, stream: int, nbytes: int) -> Tensor:
+    capture = _native.load().asrback_stream_capture_id(stream)
+    key = (device.index, stream, capture != 0)
+    held = _counters.get(key)
+    if held is None or held[0] != capture or held[1].numel() < nbytes:
+        size = max(nbytes, _MIN_COUNTER_BYTES)
+        held = (capture, torch.zeros(size, dtype=torch.uint8, device=device))
+        _counters[key] = held
+    return held[1]
+
+
+def _on(device: torch.device):
+    """A context in which ``device`` is the current one."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _int_rows(t: Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> Tensor:
+    if t.dtype != dtype or t.shape != shape or t.device != device:
+        raise ValueError(f"asrback_b200: {name} must be {shape} {dtype} on {device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.contiguous()
+
+
+def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
+    """Plans the draft trees of a step, once for all layers. ``parents``
+    ``(B, N)`` int32 on the device: node ``i``'s parent, below ``i``, or -1 for
+    a root (``N <= 64``; an expanded ``(1, N)`` serves one tree for every row).
+    ``counts`` ``(B,)`` int32: the row's first nodes that are live, the others
+    being padding (default: all). Node 0 holds the row's current token, the
+    others drafts of what follows it. A row with invalid parents or count gets
+    no nodes and sets ``_native.STATUS_TREE``."""
+    if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_cuda:
+        raise ValueError("asrback_b200: parents must be (batch, nodes) int32 on a CUDA device")
+    batch, nodes = parents.shape
+    if batch < 1 or not 1 <= nodes <= MAX_NODES:
+        raise ValueError(f"asrback_b200: a batch of trees of 1 to {MAX_NODES} nodes is needed, got "
+                         f"{tuple(parents.shape)}")
+    device = parents.device
+    if parents.stride(1) != 1 or 0 < parents.stride(0) < nodes:
+        parents = parents.contiguous()
+    if counts is not None:
+        counts = _int_rows(counts, "counts", torch.int32, (batch,), device)
+    with _on(device):
+        ancestors = torch.empty((batch, nodes), dtype=torch.int64, device=device)
+        depths = torch.empty((batch, nodes), dtype=torch.int32, device=device)
+        live = torch.empty(batch, dtype=torch.int32, device=device)
+        _native.call("asrback_draft_tree", batch, nodes, parents.data_ptr(), parents.stride(0),
+                     None if counts is None else counts.data_ptr(), ancestors.data_ptr(),
+                     depths.data_ptr(), live.data_ptr(), _state(device).status.data_ptr(),
+                     _stream(device))
+    return DraftTree(parents, live, ancestors, depths)
+
+
+def _tree_call(q: Tensor, k: Tensor, v: Tensor, rotary: tuple | None, tree: DraftTree,
+               lengths: Tensor, keys: Tensor, values: Tensor, scale: float | None,
+               weights: Tensor | None) -> Tensor:
+    """``q`` (B, N, H, D), ``k``/``v`` (B, N, KVH, D) and the caches as
+    (B, L, KVH, D) views, whatever their memory order."""
+    batch, nodes, heads, head_dim = q.shape
+    kv_heads, length = keys.shape[2], keys.shape[1]
+    device = q.device
+    dtype = _dtype_code(q, k, v, keys, values)
+    if values.shape != keys.shape or values.stride() != keys.stride():
+        raise ValueError("asrback_b200: key and value caches differ in shape or strides")
+    if q.stride(3) != 1 or k.stride(3) != 1 or v.stride(3) != 1 or keys.stride(3) != 1:
+        raise ValueError("asrback_b200: head_dim must have unit stride")
+    for t in (k, v, keys, values):
+        if t.device != device:
+            raise ValueError("asrback_b200: tensors must be on one device")
+    ancestors = _int_rows(tree.ancestors, "tree.ancestors", torch.int64, (batch, nodes), device)
+    depths = _int_rows(tree.depths, "tree.depths", torch.int32, (batch, nodes), device)
+    counts = _int_rows(tree.counts, "tree.counts", torch.int32, (batch,), device)
+    lengths = _int_rows(lengths, "lengths", torch.int64, (batch,), device)
+    if weights is None:
+        w_ptr, w_batch, w_head = None, 0, 0
+    else:
+        if weights.dtype != torch.float32 or weights.shape != (batch, kv_heads, length) \
+                or weights.device != device or (length > 1 and weights.stride(2) != 1):
+            raise ValueError(f"asrback_b200: weights must be {(batch, kv_heads, length)} float32 "
+                             "with unit last stride, on the tensors' device")
+        w_ptr, w_batch, w_head = weights.data_ptr(), weights.stride(0), weights.stride(1)
+    if rotary is None:
+        qn = kn = cos = sin = positions = None
+        eps, table_stride, table_length = 0.0, 0, 0
+    else:
+        qn, kn, eps, cos, sin, positions = rotary
+        _dtype_code(q, qn, kn, cos, sin)
+        for weight in (qn, kn):
+            if weight.shape != (head_dim,) or weight.stride(0) != 1 or weight.device != device:
+                raise ValueError("asrback_b200: norm weights must be contiguous (head_dim,)")
+        if cos.dim() != 2 or cos.shape[1] != head_dim or cos.shape != sin.shape \
+                or cos.stride(1) != 1 or cos.stride() != sin.stride() or cos.device != device \
+                or sin.device != device:
+            raise ValueError("asrback_b200: cos and sin must be (table_length, head_dim) of one "
+                             "layout")
+        positions = _int_rows(positions, "positions", torch.int64, (batch,), device)
+        qn, kn, table_stride, table_length = qn.data_ptr(), kn.data_ptr(), cos.stride(0), cos.shape[0]
+        if table_length == 1:
+            table_stride = head_dim
+        cos, sin, positions = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
+    lib = _native.load()
+    with _on(device):
+        stream = _stream(device)
+        out = torch.empty((batch, nodes, heads * head_dim), dtype=q.dtype, device=device)
+        counter_bytes = lib.asrback_tree_counter_bytes(dtype, batch, nodes, heads, kv_heads)
+        ws_bytes = lib.asrback_tree_workspace_bytes(dtype, batch, nodes, heads, kv_heads, head_dim,
+                                                    length, 0 if weights is None else 1)
+        status = _state(device).status
+        counters = _counters_for(device, stream, counter_bytes)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+        _native.call(
+            "asrback_tree_attention",
+            dtype, batch, nodes, heads, kv_heads, head_dim, length,
+            q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
+            k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+            v.data_ptr(), v.stride(0), v.stride(1), v.stride(2),
+            qn, kn, eps, cos, sin, table_stride, table_length, positions,
+            ancestors.data_ptr(), depths.data_ptr(), counts.data_ptr(), lengths.data_ptr(),
+            keys.data_ptr(), values.data_ptr(), keys.stride(0), keys.stride(1), keys.stride(2),
+            out.data_ptr(), nodes * heads * head_dim, heads * head_dim, head_dim,
+            w_ptr, w_batch, w_head,
+            scale if scale is not None else 1.0 / math.sqrt(head_dim),
+            counters.data_ptr(), counters.numel(), workspace.data_ptr(), ws_bytes,
+            status.data_ptr(), stream,
+        )
+    return out
+
+
+def qwen3_attention_tree(qkv: Tensor, q_norm_weight: Tensor, k_norm_weight: Tensor, eps: float,
+                         cos: Tensor, sin: Tensor, positions: Tensor, tree: DraftTree, keys: Tensor,
+                         values: Tensor, heads: int, kv_heads: int, scale: float | None = None,
+                         lengths: Tensor | None = None, weights: Tensor | None = None) -> Tensor:
+    """Qwen3 attention for a tree of drafted tokens per row, from ``qkv_proj``'s
+    output ``(B, N, (heads + 2 kv_heads) * D)`` to ``o_proj``'s input
+    ``(B, N, heads * D)``: q/k RMSNorm, RoPE at ``positions[b] + depth``, the
+    nodes' keys and values written to cache slots ``lengths[b] + i`` of
+    ``keys``/``values`` ``(B, L, kv_heads, D)``, then grouped-query attention of
+    node ``i`` over the cache's first ``lengths[b]`` keys and its ancestors in
+    the tree. ``lengths`` (int64) defaults to ``positions``; the two differ once
+    keys have been evicted. Padding nodes give zeros and write nothing.
+
+    ``weights`` ``(B, kv_heads, L)`` float32, if given, gathers the softmax
+    weight that every key gets, summed over the row's live nodes and the query
+    heads of its key/value head: added for cached keys, assigned for the new
+    slots (at most ``MAX_WEIGHT_ROWS`` query rows, ``N * heads / kv_heads``).
+
+    ``N = 1`` is the decode step, a chain a prompt pass of up to 64 tokens.
+    ``head_dim`` 64 or 128. A row whose nodes do not fit the cache or the RoPE
+    table gets zeros and sets ``_native.STATUS_POSITION``."""
+    if qkv.dim() != 3 or qkv.stride(2) != 1:
+        raise ValueError("asrback_b200: qkv must be (batch, nodes, width) with unit last stride")
+    if keys.dim() != 4 or keys.shape[0] != qkv.shape[0] or keys.shape[2] != kv_heads:
+        raise ValueError("asrback_b200: keys must be (batch, length, kv_heads, head_dim)")
+    batch, nodes, width = qkv.shape
+    head_dim = keys.shape[3]
+    if width != (heads + 2 * kv_heads) * head_dim:
+        raise ValueError("asrback_b200: qkv width or cache heads do not match heads/kv_heads")
+    x = qkv.unflatten(2, (heads + 2 * kv_heads, head_dim))
+    return _tree_call(x[:, :, :heads], x[:, :, heads:heads + kv_heads], x[:, :, heads + kv_heads:],
+                      (q_norm_weight, k_norm_weight, float(eps), cos, sin, positions), tree,
+                      positions if lengths is None else lengths, keys, values, scale, weights)
+
+
+def whisper_self_attention_tree(query: Tensor, key: Tensor, value: Tensor, key_cache: Tensor,
+                                value_cache: Tensor, lengths: Tensor, tree: DraftTree,
+                                scale: float | None = None, weights: Tensor | None = None) -> Tensor:
+    """Whisper decoder self-attention for a tree of drafted tokens per row:
+    writes node ``i``'s key and value to slot ``lengths[b] + i`` of the caches
+    ``(B, H, L, D)`` and attends with ``query`` to the first ``lengths[b]`` keys
+    and the node's ancestors. ``query``/``key``/``value``: ``(B, H, N, D)`` (the
+    ``_split_heads`` views); ``lengths`` ``(B,)`` int64. Returns ``(B, N, H*D)``,
+    the layout ``out_proj`` takes. The nodes' position embeddings are those of
+    ``lengths[b] + tree.depths``; their cross-attention is
+    :func:`whisper_cross_attention_prefix`. ``weights``: as in
+    :func:`qwen3_attention_tree`."""
+    if query.dim() != 4 or key.shape != query.shape or value.shape != query.shape:
+        raise ValueError("asrback_b200: query, key and value must be (batch, heads, nodes, "
+                         "head_dim) of one shape")
+    batch, heads, _, head_dim = query.shape
+    if key_cache.dim() != 4 or key_cache.shape[:2] != (batch, heads) \
+            or key_cache.shape[3] != head_dim:
+        raise ValueError(f"asrback_b200: cache {tuple(key_cache.shape)} does not match query "
+                         f"{tuple(query.shape)}")
+    query, key, value, key_cache, value_cache = (
+        t.transpose(1, 2) for t in (query, key, value, key_cache, value_cache))
+    return _tree_call(query, key, value, None, tree, lengths, key_cache, value_cache, scale, weights)

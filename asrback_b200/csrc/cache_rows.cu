@@ -1,0 +1,465 @@
+// Rows of a key/value cache moved to the front of their batch row: the commit
+// of a draft tree's accepted nodes and the eviction of keys by accumulated
+// attention weight, sm_100a.
+//
+// Both move cache row source[k] to row target + k with source ascending and
+// source[k] >= k, in place. A move then never overwrites a row that a later
+// move reads, so rows are moved in ascending order, a batch of loads before
+// its stores, with no copy of the cache. Both are bound by HBM: a moved row is
+// read once and written once.
+#include "../../include/asrback_attn.h"
+#include "capi_internal.h"
+#include "common.cuh"
+
+#include <algorithm>
+
+namespace asrback {
+namespace {
+
+struct CacheView {
+  uint8_t* base;  // strides in bytes
+  int64_t layer, batch, position, head;
+};
+
+// -------------------------------------------------------------------- commit
+
+struct CommitParams {
+  CacheView cache[2];  // keys, values
+  int layers, batch, heads, length, vectors;  // vectors: 16-byte pieces of a head's row
+  const int32_t* path;
+  const int32_t* counts;
+  const int64_t* start;
+  int nodes;
+  float* weights;  // or null
+  int64_t w_layer, w_batch, w_head;
+  int32_t* status;
+};
+
+constexpr int kMaxNodes = 64;
+constexpr int kCommitThreads = 128;
+
+// A thread owns one 16-byte column of the moved rows and moves it node by
+// node, eight loads in flight. A row of the batch accepts a few nodes of some
+// kilobytes over every layer, so the columns are what there is to spread out.
+__global__ void __launch_bounds__(kCommitThreads)
+    commit_kernel(const __grid_constant__ CommitParams p) {
+  __shared__ int path[kMaxNodes];
+  __shared__ int moved[2];  // first node that moves, one past the last
+  griddep_wait();
+  griddep_launch_dependents();
+  const int b = blockIdx.y, layer = blockIdx.z >> 1, which = blockIdx.z & 1;
+  const int column = blockIdx.x * kCommitThreads + threadIdx.x;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    const int count = p.counts[b];
+    const int64_t start = p.start[b];
+    int node[2];
+    bool bad = count < 0 || count > p.nodes;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int k = lane + 32 * u;
+      node[u] = k < p.nodes ? p.path[(int64_t)b * p.nodes + k] : -1;
+      path[k] = node[u];
+    }
+    __syncwarp();
+    uint64_t moves = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int k = lane + 32 * u;
+      if (k < count && k < p.nodes) {
+        const int before = k > 0 ? path[k - 1] : -1;
+        bad |= node[u] <= before || node[u] >= p.nodes || start < 0 ||
+               start + node[u] >= p.length;
+      }
+      moves |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, k < count && node[u] != k))
+               << (32 * u);
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) {
+      if (bad && p.status) atomicOr(p.status, ASRBACK_STATUS_POSITION);
+      moved[0] = bad || moves == 0 ? 0 : __ffsll(static_cast<long long>(moves)) - 1;
+      moved[1] = bad || moves == 0 ? 0 : count;
+    }
+  }
+  __syncthreads();
+  const int first = moved[0], last = moved[1];
+  if (first >= last) return;
+  const int64_t start = p.start[b];
+  if (which == 0 && p.weights) {
+    for (int h = column; h < p.heads; h += gridDim.x * kCommitThreads) {
+      float* row = p.weights + layer * p.w_layer + b * p.w_batch + h * p.w_head + start;
+      for (int k = first; k < last; ++k) row[k] = row[path[k]];
+    }
+  }
+  if (column >= p.heads * p.vectors) return;
+  const CacheView& c = p.cache[which];
+  uint8_t* rows = c.base + layer * c.layer + b * c.batch + (column / p.vectors) * c.head +
+                  start * c.position + (column % p.vectors) * 16;
+  for (int k = first; k < last; k += 8) {
+    uint4 piece[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (k + u < last) piece[u] = *reinterpret_cast<const uint4*>(rows + path[k + u] * c.position);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (k + u < last) *reinterpret_cast<uint4*>(rows + (k + u) * c.position) = piece[u];
+  }
+}
+
+// --------------------------------------------------------- eviction: selection
+
+struct SelectParams {
+  float* weights;
+  int64_t w_layer, w_batch, w_head;
+  const int64_t* lengths;
+  int64_t* new_lengths;
+  int32_t* kept;  // (layers, batch, heads, budget)
+  int batch, heads, length, budget, sink, recent;
+  int32_t* status;
+};
+
+// Order-preserving key of a weight: larger weight, larger key. Zeros of both
+// signs are equal, NaN counts as -inf. The protected slots' key is above every
+// weight's.
+constexpr uint32_t kProtected = 0xffffffffu;
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) w = -INFINITY;
+  if (w == 0.f) w = 0.f;
+  const uint32_t u = __float_as_uint(w);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// One CTA per (layer, row, head) finds the `budget` largest keys. The
+// threshold (the budget-th largest key) is built bit by bit from the top,
+// counting the keys at or above each candidate: the count ends early once it
+// is exactly the budget, which distinct weights do after some 10 to 20 bits.
+// Keys equal to the threshold are taken from the lowest slot up. A thread
+// holds V consecutive slots of a chunk in registers; a row of one chunk is
+// read once. The kept weights are compacted here, their slots go to `kept`.
+template <int THREADS, int V>
+__global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__ SelectParams p) {
+  constexpr int kChunk = THREADS * V;
+  constexpr int kWarps = THREADS / 32;
+  __shared__ int counter[33];
+  __shared__ int scan[2][kWarps];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t given = p.lengths[b];
+  const bool first = h == 0 && layer == 0 && tid == 0;
+  int32_t* kept = p.kept + (((int64_t)layer * p.batch + b) * p.heads + h) * p.budget;
+  if (given < 0 || given > p.length) {
+    if (first) {
+      p.new_lengths[b] = given;
+      if (p.status) atomicOr(p.status, ASRBACK_STATUS_POSITION);
+    }
+    for (int k = tid; k < p.budget; k += THREADS) kept[k] = -1;
+    return;
+  }
+  const int n = static_cast<int>(given);
+  if (first) p.new_lengths[b] = min(n, p.budget);
+  if (n <= p.budget) {
+    for (int k = tid; k < p.budget; k += THREADS) kept[k] = k < n ? k : -1;
+    return;
+  }
+  if (tid < 33) counter[tid] = 0;
+  __syncthreads();
+  float* row = p.weights + layer * p.w_layer + b * p.w_batch + h * p.w_head;
+  const int chunks = (n + kChunk - 1) / kChunk;
+  const int tail = n - p.recent;
+  uint32_t key[V];
+  // Slots past the row's end hold key 0, below every weight's.
+  auto load = [&](int chunk) {
+    const int base = chunk * kChunk + tid * V;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const int j = base + u;
+      key[u] = j >= n ? 0u : j < p.sink || j >= tail ? kProtected : weight_key(row[j]);
+    }
+  };
+  load(0);
+  uint32_t threshold = 0;
+  bool exact = false;
+  for (int bit = 31; bit >= 0 && !exact; --bit) {
+    const uint32_t candidate = threshold | 1u << bit;
+    int count = 0;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+      if (chunks > 1) load(chunk);
+#pragma unroll
+      for (int u = 0; u < V; ++u) count += key[u] >= candidate;
+    }
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (lane == 0 && count) atomicAdd(&counter[bit], count);
+    __syncthreads();
+    const int total = counter[bit];
+    if (total >= p.budget) threshold = candidate;
+    exact = total == p.budget;
+  }
+  // Keys above the threshold (or, if exact, at it) are all kept; of the ones
+  // equal to it the `ties` lowest slots.
+  int above_all = 0;
+  if (!exact) {
+    int count = 0;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+      if (chunks > 1) load(chunk);
+#pragma unroll
+      for (int u = 0; u < V; ++u) count += key[u] > threshold;
+    }
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (lane == 0 && count) atomicAdd(&counter[32], count);
+    __syncthreads();
+    above_all = counter[32];
+  }
+  const int ties = exact ? n : p.budget - above_all;
+  int above_before = 0, equal_before = 0;  // of the chunks before this one
+  for (int chunk = 0; chunk < chunks; ++chunk) {
+    if (chunks > 1) load(chunk);
+    const int base = chunk * kChunk + tid * V;
+    int above = 0, equal = 0;
+    float raw[V];
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      raw[u] = base + u < n ? row[base + u] : 0.f;
+      above += key[u] > threshold;
+      equal += key[u] == threshold;
+    }
+    int above_scan = above, equal_scan = equal;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, above_scan, o);
+      const int e = __shfl_up_sync(0xffffffffu, equal_scan, o);
+      if (lane >= o) above_scan += a, equal_scan += e;
+    }
+    __syncthreads();  // the last chunk's sums have been read, the raw weights too
+    if (lane == 31) scan[0][warp] = above_scan, scan[1][warp] = equal_scan;
+    __syncthreads();
+    int above_at = above_before + above_scan - above, equal_at = equal_before + equal_scan - equal;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) above_at += scan[0][w], equal_at += scan[1][w];
+      above_before += scan[0][w], equal_before += scan[1][w];
+    }
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const bool over = key[u] > threshold, same = key[u] == threshold;
+      if (over || (same && equal_at < ties)) {
+        const int k = above_at + min(equal_at, ties);
+        kept[k] = base + u;
+        row[k] = raw[u];
+      }
+      above_at += over;
+      equal_at += same;
+    }
+  }
+}
+
+// -------------------------------------------------------- eviction: the moves
+
+struct MoveParams {
+  CacheView cache[2];
+  const int64_t* lengths;
+  const int32_t* kept;
+  int batch, heads, length, budget;
+  int vectors;  // 16-byte pieces of the part of a row that one CTA moves
+};
+
+constexpr int kMoveThreads = 256;
+constexpr int kMoveUnroll = 4;
+
+// A CTA moves one head's kept rows of the keys or of the values (or a part of
+// their columns, where the batch has few heads), kMoveUnroll rows per thread
+// and turn. A turn's loads come before its barrier and its stores after it;
+// the next turn's loads are issued in between, since its rows lie behind all
+// that this turn writes.
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int b = blockIdx.y % p.batch, layer = blockIdx.y / p.batch;
+  const int which = blockIdx.z & 1, part = blockIdx.z >> 1, h = blockIdx.x;
+  const int64_t given = p.lengths[b];
+  if (given <= p.budget || given > p.length) return;
+  const CacheView& c = p.cache[which];
+  uint8_t* rows = c.base + layer * c.layer + b * c.batch + h * c.head +
+                  (part * p.vectors + threadIdx.x % p.vectors) * 16;
+  const int32_t* kept = p.kept + ((int64_t)blockIdx.y * p.heads + h) * p.budget;
+  const int lanes = kMoveThreads / p.vectors;  // rows per pass of the CTA
+  const int turn = lanes * kMoveUnroll;
+  const int mine = threadIdx.x / p.vectors;
+  uint4 piece[2][kMoveUnroll];
+  int from[2][kMoveUnroll];
+  auto load = [&](int set, int k0) {
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int k = k0 + u * lanes + mine;
+      from[set][u] = k < p.budget ? kept[k] : k;
+    }
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int k = k0 + u * lanes + mine;
+      if (from[set][u] != k)
+        piece[set][u] = *reinterpret_cast<const uint4*>(rows + from[set][u] * c.position);
+    }
+  };
+  auto store = [&](int set, int k0) {
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int k = k0 + u * lanes + mine;
+      if (from[set][u] != k) *reinterpret_cast<uint4*>(rows + k * c.position) = piece[set][u];
+    }
+  };
+  load(0, 0);
+  for (int k0 = 0; k0 < p.budget; k0 += 2 * turn) {
+    load(1, k0 + turn);
+    __syncthreads();
+    store(0, k0);
+    load(0, k0 + 2 * turn);
+    __syncthreads();
+    store(1, k0 + turn);
+  }
+}
+
+// Checks a cache's shape and fills `view` (strides in bytes); an ABI code.
+int cache_view(CacheView* view, const char* name, void* base, int64_t esize, int head_dim,
+               int64_t layer, int64_t batch, int64_t position, int64_t head) {
+  if (!base) return fail(ASRBACK_ERR_ARGUMENT, "null %s pointer", name);
+  if (!aligned16(base) || (layer * esize) % 16 || (batch * esize) % 16 ||
+      (position * esize) % 16 || (head * esize) % 16)
+    return fail(ASRBACK_ERR_ARGUMENT,
+                "%s rows must start on 16-byte boundaries (pointer and strides)", name);
+  if (position < head_dim || head < head_dim || layer < 0 || batch < 0)
+    return fail(ASRBACK_ERR_ARGUMENT, "%s strides do not hold rows of head_dim elements", name);
+  *view = {static_cast<uint8_t*>(base), layer * esize, batch * esize, position * esize,
+           head * esize};
+  return ASRBACK_OK;
+}
+
+int check_cache_sizes(int dtype, int layers, int batch, int heads, int head_dim, int length) {
+  if (dtype != ASRBACK_BF16 && dtype != ASRBACK_F32)
+    return fail(ASRBACK_ERR_ARGUMENT, "dtype must be ASRBACK_BF16 or ASRBACK_F32, got %d", dtype);
+  if (layers < 1 || batch < 1 || heads < 1 || length < 1)
+    return fail(ASRBACK_ERR_ARGUMENT, "layers, batch, heads and cache length must be positive");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(ASRBACK_ERR_ARGUMENT, "head_dim must be 64 or 128, got %d", head_dim);
+  return ASRBACK_OK;
+}
+
+}  // namespace
+}  // namespace asrback
+
+using namespace asrback;
+
+extern "C" int asrback_commit_tree(int dtype, int layers, int batch, int nodes, int heads,
+                                   int head_dim, int length, void* key_cache, void* value_cache,
+                                   int64_t c_stride_layer, int64_t c_stride_batch,
+                                   int64_t c_stride_position, int64_t c_stride_head, float* weights,
+                                   int64_t w_stride_layer, int64_t w_stride_batch,
+                                   int64_t w_stride_head, const int32_t* path,
+                                   const int32_t* counts, const int64_t* start, int32_t* status,
+                                   void* stream) {
+  if (int rc = check_cache_sizes(dtype, layers, batch, heads, head_dim, length)) return rc;
+  if (nodes < 1 || nodes > kMaxNodes)
+    return fail(ASRBACK_ERR_ARGUMENT, "nodes must be in [1, %d], got %d", kMaxNodes, nodes);
+  if (batch > 65535 || layers > 32767)
+    return fail(ASRBACK_ERR_ARGUMENT, "at most 65535 rows and 32767 layers, got %d and %d", batch,
+                layers);
+  if (!path || !counts || !start)
+    return fail(ASRBACK_ERR_ARGUMENT, "null path, counts or start pointer");
+  const int64_t esize = dtype == ASRBACK_BF16 ? 2 : 4;
+  CommitParams p{};
+  if (int rc = cache_view(&p.cache[0], "key_cache", key_cache, esize, head_dim, c_stride_layer,
+                          c_stride_batch, c_stride_position, c_stride_head))
+    return rc;
+  if (int rc = cache_view(&p.cache[1], "value_cache", value_cache, esize, head_dim, c_stride_layer,
+                          c_stride_batch, c_stride_position, c_stride_head))
+    return rc;
+  p.layers = layers;
+  p.batch = batch;
+  p.heads = heads;
+  p.length = length;
+  p.vectors = static_cast<int>(head_dim * esize / 16);
+  p.path = path;
+  p.counts = counts;
+  p.start = start;
+  p.nodes = nodes;
+  p.weights = weights;
+  p.w_layer = w_stride_layer;
+  p.w_batch = w_stride_batch;
+  p.w_head = w_stride_head;
+  p.status = status;
+  const unsigned columns = (heads * p.vectors + kCommitThreads - 1) / kCommitThreads;
+  if (int rc = launch_pdl(commit_kernel, dim3(columns, batch, 2 * layers), dim3(kCommitThreads), 0,
+                          static_cast<cudaStream_t>(stream), "commit launch", p))
+    return rc;
+  return ok();
+}
+
+extern "C" int asrback_evict(int dtype, int layers, int batch, int heads, int head_dim, int length,
+                             void* key_cache, void* value_cache, int64_t c_stride_layer,
+                             int64_t c_stride_batch, int64_t c_stride_position,
+                             int64_t c_stride_head, float* weights, int64_t w_stride_layer,
+                             int64_t w_stride_batch, int64_t w_stride_head, const int64_t* lengths,
+                             int budget, int sink, int recent, int64_t* new_lengths, int32_t* kept,
+                             int32_t* status, void* stream) {
+  if (int rc = check_cache_sizes(dtype, layers, batch, heads, head_dim, length)) return rc;
+  if (budget < 1 || budget > length)
+    return fail(ASRBACK_ERR_ARGUMENT, "budget must be in [1, cache length %d], got %d", length,
+                budget);
+  if (sink < 0 || recent < 0 || sink > budget - recent)
+    return fail(ASRBACK_ERR_ARGUMENT,
+                "sink and recent must not be negative and at most budget together");
+  if (static_cast<int64_t>(layers) * batch > 65535 || layers > 65535 || batch > 65535)
+    return fail(ASRBACK_ERR_ARGUMENT, "at most 65535 rows over all layers, got %d x %d", layers,
+                batch);
+  if (!weights || !lengths || !new_lengths || !kept)
+    return fail(ASRBACK_ERR_ARGUMENT, "null weights, lengths, new_lengths or kept pointer");
+  const int64_t esize = dtype == ASRBACK_BF16 ? 2 : 4;
+  MoveParams m{};
+  if (int rc = cache_view(&m.cache[0], "key_cache", key_cache, esize, head_dim, c_stride_layer,
+                          c_stride_batch, c_stride_position, c_stride_head))
+    return rc;
+  if (int rc = cache_view(&m.cache[1], "value_cache", value_cache, esize, head_dim, c_stride_layer,
+                          c_stride_batch, c_stride_position, c_stride_head))
+    return rc;
+  SelectParams s{};
+  s.weights = weights;
+  s.w_layer = w_stride_layer;
+  s.w_batch = w_stride_batch;
+  s.w_head = w_stride_head;
+  s.lengths = lengths;
+  s.new_lengths = new_lengths;
+  s.kept = kept;
+  s.batch = batch;
+  s.heads = heads;
+  s.length = length;
+  s.budget = budget;
+  s.sink = sink;
+  s.recent = recent;
+  s.status = status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid(heads, batch, layers);
+  int rc;
+  if (length <= 1024)
+    rc = launch_pdl(select_kernel<256, 4>, grid, dim3(256), 0, st, "evict selection launch", s);
+  else if (length <= 4096)
+    rc = launch_pdl(select_kernel<1024, 4>, grid, dim3(1024), 0, st, "evict selection launch", s);
+  else
+    rc = launch_pdl(select_kernel<1024, 16>, grid, dim3(1024), 0, st, "evict selection launch", s);
+  if (rc) return rc;
+  m.lengths = lengths;
+  m.kept = kept;
+  m.batch = batch;
+  m.heads = heads;
+  m.length = length;
+  m.budget = budget;
+  // A row is cut into column parts of at least 64 bytes until the launch has
+  // two CTAs per SM.
+  const int vectors = static_cast<int>(head_dim * esize / 16);
+  int parts = 1;
+  while (vectors / parts > 4 &&
+         static_cast<int64_t>(layers) * batch * heads * 2 * parts < 2 * sm_count())
+    parts *= 2;
+  m.vectors = vectors / parts;
+  rc = launch_pdl(move_kernel, dim3(heads, layers * batch, 2 * parts), dim3(kMoveThreads), 0, st,
+                  "evict move launch", m);
+  return rc ? rc : ok();
+}

@@ -14,6 +14,11 @@ bf16 runs the logits on the tensor cores (fp32 sums rounded to bf16, as the
 reference's bf16 matmul returns them); float32 runs a SIMT kernel. Sampling
 (a positive temperature) is not fused: the reference's graphs cover greedy
 steps only, and the patched ``_step`` hands sampled steps to the original.
+
+For a step that ran a tree of drafted tokens per row (speculative decoding, no
+counterpart in the reference), :func:`accept_tree` walks each tree along the
+tokens the model chose and updates the decode state by as many greedy steps as
+the drafts were right, and :func:`greedy_tree_step` does the nodes' logits too.
 """
 
 from __future__ import annotations
@@ -21,13 +26,15 @@ from __future__ import annotations
 import ctypes
 import threading
 from collections.abc import Sequence
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
 
 from . import _native, attention
 
-__all__ = ["greedy_choose", "greedy_step", "MAX_BATCH"]
+__all__ = ["greedy_choose", "greedy_step", "AcceptedPath", "accept_tree", "greedy_tree_step",
+           "MAX_BATCH"]
 
 MAX_BATCH = 128  # bf16; float32 takes up to 64 rows
 
@@ -141,3 +148,106 @@ def greedy_step(hidden: Tensor, weight: Tensor, tokens: Tensor, position: Tensor
     state = dict(tokens=tokens, position=position, end=end, finished=finished,
                  sum_logprobs=sum_logprobs, generated=generated)
     _launch(hidden, weight, suppress, None, None, state, eos_ids)
+
+
+class AcceptedPath(NamedTuple):
+    """What :func:`accept_tree` accepted: ``path`` ``(B, N)`` int32, the row's
+    accepted nodes from node 0 on, then -1; ``counts`` ``(B,)`` int32, their
+    number, which is the number of tokens emitted; ``start`` ``(B,)`` int64, the
+    cache slot of node 0."""
+
+    path: Tensor
+    counts: Tensor
+    start: Tensor
+
+
+def _node_rows(t: Tensor, name: str, dtype: torch.dtype, shape: tuple, device) -> Tensor:
+    if t.dtype != dtype or t.shape != shape or t.device != device:
+        raise ValueError(f"asrback_b200: {name} must be {shape} {dtype} on {device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t if t.stride(1) == 1 and t.stride(0) >= shape[1] else t.contiguous()
+
+
+def accept_tree(tree: attention.DraftTree, drafts: Tensor, chosen: Tensor, logprob: Tensor,
+                tokens: Tensor, position: Tensor, end: Tensor, finished: Tensor,
+                sum_logprobs: Tensor, generated: Tensor, eos_ids: Sequence[int],
+                lengths: Tensor | None = None) -> AcceptedPath:
+    """Walks each row's tree from node 0: the token ``chosen`` at a node is
+    emitted, and the walk goes on to the lowest child whose draft it is. It ends
+    when no child holds it or the row is finished (EOS, or its position at
+    ``end``). Every emitted token updates the decode state as
+    :func:`greedy_step` does; finished rows stay as they are.
+
+    ``drafts`` ``(B, N)`` int64: the nodes' tokens; ``chosen`` int64 and
+    ``logprob`` float32 ``(B, N)``: what :func:`greedy_choose` says of each
+    node's hidden state. ``lengths`` ``(B,)`` int64: the cache lengths, advanced
+    with ``position``, for a cache whose slots are not its positions. The
+    caches' rows are brought in order by :func:`asrback_b200.cache.qwen3_commit_tree`
+    or :func:`~asrback_b200.cache.whisper_commit_tree` with the returned path."""
+    batch, nodes = tree.parents.shape
+    device = tree.parents.device
+    if not tree.parents.is_cuda or tree.parents.dtype != torch.int32:
+        raise ValueError("asrback_b200: tree must be a draft_tree() plan on a CUDA device")
+    parents = tree.parents
+    if parents.stride(1) != 1 or 0 < parents.stride(0) < nodes:
+        parents = parents.contiguous()
+    counts = _vector(tree.counts, "tree.counts", torch.int32, batch)
+    drafts = _node_rows(drafts, "drafts", torch.int64, (batch, nodes), device)
+    chosen = _node_rows(chosen, "chosen", torch.int64, (batch, nodes), device)
+    logprob = _node_rows(logprob, "logprob", torch.float32, (batch, nodes), device)
+    if tokens.dtype != torch.int64 or tokens.shape[0] != batch or tokens.numel() != batch:
+        raise ValueError(f"asrback_b200: tokens must be ({batch},) or ({batch}, 1) int64")
+    position = _vector(position, "position", torch.int64, batch)
+    end = _vector(end, "end", torch.int64, batch)
+    finished = _vector(finished, "finished", torch.bool, batch)
+    sums = _vector(sum_logprobs, "sum_logprobs", torch.float32, batch)
+    if generated.dtype != torch.int64 or generated.dim() != 2 or generated.shape[0] != batch \
+            or generated.stride(1) != 1:
+        raise ValueError(f"asrback_b200: generated must be ({batch}, length) int64 with "
+                         "contiguous rows")
+    if lengths is not None:
+        lengths = _vector(lengths, "lengths", torch.int64, batch)
+    for t in (counts, tokens, position, end, finished, sums, generated, lengths):
+        if t is not None and t.device != device:
+            raise ValueError("asrback_b200: the decode state must be on the tree's device")
+    eos = [int(e) for e in eos_ids]
+    eos_host = (ctypes.c_int64 * max(len(eos), 1))(*eos)
+    with attention._on(device):
+        path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
+        accepted = torch.empty(batch, dtype=torch.int32, device=device)
+        start = torch.empty(batch, dtype=torch.int64, device=device)
+        _native.call(
+            "asrback_accept_tree", batch, nodes, parents.data_ptr(), parents.stride(0),
+            counts.data_ptr(), drafts.data_ptr(), drafts.stride(0), chosen.data_ptr(),
+            chosen.stride(0), logprob.data_ptr(), logprob.stride(0),
+            tokens.data_ptr(), tokens.stride(0) if batch > 1 else 1, position.data_ptr(),
+            end.data_ptr(), finished.data_ptr(), sums.data_ptr(), generated.data_ptr(),
+            generated.stride(0) if batch > 1 else generated.shape[1], generated.shape[1],
+            None if lengths is None else lengths.data_ptr(), eos_host, len(eos),
+            path.data_ptr(), accepted.data_ptr(), start.data_ptr(),
+            attention._state(device).status.data_ptr(), attention._stream(device))
+    return AcceptedPath(path, accepted, start)
+
+
+def greedy_tree_step(hidden: Tensor, weight: Tensor, tree: attention.DraftTree, drafts: Tensor,
+                     tokens: Tensor, position: Tensor, end: Tensor, finished: Tensor,
+                     sum_logprobs: Tensor, generated: Tensor, eos_ids: Sequence[int],
+                     suppress: Tensor | None = None, lengths: Tensor | None = None) -> AcceptedPath:
+    """A greedy step after the decoder has run a tree of drafted tokens per
+    row: every node's logits and choice from ``hidden`` ``(B, N, d)`` (as
+    :func:`greedy_choose`, ``MAX_BATCH`` rows per launch), then
+    :func:`accept_tree`."""
+    if hidden.dim() != 3 or hidden.shape[:2] != tree.parents.shape:
+        raise ValueError(f"asrback_b200: hidden must be (batch, nodes, width) for trees of "
+                         f"{tuple(tree.parents.shape)}, got {tuple(hidden.shape)}")
+    batch, nodes, width = hidden.shape
+    rows = hidden.flatten(0, 1)
+    # float32 takes 64 rows, and as many as 200 KB of shared memory hold.
+    limit = MAX_BATCH if hidden.dtype == torch.bfloat16 else max(1, min(64, 51200 // width))
+    token = torch.empty(batch * nodes, dtype=torch.int64, device=hidden.device)
+    logprob = torch.empty(batch * nodes, dtype=torch.float32, device=hidden.device)
+    for first in range(0, batch * nodes, limit):
+        part = slice(first, first + limit)
+        _launch(rows[part], weight, suppress, token[part], logprob[part], None, ())
+    return accept_tree(tree, drafts, token.view(batch, nodes), logprob.view(batch, nodes), tokens,
+                       position, end, finished, sum_logprobs, generated, eos_ids, lengths)

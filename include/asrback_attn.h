@@ -80,6 +80,7 @@ extern "C" {
 #define ASRBACK_STATUS_TIMEOUT 2  /* a bounded wait inside a kernel gave up */
 #define ASRBACK_STATUS_SEGMENT 4  /* a segment of cu_seqlens lay outside the tensor or
                                      exceeded max_length (asrback_varlen_attention) */
+#define ASRBACK_STATUS_TREE 8     /* a draft tree's parents or node count were invalid */
 
 /* Version of this ABI: (major << 16) | minor. */
 ASRBACK_API int asrback_abi_version(void);
@@ -358,6 +359,165 @@ ASRBACK_API int asrback_greedy_step(
     int64_t* generated, int64_t generated_stride, int64_t generated_cols,
     const int64_t* eos_ids, int n_eos,
     void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
+/*
+ * Draft trees (speculative decoding). A row's tree has at most 64 nodes, each
+ * holding a drafted token; parents[i] < i is node i's parent, -1 for a root.
+ * Node 0 holds the row's current token (the one a plain step would run), the
+ * others drafts of what follows. Rows may have fewer nodes than `nodes`: the
+ * first counts[b] are live, the rest is padding.
+ *
+ * asrback_draft_tree plans the trees of a step, once for all layers:
+ * parents      (batch, nodes) int32, rows at parents_stride (0: one tree for
+ *              every row)
+ * counts       (batch,) int32, or null: every node is live
+ * ancestors    (batch, nodes) int64, out: bit j of ancestors[b][i] is set if
+ *              node j is node i or an ancestor of it; 0 for padding
+ * depths       (batch, nodes) int32, out: ancestors besides the node itself
+ * live_counts  (batch,) int32, out: counts, or 0 for a row whose parents or
+ *              count are invalid (it sets ASRBACK_STATUS_TREE)
+ */
+ASRBACK_API int asrback_draft_tree(
+    int batch, int nodes, const int32_t* parents, int64_t parents_stride, const int32_t* counts,
+    int64_t* ancestors, int32_t* depths, int32_t* live_counts, int32_t* status, void* stream);
+
+/*
+ * Attention of a draft tree's nodes over a row's cache. Node i's key and value
+ * are written to cache slot lengths[b] + i; it attends to the cache's first
+ * lengths[b] keys and to the slots of the nodes in ancestors[b][i]. A node
+ * without a bit (padding) gets zeros and writes nothing. One node per row is
+ * the ordinary decode step; a chain is a prompt pass of up to 64 tokens.
+ *
+ * query        (batch, nodes, heads, head_dim) at [b*stride_batch +
+ *              i*stride_node + h*stride_head + d]; key, value likewise over
+ *              kv_heads; query head h reads key/value head h / (heads / kv_heads)
+ * q_norm_weight, k_norm_weight, eps, cos, sin, table_*, positions: if given,
+ *              query and key first get their per-head RMSNorm and rotate-half
+ *              rotary embedding at positions[b] + depths[b][i], in float32 and
+ *              rounded once (the Qwen3 form); all null: taken as they are
+ *              (Whisper). positions (batch,) int64; it differs from lengths
+ *              once keys have been evicted. positions[b] + counts[b] must not
+ *              exceed table_length.
+ * ancestors, depths, counts  from asrback_draft_tree
+ * lengths      (batch,) int64: keys in the cache before the call
+ * key_cache, value_cache  at [b*c_stride_batch + p*c_stride_position +
+ *              h*c_stride_head + d], cache_length positions: Qwen3's
+ *              position-major and Whisper's head-major caches alike
+ * out          (batch, nodes, heads, head_dim), strides o_stride_*
+ * weights      null, or (batch, kv_heads, cache_length) float at
+ *              [b*w_stride_batch + h*w_stride_head + p]: the softmax weights
+ *              that key p got, summed over the live nodes and the head's query
+ *              heads, are added to the cached keys' entries and assigned to
+ *              the new slots'. At most 16 query rows per key/value head
+ *              (nodes * heads / kv_heads).
+ * head_dim 64 or 128; nodes <= 64; batch <= 1024; dtype ASRBACK_BF16 or
+ * ASRBACK_F32; rows and pointers 16-byte aligned.
+ * A row whose counts, lengths or positions are out of range gets zeros, writes
+ * nothing else and sets ASRBACK_STATUS_POSITION.
+ *
+ * counters     asrback_tree_counter_bytes(...) bytes, zero before the first
+ *              call; every call leaves them zero. Calls that may run at the
+ *              same time (other streams, other graphs) need their own.
+ * workspace    asrback_tree_workspace_bytes(...) bytes of scratch, of any
+ *              content; likewise not shared by calls that run at the same time.
+ */
+ASRBACK_API size_t asrback_tree_counter_bytes(int dtype, int batch, int nodes, int heads,
+                                              int kv_heads);
+ASRBACK_API size_t asrback_tree_workspace_bytes(int dtype, int batch, int nodes, int heads,
+                                                int kv_heads, int head_dim, int cache_length,
+                                                int with_weights);
+ASRBACK_API int asrback_tree_attention(
+    int dtype, int batch, int nodes, int heads, int kv_heads, int head_dim, int cache_length,
+    const void* query, int64_t q_stride_batch, int64_t q_stride_node, int64_t q_stride_head,
+    const void* key, int64_t k_stride_batch, int64_t k_stride_node, int64_t k_stride_head,
+    const void* value, int64_t v_stride_batch, int64_t v_stride_node, int64_t v_stride_head,
+    const void* q_norm_weight, const void* k_norm_weight, float eps,
+    const void* cos, const void* sin, int64_t table_stride, int table_length,
+    const int64_t* positions,
+    const int64_t* ancestors, const int32_t* depths, const int32_t* counts, const int64_t* lengths,
+    void* key_cache, void* value_cache,
+    int64_t c_stride_batch, int64_t c_stride_position, int64_t c_stride_head,
+    void* out, int64_t o_stride_batch, int64_t o_stride_node, int64_t o_stride_head,
+    float* weights, int64_t w_stride_batch, int64_t w_stride_head,
+    float scale, void* counters, size_t counter_bytes, void* workspace, size_t workspace_bytes,
+    int32_t* status, void* stream);
+
+/*
+ * Greedy acceptance of a draft tree, and the decode-state update of as many
+ * greedy steps as it accepts. A row's walk begins at node 0: the token chosen
+ * there (the target's argmax after that node) is emitted; the walk goes on to
+ * the lowest child whose drafted token equals it, and ends when there is none
+ * or the row is finished (EOS, or its position reaches end). Each emitted
+ * token updates the state as asrback_greedy_step does. A finished row, and one
+ * without nodes, stays as it is.
+ *
+ * parents, counts  as in asrback_draft_tree (counts: its live_counts)
+ * drafts       (batch, nodes) int64: the nodes' tokens (node 0's is not read)
+ * chosen, logprob  (batch, nodes) int64 / float: each node's chosen token and
+ *              its log-probability; rows at their strides
+ * tokens ... eos_ids  the decode state, as in asrback_greedy_step
+ * lengths      null, or (batch,) int64 cache lengths, advanced with position
+ * path         (batch, nodes) int32, out: the walk's nodes, then -1
+ * accepted     (batch,) int32, out: the walk's length, i.e. tokens emitted
+ * start        (batch,) int64, out: the cache slot of node 0: lengths[b] (or
+ *              position[b]) before the call
+ */
+ASRBACK_API int asrback_accept_tree(
+    int batch, int nodes, const int32_t* parents, int64_t parents_stride, const int32_t* counts,
+    const int64_t* drafts, int64_t drafts_stride, const int64_t* chosen, int64_t chosen_stride,
+    const float* logprob, int64_t logprob_stride,
+    int64_t* tokens, int64_t tokens_stride, int64_t* position, const int64_t* end,
+    uint8_t* finished, float* sum_logprobs,
+    int64_t* generated, int64_t generated_stride, int64_t generated_cols,
+    int64_t* lengths, const int64_t* eos_ids, int n_eos,
+    int32_t* path, int32_t* accepted, int64_t* start, int32_t* status, void* stream);
+
+/*
+ * Commits accepted nodes: in every layer, cache row start[b] + path[b][k] moves
+ * to row start[b] + k for k < counts[b] (path ascending, as asrback_accept_tree
+ * returns it). Caches at [layer*c_stride_layer + b*c_stride_batch +
+ * p*c_stride_position + h*c_stride_head + d]; weights null or (layers, batch,
+ * heads, length) float, whose entries move along. Rows with an invalid path or
+ * start stay as they are and set ASRBACK_STATUS_POSITION.
+ */
+ASRBACK_API int asrback_commit_tree(
+    int dtype, int layers, int batch, int nodes, int heads, int head_dim, int length,
+    void* key_cache, void* value_cache,
+    int64_t c_stride_layer, int64_t c_stride_batch, int64_t c_stride_position,
+    int64_t c_stride_head,
+    float* weights, int64_t w_stride_layer, int64_t w_stride_batch, int64_t w_stride_head,
+    const int32_t* path, const int32_t* counts, const int64_t* start,
+    int32_t* status, void* stream);
+
+/*
+ * Evicts keys by accumulated attention weight: each row with more than
+ * `budget` keys keeps, per layer and head, its first `sink` slots, its last
+ * `recent` slots and of the others those with the largest weights (the lower
+ * slot on ties; NaN counts as -inf), `budget` in all. Kept keys, values and
+ * weights move to slots 0..budget-1 in their old order; what lies behind stays
+ * as it is. Rows with at most `budget` keys are left alone.
+ *
+ * caches, weights  as in asrback_commit_tree
+ * lengths      (batch,) int64: keys per row; outside [0, length] the row is
+ *              left alone and sets ASRBACK_STATUS_POSITION
+ * new_lengths  (batch,) int64, out: min(lengths, budget)
+ * kept         (layers, batch, heads, budget) int32, out: the old slots of the
+ *              kept keys, ascending, then -1
+ */
+ASRBACK_API int asrback_evict(
+    int dtype, int layers, int batch, int heads, int head_dim, int length,
+    void* key_cache, void* value_cache,
+    int64_t c_stride_layer, int64_t c_stride_batch, int64_t c_stride_position,
+    int64_t c_stride_head,
+    float* weights, int64_t w_stride_layer, int64_t w_stride_batch, int64_t w_stride_head,
+    const int64_t* lengths, int budget, int sink, int recent,
+    int64_t* new_lengths, int32_t* kept, int32_t* status, void* stream);
+
+/*
+ * The id of the CUDA graph capture that `stream` is in, 0 if it is in none:
+ * for callers that keep zeroed counters per graph.
+ */
+ASRBACK_API uint64_t asrback_stream_capture_id(void* stream);
 
 /*
  * Self-test of the kernels' bounded waits: one CTA waits on an mbarrier that
