@@ -142,7 +142,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
         _c_int,
     ),
     "asrback_tree_counter_bytes": ([_c_int] * 5, _c_size),
-    "asrback_tree_workspace_bytes": ([_c_int] * 8, _c_size),
+    "asrback_tree_workspace_bytes": ([_c_int] * 9, _c_size),
     "asrback_tree_attention": (
         [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
          _c_p, _c_i64, _c_i64, _c_i64,

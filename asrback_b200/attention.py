@@ -616,7 +616,8 @@ def _tree_call(q: Tensor, k: Tensor, v: Tensor, rotary: tuple | None, tree: Draf
         out = torch.empty((batch, nodes, heads * head_dim), dtype=q.dtype, device=device)
         counter_bytes = lib.asrback_tree_counter_bytes(dtype, batch, nodes, heads, kv_heads)
         ws_bytes = lib.asrback_tree_workspace_bytes(dtype, batch, nodes, heads, kv_heads, head_dim,
-                                                    length, 0 if weights is None else 1)
+                                                    length, 0 if rotary is None else 1,
+                                                    0 if weights is None else 1)
         status = _state(device).status
         counters = _counters_for(device, stream, counter_bytes)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)

@@ -23,379 +23,23 @@
 // re-arms) merges the parts in list order, so results do not depend on which
 // CTA was last.
 //
-// The tree is an item's last tile. Its keys and values come from the call's
-// inputs, not from the cache: the CTA that owns the tile normalises and
-// rotates them, writes them to the cache and uses them from shared memory, so
-// no CTA waits for another's cache write.
+// A first, small kernel (tree_prepare.cu) writes the nodes' keys and values to
+// the cache and the prepared query rows to the workspace; the nodes then are an
+// item's last keys, masked by the rows' ancestors. Every CTA of the attention
+// works on its own: none waits for another.
 #include "../../include/asrback_attn.h"
 #include "capi_internal.h"
 #include "common.cuh"
 #include "tree_attention.cuh"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace asrback {
 namespace {
 
 using namespace tree;
 
-// ----------------------------------------------------------- bf16, mma.sync
-//
-// Four warps; a warp owns 16 of a tile's 64 keys and all the block's query
-// rows (16 or 32), with its own softmax state, its own part of the ring and
-// no barrier with the other warps until the end of a stretch.
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// 16 bytes global to shared, or 16 zero bytes where `valid` is false.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(valid ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-
-// Byte offset of 16-byte piece `piece` of row `row` in a [rows][D] bf16 tile:
-// pieces permuted within a row so that eight rows' same piece (an ldmatrix
-// phase) and one row's pieces (a copy) both touch all banks once.
-template <int D>
-__device__ __forceinline__ int swz(int row, int piece) {
-  return row * (D * 2) + ((piece ^ (row & 7)) << 4);
-}
-
-template <int D, int MT, bool kWeights>
-struct MmaShape {
-  static constexpr int kRows = 16 * MT;
-  static constexpr int kStages = 3;
-  static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kRingBytes = kStages * 2 * kTileBytes;  // [stage][keys, values], at 0
-  static constexpr int kOffQ = kRingBytes;  // q rounded to bf16; then, with weights, the rest
-  static constexpr int kQBytes = kRows * D * 2;
-  static constexpr int kOffCommon = kOffQ + (kWeights ? 2 : 1) * kQBytes;
-  static constexpr int kSmem = kOffCommon + (int)sizeof(Common<kRows>);
-  // The warps' results at the end of a stretch, in the ring.
-  static constexpr int kMergeFloats = 4 * kRows * (D + 2);
-  static_assert(kMergeFloats * 4 <= kRingBytes, "the merge buffer must fit the ring");
-};
-
-template <int D, int MT, bool kWeights>
-__global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1)
-    tree_mma_kernel(const __grid_constant__ TreeParams p) {
-  using Sh = MmaShape<D, MT, kWeights>;
-  using T = __nv_bfloat16;
-  constexpr int kRows = Sh::kRows, kStages = Sh::kStages;
-  constexpr int kPieces = D / 8;             // 16-byte pieces of a row
-  constexpr int kPasses = 16 * kPieces / 32;  // copies per lane for 16 rows
-  constexpr int kRowStep = 32 / kPieces;      // rows between a lane's copies
-  extern __shared__ __align__(1024) uint8_t smem[];
-  auto& cm = *reinterpret_cast<Common<kRows>*>(smem + Sh::kOffCommon);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quad = lane & 3, group_row = lane >> 2;
-
-  griddep_wait();
-  griddep_launch_dependents();
-  Stretch st = begin_stretch(p, cm);
-  const uint32_t ring = smem_addr(smem);
-  const uint32_t q_smem = smem_addr(smem + Sh::kOffQ);
-  // ldmatrix addresses: lane l gives row l % 8 of matrix l / 8.
-  const int mat = lane >> 3, mrow = lane & 7;
-
-  while (next_segment(p, cm, st)) {
-    const Segment& sg = st.seg;
-    // Query rows of the block: normalised, rotated, rounded once to bf16. With
-    // weights, q = hi + lo in two bf16 parts, since a rounding of q to 8 bits
-    // would put 2^-9 * |s| into every accumulated weight.
-    prepare_rows<D, kRows, T>(p, sg, cm, warp, lane, [&](int r, int e, const float* x, int n) {
-      uint8_t* hi = smem + Sh::kOffQ + swz<D>(r, e / 8) + (e % 8) * 2;
-#pragma unroll
-      for (int j = 0; j < n; j += 2) {
-        const uint32_t h = bf16_pair(x[j], x[j + 1]);
-        *reinterpret_cast<uint32_t*>(hi + 2 * j) = h;
-        if constexpr (kWeights)
-          *reinterpret_cast<uint32_t*>(hi + Sh::kQBytes + 2 * j) =
-              bf16_pair(x[j] - __uint_as_float(h << 16), x[j + 1] - __uint_as_float(h & 0xffff0000u));
-      }
-    });
-    __syncthreads();
-    uint32_t qa[MT][D / 16][4];
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks)
-        ldsm4(qa[t][ks], q_smem + swz<D>(16 * t + (mat & 1) * 8 + mrow, 2 * ks + (mat >> 1)));
-
-    float o[MT][D / 8][4], m[MT][2], l[MT][2];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      m[t][0] = m[t][1] = -INFINITY;
-      l[t][0] = l[t][1] = 0.f;
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[t][n][j] = 0.f;
-    }
-
-    const T* kbase = static_cast<const T*>(p.key_cache) + sg.b * p.c_sb + sg.h * p.c_sh;
-    const T* vbase = static_cast<const T*>(p.value_cache) + sg.b * p.c_sb + sg.h * p.c_sh;
-    const int copy_row = lane / kPieces, copy_piece = lane % kPieces;
-    auto copy_tile = [&](int stage, int tile) {
-      const uint32_t dst = ring + stage * 2 * Sh::kTileBytes;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int row = 16 * warp + copy_row + i * kRowStep;
-        const int key = tile * kTile + row;
-        const bool in = key < sg.length;
-        const int64_t at = (int64_t)(in ? key : 0) * p.c_sp + copy_piece * 8;
-        cp_async16(dst + swz<D>(row, copy_piece), kbase + at, in);
-        cp_async16(dst + Sh::kTileBytes + swz<D>(row, copy_piece), vbase + at, in);
-      }
-    };
-
-    // One warp's 16 keys against the block's rows. `visible(t, row half, key in
-    // the tile)` masks; kMask is off for full cache tiles.
-    // `finite` is false only where a node's value is not.
-    auto compute = [&](int stage, auto masked, int first_key, bool finite, auto visible) {
-      constexpr bool kMask = decltype(masked)::value;
-      const uint32_t kt = ring + stage * 2 * Sh::kTileBytes, vt = kt + Sh::kTileBytes;
-      float s[MT][2][4];
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[t][n][j] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t kb[4];
-        ldsm4(kb, kt + swz<D>(16 * warp + (mat >> 1) * 8 + mrow, 2 * ks + (mat & 1)));
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          mma16816(s[t][0], qa[t][ks], kb[0], kb[1]);
-          mma16816(s[t][1], qa[t][ks], kb[2], kb[3]);
-          if constexpr (kWeights) {
-            uint32_t lo[4];
-            ldsm4(lo, q_smem + Sh::kQBytes +
-                          swz<D>(16 * t + (mat & 1) * 8 + mrow, 2 * ks + (mat >> 1)));
-            mma16816(s[t][0], lo, kb[0], kb[1]);
-            mma16816(s[t][1], lo, kb[2], kb[3]);
-          }
-        }
-      }
-      uint32_t pa[MT][4];
-      bool moved = false;
-      float alpha[MT][2];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float& x = s[t][n][2 * half + j];
-              x *= p.scale_log2;
-              if constexpr (kMask) {
-                if (!visible(16 * t + 8 * half + group_row, 16 * warp + 8 * n + 2 * quad + j))
-                  x = -INFINITY;
-              }
-              top = fmaxf(top, x);
-            }
-          if constexpr (kWeights) {
-            const int r = 16 * t + 8 * half + group_row;
-            if (r < p.rows) {
-              float* out = score_row(p, sg, r) + first_key + 16 * warp + 2 * quad;
-#pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                  if (!kMask || 16 * warp + 8 * n + 2 * quad + j < sg.tile_keys(first_key))
-                    out[8 * n + j] = s[t][n][2 * half + j];
-            }
-          }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float now = fmaxf(m[t][half], top);
-          const float ref = now == -INFINITY ? 0.f : now;
-          alpha[t][half] = fast_exp2(m[t][half] - ref);
-          moved |= now != m[t][half];
-          m[t][half] = now;
-          float sum = 0.f;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float& x = s[t][n][2 * half + j];
-              x = fast_exp2(x - ref);
-              sum += x;
-            }
-          l[t][half] = l[t][half] * alpha[t][half] + sum;
-        }
-        // Probabilities are rounded to bf16 for the second product: 2^-9 apart
-        // at most, against an output rounded to bf16 itself; their sum is not.
-        pa[t][0] = bf16_pair(s[t][0][0], s[t][0][1]);
-        pa[t][1] = bf16_pair(s[t][0][2], s[t][0][3]);
-        pa[t][2] = bf16_pair(s[t][1][0], s[t][1][1]);
-        pa[t][3] = bf16_pair(s[t][1][2], s[t][1][3]);
-      }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[t][n][j] *= alpha[t][j >> 1];
-      }
-      if (!kMask || finite) {
-#pragma unroll
-        for (int dp = 0; dp < D / 16; ++dp) {
-          uint32_t vb[4];
-          ldsm4_t(vb, vt + swz<D>(16 * warp + (mat & 1) * 8 + mrow, 2 * dp + (mat >> 1)));
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            mma16816(o[t][2 * dp], pa[t], vb[0], vb[1]);
-            mma16816(o[t][2 * dp + 1], pa[t], vb[2], vb[3]);
-          }
-        }
-      }
-      if constexpr (kMask) {
-        if (finite) return;
-        // A node's infinite or NaN value must not reach the nodes that do not
-        // see it, as a product with zero would let it: one key at a time,
-        // added only where it is visible.
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            for (int key = 0; key < 16; ++key) {
-              // Key `key` of the warp lies in half key % 2 of a register of
-              // the quad's lane (key % 8) / 2.
-              const uint32_t pair = __shfl_sync(
-                  0xffffffffu, key < 8 ? pa[t][half] : pa[t][2 + half], (lane & ~3) | ((key & 7) >> 1));
-              const float w = __uint_as_float(key & 1 ? pair & 0xffff0000u : pair << 16);
-              if (!visible(16 * t + 8 * half + group_row, 16 * warp + key)) continue;
-#pragma unroll
-              for (int n = 0; n < D / 8; ++n) {
-                const uint32_t v = *reinterpret_cast<const uint32_t*>(
-                    smem + (vt - ring) + swz<D>(16 * warp + key, n) + 4 * quad);
-                o[t][n][2 * half] = fmaf(w, __uint_as_float(v << 16), o[t][n][2 * half]);
-                o[t][n][2 * half + 1] =
-                    fmaf(w, __uint_as_float(v & 0xffff0000u), o[t][n][2 * half + 1]);
-              }
-            }
-      }
-    };
-
-    // The stretch's cache tiles, kStages - 1 in flight.
-    const int last = min(sg.tile1, sg.tiles - 1);  // one past the last cache tile
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      if (sg.tile0 + s < last) copy_tile(s, sg.tile0 + s);
-      cp_commit();
-    }
-    int stage = 0;
-    for (int tile = sg.tile0; tile < last; ++tile) {
-      cp_wait<kStages - 2>();
-      __syncwarp();
-      const int ahead = tile + kStages - 1;
-      if (ahead < last) copy_tile(stage == 0 ? kStages - 1 : stage - 1, ahead);
-      cp_commit();
-      if ((tile + 1) * kTile <= sg.length)
-        compute(stage, std::false_type{}, tile * kTile, true, [](int, int) { return true; });
-      else
-        compute(stage, std::true_type{}, tile * kTile, true,
-                [&](int, int key) { return tile * kTile + key < sg.length; });
-      __syncwarp();
-      stage = stage == kStages - 1 ? 0 : stage + 1;
-    }
-
-    // The tree's own tile.
-    if (sg.tile1 == sg.tiles && sg.count > 0) {
-      __syncthreads();  // every warp is done with its part of stage 0
-      const bool finite = load_tree_tile<D, T>(
-          p, sg, cm, warp, lane, [&](int i, int e, const float* k, const float* v, int n) {
-            uint8_t* dst = smem + swz<D>(i, e / 8) + (e % 8) * 2;
-#pragma unroll
-            for (int j = 0; j < n; j += 2) {
-              *reinterpret_cast<uint32_t*>(dst + 2 * j) = bf16_pair(k[j], k[j + 1]);
-              *reinterpret_cast<uint32_t*>(dst + Sh::kTileBytes + 2 * j) =
-                  bf16_pair(v[j], v[j + 1]);
-            }
-          });
-      if (16 * warp < sg.count)
-        compute(0, std::true_type{}, sg.length, finite,
-                [&](int r, int key) { return (cm.mask[r] >> key & 1) != 0; });
-    }
-
-    // The four warps' states become one.
-    __syncthreads();
-    float* part_m = reinterpret_cast<float*>(smem);  // [warp][row] m, then l, then o
-    float* part_l = part_m + 4 * kRows;
-    float* part_o = part_l + 4 * kRows;
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = 16 * t + 8 * half + group_row;
-        float sum = l[t][half];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (quad == 0) {
-          part_m[warp * kRows + r] = m[t][half];
-          part_l[warp * kRows + r] = sum;
-        }
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-          *reinterpret_cast<float2*>(part_o + (warp * kRows + r) * D + 8 * n + 2 * quad) =
-              make_float2(o[t][n][2 * half], o[t][n][2 * half + 1]);
-      }
-    __syncthreads();
-    finish_segment<D, kRows, T>(p, st, cm, [&](int r, int e, float& rm, float& rl, float4& ro) {
-      rm = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) rm = fmaxf(rm, part_m[w * kRows + r]);
-      const float ref = rm == -INFINITY ? 0.f : rm;
-      rl = 0.f;
-      ro = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float a = fast_exp2(part_m[w * kRows + r] - ref);
-        rl += part_l[w * kRows + r] * a;
-        const float4 x = *reinterpret_cast<const float4*>(part_o + (w * kRows + r) * D + e);
-        ro.x += x.x * a, ro.y += x.y * a, ro.z += x.z * a, ro.w += x.w * a;
-      }
-    });
-    __syncthreads();
-  }
-}
+constexpr int kThreads = 128;
 
 // ------------------------------------------------------------ float32, SIMT
 //
@@ -413,8 +57,10 @@ struct SimtShape {
   static constexpr int kOffS = kOffQ + kRows * D * 4;        // scores, then probabilities
   static constexpr int kOffState = kOffS + kRows * kTile * 4;  // m, l, alpha
   static constexpr int kOffO = kOffState + 3 * kRows * 4;
-  static constexpr int kOffCommon = kOffO + kRows * D * 4;
-  static constexpr int kSmem = kOffCommon + (int)sizeof(Common<kRows>);
+  static constexpr int kOffMasks = kOffO + kRows * D * 4;
+  static constexpr int kOffScratch = kOffMasks + kRows * 8;  // a flag, then begin_stretch's
+  static constexpr int kOffList = kOffScratch + 32;
+  static constexpr int bytes(int batch) { return kOffList + list_bytes(batch); }
 };
 
 template <int D>
@@ -425,7 +71,9 @@ __global__ void __launch_bounds__(kThreads)
   constexpr int kHalves = kThreads / D;     // threads per output column
   constexpr int kMine = kRows / kHalves;    // rows per thread in the second product
   extern __shared__ __align__(1024) uint8_t smem[];
-  auto& cm = *reinterpret_cast<Common<kRows>*>(smem + Sh::kOffCommon);
+  auto* masks = reinterpret_cast<unsigned long long*>(smem + Sh::kOffMasks);
+  int* scratch = reinterpret_cast<int*>(smem + Sh::kOffScratch);
+  TileList list(smem + Sh::kOffList, p.batch);
   float* ks = reinterpret_cast<float*>(smem + Sh::kOffK);
   float* vs = reinterpret_cast<float*>(smem + Sh::kOffV);
   float* qs = reinterpret_cast<float*>(smem + Sh::kOffQ);
@@ -438,44 +86,35 @@ __global__ void __launch_bounds__(kThreads)
 
   griddep_wait();
   griddep_launch_dependents();
-  Stretch st = begin_stretch(p, cm);
-  while (next_segment(p, cm, st)) {
+  Stretch st = begin_stretch<kThreads>(p, list, scratch + 4);
+  while (next_segment(p, list, st)) {
     const Segment& sg = st.seg;
-    prepare_rows<D, kRows, float>(p, sg, cm, warp, lane, [&](int r, int e, const float* x, int n) {
-      for (int j = 0; j < n; ++j) qs[r * D + e + j] = x[j];
-    });
+    const uint8_t* block = p.q_blocks + (int64_t)sg.item * p.q_block_bytes;
+    for (int i = tid; i < kRows * D / 4; i += kThreads)
+      reinterpret_cast<float4*>(qs)[i] = __ldcg(reinterpret_cast<const float4*>(block) + i);
+    if (tid < kRows)
+      masks[tid] = __ldcg(reinterpret_cast<const unsigned long long*>(block + kRows * D * 4) + tid);
     if (tid < kRows) state_m[tid] = -INFINITY, state_l[tid] = 0.f;
     float o[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) o[i] = 0.f;
     const float* kbase = static_cast<const float*>(p.key_cache) + sg.b * p.c_sb + sg.h * p.c_sh;
     const float* vbase = static_cast<const float*>(p.value_cache) + sg.b * p.c_sb + sg.h * p.c_sh;
-    for (int tile = sg.tile0; tile < sg.tile1; ++tile) {
-      const bool tree = tile == sg.tiles - 1;
-      if (tree && sg.count == 0) break;
-      const int first_key = tree ? sg.length : tile * kTile;
-      const int keys = tree ? sg.count : min(kTile, sg.length - first_key);
+    const int total = sg.length + sg.count;
+    for (int tile = sg.tile0; tile < sg.tile1 && total > 0; ++tile) {
+      const int first_key = tile * kTile, keys = min(kTile, total - first_key);
+      const bool edge = first_key + kTile > sg.length;  // nodes in the tile
       __syncthreads();
-      if (tree) {
-        load_tree_tile<D, float>(p, sg, cm, warp, lane,
-                                 [&](int i, int e, const float* k, const float* v, int n) {
-                                   for (int j = 0; j < n; ++j) {
-                                     ks[i * kPitch + e + j] = k[j];
-                                     vs[i * D + e + j] = v[j];
-                                   }
-                                 });
-      } else {
-        for (int i = tid; i < kTile * D / 4; i += kThreads) {
-          const int row = i / (D / 4), e = i % (D / 4) * 4;
-          float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-          if (row < keys) {
-            const int64_t at = (int64_t)(first_key + row) * p.c_sp + e;
-            k = *reinterpret_cast<const float4*>(kbase + at);
-            v = *reinterpret_cast<const float4*>(vbase + at);
-          }
-          *reinterpret_cast<float4*>(ks + row * kPitch + e) = k;
-          *reinterpret_cast<float4*>(vs + row * D + e) = v;
+      for (int i = tid; i < kTile * D / 4; i += kThreads) {
+        const int row = i / (D / 4), e = i % (D / 4) * 4;
+        float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+        if (row < keys) {
+          const int64_t at = (int64_t)(first_key + row) * p.c_sp + e;
+          k = *reinterpret_cast<const float4*>(kbase + at);
+          v = *reinterpret_cast<const float4*>(vbase + at);
         }
+        *reinterpret_cast<float4*>(ks + row * kPitch + e) = k;
+        *reinterpret_cast<float4*>(vs + row * D + e) = v;
       }
       __syncthreads();
       {
@@ -495,7 +134,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int i = 0; i < kRows / 2; ++i) {
           const int r = half * (kRows / 2) + i;
-          const bool seen = key < keys && (!tree || (cm.mask[r] >> key & 1) != 0);
+          const int age = first_key + key - sg.length;
+          const bool seen = key < keys && (age < 0 || (masks[r] >> age & 1) != 0);
           const float x = seen ? s[i] * p.scale_log2 : -INFINITY;
           ss[r * kTile + key] = x;
           if (p.weights && key < keys && r < p.rows) score_row(p, sg, r)[first_key + key] = x;
@@ -531,8 +171,9 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
           const float w = ss[(row0 + i) * kTile + key];
-          // An unseen key's value may be infinite or NaN: no product with zero.
-          if (!tree || (cm.mask[row0 + i] >> key & 1) != 0) o[i] = fmaf(w, v, o[i]);
+          // An unseen node's value may be infinite or NaN: no product with zero.
+          const int age = first_key + key - sg.length;
+          if (!edge || age < 0 || (masks[row0 + i] >> age & 1) != 0) o[i] = fmaf(w, v, o[i]);
         }
       }
     }
@@ -541,12 +182,27 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int i = 0; i < kMine; ++i) os[(row0 + i) * D + column] = o[i];
     __syncthreads();
-    finish_segment<D, kRows, float>(p, st, cm,
-                                    [&](int r, int e, float& rm, float& rl, float4& ro) {
-                                      rm = state_m[r];
-                                      rl = state_l[r];
-                                      ro = *reinterpret_cast<const float4*>(os + r * D + e);
-                                    });
+    constexpr int kPieces = D / 4;
+    if (sg.first_cta == sg.last_cta) {
+      for (int i = tid; i < kRows * kPieces; i += kThreads) {
+        const int r = i / kPieces, e = i % kPieces * 4;
+        write_row<kRows, float>(p, sg, masks, r, e, state_m[r], state_l[r],
+                                *reinterpret_cast<const float4*>(os + r * D + e));
+      }
+    } else {
+      float* part = Parts<D, kRows>::mine(p, st);
+      for (int i = tid; i < kRows * kPieces; i += kThreads)
+        reinterpret_cast<float4*>(part + 2 * kRows)[i] = reinterpret_cast<const float4*>(os)[i];
+      if (tid < kRows) part[tid] = state_m[tid], part[kRows + tid] = state_l[tid];
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) scratch[0] = take_ticket(sg, p.counters + sg.item);
+      __syncthreads();
+      if (scratch[0]) {
+        __threadfence();
+        merge_parts<D, kRows, kRows, kThreads, float>(p, st, masks, 0, tid);
+      }
+    }
     __syncthreads();
   }
 }
@@ -581,44 +237,51 @@ __global__ void __launch_bounds__(kWeightThreads)
 
 // ------------------------------------------------------------------ host side
 
-template <typename Kernel>
-int launch(Kernel kernel, int smem, const TreeParams& p, cudaStream_t stream,
-           const char* what) {
-  if (int rc = check_cuda(
-          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what))
+template <int D>
+int launch_simt(const TreeParams& p, cudaStream_t stream) {
+  const int smem = SimtShape<D>::bytes(p.batch);
+  if (int rc = check_cuda(cudaFuncSetAttribute(tree_simt_kernel<D>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                          "cudaFuncSetAttribute(tree attention f32)"))
     return rc;
-  return launch_pdl(kernel, dim3(p.ctas), dim3(kThreads), smem, stream, what, p);
+  return launch_pdl(tree_simt_kernel<D>, dim3(p.ctas), dim3(kThreads), smem, stream,
+                    "tree attention (f32) launch", p);
 }
 
 // Query rows that one CTA holds against a key tile, by dtype and rows per
 // key/value head.
 int rows_per_block(int dtype, int rows) {
   if (dtype == ASRBACK_F32) return 16;
-  return rows <= 16 ? 16 : 32;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
 struct Plan {
   int block_rows, mblocks, ctas;
-  size_t counter_bytes, part_bytes, lse_bytes, score_bytes;
+  int q_block_bytes;
+  size_t counter_bytes, q_bytes, part_bytes, lse_bytes, score_bytes;
   int64_t score_stride;
-  size_t total() const { return counter_bytes + part_bytes + lse_bytes + score_bytes; }
+  size_t workspace() const { return q_bytes + part_bytes + lse_bytes + score_bytes; }
 };
 
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
 Plan plan_for(int dtype, int batch, int nodes, int heads, int kv_heads, int head_dim,
-              int cache_length, bool weights) {
+              int cache_length, bool rotary, bool weights) {
   Plan plan{};
   const int rows = nodes * (heads / kv_heads);
   plan.block_rows = rows_per_block(dtype, rows);
   plan.mblocks = (rows + plan.block_rows - 1) / plan.block_rows;
   const int64_t items = (int64_t)batch * kv_heads * plan.mblocks;
-  const int64_t tiles = items * ((cache_length + kTile - 1) / kTile + 1);
-  // Resident CTAs per SM: two of the 16-row kernel (96 KB rings), one of the
-  // 32-row kernel's register count.
-  const int per_sm = dtype == ASRBACK_BF16 && plan.block_rows == 16 ? 2 : 1;
+  const int64_t tiles = items * ((cache_length + kTile - 1) / kTile);
+  // As many CTAs as are resident at once.
+  const int per_sm = dtype == ASRBACK_BF16 ? mma_ctas_per_sm(head_dim, plan.block_rows)
+                                           : head_dim == 128 ? 2 : 3;
   plan.ctas = static_cast<int>(std::min<int64_t>(tiles, (int64_t)per_sm * sm_count()));
-  plan.counter_bytes = up16(items * sizeof(int));
+  plan.counter_bytes = up16(items * (plan.block_rows / 16) * sizeof(int));
+  // float32, bf16 as it comes, or (rotary) two bf16 parts; then the masks.
+  const int row_bytes = head_dim * (dtype == ASRBACK_F32 || rotary ? 4 : 2) + 8;
+  plan.q_block_bytes = plan.block_rows * row_bytes;
+  plan.q_bytes = up16((size_t)items * plan.q_block_bytes);
   plan.part_bytes = up16((size_t)2 * plan.ctas * plan.block_rows * (head_dim + 2) * sizeof(float));
   if (weights) {
     plan.score_stride = (cache_length + 3) / 4 * 4;
@@ -637,18 +300,18 @@ using namespace asrback::tree;
 extern "C" size_t asrback_tree_counter_bytes(int dtype, int batch, int nodes, int heads,
                                              int kv_heads) {
   if (batch < 1 || nodes < 1 || kv_heads < 1 || heads < kv_heads) return 0;
-  return plan_for(dtype, batch, nodes, heads, kv_heads, 64, 1, false).counter_bytes;
+  return plan_for(dtype, batch, nodes, heads, kv_heads, 64, 1, false, false).counter_bytes;
 }
 
 extern "C" size_t asrback_tree_workspace_bytes(int dtype, int batch, int nodes, int heads,
                                                int kv_heads, int head_dim, int cache_length,
-                                               int with_weights) {
+                                               int rotary, int with_weights) {
   if (batch < 1 || nodes < 1 || kv_heads < 1 || heads < kv_heads || head_dim < 1 ||
       cache_length < 1)
     return 0;
-  const Plan plan = plan_for(dtype, batch, nodes, heads, kv_heads, head_dim, cache_length,
-                             with_weights != 0);
-  return plan.total() - plan.counter_bytes;
+  return plan_for(dtype, batch, nodes, heads, kv_heads, head_dim, cache_length, rotary != 0,
+                  with_weights != 0)
+      .workspace();
 }
 
 extern "C" int asrback_tree_attention(
@@ -715,12 +378,12 @@ extern "C" int asrback_tree_attention(
                 kMaxWeightRows, rows);
   if (weights && kv_heads > 65535)
     return fail(ASRBACK_ERR_ARGUMENT, "weights take at most 65535 key/value heads");
-  const Plan plan = plan_for(dtype, batch, nodes, heads, kv_heads, head_dim, cache_length,
+  const Plan plan = plan_for(dtype, batch, nodes, heads, kv_heads, head_dim, cache_length, rotary,
                              weights != nullptr);
-  if ((int64_t)batch * kv_heads * plan.mblocks * ((cache_length + kTile - 1) / kTile + 1) >
+  if ((int64_t)batch * kv_heads * plan.mblocks * ((cache_length + kTile - 1) / kTile) >
       (int64_t)1 << 30)
     return fail(ASRBACK_ERR_ARGUMENT, "too many key tiles for one call");
-  const size_t need = plan.total() - plan.counter_bytes;
+  const size_t need = plan.workspace();
   if (!counters || counter_bytes < plan.counter_bytes)
     return fail(ASRBACK_ERR_WORKSPACE, "counters of %zu bytes, %zu needed",
                 counters ? counter_bytes : (size_t)0, plan.counter_bytes);
@@ -747,6 +410,9 @@ extern "C" int asrback_tree_attention(
   p.rows = rows, p.mblocks = plan.mblocks, p.cache_length = cache_length, p.ctas = plan.ctas;
   uint8_t* at = static_cast<uint8_t*>(workspace);
   p.counters = static_cast<int*>(counters);
+  p.q_blocks = at;
+  p.q_block_bytes = plan.q_block_bytes;
+  at += plan.q_bytes;
   p.parts = reinterpret_cast<float*>(at);
   at += plan.part_bytes;
   p.lse = reinterpret_cast<float*>(at);
@@ -756,28 +422,12 @@ extern "C" int asrback_tree_attention(
   p.status = status;
 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int rc;
-  const char* what = "tree attention launch";
-  auto mma = [&](auto dim, auto mt, auto held) {
-    constexpr int D = decltype(dim)::value, MT = decltype(mt)::value;
-    constexpr bool W = decltype(held)::value;
-    return launch(tree_mma_kernel<D, MT, W>, MmaShape<D, MT, W>::kSmem, p, s, what);
-  };
-  using std::integral_constant;
-  using one = integral_constant<int, 1>;
-  using two = integral_constant<int, 2>;
-  auto by_rows = [&](auto dim) {
-    if (weights) return mma(dim, one{}, std::true_type{});
-    if (plan.block_rows == 16) return mma(dim, one{}, std::false_type{});
-    return mma(dim, two{}, std::false_type{});
-  };
+  int rc = launch_prepare(dtype, head_dim, plan.block_rows, p, s);
+  if (rc) return rc;
   if (dtype == ASRBACK_BF16)
-    rc = head_dim == 64 ? by_rows(integral_constant<int, 64>{})
-                        : by_rows(integral_constant<int, 128>{});
-  else if (head_dim == 64)
-    rc = launch(tree_simt_kernel<64>, SimtShape<64>::kSmem, p, s, what);
+    rc = launch_mma(head_dim, plan.block_rows, p, s);
   else
-    rc = launch(tree_simt_kernel<128>, SimtShape<128>::kSmem, p, s, what);
+    rc = head_dim == 64 ? launch_simt<64>(p, s) : launch_simt<128>(p, s);
   if (rc) return rc;
   if (weights) {
     const dim3 grid((cache_length + kWeightThreads - 1) / kWeightThreads, kv_heads, batch);

@@ -1,6 +1,6 @@
-// What the draft-tree attention kernels share: the stretch of the tile list
-// that a CTA works through, the query rows' and the tree's own tile's
-// preparation, and the end of a segment (output, or part and merge).
+// What the draft-tree attention kernels share: the call's parameters, the
+// stretch of the tile list that a CTA works through, and the end of a segment
+// (output, or part and merge).
 #pragma once
 
 #include "common.cuh"
@@ -8,8 +8,8 @@
 namespace asrback {
 namespace tree {
 
-constexpr int kTile = 64;            // keys per tile; the tree (at most 64 nodes) is one tile
-constexpr int kThreads = 128;
+constexpr int kTile = 64;            // keys per tile
+constexpr int kMaxNodes = 64;
 constexpr int kMaxBatch = 1024;      // rows whose tile counts fit the CTA's shared memory
 constexpr int kMaxWeightRows = 16;   // query rows per key/value head of a call with weights
 constexpr int kMaxLength = 1 << 24;  // cache positions (packed with the node count)
@@ -31,7 +31,11 @@ struct TreeParams {
   int64_t w_sb, w_sh;
   float scale_log2;  // softmax scale times log2(e)
   int batch, nodes, kv_heads, group, rows, mblocks, cache_length, ctas;
-  int* counters;  // one per item, zero between calls
+  // The prepared query rows, a block per item: kQParts x [block rows][D]
+  // (bf16: laid out as the products read it), then the rows' masks.
+  uint8_t* q_blocks;
+  int q_block_bytes;
+  int* counters;  // per item and group of 16 rows, zero between calls
   float* parts;   // two per CTA: [rows] m, [rows] l, [rows][D] o
   float* lse;     // with weights: (batch, kv_heads, rows), base 2, +inf for an empty row
   float* scores;  // with weights: (batch, kv_heads, rows, score_stride), base 2
@@ -56,27 +60,27 @@ __device__ __forceinline__ RowSpan row_span(const TreeParams& p, int b) {
   return {static_cast<int>(length), count, false};
 }
 
-__device__ __forceinline__ int row_tiles(int length) { return (length + kTile - 1) / kTile + 1; }
+// Tiles over the row's keys, the tree's behind the cached ones; a row that is
+// skipped has one, for its zeros.
+__device__ __forceinline__ int row_tiles(int keys) { return max(1, (keys + kTile - 1) / kTile); }
 
-template <int kRows>
-struct Common {
-  unsigned long long mask[kRows];  // the tree's nodes that a query row sees; 0: an empty row
-  int prefix[kMaxBatch];           // tiles of rows 0..b
-  uint32_t span[kMaxBatch];        // length << 7 | count
-  int warp_sum[kThreads / 32];
-  int is_last;
+// The tile list of the call, in the CTA's shared memory: list_bytes(batch) at
+// `prefix`, the spans behind the prefix.
+struct TileList {
+  int* prefix;     // tiles of rows 0..b
+  uint32_t* span;  // length << 7 | count
+  __device__ __forceinline__ TileList(uint8_t* at, int batch)
+      : prefix(reinterpret_cast<int*>(at)), span(reinterpret_cast<uint32_t*>(at) + batch) {}
 };
+__host__ __device__ constexpr int list_bytes(int batch) { return (8 * batch + 15) / 16 * 16; }
 
 struct Segment {
   int b, h, mblock, item;
   int length, count;
-  int tiles;         // of the item: cache tiles, then the tree
+  int tiles;         // of the item
   int tile0, tile1;  // this segment's
   int begin;         // tile0 in the list of all tiles
   int first_cta, last_cta;
-  __device__ __forceinline__ int tile_keys(int first_key) const {
-    return first_key == length ? count : length - first_key;
-  }
 };
 
 // A CTA's stretch [lo, hi) of the list of all items' tiles, `per` tiles each.
@@ -85,8 +89,11 @@ struct Stretch {
   Segment seg;
 };
 
-template <int kRows>
-__device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, Common<kRows>& cm) {
+// Fills the tile list and finds the CTA's stretch. All kThreads threads of the
+// CTA call it; `scratch` holds kThreads / 32 ints.
+template <int kThreads>
+__device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, const TileList& list,
+                                                 int* scratch) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int carry = 0;
   for (int base = 0; base < p.batch; base += kThreads) {
@@ -94,9 +101,8 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, Common<kRo
     int tiles = 0;
     if (b < p.batch) {
       const RowSpan s = row_span(p, b);
-      if (s.bad && blockIdx.x == 0 && p.status) atomicOr(p.status, ASRBACK_STATUS_POSITION);
-      cm.span[b] = static_cast<uint32_t>(s.length) << 7 | s.count;
-      tiles = row_tiles(s.length) * p.kv_heads * p.mblocks;
+      list.span[b] = static_cast<uint32_t>(s.length) << 7 | s.count;
+      tiles = row_tiles(s.length + s.count) * p.kv_heads * p.mblocks;
     }
     int sum = tiles;
 #pragma unroll
@@ -104,13 +110,16 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, Common<kRo
       const int x = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += x;
     }
-    if (lane == 31) cm.warp_sum[warp] = sum;
+    if (lane == 31) scratch[warp] = sum;
     __syncthreads();
+    sum += carry;
+#pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) sum += cm.warp_sum[w];
+      const int s = scratch[w];
+      if (w < warp) sum += s;
+      carry += s;
     }
-    if (b < p.batch) cm.prefix[b] = sum + carry;
-    for (int w = 0; w < kThreads / 32; ++w) carry += cm.warp_sum[w];
+    if (b < p.batch) list.prefix[b] = sum;
     __syncthreads();
   }
   Stretch st;
@@ -122,7 +131,7 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, Common<kRo
   int low = 0, high = p.batch - 1;  // the first row whose prefix lies past lo
   while (low < high) {
     const int mid = (low + high) >> 1;
-    if (cm.prefix[mid] > st.lo) high = mid;
+    if (list.prefix[mid] > st.lo) high = mid;
     else low = mid + 1;
   }
   st.row = low;
@@ -130,17 +139,16 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, Common<kRo
 }
 
 // The next (part of an) item of the stretch; false at its end.
-template <int kRows>
-__device__ __forceinline__ bool next_segment(const TreeParams& p, const Common<kRows>& cm,
+__device__ __forceinline__ bool next_segment(const TreeParams& p, const TileList& list,
                                              Stretch& st) {
   if (st.cur >= st.hi) return false;
-  while (cm.prefix[st.row] <= st.cur) ++st.row;
+  while (list.prefix[st.row] <= st.cur) ++st.row;
   Segment& s = st.seg;
-  const int base = st.row > 0 ? cm.prefix[st.row - 1] : 0;
+  const int base = st.row > 0 ? list.prefix[st.row - 1] : 0;
   s.b = st.row;
-  s.length = static_cast<int>(cm.span[s.b] >> 7);
-  s.count = static_cast<int>(cm.span[s.b] & 127u);
-  s.tiles = row_tiles(s.length);
+  s.length = static_cast<int>(list.span[s.b] >> 7);
+  s.count = static_cast<int>(list.span[s.b] & 127u);
+  s.tiles = row_tiles(s.length + s.count);
   const int index = (st.cur - base) / s.tiles;
   s.h = index / p.mblocks;
   s.mblock = index % p.mblocks;
@@ -159,233 +167,119 @@ __device__ __forceinline__ float* score_row(const TreeParams& p, const Segment& 
   return p.scores + (((int64_t)s.b * p.kv_heads + s.h) * p.rows + r) * p.score_stride;
 }
 
-// A lane's D / 32 consecutive elements of a row.
-template <int D, typename T>
-__device__ __forceinline__ void load_lane(const void* row, int lane, float* x) {
-  if constexpr (sizeof(T) == 4) {
-    if constexpr (D == 128) {
-      const float4 v = __ldg(static_cast<const float4*>(row) + lane);
-      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    } else {
-      const float2 v = __ldg(static_cast<const float2*>(row) + lane);
-      x[0] = v.x, x[1] = v.y;
-    }
-  } else {
-    uint32_t u[D / 64];
-    if constexpr (D == 128) {
-      const uint2 v = __ldg(static_cast<const uint2*>(row) + lane);
-      u[0] = v.x, u[1] = v.y;
-    } else {
-      u[0] = __ldg(static_cast<const uint32_t*>(row) + lane);
-    }
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      x[2 * i] = __uint_as_float(u[i] << 16);
-      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
-  }
-}
-
-template <int D, typename T>
-__device__ __forceinline__ void store_lane(void* row, int lane, const float* x) {
-  if constexpr (sizeof(T) == 4) {
-    if constexpr (D == 128)
-      static_cast<float4*>(row)[lane] = make_float4(x[0], x[1], x[2], x[3]);
-    else
-      static_cast<float2*>(row)[lane] = make_float2(x[0], x[1]);
-  } else {
-    __nv_bfloat162 h[D / 64];
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    if constexpr (D == 128)
-      static_cast<uint2*>(row)[lane] = *reinterpret_cast<uint2*>(h);
-    else
-      static_cast<uint32_t*>(row)[lane] = *reinterpret_cast<uint32_t*>(h);
-  }
-}
-
-// RMSNorm, then rotate-half rotary embedding of one head's row, D / 32
-// consecutive elements per lane, all in float32: element d pairs with d +- D/2,
-// which lane ^ 16 holds.
-template <int D, typename T>
-__device__ __forceinline__ void norm_rotate(const TreeParams& p, const void* weight, int64_t place,
-                                            int lane, float* x) {
-  constexpr int E = D / 32;
-  float w[E], cs[E], sn[E];
-  load_lane<D, T>(weight, lane, w);
-  load_lane<D, T>(static_cast<const T*>(p.cos) + place * p.table_stride, lane, cs);
-  load_lane<D, T>(static_cast<const T*>(p.sin) + place * p.table_stride, lane, sn);
-  float ss = 0.f;
-#pragma unroll
-  for (int j = 0; j < E; ++j) ss = fmaf(x[j], x[j], ss);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float r = rsqrtf(ss / D + p.eps);
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const float y = x[j] * r * w[j];
-    const float pair = __shfl_xor_sync(0xffffffffu, y, 16);
-    x[j] = y * cs[j] + (lane < 16 ? -pair : pair) * sn[j];
-  }
-}
-
-// The block's query rows: row r is node r / group, head r % group. Fills
-// cm.mask and calls store(row, element, values, count) for each lane's piece;
-// empty rows (no such node, or a mask without bits) are zeros.
-template <int D, int kRows, typename T, typename Store>
-__device__ __forceinline__ void prepare_rows(const TreeParams& p, const Segment& s,
-                                             Common<kRows>& cm, int warp, int lane, Store store) {
-  constexpr int E = D / 32;
-  const unsigned long long live = s.count >= 64 ? ~0ull : (1ull << s.count) - 1;
-  const int64_t position = p.q_norm ? p.positions[s.b] : 0;
-#pragma unroll 4
-  for (int i = 0; i < kRows / 4; ++i) {
-    const int r = warp + 4 * i, row = s.mblock * kRows + r;
-    const int node = row / p.group, head = s.h * p.group + row % p.group;
-    float x[E];
-#pragma unroll
-    for (int j = 0; j < E; ++j) x[j] = 0.f;
-    unsigned long long mask = 0;
-    if (row < p.rows && node < s.count) {
-      mask = static_cast<unsigned long long>(__ldg(p.ancestors + (int64_t)s.b * p.nodes + node)) &
-             live;
-      if (mask) {
-        load_lane<D, T>(static_cast<const T*>(p.q) + s.b * p.q_sb + node * p.q_sn + head * p.q_sh,
-                        lane, x);
-        if (p.q_norm) {
-          const int depth = min(max(__ldg(p.depths + (int64_t)s.b * p.nodes + node), 0), node);
-          norm_rotate<D, T>(p, p.q_norm, position + depth, lane, x);
-        }
-      }
-    }
-    if (lane == 0) cm.mask[r] = mask;
-    store(r, lane * E, x, E);
-  }
-}
-
-// The tree's keys and values: normalised and rotated, rounded to T, written to
-// the cache (by the first block of query rows) and handed to store(node,
-// element, key, value, count). Nodes up to the next multiple of 16 are zeros.
-// Returns, after a barrier, whether every value is finite.
-template <int D, typename T, int kRows, typename Store>
-__device__ __forceinline__ bool load_tree_tile(const TreeParams& p, const Segment& s,
-                                               Common<kRows>& cm, int warp, int lane, Store store) {
-  constexpr int E = D / 32;
-  const int64_t position = p.q_norm ? p.positions[s.b] : 0;
-  bool finite = true;
-#pragma unroll 2
-  for (int i = warp; i < (s.count + 15) / 16 * 16; i += 4) {
-    float k[E], v[E];
-#pragma unroll
-    for (int j = 0; j < E; ++j) k[j] = v[j] = 0.f;
-    if (i < s.count) {
-      load_lane<D, T>(static_cast<const T*>(p.k) + s.b * p.k_sb + i * p.k_sn + s.h * p.k_sh, lane,
-                      k);
-      load_lane<D, T>(static_cast<const T*>(p.v) + s.b * p.v_sb + i * p.v_sn + s.h * p.v_sh, lane,
-                      v);
-      if (p.q_norm) {
-        const int depth = min(max(__ldg(p.depths + (int64_t)s.b * p.nodes + i), 0), i);
-        norm_rotate<D, T>(p, p.k_norm, position + depth, lane, k);
-      }
-      if (s.mblock == 0) {
-        const int64_t at = s.b * p.c_sb + (int64_t)(s.length + i) * p.c_sp + s.h * p.c_sh;
-        store_lane<D, T>(static_cast<T*>(p.key_cache) + at, lane, k);
-        store_lane<D, T>(static_cast<T*>(p.value_cache) + at, lane, v);
-      }
-#pragma unroll
-      for (int j = 0; j < E; ++j) finite &= fabsf(v[j]) < INFINITY;
-    }
-    store(i, lane * E, k, v, E);
-  }
-  return __syncthreads_and(finite) != 0;
-}
-
-// The end of a segment. get(row, element, m, l, o) gives the CTA's state of a
-// query row and four elements of its unnormalised output. An item that lies
-// in one CTA is written out; otherwise the part goes to the workspace and the
-// item's last CTA merges all of them, in the order of the tile list.
-template <int D, int kRows, typename T, typename Get>
-__device__ __forceinline__ void finish_segment(const TreeParams& p, const Stretch& st,
-                                               Common<kRows>& cm, Get get) {
-  constexpr int kPieces = D / 4;
-  constexpr int kPart = kRows * (D + 2);
-  const Segment& s = st.seg;
-  const int tid = threadIdx.x;
-  auto write = [&](int r, int e, float m, float l, float4 o) {
-    const int row = s.mblock * kRows + r;
-    if (row >= p.rows) return;
-    const bool empty = cm.mask[r] == 0;
-    if (p.weights && e == 0)
-      p.lse[((int64_t)s.b * p.kv_heads + s.h) * p.rows + row] = empty ? INFINITY : m + log2f(l);
-    const float f = empty ? 0.f : 1.f / l;
-    if (empty) o = make_float4(0.f, 0.f, 0.f, 0.f);
-    T* out = static_cast<T*>(p.out) + s.b * p.o_sb + (row / p.group) * p.o_sn +
-             (s.h * p.group + row % p.group) * p.o_sh + e;
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(out) = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-    } else {
-      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(o.x * f, o.y * f),
-                             __floats2bfloat162_rn(o.z * f, o.w * f)};
-      *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(h);
-    }
-  };
-  if (s.first_cta == s.last_cta) {
-    for (int i = tid; i < kRows * kPieces; i += kThreads) {
-      float m, l;
-      float4 o;
-      get(i / kPieces, i % kPieces * 4, m, l, o);
-      write(i / kPieces, i % kPieces * 4, m, l, o);
-    }
-    return;
-  }
+// Where a segment's result goes.
+template <int D, int kRows>
+struct Parts {
+  static constexpr int kFloats = kRows * (D + 2);  // [rows] m, [rows] l, [rows][D] o
   // A CTA's first segment leaves part 0, a later one (its last) part 1.
-  const int cta = blockIdx.x;
-  float* part = p.parts + (int64_t)(2 * cta + (s.begin == st.lo ? 0 : 1)) * kPart;
-  for (int i = tid; i < kRows * kPieces; i += kThreads) {
-    const int r = i / kPieces, e = i % kPieces * 4;
-    float m, l;
-    float4 o;
-    get(r, e, m, l, o);
-    if (e == 0) part[r] = m, part[kRows + r] = l;
-    *reinterpret_cast<float4*>(part + 2 * kRows + r * D + e) = o;
+  __device__ __forceinline__ static float* mine(const TreeParams& p, const Stretch& st) {
+    return p.parts + (int64_t)(2 * blockIdx.x + (st.seg.begin == st.lo ? 0 : 1)) * kFloats;
   }
-  __threadfence();
-  __syncthreads();
-  const int ctas = s.last_cta - s.first_cta + 1;
-  if (tid == 0) {
-    cm.is_last = atomicAdd(p.counters + s.item, 1) == ctas - 1;
-    if (cm.is_last) p.counters[s.item] = 0;
+  // Part c of the item; its first CTA may have begun it behind another item.
+  __device__ __forceinline__ static const float* of(const TreeParams& p, const Stretch& st, int c) {
+    const Segment& s = st.seg;
+    const int start = s.begin - s.tile0;
+    const int second = c == 0 && start != s.first_cta * st.per ? 1 : 0;
+    return p.parts + (int64_t)(2 * (s.first_cta + c) + second) * kFloats;
   }
-  __syncthreads();
-  if (!cm.is_last) return;
-  __threadfence();
-  // The item's first CTA may have begun it behind another item (part 1).
-  const int start = s.begin - s.tile0;
-  const float* parts0 =
-      p.parts + (int64_t)(2 * s.first_cta + (start == s.first_cta * st.per ? 0 : 1)) * kPart;
-  auto part_of = [&](int c) {
-    return c == 0 ? parts0 : p.parts + (int64_t)(2 * (s.first_cta + c)) * kPart;
-  };
-  for (int i = tid; i < kRows * kPieces; i += kThreads) {
-    const int r = i / kPieces, e = i % kPieces * 4;
-    if (s.mblock * kRows + r >= p.rows) continue;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = 0; c < ctas; ++c) m = fmaxf(m, __ldcg(part_of(c) + r));
-    const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-    for (int c = 0; c < ctas; ++c) {
-      const float* x = part_of(c);
-      const float a = fast_exp2(__ldcg(x + r) - ref);
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(x + 2 * kRows + r * D + e));
-      l = fmaf(__ldcg(x + kRows + r), a, l);
-      o.x = fmaf(y.x, a, o.x), o.y = fmaf(y.y, a, o.y);
-      o.z = fmaf(y.z, a, o.z), o.w = fmaf(y.w, a, o.w);
-    }
-    write(r, e, m, l, o);
+};
+
+// Four elements of an output row from its unnormalised sum, and (with weights)
+// the row's log-sum-exp. Empty rows give zeros.
+template <int kRows, typename T>
+__device__ __forceinline__ void write_row(const TreeParams& p, const Segment& s,
+                                          const unsigned long long* masks, int r, int e, float m,
+                                          float l, float4 o) {
+  const int row = s.mblock * kRows + r;
+  if (row >= p.rows) return;
+  const bool empty = masks[r] == 0;
+  if (p.weights && e == 0)
+    p.lse[((int64_t)s.b * p.kv_heads + s.h) * p.rows + row] = empty ? INFINITY : m + log2f(l);
+  const float f = 1.f / l;
+  o = empty ? make_float4(0.f, 0.f, 0.f, 0.f)
+            : make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+  T* out = static_cast<T*>(p.out) + s.b * p.o_sb + (row / p.group) * p.o_sn +
+           (s.h * p.group + row % p.group) * p.o_sh + e;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(out) = o;
+  } else {
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(o.x, o.y), __floats2bfloat162_rn(o.z, o.w)};
+    *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(h);
   }
 }
+
+// Merges rows row0 .. row0 + kCount - 1 of the item's parts, in the order of the
+// tile list, and writes them out; kThreads threads call it, after the last
+// ticket of the rows has been taken. A thread's elements of a part are loaded
+// together, so that a part costs one latency.
+template <int D, int kRows, int kCount, int kThreads, typename T>
+__device__ __forceinline__ void merge_parts(const TreeParams& p, const Stretch& st,
+                                            const unsigned long long* masks, int row0, int tid) {
+  constexpr int kPieces = D / 4;
+  constexpr int kMine = kCount * kPieces / kThreads;
+  static_assert(kCount * kPieces % kThreads == 0, "the rows are shared out evenly");
+  const Segment& s = st.seg;
+  const int ctas = s.last_cta - s.first_cta + 1;
+  float m[kMine], l[kMine];
+  float4 o[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll 2
+  for (int c = 0; c < ctas; ++c) {
+    const float* x = Parts<D, kRows>::of(p, st, c);
+    float m2[kMine], l2[kMine];
+    float4 y[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int at = tid + i * kThreads, r = row0 + at / kPieces, e = at % kPieces * 4;
+      m2[i] = __ldcg(x + r);
+      l2[i] = __ldcg(x + kRows + r);
+      y[i] = __ldcg(reinterpret_cast<const float4*>(x + 2 * kRows + r * D + e));
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const float now = fmaxf(m[i], m2[i]), ref = now == -INFINITY ? 0.f : now;
+      const float a = fast_exp2(m[i] - ref), b = fast_exp2(m2[i] - ref);
+      m[i] = now;
+      l[i] = l[i] * a + l2[i] * b;
+      o[i].x = o[i].x * a + y[i].x * b, o[i].y = o[i].y * a + y[i].y * b;
+      o[i].z = o[i].z * a + y[i].z * b, o[i].w = o[i].w * a + y[i].w * b;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = tid + i * kThreads;
+    write_row<kRows, T>(p, s, masks, row0 + at / kPieces, at % kPieces * 4, m[i], l[i], o[i]);
+  }
+}
+
+// Takes a ticket of the item (one thread, once its CTA's part is in memory):
+// true for the last of the item's CTAs, which also re-arms the counter.
+__device__ __forceinline__ bool take_ticket(const Segment& s, int* counter) {
+  const bool last = atomicAdd(counter, 1) == s.last_cta - s.first_cta;
+  if (last) *counter = 0;
+  return last;
+}
+
+// Byte offset of 16-byte piece `piece` of row `row` in a tile of `rows` rows of
+// D bf16, as a 128-byte-swizzled TMA box lays it out: columns in blocks of 64
+// elements, pieces permuted within a row's 128 bytes.
+template <int D>
+__device__ __forceinline__ int tile_at(int rows, int row, int piece) {
+  return (piece >> 3) * rows * 128 + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+}
+
+// tree_prepare.cu: the query blocks, and the nodes' keys and values in the
+// cache. `split`: q times the scale, in two bf16 parts.
+int launch_prepare(int dtype, int head_dim, int block_rows, const TreeParams& p,
+                   cudaStream_t stream);
+// tree_attention_mma.cu: bf16, blocks of 16, 32 or 64 query rows.
+int mma_ctas_per_sm(int head_dim, int block_rows);
+int launch_mma(int head_dim, int block_rows, const TreeParams& p, cudaStream_t stream);
 
 }  // namespace tree
 }  // namespace asrback

@@ -418,14 +418,15 @@ ASRBACK_API int asrback_draft_tree(
  * counters     asrback_tree_counter_bytes(...) bytes, zero before the first
  *              call; every call leaves them zero. Calls that may run at the
  *              same time (other streams, other graphs) need their own.
- * workspace    asrback_tree_workspace_bytes(...) bytes of scratch, of any
+ * workspace    asrback_tree_workspace_bytes(...) bytes of scratch (rotary:
+ *              q_norm_weight is given, with_weights: weights are), of any
  *              content; likewise not shared by calls that run at the same time.
  */
 ASRBACK_API size_t asrback_tree_counter_bytes(int dtype, int batch, int nodes, int heads,
                                               int kv_heads);
 ASRBACK_API size_t asrback_tree_workspace_bytes(int dtype, int batch, int nodes, int heads,
                                                 int kv_heads, int head_dim, int cache_length,
-                                                int with_weights);
+                                                int rotary, int with_weights);
 ASRBACK_API int asrback_tree_attention(
     int dtype, int batch, int nodes, int heads, int kv_heads, int head_dim, int cache_length,
     const void* query, int64_t q_stride_batch, int64_t q_stride_node, int64_t q_stride_head,

@@ -40,7 +40,7 @@ def norm_rotate(x, weight, cos, sin, eps):
 
 
 def tree_attention(q, k, v, keys, values, lengths, above, counts, scale, weights=None,
-                   rotary=None, bf16=False, round_q=False):
+                   rotary=None, bf16=False):
     """``q`` (B, N, H, D), ``k``/``v`` (B, N, KVH, D), caches (B, L, KVH, D):
     returns ``out`` (B, N, H, D), the caches and weights after the call, and for
     tolerances ``mass`` (the outputs' sums of |p v|) and ``reach`` (each row's
@@ -65,8 +65,6 @@ def tree_attention(q, k, v, keys, values, lengths, above, counts, scale, weights
             kb = norm_rotate(kb, wk, cos[at][:, None], sin[at][:, None], eps)
         if bf16:
             kb = bf16_round(kb.astype(np.float32)).astype(np.float64)
-            if round_q:
-                qb = bf16_round(qb.astype(np.float32)).astype(np.float64)
         keys[b, m:m + n], values[b, m:m + n] = kb, v[b, :n]
         if weights is not None:
             weights[b, :, m:m + n] = 0

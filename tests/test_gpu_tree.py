@@ -3,10 +3,10 @@ float64 oracle (``oracle/tree.py``).
 
 Tolerances. A bf16 output is rounded once (2^-8 of it at most, half a step) and
 its probabilities once before the second product (2^-8 of the sum of |p v|, the
-``mass``). The oracle rounds q where the kernel does; a float32 q or k that
-falls on the other side of a rounding border moves one element by a step
-(2^-7): two such elements per row are allowed for, each worth 2^-7 * max |q k|
-in its score. Float32 sums of n terms add n * 2^-24 of the terms' sum. A score
+``mass``). A rotated q is taken in two bf16 parts (2^-17). A rotated k that
+falls on the other side of a rounding border in float32 than in float64 moves
+one element by a step (2^-7): two such elements per key are allowed for, each
+worth 2^-7 * max |q k| in its score. Float32 sums of n terms add n * 2^-24 of the terms' sum. A score
 off by d moves a probability by the factor e^(2 d) at most (once itself, once
 in the sum).
 """
@@ -111,8 +111,7 @@ def _want(x):
                   depths)
     weights = None if x["weights"] is None else _np(x["weights"])
     return oracle.tree_attention(q, k, v, keys, values, x["lengths"], above, x["counts"],
-                                 dim ** -0.5, weights, rotary, x["tag"] == "bf16",
-                                 round_q=x["weights"] is None)
+                                 dim ** -0.5, weights, rotary, x["tag"] == "bf16")
 
 
 def _check(x, got, want):
@@ -122,9 +121,7 @@ def _check(x, got, want):
     n_keys = int(x["lengths"].max()) + 64
     d = dim * 2.0 ** -24 * full + 2.0 ** -22 * (1 + full)
     if bf16 and x["family"] == "qwen3":
-        d = d + 2 * 2.0 ** -7 * top
-    if bf16 and x["weights"] is not None:
-        d = d + 2.0 ** -17 * full
+        d = d + 2 * 2.0 ** -7 * top + 2.0 ** -17 * full
     shift = np.expm1(2 * d)
     rounding = 2.0 ** -8 if bf16 else 2.0 ** -24
     tol = rounding * np.abs(want["out"]) + want["mass"] * (
