@@ -183,24 +183,28 @@ __global__ void __launch_bounds__(kThreads)
     for (int i = 0; i < kMine; ++i) os[(row0 + i) * D + column] = o[i];
     __syncthreads();
     constexpr int kPieces = D / 4;
-    if (sg.first_cta == sg.last_cta) {
+    if (sg.whole()) {
       for (int i = tid; i < kRows * kPieces; i += kThreads) {
-        const int r = i / kPieces, e = i % kPieces * 4;
-        write_row<kRows, float>(p, sg, masks, r, e, state_m[r], state_l[r],
-                                *reinterpret_cast<const float4*>(os + r * D + e));
+        const int r = i / kPieces, e = i % kPieces * 4, row = sg.mblock * kRows + r;
+        if (row >= p.rows) break;
+        const bool empty = masks[r] == 0;
+        write_four<float>(out_row<float>(p, sg, row) + e, empty, state_l[r],
+                          *reinterpret_cast<const float4*>(os + r * D + e));
+        if (p.weights && e == 0) write_lse(p, sg, row, empty, state_m[r], state_l[r]);
       }
     } else {
-      float* part = Parts<D, kRows>::mine(p, st);
+      float* part = Parts<D>::mine(p, st);
       for (int i = tid; i < kRows * kPieces; i += kThreads)
         reinterpret_cast<float4*>(part + 2 * kRows)[i] = reinterpret_cast<const float4*>(os)[i];
       if (tid < kRows) part[tid] = state_m[tid], part[kRows + tid] = state_l[tid];
       __threadfence();
       __syncthreads();
-      if (tid == 0) scratch[0] = take_ticket(sg, p.counters + sg.item);
+      const Sharers by(st);
+      if (tid == 0) scratch[0] = take_ticket(by, p.counters + sg.item);
       __syncthreads();
       if (scratch[0]) {
         __threadfence();
-        merge_parts<D, kRows, kRows, kThreads, float>(p, st, masks, 0, tid);
+        merge_parts<D, kThreads, float>(p, sg, by, masks, state_m, state_l, tid, [] { __syncthreads(); });
       }
     }
     __syncthreads();
@@ -249,11 +253,15 @@ int launch_simt(const TreeParams& p, cudaStream_t stream) {
 }
 
 // Query rows that one CTA holds against a key tile, by dtype and rows per
-// key/value head.
+// key/value head: in bf16 whole warps of TMEM lanes.
 int rows_per_block(int dtype, int rows) {
   if (dtype == ASRBACK_F32) return 16;
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  return std::min((rows + 31) / 32 * 32, 128);
 }
+
+// Fewest tiles of a CTA: below, the merge of the parts takes longer than the
+// tiles it saves. (A float32 tile on the FMA pipes takes longer than a merge.)
+int min_tiles(int dtype) { return dtype == ASRBACK_F32 ? 1 : 4; }
 
 struct Plan {
   int block_rows, mblocks, ctas;
@@ -274,17 +282,16 @@ Plan plan_for(int dtype, int batch, int nodes, int heads, int kv_heads, int head
   const int64_t items = (int64_t)batch * kv_heads * plan.mblocks;
   const int64_t tiles = items * ((cache_length + kTile - 1) / kTile);
   // As many CTAs as are resident at once.
-  const int per_sm = dtype == ASRBACK_BF16 ? mma_ctas_per_sm(head_dim, plan.block_rows)
-                                           : head_dim == 128 ? 2 : 3;
+  const int per_sm = dtype == ASRBACK_BF16 ? 1 : head_dim == 128 ? 2 : 3;
   plan.ctas = static_cast<int>(std::min<int64_t>(tiles, (int64_t)per_sm * sm_count()));
-  plan.counter_bytes = up16(items * (plan.block_rows / 16) * sizeof(int));
+  plan.counter_bytes = up16(items * sizeof(int));
   // float32, bf16 as it comes, or (rotary) two bf16 parts; then the masks.
   const int row_bytes = head_dim * (dtype == ASRBACK_F32 || rotary ? 4 : 2) + 8;
   plan.q_block_bytes = plan.block_rows * row_bytes;
   plan.q_bytes = up16((size_t)items * plan.q_block_bytes);
   plan.part_bytes = up16((size_t)2 * plan.ctas * plan.block_rows * (head_dim + 2) * sizeof(float));
   if (weights) {
-    plan.score_stride = (cache_length + 3) / 4 * 4;
+    plan.score_stride = (cache_length + kTile - 1) / kTile * kTile;
     plan.lse_bytes = up16((size_t)batch * kv_heads * rows * sizeof(float));
     plan.score_bytes = (size_t)batch * kv_heads * rows * plan.score_stride * sizeof(float);
   }
@@ -407,7 +414,9 @@ extern "C" int asrback_tree_attention(
   p.weights = weights, p.w_sb = w_stride_batch, p.w_sh = w_stride_head;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.batch = batch, p.nodes = nodes, p.kv_heads = kv_heads, p.group = heads / kv_heads;
-  p.rows = rows, p.mblocks = plan.mblocks, p.cache_length = cache_length, p.ctas = plan.ctas;
+  p.cache_length = cache_length, p.rows = rows;
+  p.block_rows = plan.block_rows, p.mblocks = plan.mblocks;
+  p.ctas = plan.ctas, p.min_tiles = min_tiles(dtype);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   p.counters = static_cast<int*>(counters);
   p.q_blocks = at;
@@ -422,10 +431,10 @@ extern "C" int asrback_tree_attention(
   p.status = status;
 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int rc = launch_prepare(dtype, head_dim, plan.block_rows, p, s);
+  int rc = launch_prepare(dtype, head_dim, p, s);
   if (rc) return rc;
   if (dtype == ASRBACK_BF16)
-    rc = launch_mma(head_dim, plan.block_rows, p, s);
+    rc = launch_tc(head_dim, p, s);
   else
     rc = head_dim == 64 ? launch_simt<64>(p, s) : launch_simt<128>(p, s);
   if (rc) return rc;

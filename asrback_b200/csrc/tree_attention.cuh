@@ -30,13 +30,15 @@ struct TreeParams {
   float* weights;
   int64_t w_sb, w_sh;
   float scale_log2;  // softmax scale times log2(e)
-  int batch, nodes, kv_heads, group, rows, mblocks, cache_length, ctas;
-  // The prepared query rows, a block per item: kQParts x [block rows][D]
-  // (bf16: laid out as the products read it), then the rows' masks.
+  int batch, nodes, kv_heads, group, cache_length;
+  int rows, block_rows, mblocks;  // query rows per key/value head, in blocks
+  int ctas, min_tiles;            // fewest tiles of a CTA's stretch
+  // The prepared query rows, a block per item: [block rows][D] (bf16: laid out as
+  // the products read it, in two parts if rotated), then the rows' masks.
   uint8_t* q_blocks;
   int q_block_bytes;
-  int* counters;  // per item and group of 16 rows, zero between calls
-  float* parts;   // two per CTA: [rows] m, [rows] l, [rows][D] o
+  int* counters;  // one per item, zero between calls
+  float* parts;   // two per CTA: [block rows] m, l, [block rows][D] o
   float* lse;     // with weights: (batch, kv_heads, rows), base 2, +inf for an empty row
   float* scores;  // with weights: (batch, kv_heads, rows, score_stride), base 2
   int64_t score_stride;
@@ -80,12 +82,14 @@ struct Segment {
   int tiles;         // of the item
   int tile0, tile1;  // this segment's
   int begin;         // tile0 in the list of all tiles
-  int first_cta, last_cta;
+  __device__ __forceinline__ bool whole() const { return tile1 - tile0 == tiles; }
 };
 
-// A CTA's stretch [lo, hi) of the list of all items' tiles, `per` tiles each.
+// A CTA's stretch [cur, hi) of the list of all items' tiles, `per` tiles each
+// from `lo` on: `cur` is tile `tile` of item (row, h, mblock).
 struct Stretch {
-  int lo, hi, cur, per, row;
+  int lo, hi, cur, per;
+  int row, h, mblock, tile;
   Segment seg;
 };
 
@@ -124,7 +128,7 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, const Tile
   }
   Stretch st;
   const int total = carry;
-  st.per = (total + p.ctas - 1) / p.ctas;
+  st.per = max((total + p.ctas - 1) / p.ctas, p.min_tiles);
   st.lo = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * st.per, (int64_t)total));
   st.hi = min(st.lo + st.per, total);
   st.cur = st.lo;
@@ -135,6 +139,11 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, const Tile
     else low = mid + 1;
   }
   st.row = low;
+  const int tiles = row_tiles(static_cast<int>((list.span[low] >> 7) + (list.span[low] & 127u)));
+  const int off = st.lo - (low > 0 ? list.prefix[low - 1] : 0), index = off / tiles;
+  st.tile = off - index * tiles;
+  st.h = index / p.mblocks;
+  st.mblock = index - st.h * p.mblocks;
   return st;
 }
 
@@ -142,64 +151,79 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, const Tile
 __device__ __forceinline__ bool next_segment(const TreeParams& p, const TileList& list,
                                              Stretch& st) {
   if (st.cur >= st.hi) return false;
-  while (list.prefix[st.row] <= st.cur) ++st.row;
   Segment& s = st.seg;
-  const int base = st.row > 0 ? list.prefix[st.row - 1] : 0;
   s.b = st.row;
+  s.h = st.h;
+  s.mblock = st.mblock;
+  s.item = (s.b * p.kv_heads + s.h) * p.mblocks + s.mblock;
   s.length = static_cast<int>(list.span[s.b] >> 7);
   s.count = static_cast<int>(list.span[s.b] & 127u);
   s.tiles = row_tiles(s.length + s.count);
-  const int index = (st.cur - base) / s.tiles;
-  s.h = index / p.mblocks;
-  s.mblock = index % p.mblocks;
-  s.item = s.b * p.kv_heads * p.mblocks + index;
-  const int start = base + index * s.tiles;
-  s.tile0 = st.cur - start;
-  s.tile1 = min(s.tiles, st.hi - start);
-  s.first_cta = start / st.per;
-  s.last_cta = (start + s.tiles - 1) / st.per;
+  s.tile0 = st.tile;
   s.begin = st.cur;
-  st.cur = start + s.tile1;
+  s.tile1 = min(s.tiles, s.tile0 + st.hi - st.cur);
+  st.cur += s.tile1 - s.tile0;
+  st.tile = 0;
+  if (++st.mblock == p.mblocks) {
+    st.mblock = 0;
+    if (++st.h == p.kv_heads) {
+      st.h = 0;
+      ++st.row;
+    }
+  }
   return true;
 }
+
+// The CTAs that hold parts of the segment's item.
+struct Sharers {
+  int first, count;
+  bool begins;  // the item begins the first one's stretch
+  __device__ __forceinline__ Sharers(const Stretch& st) {
+    const int start = st.seg.begin - st.seg.tile0;
+    first = start / st.per;
+    count = (start + st.seg.tiles - 1) / st.per - first + 1;
+    begins = start == first * st.per;
+  }
+};
 
 __device__ __forceinline__ float* score_row(const TreeParams& p, const Segment& s, int r) {
   return p.scores + (((int64_t)s.b * p.kv_heads + s.h) * p.rows + r) * p.score_stride;
 }
 
-// Where a segment's result goes.
-template <int D, int kRows>
+// Where a segment's result goes, if other CTAs hold the rest of its item: m and l
+// of the block's rows, then their unnormalised outputs.
+template <int D>
 struct Parts {
-  static constexpr int kFloats = kRows * (D + 2);  // [rows] m, [rows] l, [rows][D] o
+  __device__ __forceinline__ static int64_t floats(const TreeParams& p) {
+    return (int64_t)p.block_rows * (D + 2);
+  }
   // A CTA's first segment leaves part 0, a later one (its last) part 1.
   __device__ __forceinline__ static float* mine(const TreeParams& p, const Stretch& st) {
-    return p.parts + (int64_t)(2 * blockIdx.x + (st.seg.begin == st.lo ? 0 : 1)) * kFloats;
+    return p.parts + (2 * blockIdx.x + (st.seg.begin == st.lo ? 0 : 1)) * floats(p);
   }
   // Part c of the item; its first CTA may have begun it behind another item.
-  __device__ __forceinline__ static const float* of(const TreeParams& p, const Stretch& st, int c) {
-    const Segment& s = st.seg;
-    const int start = s.begin - s.tile0;
-    const int second = c == 0 && start != s.first_cta * st.per ? 1 : 0;
-    return p.parts + (int64_t)(2 * (s.first_cta + c) + second) * kFloats;
+  __device__ __forceinline__ static const float* of(const TreeParams& p, const Sharers& by, int c) {
+    return p.parts + (2 * (by.first + c) + (c == 0 && !by.begins ? 1 : 0)) * floats(p);
   }
 };
 
-// Four elements of an output row from its unnormalised sum, and (with weights)
-// the row's log-sum-exp. Empty rows give zeros.
-template <int kRows, typename T>
-__device__ __forceinline__ void write_row(const TreeParams& p, const Segment& s,
-                                          const unsigned long long* masks, int r, int e, float m,
-                                          float l, float4 o) {
-  const int row = s.mblock * kRows + r;
-  if (row >= p.rows) return;
-  const bool empty = masks[r] == 0;
-  if (p.weights && e == 0)
-    p.lse[((int64_t)s.b * p.kv_heads + s.h) * p.rows + row] = empty ? INFINITY : m + log2f(l);
+// An output row's elements from `e` on, and its log-sum-exp (with weights).
+template <typename T>
+__device__ __forceinline__ T* out_row(const TreeParams& p, const Segment& s, int row) {
+  return static_cast<T*>(p.out) + s.b * p.o_sb + (row / p.group) * p.o_sn +
+         (s.h * p.group + row % p.group) * p.o_sh;
+}
+__device__ __forceinline__ void write_lse(const TreeParams& p, const Segment& s, int row,
+                                          bool empty, float m, float l) {
+  p.lse[((int64_t)s.b * p.kv_heads + s.h) * p.rows + row] = empty ? INFINITY : m + log2f(l);
+}
+
+// Four elements of a row from its unnormalised sum; zeros for an empty row.
+template <typename T>
+__device__ __forceinline__ void write_four(T* out, bool empty, float l, float4 o) {
   const float f = 1.f / l;
   o = empty ? make_float4(0.f, 0.f, 0.f, 0.f)
             : make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-  T* out = static_cast<T*>(p.out) + s.b * p.o_sb + (row / p.group) * p.o_sn +
-           (s.h * p.group + row % p.group) * p.o_sh + e;
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(out) = o;
   } else {
@@ -208,59 +232,87 @@ __device__ __forceinline__ void write_row(const TreeParams& p, const Segment& s,
   }
 }
 
-// Merges rows row0 .. row0 + kCount - 1 of the item's parts, in the order of the
-// tile list, and writes them out; kThreads threads call it, after the last
-// ticket of the rows has been taken. A thread's elements of a part are loaded
-// together, so that a part costs one latency.
-template <int D, int kRows, int kCount, int kThreads, typename T>
-__device__ __forceinline__ void merge_parts(const TreeParams& p, const Stretch& st,
-                                            const unsigned long long* masks, int row0, int tid) {
-  constexpr int kPieces = D / 4;
-  constexpr int kMine = kCount * kPieces / kThreads;
-  static_assert(kCount * kPieces % kThreads == 0, "the rows are shared out evenly");
-  const Segment& s = st.seg;
-  const int ctas = s.last_cta - s.first_cta + 1;
-  float m[kMine], l[kMine];
-  float4 o[kMine];
+// Merges the item's parts, in the order of the tile list, and writes its rows
+// out; kThreads threads (all of a group that `sync` joins) call it, after the
+// item's last ticket. First a thread per row finds the row's reference and sum,
+// then the outputs are added up, kDeep loads in flight per thread. `rows_m` and
+// `rows_l` hold a float per row of the block.
+template <int D, int kThreads, typename T, typename Sync>
+__device__ __forceinline__ void merge_parts(const TreeParams& p, const Segment& s,
+                                            const Sharers& by, const unsigned long long* masks,
+                                            float* rows_m, float* rows_l, int tid, Sync sync) {
+  constexpr int kPieces = D / 4, kDeep = 4;
+  const int ctas = by.count;
+  const int rows = min(p.block_rows, p.rows - s.mblock * p.block_rows);
+  for (int r = tid; r < rows; r += kThreads) {
+    float m = -INFINITY, l = 0.f;
+    for (int c0 = 0; c0 < ctas; c0 += kDeep) {
+      float m2[kDeep], l2[kDeep];
 #pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-    o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < kDeep; ++c) {
+        const bool in = c0 + c < ctas;
+        const float* x = Parts<D>::of(p, by, in ? c0 + c : 0);
+        m2[c] = in ? __ldcg(x + r) : -INFINITY;
+        l2[c] = in ? __ldcg(x + p.block_rows + r) : 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < kDeep; ++c) {
+        const float now = fmaxf(m, m2[c]), ref = now == -INFINITY ? 0.f : now;
+        l = l * fast_exp2(m - ref) + l2[c] * fast_exp2(m2[c] - ref);
+        m = now;
+      }
+    }
+    rows_m[r] = m == -INFINITY ? 0.f : m;
+    rows_l[r] = l;
+    if (p.weights) write_lse(p, s, s.mblock * p.block_rows + r, masks[r] == 0, m, l);
   }
+  sync();
+  // Parts lie a fixed distance apart but for the first.
+  const float* first = Parts<D>::of(p, by, 0);
+  const float* second = Parts<D>::of(p, by, 1);
+  const int64_t step = 2 * Parts<D>::floats(p);
+  const int body = 2 * p.block_rows;
+  for (int at0 = tid; at0 < rows * kPieces; at0 += kDeep * kThreads) {
+    float4 o[kDeep];
+    float m[kDeep];
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      m[u] = rows_m[min(at0 + u * kThreads, rows * kPieces - 1) / kPieces];
+    }
+    const float* x = first;
 #pragma unroll 2
-  for (int c = 0; c < ctas; ++c) {
-    const float* x = Parts<D, kRows>::of(p, st, c);
-    float m2[kMine], l2[kMine];
-    float4 y[kMine];
+    for (int c = 0; c < ctas; ++c) {
+      float4 y[kDeep];
+      float a[kDeep];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int at = tid + i * kThreads, r = row0 + at / kPieces, e = at % kPieces * 4;
-      m2[i] = __ldcg(x + r);
-      l2[i] = __ldcg(x + kRows + r);
-      y[i] = __ldcg(reinterpret_cast<const float4*>(x + 2 * kRows + r * D + e));
+      for (int u = 0; u < kDeep; ++u) {
+        const int at = min(at0 + u * kThreads, rows * kPieces - 1);
+        a[u] = __ldcg(x + at / kPieces);
+        y[u] = __ldcg(reinterpret_cast<const float4*>(x + body + 4 * at));
+      }
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        const float f = fast_exp2(a[u] - m[u]);
+        o[u].x = fmaf(y[u].x, f, o[u].x), o[u].y = fmaf(y[u].y, f, o[u].y);
+        o[u].z = fmaf(y[u].z, f, o[u].z), o[u].w = fmaf(y[u].w, f, o[u].w);
+      }
+      x = c == 0 ? second : x + step;
     }
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const float now = fmaxf(m[i], m2[i]), ref = now == -INFINITY ? 0.f : now;
-      const float a = fast_exp2(m[i] - ref), b = fast_exp2(m2[i] - ref);
-      m[i] = now;
-      l[i] = l[i] * a + l2[i] * b;
-      o[i].x = o[i].x * a + y[i].x * b, o[i].y = o[i].y * a + y[i].y * b;
-      o[i].z = o[i].z * a + y[i].z * b, o[i].w = o[i].w * a + y[i].w * b;
+    for (int u = 0; u < kDeep; ++u) {
+      const int at = at0 + u * kThreads, r = at / kPieces, e = at % kPieces * 4;
+      if (at >= rows * kPieces) break;
+      write_four<T>(out_row<T>(p, s, s.mblock * p.block_rows + r) + e, masks[r] == 0, rows_l[r],
+                    o[u]);
     }
-  }
-#pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    const int at = tid + i * kThreads;
-    write_row<kRows, T>(p, s, masks, row0 + at / kPieces, at % kPieces * 4, m[i], l[i], o[i]);
   }
 }
 
 // Takes a ticket of the item (one thread, once its CTA's part is in memory):
 // true for the last of the item's CTAs, which also re-arms the counter.
-__device__ __forceinline__ bool take_ticket(const Segment& s, int* counter) {
-  const bool last = atomicAdd(counter, 1) == s.last_cta - s.first_cta;
+__device__ __forceinline__ bool take_ticket(const Sharers& by, int* counter) {
+  const bool last = atomicAdd(counter, 1) == by.count - 1;
   if (last) *counter = 0;
   return last;
 }
@@ -268,18 +320,15 @@ __device__ __forceinline__ bool take_ticket(const Segment& s, int* counter) {
 // Byte offset of 16-byte piece `piece` of row `row` in a tile of `rows` rows of
 // D bf16, as a 128-byte-swizzled TMA box lays it out: columns in blocks of 64
 // elements, pieces permuted within a row's 128 bytes.
-template <int D>
 __device__ __forceinline__ int tile_at(int rows, int row, int piece) {
   return (piece >> 3) * rows * 128 + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
 }
 
 // tree_prepare.cu: the query blocks, and the nodes' keys and values in the
-// cache. `split`: q times the scale, in two bf16 parts.
-int launch_prepare(int dtype, int head_dim, int block_rows, const TreeParams& p,
-                   cudaStream_t stream);
-// tree_attention_mma.cu: bf16, blocks of 16, 32 or 64 query rows.
-int mma_ctas_per_sm(int head_dim, int block_rows);
-int launch_mma(int head_dim, int block_rows, const TreeParams& p, cudaStream_t stream);
+// cache. In bf16 a rotated q is multiplied by the scale and taken in two parts.
+int launch_prepare(int dtype, int head_dim, const TreeParams& p, cudaStream_t stream);
+// tree_attention_tc.cu: bf16.
+int launch_tc(int head_dim, const TreeParams& p, cudaStream_t stream);
 
 }  // namespace tree
 }  // namespace asrback

@@ -1,0 +1,668 @@
+// Draft-tree attention in bf16 on the 5th-generation tensor cores, sm_100a. The
+// split of the work is tree_attention.cu's.
+//
+// A block of query rows (the nodes of a row times the query heads of one
+// key/value head, up to 128) is one 128-row tcgen05 tile against the row's keys
+// in tiles of 64. The call is bound by streaming the cache, so the TMA warps run
+// ahead of everything through the CTA's whole stretch, across items. Tiles
+// alternate between two slots, each with its own scores, probabilities, output
+// accumulator and softmax state, so that one slot's softmax runs beside the
+// other's products; the two states of an item are merged when it ends, by warps
+// of their own, while the next item is under way. Roles:
+//   warp 0      TMA: a segment's query block, the tiles' keys;
+//   warp 2      TMA: the tiles' values. (Two warps, since one issues tiles more
+//               slowly than they arrive.) A full tile is one copy of 64
+//               positions x D, of the row's last one only the blocks of 16
+//               positions that hold keys;
+//   warp 1      TMEM allocation and the MMAs: S_x = Q K^T two tiles ahead of
+//               O_x (+)= P_x V. A rotated query is two bf16 parts (their sum has
+//               2^-17 of rounding), whose products are added up in S;
+//   warp 3      passes the values on; behind the cached keys: zeros behind the
+//               last node, nothing infinite or NaN;
+//   warps 4-7   softmax of slot 0, warps 8-11 of slot 1: thread = TMEM lane =
+//               query row; only the warps that hold rows run. A row's reference
+//               moves, and its O is rescaled, only when a score passes it by
+//               more than 8 (base 2);
+//   warps 12-15 an item's end: merge of the slots, output, or the part for the
+//               workspace, and the merge of the parts by the item's last CTA.
+#include <algorithm>
+#include <type_traits>
+
+#include "tcgen05.cuh"
+#include "tree_attention.cuh"
+
+namespace asrback {
+namespace {
+
+using namespace tree;
+
+constexpr int kThreads = 512;
+constexpr int kTailKeys = 16;  // positions per copy of a row's last tile
+constexpr int kMaxUnits = 16;  // tiles of keys, and of values, in their rings
+constexpr float kMoveThreshold = 8.0f;
+constexpr int kTmemCols = 512;
+constexpr int col_s(int x) { return kTile * x; }  // P over its first half
+constexpr int col_o(int x) { return 2 * kTile + 128 * x; }
+
+// What a softmax warp hands to the item's end, per slot and row.
+struct RowState {
+  float m, l;
+  unsigned long long mask;
+};
+
+// Shared memory: the query blocks, the rings of keys and of values, then the
+// rest. The tensor core reads 128 rows from a block's start whatever its rows:
+// what follows are keys, as rows of no one.
+struct Layout {
+  int slots, slot_bytes, units, unit_bytes;
+  __host__ __device__ int keys() const { return slots * slot_bytes; }
+  __host__ __device__ int values() const { return keys() + units * unit_bytes; }
+  __host__ __device__ int rest() const { return values() + units * unit_bytes; }
+};
+
+// Tensor maps of the cache: whole tiles (a box of 64 positions x D) and blocks
+// of kTailKeys positions x 64 columns.
+struct Maps {
+  CUtensorMap tile[2], tail[2];  // keys, values
+};
+
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                            int c3, int c4, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+constexpr int kOffStates = 0;                                // [slot][128] RowState
+constexpr int kOffMasks = kOffStates + 2 * 128 * 16;         // [128], the end's
+constexpr int kOffSums = kOffMasks + 128 * 8;                 // [2][128] float, the end's
+constexpr int kOffBars = kOffSums + 2 * 128 * 4;
+// full, empty per unit of keys and of values; q_full, q_empty per block; s_full,
+// p_full, o_done, state_full, state_empty per slot; o_free; v_ready per unit
+constexpr int kNumBars = 5 * kMaxUnits + 4 + 10 + 1;
+constexpr int kOffInts = kOffBars + kNumBars * 8;            // scratch[16], odd[17], last, tmem
+constexpr int kOffList = (kOffInts + (16 + kMaxUnits + 3) * 4 + 15) / 16 * 16;
+constexpr int rest_bytes(int batch) { return kOffList + list_bytes(batch); }
+constexpr int kBudget = 227 * 1024 - 1024;  // less the alignment of the base
+
+template <int D, bool kSplit, bool kWeights>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ TreeParams p,
+                   const Layout lay) {
+  using T = __nv_bfloat16;
+  constexpr int kUnitBytes = kTile * D * 2;
+  constexpr int kHalves = D / 64;  // 128-byte column blocks
+  constexpr int kParts = kSplit ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* rest = smem + lay.rest();
+  RowState* states = reinterpret_cast<RowState*>(rest + kOffStates);
+  auto* end_masks = reinterpret_cast<unsigned long long*>(rest + kOffMasks);
+  float* end_m = reinterpret_cast<float*>(rest + kOffSums);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(rest + kOffBars);  // [unit]
+  uint64_t* k_empty = k_full + kMaxUnits;
+  uint64_t* v_full = k_empty + kMaxUnits;
+  uint64_t* v_empty = v_full + kMaxUnits;
+  uint64_t* q_full = v_empty + kMaxUnits;  // [block buffer]
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* s_full = q_empty + 2;  // [slot] from here
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_done = p_full + 2;
+  uint64_t* state_full = o_done + 2;
+  uint64_t* state_empty = state_full + 2;
+  uint64_t* o_free = state_empty + 2;
+  uint64_t* v_ready = o_free + 1;  // [unit]
+  int* scratch = reinterpret_cast<int*>(rest + kOffInts);  // [16]
+  int* odd_unit = scratch + 16;  // [unit] the tile's nodes hold infinite or NaN values
+  int* odd_segment = odd_unit + kMaxUnits;
+  int* is_last = odd_segment + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(is_last + 1);
+  TileList list(rest + kOffList, p.batch);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row_warps = p.block_rows / 32;
+
+  if (threadIdx.x == 0) {
+    for (int u = 0; u < lay.units; ++u) {
+      mbar_init(&k_full[u], 1);
+      mbar_init(&k_empty[u], 1);
+      mbar_init(&v_full[u], 1);
+      mbar_init(&v_empty[u], 1);
+      mbar_init(&v_ready[u], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1 + 2 * row_warps);  // the MMA warp, the softmax warps
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], row_warps);
+      mbar_init(&o_done[s], 1);
+      mbar_init(&state_full[s], row_warps);
+      mbar_init(&state_empty[s], row_warps);
+    }
+    mbar_init(o_free, row_warps);
+    fence_barrier_init();
+  }
+  if (warp == 1) tc::tmem_alloc(tmem_slot, kTmemCols);
+  griddep_launch_dependents();
+  tc::tc_fence_before();
+  // The lengths and counts are older than the preparation kernel, which began
+  // behind them: only what that kernel writes is waited for, further down.
+  Stretch st = begin_stretch<kThreads>(p, list, scratch);  // has barriers: inits are visible
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Segment& sg = st.seg;
+  auto wait = [](uint64_t* bar, int parity) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity & 1)) != 0;
+  };
+  auto tiles_of = [](const Segment& s) {
+    return s.length + s.count > 0 ? s.tile1 - s.tile0 : 0;  // a skipped row has none
+  };
+  bool ok = true;
+  // A ring's or buffer's place and lap, counted on without divisions.
+  struct Turn {
+    int at = 0, lap = 0;
+    __device__ __forceinline__ void next(int size) {
+      if (++at == size) at = 0, ++lap;
+    }
+  };
+
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------------------- TMA
+    const int which = warp >> 1;  // keys or values
+    uint64_t* full = which ? v_full : k_full;
+    uint64_t* empty = which ? v_empty : k_empty;
+    uint8_t* ring = smem + (which ? lay.values() : lay.keys());
+    const bool leader = tc::elect_one();
+    if (leader) {
+      tc::prefetch_tensormap(&maps.tile[which]);
+      tc::prefetch_tensormap(&maps.tail[which]);
+    }
+    __syncwarp();
+    const uint64_t policy = l2_evict_first_policy();
+    bool waited = false;
+    Turn unit, block;
+    for (; ok && next_segment(p, list, st); block.next(lay.slots)) {
+      // The query block is loaded as soon as its buffer is free, and at the
+      // latest when the products could not go on without it: before the ring
+      // waits for a unit that this segment itself has filled.
+      const int slot = block.at, q_lap = block.lap;
+      bool q_due = which == 0;
+      auto load_q = [&](bool now) {
+        if (!q_due || (!now && !waited)) return;
+        if (!waited) griddep_wait();
+        waited = true;
+        if (q_lap > 0) {
+          if (!now && !__all_sync(0xffffffffu, mbar_test(&q_empty[slot], (q_lap - 1) & 1))) return;
+          ok = wait(&q_empty[slot], q_lap - 1);
+        }
+        q_due = false;
+        if (ok && leader) {
+          mbar_arrive_expect_tx(&q_full[slot], p.q_block_bytes);
+          bulk_g2s(smem + slot * lay.slot_bytes, p.q_blocks + (int64_t)sg.item * p.q_block_bytes,
+                   p.q_block_bytes, &q_full[slot], policy);
+        }
+        __syncwarp();
+      };
+      const int total = sg.length + sg.count, tiles = tiles_of(sg);
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int key = (sg.tile0 + i) * kTile, keys = min(kTile, total - key);
+        load_q(i >= lay.units);
+        // A tile with nodes in it comes after the preparation.
+        if (!waited && key + kTile > sg.length) {
+          load_q(true);
+          if (!waited) griddep_wait();
+          waited = true;
+        }
+        uint64_t* bar = &full[unit.at];
+        if (ok && unit.lap > 0) ok = wait(&empty[unit.at], unit.lap - 1);
+        if (ok && leader) {
+          uint8_t* dst = ring + unit.at * kUnitBytes;
+          if (keys == kTile) {
+            mbar_arrive_expect_tx(bar, kUnitBytes);
+            tma_load_5d(dst, &maps.tile[which], 0, key, 0, sg.h, sg.b, bar);
+          } else {
+            const int blocks = (keys + kTailKeys - 1) / kTailKeys;
+            mbar_arrive_expect_tx(bar, blocks * kTailKeys * D * 2);
+            for (int k = 0; k < blocks * kTailKeys; k += kTailKeys)
+#pragma unroll
+              for (int c = 0; c < kHalves; ++c)
+                tc::tma_load_4d(dst + c * kTile * 128 + k * 128, &maps.tail[which], 64 * c, key + k,
+                                sg.h, sg.b, bar);
+          }
+        }
+        __syncwarp();
+        if (ok) unit.next(lay.units);
+      }
+      if (ok) load_q(true);
+    }
+    // A wait gave up: the copies in flight still have to land before the CTA
+    // may end.
+    if (!ok)
+      for (int u = 0; u < lay.units; ++u) {
+        const int laps = unit.lap + (u < unit.at ? 1 : 0);
+        if (laps > 0) wait(&full[u], laps - 1);
+      }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------- MMA
+    const bool leader = tc::elect_one();
+    constexpr uint32_t kIdescQK = tc::idesc_bf16(128, kTile, false);
+    constexpr uint32_t kIdescPV = tc::idesc_bf16(128, D, true);
+    const uint64_t q_desc = tc::sw128_desc(smem_addr(smem), 16, 1024);
+    const uint64_t k_desc = tc::sw128_desc(smem_addr(smem + lay.keys()), 16, 1024);
+    const uint64_t v_desc = tc::sw128_desc(smem_addr(smem + lay.values()), kTile * 128, 1024);
+    const int half_bytes = p.block_rows * 128;
+    // S of tile gq, in list order, two tiles ahead of the P V below.
+    Stretch front = st;
+    Turn keys, block;
+    int gq = 0, front_left = 0, slot = 0;
+    auto scores = [&] {
+      while (front_left == 0) {
+        if (!next_segment(p, list, front)) return;
+        slot = block.at;
+        ok = ok && wait(&q_full[slot], block.lap);
+        block.next(lay.slots);
+        front_left = tiles_of(front.seg);
+        if (front_left == 0 && leader) mbar_arrive(&q_empty[slot]);
+      }
+      const int u = keys.at;
+      ok = ok && wait(&k_full[u], keys.lap);
+      if (!ok) return;
+      keys.next(lay.units);
+      tc::tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+#pragma unroll
+          for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc::mma_ss(tmem + col_s(gq & 1),
+                         q_desc + ((slot * lay.slot_bytes + (part * kHalves + c) * half_bytes +
+                                    32 * k) >> 4),
+                         k_desc + ((u * kUnitBytes + c * kTile * 128 + 32 * k) >> 4), kIdescQK,
+                         part > 0 || c > 0 || k > 0);
+        tc::mma_commit(&s_full[gq & 1]);
+        tc::mma_commit(&k_empty[u]);
+        if (front_left == 1) tc::mma_commit(&q_empty[slot]);
+      }
+      __syncwarp();
+      --front_left;
+      ++gq;
+    };
+    scores();
+    scores();
+    Turn values;
+    int g = 0;
+    for (int n = 0; ok && next_segment(p, list, st); ++n) {
+      const int tiles = tiles_of(sg);
+      // The segment's first products overwrite the accumulators.
+      if (n > 0) ok = wait(o_free, n - 1);
+      if (leader) *odd_segment = 0;  // its last reader has freed the accumulators
+      for (int i = 0; i < tiles && ok; ++i, ++g) {
+        const int x = g & 1, u = values.at;
+        const int key = (sg.tile0 + i) * kTile;
+        const bool edge = key + kTile > sg.length;
+        ok = wait(&p_full[x], g >> 1) && wait(&v_ready[u], values.lap);
+        if (!ok) break;
+        values.next(lay.units);
+        tc::tc_fence_after();
+        if (leader) {
+          if (edge && odd_unit[u]) {
+            *odd_segment = 1;
+            __threadfence_block();
+          }
+          const int steps = min(kTile, sg.length + sg.count - key + 15) / 16;
+          for (int k = 0; k < steps; ++k)
+            tc::mma_ts(tmem + col_o(x), tmem + col_s(x) + 8 * k,
+                       v_desc + ((u * kUnitBytes + k * 2048) >> 4), kIdescPV, i > 1 || k > 0);
+          tc::mma_commit(&o_done[x]);
+          tc::mma_commit(&v_empty[u]);
+        }
+        __syncwarp();
+        scores();
+      }
+    }
+  } else if (warp == 3) {
+    // ---------------------------------------- values behind the cached keys
+    // Zeros behind the last node, for the product with zero probabilities. A
+    // node's infinite or NaN value becomes zero too, since that product would
+    // pass it on to the nodes that do not see it: the item's end adds it where
+    // it is seen.
+    for (Turn unit; ok && next_segment(p, list, st);) {
+      const int tiles = tiles_of(sg), total = sg.length + sg.count;
+      for (int i = 0; i < tiles && ok; ++i, unit.next(lay.units)) {
+        const int key = (sg.tile0 + i) * kTile, u = unit.at;
+        ok = wait(&v_full[u], unit.lap);
+        if (!ok) break;
+        if (key + kTile <= sg.length) {
+          if (lane == 0) mbar_arrive(&v_ready[u]);
+          continue;
+        }
+        uint8_t* values = smem + lay.values() + u * kUnitBytes;
+        const int row0 = max(sg.length - key, 0), nodes_end = min(total - key, kTile);
+        const int rows_end = min((nodes_end + 15) & ~15, kTile);
+        bool odd = false;
+#pragma unroll 4
+        for (int at = row0 * (D / 8) + lane; at < rows_end * (D / 8); at += 32) {
+          uint4* to = reinterpret_cast<uint4*>(values + tile_at(kTile, at / (D / 8), at % (D / 8)));
+          const bool node = at / (D / 8) < nodes_end;
+          uint4 v = *to;
+          uint32_t* words = &v.x;
+          bool fix = !node;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool low = (words[j] & 0x7f80u) == 0x7f80u;
+            const bool high = (words[j] & 0x7f800000u) == 0x7f800000u;
+            odd |= node && (low || high);
+            fix |= low || high;
+            words[j] = node ? words[j] & (low ? 0xffff0000u : ~0u) & (high ? 0xffffu : ~0u) : 0u;
+          }
+          if (fix) *to = v;
+        }
+        odd = __any_sync(0xffffffffu, odd);
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          odd_unit[u] = odd;
+          mbar_arrive(&v_ready[u]);
+        }
+      }
+    }
+  } else if (warp >= 4 && warp < 12 && (warp & 3) < row_warps) {
+    // --------------------------------------------------------------- softmax
+    const int x = (warp >> 2) - 1, quarter = warp & 3;
+    const int r = 32 * quarter + lane;  // this thread's row of the block
+    const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
+    const uint32_t t_s = tmem + lanes + col_s(x), t_o = tmem + lanes + col_o(x);
+    Turn block;
+    int g = 0;
+    for (int n = 0; next_segment(p, list, st); ++n, block.next(lay.slots)) {
+      const int slot = block.at;
+      if (ok) ok = wait(&q_full[slot], block.lap);
+      const unsigned long long mask =
+          ok ? reinterpret_cast<const unsigned long long*>(smem + slot * lay.slot_bytes +
+                                                           p.q_block_bytes)[r - p.block_rows]
+             : 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[slot]);
+      float m = -INFINITY, l = 0.f;
+      const int total = sg.length + sg.count, g0 = g, end = g + tiles_of(sg);
+      // This slot's tiles: every second one of the CTA's.
+      for (g += (g ^ x) & 1; g < end && ok; g += 2) {
+        const int tile = sg.tile0 + g - g0;
+        ok = wait(&s_full[x], g >> 1);
+        if (!ok) break;
+        tc::tc_fence_after();
+        float s[kTile];
+        tc::tmem_ld64(t_s, s);
+        if constexpr (!kSplit) {
+#pragma unroll
+          for (int i = 0; i < kTile; ++i) s[i] *= p.scale_log2;
+        }
+        const int cached = sg.length - tile * kTile;  // columns before the nodes
+        if (cached < kTile) {
+          // Behind the cached keys lie the nodes, behind them nothing (a mask
+          // has no bits there).
+          const unsigned long long older = cached > 0 ? (1ull << cached) - 1 : 0;
+          const unsigned long long seen = older | (cached >= 0 ? mask << cached : mask >> -cached);
+#pragma unroll
+          for (int i = 0; i < kTile; ++i)
+            if ((seen >> i & 1) == 0) s[i] = -INFINITY;
+        }
+        if constexpr (kWeights) {
+          if (r < p.rows) {
+            float4* to = reinterpret_cast<float4*>(
+                p.scores + (((int64_t)sg.b * p.kv_heads + sg.h) * p.rows + r) * p.score_stride +
+                tile * kTile);
+#pragma unroll
+            for (int i = 0; i < kTile; i += 4)
+              to[i / 4] = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+          }
+        }
+        float top[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[i] = fmaxf(s[i], s[i + 4]);
+#pragma unroll
+        for (int i = 8; i < kTile; i += 8)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top[j] = fmax3(top[j], s[i + j], s[i + j + 4]);
+        const float highest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const bool moves = highest > m + kMoveThreshold;
+        if (__any_sync(0xffffffffu, moves)) {
+          const float now = moves ? highest : m;
+          if (g - g0 > 1) {
+            // The slot's O of this segment has to be at rest.
+            ok = wait(&o_done[x], (g >> 1) - 1);
+            if (!ok) break;
+            tc::tc_fence_after();
+            const float a = moves ? fast_exp2(m - now) : 1.f;
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tc::tmem_ld16(t_o + c, o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] *= a;
+              tc::tmem_st16f(t_o + c, o);
+            }
+            tc::tmem_wait_st();
+            l *= a;
+          }
+          m = now;
+        }
+        // Probabilities are rounded to bf16 for the second product (2^-8 at
+        // most, against an output in bf16 itself); their sum is not.
+        const float ref = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t packed[kTile / 2];
+#pragma unroll
+        for (int i = 0; i < kTile; i += 2) {
+          const float p0 = fast_exp2(s[i] - ref), p1 = fast_exp2(s[i + 1] - ref);
+          sum[(i >> 1) & 3] += p0 + p1;
+          packed[i / 2] = tc::bf16x2(p0, p1);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc::tmem_st32u(t_s, packed);
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+      }
+      g = end;
+      if (n > 0 && ok) ok = wait(&state_empty[x], n - 1);
+      states[128 * x + r] = RowState{m, l, mask};
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&state_full[x]);
+      if (!ok) break;
+    }
+  } else if (warp >= 12) {
+    // ---------------------------------------------------------- an item's end
+    const int quarter = warp & 3, r = 32 * quarter + lane;
+    const bool has_rows = quarter < row_warps;
+    const uint32_t t_o = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+    int g = 0;
+    for (int n = 0; next_segment(p, list, st); ++n) {
+      const int tiles = tiles_of(sg), end = g + tiles;
+      const bool whole = sg.whole();
+      const int row = sg.mblock * p.block_rows + r;
+      float* part = Parts<D>::mine(p, st);
+      if (has_rows) {
+        ok = ok && wait(&state_full[0], n) && wait(&state_full[1], n);
+        const RowState a = states[r], b = states[128 + r];
+        const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
+        const float fa = fast_exp2(a.m - ref), fb = fast_exp2(b.m - ref);
+        const float l = a.l * fa + b.l * fb;
+        end_masks[r] = a.mask;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&state_empty[0]), mbar_arrive(&state_empty[1]);
+        // Each slot's last P V of the segment; a slot without a tile has none.
+        const bool used[2] = {tiles > 1 || (tiles == 1 && (g & 1) == 0),
+                              tiles > 1 || (tiles == 1 && (g & 1) == 1)};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int last = ((end - 1) & 1) == x ? end - 1 : end - 2;
+          if (used[x] && ok) ok = wait(&o_done[x], last >> 1);
+        }
+        tc::tc_fence_after();
+        const bool odd = tiles > 0 && *odd_segment != 0;
+        const bool live = row < p.rows;
+        const float f = whole ? 1.f / l : 1.f;
+        const float f0 = fa * f, f1 = fb * f;
+        T* out = out_row<T>(p, sg, live ? row : 0);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32], o1[32];
+          tc::tmem_ld32(t_o + col_o(0) + c, o);
+          tc::tmem_ld32(t_o + col_o(1) + c, o1);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = (used[0] ? o[i] * f0 : 0.f) + (used[1] ? o1[i] * f1 : 0.f);
+          if (c == D - 32) {
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
+          }
+          if (!live) continue;
+          if (odd) {
+            // The infinite and NaN values of the nodes that the row sees, among
+            // the segment's tiles.
+            for (int i = 0; i < sg.count; ++i) {
+              const int at = sg.length + i - sg.tile0 * kTile;
+              if ((a.mask >> i & 1) == 0 || at < 0 || at >= tiles * kTile) continue;
+              const T* v = static_cast<const T*>(p.value_cache) + sg.b * p.c_sb +
+                           (int64_t)(sg.length + i) * p.c_sp + sg.h * p.c_sh + c;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float value = __bfloat162float(v[j]);
+                if (!(fabsf(value) < INFINITY)) o[j] += value;
+              }
+            }
+          }
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 w = make_uint4(0u, 0u, 0u, 0u);
+              if (a.mask != 0)
+                w = make_uint4(tc::bf16x2(o[i], o[i + 1]), tc::bf16x2(o[i + 2], o[i + 3]),
+                               tc::bf16x2(o[i + 4], o[i + 5]), tc::bf16x2(o[i + 6], o[i + 7]));
+              *reinterpret_cast<uint4*>(out + c + i) = w;
+            }
+          } else {
+            float4* to = reinterpret_cast<float4*>(part + 2 * p.block_rows + r * D + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+        if (live && whole && p.weights) write_lse(p, sg, row, a.mask == 0, m, l);
+        if (live && !whole) part[r] = m, part[p.block_rows + r] = l;
+      }
+      g = end;
+      if (!whole) {
+        __threadfence();
+        named_sync(1, 128);
+        const Sharers by(st);
+        if (threadIdx.x == 32 * 12) *is_last = take_ticket(by, p.counters + sg.item);
+        named_sync(1, 128);
+        if (*is_last && ok) {
+          __threadfence();
+          merge_parts<D, 128, T>(p, sg, by, end_masks, end_m, end_m + 128, threadIdx.x - 32 * 12,
+                                 [] { named_sync(1, 128); });
+        }
+        named_sync(1, 128);  // the masks may be overwritten
+      }
+    }
+  }
+  if (!ok && lane == 0 && p.status) atomicOr(p.status, ASRBACK_STATUS_TIMEOUT);
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// The cache as a map {64 columns, position, column block, head, row} with a box
+// of 64 positions of all column blocks, and as one {column, position, head, row}
+// with a box of 64 columns of kTailKeys positions.
+int make_maps(CUtensorMap* tile, CUtensorMap* tail, void* base, const TreeParams& p,
+              int head_dim) {
+  int rc = ASRBACK_OK;
+  auto encode = tc::tensor_map_encoder(&rc);
+  if (!encode) return rc;
+  // A dimension of one may have any stride; the encoder wants a plausible one.
+  const auto bytes = [&](int64_t stride, int64_t size) {
+    return static_cast<cuuint64_t>((size > 1 ? stride : head_dim) * 2);
+  };
+  const cuuint64_t position = bytes(p.c_sp, p.cache_length), head = bytes(p.c_sh, p.kv_heads),
+                   row = bytes(p.c_sb, p.batch);
+  const cuuint64_t length = p.cache_length, heads = p.kv_heads, rows = p.batch;
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  const auto make = [&](CUtensorMap* map, int rank, const cuuint64_t* dims,
+                        const cuuint64_t* strides, const cuuint32_t* box) {
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, base, dims, strides, box, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  const cuuint64_t blocks = head_dim / 64;
+  const cuuint64_t dims5[5] = {64, length, blocks, heads, rows};
+  const cuuint64_t strides5[4] = {position, 128, head, row};
+  const cuuint32_t box5[5] = {64, kTile, (cuuint32_t)blocks, 1, 1};
+  const cuuint64_t dims4[4] = {(cuuint64_t)head_dim, length, heads, rows};
+  const cuuint64_t strides4[3] = {position, head, row};
+  const cuuint32_t box4[4] = {64, kTailKeys, 1, 1};
+  CUresult res = make(tile, 5, dims5, strides5, box5);
+  if (res == CUDA_SUCCESS) res = make(tail, 4, dims4, strides4, box4);
+  if (res != CUDA_SUCCESS)
+    return fail(ASRBACK_ERR_ARGUMENT,
+                "cuTensorMapEncodeTiled rejected the cache (error %d): strides (%lld, %lld, %lld)",
+                (int)res, (long long)p.c_sb, (long long)p.c_sp, (long long)p.c_sh);
+  return ASRBACK_OK;
+}
+
+template <int D, bool kSplit, bool kWeights>
+int launch(const TreeParams& p, cudaStream_t stream) {
+  auto kernel = tree_tc_kernel<D, kSplit, kWeights>;
+  Maps maps;
+  if (int rc = make_maps(&maps.tile[0], &maps.tail[0], p.key_cache, p, D)) return rc;
+  if (int rc = make_maps(&maps.tile[1], &maps.tail[1], p.value_cache, p, D)) return rc;
+  static thread_local int prepared_device = -1;
+  int device = 0;
+  if (int rc = check_cuda(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+  if (prepared_device != device) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(
+                                kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024),
+                            "cudaFuncSetAttribute(tree attention)"))
+      return rc;
+    prepared_device = device;
+  }
+  // Two query blocks where they leave the ring most of the shared memory.
+  Layout lay{};
+  lay.slot_bytes = (p.q_block_bytes + 1023) / 1024 * 1024;
+  lay.slots = lay.slot_bytes <= 40 * 1024 ? 2 : 1;
+  lay.unit_bytes = kTile * D * 2;
+  lay.units = std::min((kBudget - rest_bytes(p.batch) - lay.keys()) / lay.unit_bytes / 2, kMaxUnits);
+  return launch_pdl(kernel, dim3(p.ctas), dim3(kThreads), 1024 + lay.rest() + rest_bytes(p.batch),
+                    stream, "tree attention launch", maps, p, lay);
+}
+
+}  // namespace
+
+namespace tree {
+
+int launch_tc(int head_dim, const TreeParams& p, cudaStream_t stream) {
+  auto pick = [&](auto dim, auto split) {
+    constexpr int D = decltype(dim)::value;
+    constexpr bool kSplit = decltype(split)::value;
+    return p.weights ? launch<D, kSplit, true>(p, stream) : launch<D, kSplit, false>(p, stream);
+  };
+  using std::integral_constant;
+  if (head_dim == 64)
+    return p.q_norm ? pick(integral_constant<int, 64>{}, std::true_type{})
+                    : pick(integral_constant<int, 64>{}, std::false_type{});
+  return p.q_norm ? pick(integral_constant<int, 128>{}, std::true_type{})
+                  : pick(integral_constant<int, 128>{}, std::false_type{});
+}
+
+}  // namespace tree
+}  // namespace asrback

@@ -107,12 +107,13 @@ __device__ __forceinline__ void norm_rotate(float eps, const RowSlice<D, T>& w,
 // bf16 parts, so that rounding it costs the scores 2^-17 and not 2^-9.
 template <int D, typename T, bool kSplit>
 __global__ void __launch_bounds__(kThreads)
-    tree_prepare_kernel(const __grid_constant__ TreeParams p, const int block_rows) {
+    tree_prepare_kernel(const __grid_constant__ TreeParams p) {
   using Slice = RowSlice<D, T>;
   griddep_wait();
   griddep_launch_dependents();
   const int b = blockIdx.y, c = threadIdx.x % Slice::kLanes;
   const int task = blockIdx.x * (kThreads / Slice::kLanes) + threadIdx.x / Slice::kLanes;
+  const int block_rows = p.block_rows;
   const int q_rows = p.kv_heads * p.mblocks * block_rows;
   const RowSpan span = row_span(p, b);
   if (span.bad && blockIdx.x == 0 && threadIdx.x == 0 && p.status)
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kThreads)
                                                           a1 - __uint_as_float(hi[j] & 0xffff0000u));
         lo[j] = *reinterpret_cast<const uint32_t*>(&rest);
       }
-      uint8_t* to = out + tile_at<D>(block_rows, r, e / 8);
+      uint8_t* to = out + tile_at(block_rows, r, e / 8);
       *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       if constexpr (kSplit)
         *reinterpret_cast<uint4*>(to + block_rows * D * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -205,29 +206,28 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 template <int D, typename T, bool kSplit>
-int launch(int block_rows, const TreeParams& p, cudaStream_t stream) {
+int launch(const TreeParams& p, cudaStream_t stream) {
   constexpr int kPerCta = kThreads / RowSlice<D, T>::kLanes;
-  const int tasks = p.kv_heads * (p.mblocks * block_rows + p.nodes);
+  const int tasks = p.kv_heads * (p.mblocks * p.block_rows + p.nodes);
   return launch_pdl(tree_prepare_kernel<D, T, kSplit>,
                     dim3((tasks + kPerCta - 1) / kPerCta, p.batch), dim3(kThreads), 0, stream,
-                    "tree preparation launch", p, block_rows);
+                    "tree preparation launch", p);
 }
 
 }  // namespace
 
 namespace tree {
 
-int launch_prepare(int dtype, int head_dim, int block_rows, const TreeParams& p,
-                   cudaStream_t stream) {
+int launch_prepare(int dtype, int head_dim, const TreeParams& p, cudaStream_t stream) {
   using bf16 = __nv_bfloat16;
   if (dtype == ASRBACK_F32)
-    return head_dim == 64 ? launch<64, float, false>(block_rows, p, stream)
-                          : launch<128, float, false>(block_rows, p, stream);
+    return head_dim == 64 ? launch<64, float, false>(p, stream)
+                          : launch<128, float, false>(p, stream);
   if (p.q_norm)
-    return head_dim == 64 ? launch<64, bf16, true>(block_rows, p, stream)
-                          : launch<128, bf16, true>(block_rows, p, stream);
-  return head_dim == 64 ? launch<64, bf16, false>(block_rows, p, stream)
-                        : launch<128, bf16, false>(block_rows, p, stream);
+    return head_dim == 64 ? launch<64, bf16, true>(p, stream)
+                          : launch<128, bf16, true>(p, stream);
+  return head_dim == 64 ? launch<64, bf16, false>(p, stream)
+                        : launch<128, bf16, false>(p, stream);
 }
 
 }  // namespace tree
