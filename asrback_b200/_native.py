@@ -141,7 +141,6 @@ SIGNATURES: dict[str, tuple[list, object]] = {
         [_c_int, _c_int, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
         _c_int,
     ),
-    "asrback_tree_counter_bytes": ([_c_int] * 5, _c_size),
     "asrback_tree_workspace_bytes": ([_c_int] * 9, _c_size),
     "asrback_tree_attention": (
         [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
@@ -156,8 +155,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
          _c_i64, _c_i64, _c_i64,
          _c_p, _c_i64, _c_i64, _c_i64,
          _c_p, _c_i64, _c_i64,
-         _c_f, _c_p, _c_size, _c_p, _c_size,
-         _c_p, _c_p],
+         _c_f, _c_p, _c_size, _c_p, _c_p],
         _c_int,
     ),
     "asrback_accept_tree": (
@@ -189,7 +187,6 @@ SIGNATURES: dict[str, tuple[list, object]] = {
          _c_p, _c_p, _c_p, _c_p],
         _c_int,
     ),
-    "asrback_stream_capture_id": ([_c_p], ctypes.c_uint64),
     "asrback_selftest_bounded_wait": ([_c_i64, _c_p, _c_p], _c_int),
 }
 

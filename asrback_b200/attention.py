@@ -502,25 +502,6 @@ class DraftTree(NamedTuple):
     depths: Tensor
 
 
-# Zeroed counters of the tree kernels, one buffer per stream, and one more per
-# graph capture on it: calls that may run at the same time never share them.
-# The kernels leave them at zero. A capture's buffer is zeroed by the graph
-# itself, on every replay.
-_counters: dict[tuple[int, int, bool], tuple[int, Tensor]] = {}
-_MIN_COUNTER_BYTES = 1 << 16
-
-
-def _counters_for(device: torch.device, stream: int, nbytes: int) -> Tensor:
-    capture = _native.load().asrback_stream_capture_id(stream)
-    key = (device.index, stream, capture != 0)
-    held = _counters.get(key)
-    if held is None or held[0] != capture or held[1].numel() < nbytes:
-        size = max(nbytes, _MIN_COUNTER_BYTES)
-        held = (capture, torch.zeros(size, dtype=torch.uint8, device=device))
-        _counters[key] = held
-    return held[1]
-
-
 def _on(device: torch.device):
     """A context in which ``device`` is the current one."""
     return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
@@ -614,12 +595,10 @@ def _tree_call(q: Tensor, k: Tensor, v: Tensor, rotary: tuple | None, tree: Draf
     with _on(device):
         stream = _stream(device)
         out = torch.empty((batch, nodes, heads * head_dim), dtype=q.dtype, device=device)
-        counter_bytes = lib.asrback_tree_counter_bytes(dtype, batch, nodes, heads, kv_heads)
         ws_bytes = lib.asrback_tree_workspace_bytes(dtype, batch, nodes, heads, kv_heads, head_dim,
                                                     length, 0 if rotary is None else 1,
                                                     0 if weights is None else 1)
         status = _state(device).status
-        counters = _counters_for(device, stream, counter_bytes)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
         _native.call(
             "asrback_tree_attention",
@@ -633,8 +612,7 @@ def _tree_call(q: Tensor, k: Tensor, v: Tensor, rotary: tuple | None, tree: Draf
             out.data_ptr(), nodes * heads * head_dim, heads * head_dim, head_dim,
             w_ptr, w_batch, w_head,
             scale if scale is not None else 1.0 / math.sqrt(head_dim),
-            counters.data_ptr(), counters.numel(), workspace.data_ptr(), ws_bytes,
-            status.data_ptr(), stream,
+            workspace.data_ptr(), ws_bytes, status.data_ptr(), stream,
         )
     return out
 

@@ -79,15 +79,6 @@ int asrback_selftest_bounded_wait(int64_t budget_ns, int32_t* status, void* stre
 
 int asrback_abi_version(void) { return (1 << 16) | 4; }
 
-uint64_t asrback_stream_capture_id(void* stream) {
-  cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
-  unsigned long long id = 0;
-  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &state, &id) != cudaSuccess ||
-      state != cudaStreamCaptureStatusActive)
-    return 0;
-  return id;
-}
-
 const char* asrback_last_error(void) { return asrback::g_last_error; }
 
 int asrback_device_sm_count(void) { return asrback::sm_count(); }

@@ -19,14 +19,13 @@
 // block of query rows); each CTA takes an equal stretch of that list, whatever
 // the rows' lengths, so all CTAs stream the same number of bytes. A stretch
 // that covers only part of an item leaves its unnormalised result (m, l, o) in
-// the workspace; the last CTA of the item to finish (an atomic ticket that it
-// re-arms) merges the parts in list order, so results do not depend on which
-// CTA was last.
+// the workspace. Three launches: tree_prepare.cu writes the nodes' keys and
+// values to the cache and the prepared query rows to the workspace (the nodes
+// then are an item's last keys, masked by the rows' ancestors), the attention
+// (tree_attention_tc.cu in bf16, below in float32), and tree_finish.cu, which
+// merges the parts in list order. Each launch begins while the one before it
+// ends; no CTA waits for another, and results do not depend on their order.
 //
-// A first, small kernel (tree_prepare.cu) writes the nodes' keys and values to
-// the cache and the prepared query rows to the workspace; the nodes then are an
-// item's last keys, masked by the rows' ancestors. Every CTA of the attention
-// works on its own: none waits for another.
 #include "../../include/asrback_attn.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -58,8 +57,8 @@ struct SimtShape {
   static constexpr int kOffState = kOffS + kRows * kTile * 4;  // m, l, alpha
   static constexpr int kOffO = kOffState + 3 * kRows * 4;
   static constexpr int kOffMasks = kOffO + kRows * D * 4;
-  static constexpr int kOffScratch = kOffMasks + kRows * 8;  // a flag, then begin_stretch's
-  static constexpr int kOffList = kOffScratch + 32;
+  static constexpr int kOffScratch = kOffMasks + kRows * 8;
+  static constexpr int kOffList = kOffScratch + 16;
   static constexpr int bytes(int batch) { return kOffList + list_bytes(batch); }
 };
 
@@ -86,7 +85,7 @@ __global__ void __launch_bounds__(kThreads)
 
   griddep_wait();
   griddep_launch_dependents();
-  Stretch st = begin_stretch<kThreads>(p, list, scratch + 4);
+  Stretch st = begin_stretch<kThreads>(p, list, scratch);
   while (next_segment(p, list, st)) {
     const Segment& sg = st.seg;
     const uint8_t* block = p.q_blocks + (int64_t)sg.item * p.q_block_bytes;
@@ -187,56 +186,18 @@ __global__ void __launch_bounds__(kThreads)
       for (int i = tid; i < kRows * kPieces; i += kThreads) {
         const int r = i / kPieces, e = i % kPieces * 4, row = sg.mblock * kRows + r;
         if (row >= p.rows) break;
-        const bool empty = masks[r] == 0;
-        write_four<float>(out_row<float>(p, sg, row) + e, empty, state_l[r],
+        write_four<float>(out_row<float>(p, sg.b, sg.h, row) + e, masks[r] == 0, state_l[r],
                           *reinterpret_cast<const float4*>(os + r * D + e));
-        if (p.weights && e == 0) write_lse(p, sg, row, empty, state_m[r], state_l[r]);
+        if (p.weights && e == 0) write_lse(p, sg, row, state_m[r], state_l[r]);
       }
     } else {
       float* part = Parts<D>::mine(p, st);
       for (int i = tid; i < kRows * kPieces; i += kThreads)
         reinterpret_cast<float4*>(part + 2 * kRows)[i] = reinterpret_cast<const float4*>(os)[i];
       if (tid < kRows) part[tid] = state_m[tid], part[kRows + tid] = state_l[tid];
-      __threadfence();
-      __syncthreads();
-      const Sharers by(st);
-      if (tid == 0) scratch[0] = take_ticket(by, p.counters + sg.item);
-      __syncthreads();
-      if (scratch[0]) {
-        __threadfence();
-        merge_parts<D, kThreads, float>(p, sg, by, masks, state_m, state_l, tid, [] { __syncthreads(); });
-      }
     }
     __syncthreads();
   }
-}
-
-// ---------------------------------------------------- the accumulated weights
-//
-// The attention kernel leaves its scaled scores (base-2) of at most 16 query
-// rows per key/value head and each row's log-sum-exp: this one turns a key's
-// scores into weights and adds them up, in row order. It moves 4 bytes per row
-// and key against the 4 D of the key and value.
-constexpr int kWeightThreads = 256;
-__global__ void __launch_bounds__(kWeightThreads)
-    tree_weights_kernel(const __grid_constant__ TreeParams p) {
-  __shared__ float lse[kMaxWeightRows];
-  griddep_wait();
-  griddep_launch_dependents();
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int64_t unit = (int64_t)b * p.kv_heads + h;
-  const RowSpan span = row_span(p, b);
-  const int n = span.length + span.count;
-  const int j0 = (blockIdx.x * kWeightThreads + threadIdx.x);
-  if (threadIdx.x < p.rows) lse[threadIdx.x] = p.lse[unit * p.rows + threadIdx.x];
-  __syncthreads();
-  if (span.count == 0 || j0 >= n) return;
-  float sum = 0.f;
-  for (int r = 0; r < p.rows; ++r)
-    if (lse[r] != INFINITY)  // an empty row has no weights
-      sum += fast_exp2(p.scores[(unit * p.rows + r) * p.score_stride + j0] - lse[r]);
-  float* w = p.weights + b * p.w_sb + h * p.w_sh + j0;
-  *w = j0 < span.length ? *w + sum : sum;
 }
 
 // ------------------------------------------------------------------ host side
@@ -266,7 +227,7 @@ int min_tiles(int dtype) { return dtype == ASRBACK_F32 ? 1 : 4; }
 struct Plan {
   int block_rows, mblocks, ctas;
   int q_block_bytes;
-  size_t counter_bytes, q_bytes, part_bytes, lse_bytes, score_bytes;
+  size_t q_bytes, part_bytes, lse_bytes, score_bytes;
   int64_t score_stride;
   size_t workspace() const { return q_bytes + part_bytes + lse_bytes + score_bytes; }
 };
@@ -284,7 +245,6 @@ Plan plan_for(int dtype, int batch, int nodes, int heads, int kv_heads, int head
   // As many CTAs as are resident at once.
   const int per_sm = dtype == ASRBACK_BF16 ? 1 : head_dim == 128 ? 2 : 3;
   plan.ctas = static_cast<int>(std::min<int64_t>(tiles, (int64_t)per_sm * sm_count()));
-  plan.counter_bytes = up16(items * sizeof(int));
   // float32, bf16 as it comes, or (rotary) two bf16 parts; then the masks.
   const int row_bytes = head_dim * (dtype == ASRBACK_F32 || rotary ? 4 : 2) + 8;
   plan.q_block_bytes = plan.block_rows * row_bytes;
@@ -303,12 +263,6 @@ Plan plan_for(int dtype, int batch, int nodes, int heads, int kv_heads, int head
 
 using namespace asrback;
 using namespace asrback::tree;
-
-extern "C" size_t asrback_tree_counter_bytes(int dtype, int batch, int nodes, int heads,
-                                             int kv_heads) {
-  if (batch < 1 || nodes < 1 || kv_heads < 1 || heads < kv_heads) return 0;
-  return plan_for(dtype, batch, nodes, heads, kv_heads, 64, 1, false, false).counter_bytes;
-}
 
 extern "C" size_t asrback_tree_workspace_bytes(int dtype, int batch, int nodes, int heads,
                                                int kv_heads, int head_dim, int cache_length,
@@ -332,8 +286,7 @@ extern "C" int asrback_tree_attention(
     void* key_cache, void* value_cache, int64_t c_stride_batch, int64_t c_stride_position,
     int64_t c_stride_head, void* out, int64_t o_stride_batch, int64_t o_stride_node,
     int64_t o_stride_head, float* weights, int64_t w_stride_batch, int64_t w_stride_head,
-    float scale, void* counters, size_t counter_bytes, void* workspace, size_t workspace_bytes,
-    int32_t* status, void* stream) {
+    float scale, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   if (dtype != ASRBACK_BF16 && dtype != ASRBACK_F32)
     return fail(ASRBACK_ERR_ARGUMENT, "dtype must be ASRBACK_BF16 or ASRBACK_F32, got %d", dtype);
   if (head_dim != 64 && head_dim != 128)
@@ -383,22 +336,18 @@ extern "C" int asrback_tree_attention(
                 "weights take at most %d query rows per key/value head (nodes x heads / kv_heads), "
                 "got %d",
                 kMaxWeightRows, rows);
-  if (weights && kv_heads > 65535)
-    return fail(ASRBACK_ERR_ARGUMENT, "weights take at most 65535 key/value heads");
   const Plan plan = plan_for(dtype, batch, nodes, heads, kv_heads, head_dim, cache_length, rotary,
                              weights != nullptr);
   if ((int64_t)batch * kv_heads * plan.mblocks * ((cache_length + kTile - 1) / kTile) >
-      (int64_t)1 << 30)
-    return fail(ASRBACK_ERR_ARGUMENT, "too many key tiles for one call");
+          (int64_t)1 << 30 ||
+      kv_heads * plan.mblocks > 65535)
+    return fail(ASRBACK_ERR_ARGUMENT, "too many key tiles or heads for one call");
   const size_t need = plan.workspace();
-  if (!counters || counter_bytes < plan.counter_bytes)
-    return fail(ASRBACK_ERR_WORKSPACE, "counters of %zu bytes, %zu needed",
-                counters ? counter_bytes : (size_t)0, plan.counter_bytes);
   if (!workspace || workspace_bytes < need)
     return fail(ASRBACK_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed",
                 workspace ? workspace_bytes : (size_t)0, need);
-  if (!aligned16(workspace) || !aligned16(counters))
-    return fail(ASRBACK_ERR_ARGUMENT, "counters and workspace must be 16-byte aligned");
+  if (!aligned16(workspace))
+    return fail(ASRBACK_ERR_ARGUMENT, "workspace must be 16-byte aligned");
 
   TreeParams p{};
   p.q = query, p.q_sb = q_stride_batch, p.q_sn = q_stride_node, p.q_sh = q_stride_head;
@@ -418,7 +367,6 @@ extern "C" int asrback_tree_attention(
   p.block_rows = plan.block_rows, p.mblocks = plan.mblocks;
   p.ctas = plan.ctas, p.min_tiles = min_tiles(dtype);
   uint8_t* at = static_cast<uint8_t*>(workspace);
-  p.counters = static_cast<int*>(counters);
   p.q_blocks = at;
   p.q_block_bytes = plan.q_block_bytes;
   at += plan.q_bytes;
@@ -437,10 +385,6 @@ extern "C" int asrback_tree_attention(
     rc = launch_tc(head_dim, p, s);
   else
     rc = head_dim == 64 ? launch_simt<64>(p, s) : launch_simt<128>(p, s);
-  if (rc) return rc;
-  if (weights) {
-    const dim3 grid((cache_length + kWeightThreads - 1) / kWeightThreads, kv_heads, batch);
-    rc = launch_pdl(tree_weights_kernel, grid, dim3(kWeightThreads), 0, s, "tree weights launch", p);
-  }
+  if (!rc) rc = launch_finish(dtype, head_dim, p, s);
   return rc ? rc : ok();
 }

@@ -1,6 +1,5 @@
 // What the draft-tree attention kernels share: the call's parameters, the
-// stretch of the tile list that a CTA works through, and the end of a segment
-// (output, or part and merge).
+// stretch of the tile list that a CTA works through, and where results go.
 #pragma once
 
 #include "common.cuh"
@@ -37,9 +36,8 @@ struct TreeParams {
   // the products read it, in two parts if rotated), then the rows' masks.
   uint8_t* q_blocks;
   int q_block_bytes;
-  int* counters;  // one per item, zero between calls
   float* parts;   // two per CTA: [block rows] m, l, [block rows][D] o
-  float* lse;     // with weights: (batch, kv_heads, rows), base 2, +inf for an empty row
+  float* lse;     // with weights: (batch, kv_heads, rows), base 2, of items in one part
   float* scores;  // with weights: (batch, kv_heads, rows, score_stride), base 2
   int64_t score_stride;
   int32_t* status;
@@ -93,6 +91,21 @@ struct Stretch {
   Segment seg;
 };
 
+// The CTAs that hold parts of an item of `tiles` tiles from `start` on in the list.
+struct Sharers {
+  int first, count;
+  bool begins;  // the item begins the first one's stretch
+  __device__ __forceinline__ Sharers(int start, int tiles, int per) {
+    first = start / per;
+    count = (start + tiles - 1) / per - first + 1;
+    begins = start == first * per;
+  }
+};
+
+__device__ __forceinline__ int stretch_tiles(const TreeParams& p, int total) {
+  return max((total + p.ctas - 1) / p.ctas, p.min_tiles);
+}
+
 // Fills the tile list and finds the CTA's stretch. All kThreads threads of the
 // CTA call it; `scratch` holds kThreads / 32 ints.
 template <int kThreads>
@@ -128,7 +141,7 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, const Tile
   }
   Stretch st;
   const int total = carry;
-  st.per = max((total + p.ctas - 1) / p.ctas, p.min_tiles);
+  st.per = stretch_tiles(p, total);
   st.lo = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * st.per, (int64_t)total));
   st.hi = min(st.lo + st.per, total);
   st.cur = st.lo;
@@ -174,18 +187,6 @@ __device__ __forceinline__ bool next_segment(const TreeParams& p, const TileList
   return true;
 }
 
-// The CTAs that hold parts of the segment's item.
-struct Sharers {
-  int first, count;
-  bool begins;  // the item begins the first one's stretch
-  __device__ __forceinline__ Sharers(const Stretch& st) {
-    const int start = st.seg.begin - st.seg.tile0;
-    first = start / st.per;
-    count = (start + st.seg.tiles - 1) / st.per - first + 1;
-    begins = start == first * st.per;
-  }
-};
-
 __device__ __forceinline__ float* score_row(const TreeParams& p, const Segment& s, int r) {
   return p.scores + (((int64_t)s.b * p.kv_heads + s.h) * p.rows + r) * p.score_stride;
 }
@@ -209,13 +210,13 @@ struct Parts {
 
 // An output row's elements from `e` on, and its log-sum-exp (with weights).
 template <typename T>
-__device__ __forceinline__ T* out_row(const TreeParams& p, const Segment& s, int row) {
-  return static_cast<T*>(p.out) + s.b * p.o_sb + (row / p.group) * p.o_sn +
-         (s.h * p.group + row % p.group) * p.o_sh;
+__device__ __forceinline__ T* out_row(const TreeParams& p, int b, int h, int row) {
+  return static_cast<T*>(p.out) + b * p.o_sb + (row / p.group) * p.o_sn +
+         (h * p.group + row % p.group) * p.o_sh;
 }
-__device__ __forceinline__ void write_lse(const TreeParams& p, const Segment& s, int row,
-                                          bool empty, float m, float l) {
-  p.lse[((int64_t)s.b * p.kv_heads + s.h) * p.rows + row] = empty ? INFINITY : m + log2f(l);
+__device__ __forceinline__ void write_lse(const TreeParams& p, const Segment& s, int row, float m,
+                                          float l) {
+  p.lse[((int64_t)s.b * p.kv_heads + s.h) * p.rows + row] = m + log2f(l);
 }
 
 // Four elements of a row from its unnormalised sum; zeros for an empty row.
@@ -232,91 +233,6 @@ __device__ __forceinline__ void write_four(T* out, bool empty, float l, float4 o
   }
 }
 
-// Merges the item's parts, in the order of the tile list, and writes its rows
-// out; kThreads threads (all of a group that `sync` joins) call it, after the
-// item's last ticket. First a thread per row finds the row's reference and sum,
-// then the outputs are added up, kDeep loads in flight per thread. `rows_m` and
-// `rows_l` hold a float per row of the block.
-template <int D, int kThreads, typename T, typename Sync>
-__device__ __forceinline__ void merge_parts(const TreeParams& p, const Segment& s,
-                                            const Sharers& by, const unsigned long long* masks,
-                                            float* rows_m, float* rows_l, int tid, Sync sync) {
-  constexpr int kPieces = D / 4, kDeep = 4;
-  const int ctas = by.count;
-  const int rows = min(p.block_rows, p.rows - s.mblock * p.block_rows);
-  for (int r = tid; r < rows; r += kThreads) {
-    float m = -INFINITY, l = 0.f;
-    for (int c0 = 0; c0 < ctas; c0 += kDeep) {
-      float m2[kDeep], l2[kDeep];
-#pragma unroll
-      for (int c = 0; c < kDeep; ++c) {
-        const bool in = c0 + c < ctas;
-        const float* x = Parts<D>::of(p, by, in ? c0 + c : 0);
-        m2[c] = in ? __ldcg(x + r) : -INFINITY;
-        l2[c] = in ? __ldcg(x + p.block_rows + r) : 0.f;
-      }
-#pragma unroll
-      for (int c = 0; c < kDeep; ++c) {
-        const float now = fmaxf(m, m2[c]), ref = now == -INFINITY ? 0.f : now;
-        l = l * fast_exp2(m - ref) + l2[c] * fast_exp2(m2[c] - ref);
-        m = now;
-      }
-    }
-    rows_m[r] = m == -INFINITY ? 0.f : m;
-    rows_l[r] = l;
-    if (p.weights) write_lse(p, s, s.mblock * p.block_rows + r, masks[r] == 0, m, l);
-  }
-  sync();
-  // Parts lie a fixed distance apart but for the first.
-  const float* first = Parts<D>::of(p, by, 0);
-  const float* second = Parts<D>::of(p, by, 1);
-  const int64_t step = 2 * Parts<D>::floats(p);
-  const int body = 2 * p.block_rows;
-  for (int at0 = tid; at0 < rows * kPieces; at0 += kDeep * kThreads) {
-    float4 o[kDeep];
-    float m[kDeep];
-#pragma unroll
-    for (int u = 0; u < kDeep; ++u) {
-      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      m[u] = rows_m[min(at0 + u * kThreads, rows * kPieces - 1) / kPieces];
-    }
-    const float* x = first;
-#pragma unroll 2
-    for (int c = 0; c < ctas; ++c) {
-      float4 y[kDeep];
-      float a[kDeep];
-#pragma unroll
-      for (int u = 0; u < kDeep; ++u) {
-        const int at = min(at0 + u * kThreads, rows * kPieces - 1);
-        a[u] = __ldcg(x + at / kPieces);
-        y[u] = __ldcg(reinterpret_cast<const float4*>(x + body + 4 * at));
-      }
-#pragma unroll
-      for (int u = 0; u < kDeep; ++u) {
-        const float f = fast_exp2(a[u] - m[u]);
-        o[u].x = fmaf(y[u].x, f, o[u].x), o[u].y = fmaf(y[u].y, f, o[u].y);
-        o[u].z = fmaf(y[u].z, f, o[u].z), o[u].w = fmaf(y[u].w, f, o[u].w);
-      }
-      x = c == 0 ? second : x + step;
-    }
-#pragma unroll
-    for (int u = 0; u < kDeep; ++u) {
-      const int at = at0 + u * kThreads, r = at / kPieces, e = at % kPieces * 4;
-      if (at >= rows * kPieces) break;
-      write_four<T>(out_row<T>(p, s, s.mblock * p.block_rows + r) + e, masks[r] == 0, rows_l[r],
-                    o[u]);
-    }
-  }
-}
-
-// Takes a ticket of the item (one thread, once its CTA's part is in memory):
-// true for the last of the item's CTAs, which also re-arms the counter.
-__device__ __forceinline__ bool take_ticket(const Sharers& by, int* counter) {
-  const bool last = atomicAdd(counter, 1) == by.count - 1;
-  if (last) *counter = 0;
-  return last;
-}
-
 // Byte offset of 16-byte piece `piece` of row `row` in a tile of `rows` rows of
 // D bf16, as a 128-byte-swizzled TMA box lays it out: columns in blocks of 64
 // elements, pieces permuted within a row's 128 bytes.
@@ -327,6 +243,8 @@ __device__ __forceinline__ int tile_at(int rows, int row, int piece) {
 // tree_prepare.cu: the query blocks, and the nodes' keys and values in the
 // cache. In bf16 a rotated q is multiplied by the scale and taken in two parts.
 int launch_prepare(int dtype, int head_dim, const TreeParams& p, cudaStream_t stream);
+// tree_finish.cu: the merge of split items, the accumulated weights.
+int launch_finish(int dtype, int head_dim, const TreeParams& p, cudaStream_t stream);
 // tree_attention_tc.cu: bf16.
 int launch_tc(int head_dim, const TreeParams& p, cudaStream_t stream);
 

@@ -14,17 +14,18 @@
 //               slowly than they arrive.) A full tile is one copy of 64
 //               positions x D, of the row's last one only the blocks of 16
 //               positions that hold keys;
-//   warp 1      TMEM allocation and the MMAs: S_x = Q K^T two tiles ahead of
-//               O_x (+)= P_x V. A rotated query is two bf16 parts (their sum has
-//               2^-17 of rounding), whose products are added up in S;
-//   warp 3      passes the values on; behind the cached keys: zeros behind the
-//               last node, nothing infinite or NaN;
+//   warp 1      TMEM allocation, S_x = Q K^T. A rotated query is two bf16 parts
+//               (their sum has 2^-17 of rounding), whose products are added up
+//               in S;
+//   warp 3      O_x (+)= P_x V, and of the values behind the cached keys: zeros
+//               behind the last node, nothing infinite or NaN. (Two warps issue
+//               MMAs, since the waits and descriptors of a tile take one of them
+//               longer than the tile's share of the stream.)
 //   warps 4-7   softmax of slot 0, warps 8-11 of slot 1: thread = TMEM lane =
 //               query row; only the warps that hold rows run. A row's reference
 //               moves, and its O is rescaled, only when a score passes it by
 //               more than 8 (base 2);
-//   warps 12-15 an item's end: merge of the slots, output, or the part for the
-//               workspace, and the merge of the parts by the item's last CTA.
+//   warps 12-15 an item's end: merge of the slots, output or part.
 #include <algorithm>
 #include <type_traits>
 
@@ -76,14 +77,12 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 constexpr int kOffStates = 0;                                // [slot][128] RowState
-constexpr int kOffMasks = kOffStates + 2 * 128 * 16;         // [128], the end's
-constexpr int kOffSums = kOffMasks + 128 * 8;                 // [2][128] float, the end's
-constexpr int kOffBars = kOffSums + 2 * 128 * 4;
+constexpr int kOffBars = kOffStates + 2 * 128 * 16;
 // full, empty per unit of keys and of values; q_full, q_empty per block; s_full,
-// p_full, o_done, state_full, state_empty per slot; o_free; v_ready per unit
-constexpr int kNumBars = 5 * kMaxUnits + 4 + 10 + 1;
-constexpr int kOffInts = kOffBars + kNumBars * 8;            // scratch[16], odd[17], last, tmem
-constexpr int kOffList = (kOffInts + (16 + kMaxUnits + 3) * 4 + 15) / 16 * 16;
+// p_full, o_done, state_full, state_empty per slot; o_free
+constexpr int kNumBars = 4 * kMaxUnits + 4 + 10 + 1;
+constexpr int kOffInts = kOffBars + kNumBars * 8;            // scratch[16], odd_segment, tmem
+constexpr int kOffList = (kOffInts + 20 * 4 + 15) / 16 * 16;
 constexpr int rest_bytes(int batch) { return kOffList + list_bytes(batch); }
 constexpr int kBudget = 227 * 1024 - 1024;  // less the alignment of the base
 
@@ -100,8 +99,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* rest = smem + lay.rest();
   RowState* states = reinterpret_cast<RowState*>(rest + kOffStates);
-  auto* end_masks = reinterpret_cast<unsigned long long*>(rest + kOffMasks);
-  float* end_m = reinterpret_cast<float*>(rest + kOffSums);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(rest + kOffBars);  // [unit]
   uint64_t* k_empty = k_full + kMaxUnits;
   uint64_t* v_full = k_empty + kMaxUnits;
@@ -114,12 +111,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* state_full = o_done + 2;
   uint64_t* state_empty = state_full + 2;
   uint64_t* o_free = state_empty + 2;
-  uint64_t* v_ready = o_free + 1;  // [unit]
   int* scratch = reinterpret_cast<int*>(rest + kOffInts);  // [16]
-  int* odd_unit = scratch + 16;  // [unit] the tile's nodes hold infinite or NaN values
-  int* odd_segment = odd_unit + kMaxUnits;
-  int* is_last = odd_segment + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(is_last + 1);
+  int* odd_segment = scratch + 16;  // the segment's nodes hold infinite or NaN values
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(odd_segment + 1);
   TileList list(rest + kOffList, p.batch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row_warps = p.block_rows / 32;
@@ -130,7 +124,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&k_empty[u], 1);
       mbar_init(&v_full[u], 1);
       mbar_init(&v_empty[u], 1);
-      mbar_init(&v_ready[u], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
@@ -160,6 +153,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     return s.length + s.count > 0 ? s.tile1 - s.tile0 : 0;  // a skipped row has none
   };
   bool ok = true;
+  // The same in every lane, and known to be: descriptors built from it are kept in
+  // uniform registers, which the issue of an MMA reads.
+  auto uniform = [](uint32_t x) { return __reduce_max_sync(0xffffffffu, x); };
   // A ring's or buffer's place and lap, counted on without divisions.
   struct Turn {
     int at = 0, lap = 0;
@@ -245,130 +241,112 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (laps > 0) wait(&full[u], laps - 1);
       }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------- MMA
+    // ------------------------------------------------------------ S = Q K^T
     const bool leader = tc::elect_one();
-    constexpr uint32_t kIdescQK = tc::idesc_bf16(128, kTile, false);
-    constexpr uint32_t kIdescPV = tc::idesc_bf16(128, D, true);
+    constexpr uint32_t kIdesc = tc::idesc_bf16(128, kTile, false);
     const uint64_t q_desc = tc::sw128_desc(smem_addr(smem), 16, 1024);
     const uint64_t k_desc = tc::sw128_desc(smem_addr(smem + lay.keys()), 16, 1024);
+    const uint32_t half_step = p.block_rows * 128 >> 4;
+    Turn unit, block;
+    int g = 0;
+    for (; ok && next_segment(p, list, st); block.next(lay.slots)) {
+      const int tiles = tiles_of(sg), slot = block.at;
+      ok = wait(&q_full[slot], block.lap);
+      if (tiles == 0 && leader) mbar_arrive(&q_empty[slot]);
+      for (int i = 0; i < tiles && ok; ++i, ++g, unit.next(lay.units)) {
+        const int u = unit.at;
+        ok = wait(&k_full[u], unit.lap);
+        // S_x holds P_x until the P V of two tiles before is done.
+        if (g >= 2) ok = ok && wait(&o_done[g & 1], (g >> 1) - 1);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint32_t t_s = tmem + uniform(g & 1) * kTile;
+        const uint64_t qd = q_desc + uniform(slot * lay.slot_bytes >> 4);
+        const uint64_t kd = k_desc + uniform(u * (kUnitBytes >> 4));
+        if (leader) {
+#pragma unroll
+          for (int part = 0; part < kParts; ++part)
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tc::mma_ss(t_s, qd + (part * kHalves + c) * half_step + 2 * k,
+                           kd + c * (kTile * 128 >> 4) + 2 * k, kIdesc,
+                           part > 0 || c > 0 || k > 0);
+          tc::mma_commit(&s_full[g & 1]);
+          tc::mma_commit(&k_empty[u]);
+          if (i == tiles - 1) tc::mma_commit(&q_empty[slot]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 3) {
+    // ---------------------------------------------------------- O (+)= P V
+    const bool leader = tc::elect_one();
+    constexpr uint32_t kIdesc = tc::idesc_bf16(128, D, true);
     const uint64_t v_desc = tc::sw128_desc(smem_addr(smem + lay.values()), kTile * 128, 1024);
-    const int half_bytes = p.block_rows * 128;
-    // S of tile gq, in list order, two tiles ahead of the P V below.
-    Stretch front = st;
-    Turn keys, block;
-    int gq = 0, front_left = 0, slot = 0;
-    auto scores = [&] {
-      while (front_left == 0) {
-        if (!next_segment(p, list, front)) return;
-        slot = block.at;
-        ok = ok && wait(&q_full[slot], block.lap);
-        block.next(lay.slots);
-        front_left = tiles_of(front.seg);
-        if (front_left == 0 && leader) mbar_arrive(&q_empty[slot]);
-      }
-      const int u = keys.at;
-      ok = ok && wait(&k_full[u], keys.lap);
-      if (!ok) return;
-      keys.next(lay.units);
-      tc::tc_fence_after();
-      if (leader) {
-#pragma unroll
-        for (int part = 0; part < kParts; ++part)
-#pragma unroll
-          for (int c = 0; c < kHalves; ++c)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tc::mma_ss(tmem + col_s(gq & 1),
-                         q_desc + ((slot * lay.slot_bytes + (part * kHalves + c) * half_bytes +
-                                    32 * k) >> 4),
-                         k_desc + ((u * kUnitBytes + c * kTile * 128 + 32 * k) >> 4), kIdescQK,
-                         part > 0 || c > 0 || k > 0);
-        tc::mma_commit(&s_full[gq & 1]);
-        tc::mma_commit(&k_empty[u]);
-        if (front_left == 1) tc::mma_commit(&q_empty[slot]);
-      }
-      __syncwarp();
-      --front_left;
-      ++gq;
-    };
-    scores();
-    scores();
-    Turn values;
+    Turn unit;
     int g = 0;
     for (int n = 0; ok && next_segment(p, list, st); ++n) {
-      const int tiles = tiles_of(sg);
-      // The segment's first products overwrite the accumulators.
-      if (n > 0) ok = wait(o_free, n - 1);
-      if (leader) *odd_segment = 0;  // its last reader has freed the accumulators
-      for (int i = 0; i < tiles && ok; ++i, ++g) {
-        const int x = g & 1, u = values.at;
-        const int key = (sg.tile0 + i) * kTile;
-        const bool edge = key + kTile > sg.length;
-        ok = wait(&p_full[x], g >> 1) && wait(&v_ready[u], values.lap);
+      const int tiles = tiles_of(sg), total = sg.length + sg.count;
+      bool odd_in_segment = false;
+      for (int i = 0; i < tiles && ok; ++i, ++g, unit.next(lay.units)) {
+        const int x = g & 1, u = unit.at, key = (sg.tile0 + i) * kTile;
+        ok = wait(&v_full[u], unit.lap);
         if (!ok) break;
-        values.next(lay.units);
-        tc::tc_fence_after();
-        if (leader) {
-          if (edge && odd_unit[u]) {
-            *odd_segment = 1;
-            __threadfence_block();
+        if (key + kTile > sg.length) {
+          // Behind the last node: zeros, for the product with zero
+          // probabilities. A node's infinite or NaN value becomes zero too,
+          // since that product would pass it on to the nodes that do not see
+          // it: the item's end adds it where it is seen.
+          uint8_t* values = smem + lay.values() + u * kUnitBytes;
+          const int row0 = max(sg.length - key, 0), nodes_end = min(total - key, kTile);
+          const int rows_end = min((nodes_end + 15) & ~15, kTile);
+          bool odd = false;
+#pragma unroll 4
+          for (int at = row0 * (D / 8) + lane; at < rows_end * (D / 8); at += 32) {
+            uint4* to = reinterpret_cast<uint4*>(values + tile_at(kTile, at / (D / 8), at % (D / 8)));
+            const bool node = at / (D / 8) < nodes_end;
+            uint4 v = *to;
+            uint32_t* words = &v.x;
+            bool fix = !node;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool low = (words[j] & 0x7f80u) == 0x7f80u;
+              const bool high = (words[j] & 0x7f800000u) == 0x7f800000u;
+              odd |= node && (low || high);
+              fix |= low || high;
+              words[j] = node ? words[j] & (low ? 0xffff0000u : ~0u) & (high ? 0xffffu : ~0u) : 0u;
+            }
+            if (fix) *to = v;
           }
-          const int steps = min(kTile, sg.length + sg.count - key + 15) / 16;
-          for (int k = 0; k < steps; ++k)
-            tc::mma_ts(tmem + col_o(x), tmem + col_s(x) + 8 * k,
-                       v_desc + ((u * kUnitBytes + k * 2048) >> 4), kIdescPV, i > 1 || k > 0);
+          odd_in_segment |= __any_sync(0xffffffffu, odd) != 0;
+          tc::fence_proxy_async();
+          __syncwarp();
+        }
+        // The segment's first products overwrite the accumulators, once the
+        // last segment's have been read.
+        if (i == 0 && n > 0) ok = wait(o_free, n - 1);
+        ok = ok && wait(&p_full[x], g >> 1);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint32_t t_o = tmem + col_o(0) + uniform(x) * (col_o(1) - col_o(0));
+        const uint32_t t_p = tmem + uniform(x) * kTile;
+        const uint64_t vd = v_desc + uniform(u * (kUnitBytes >> 4));
+        if (leader) {
+          *odd_segment = odd_in_segment;
+          __threadfence_block();
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            if (16 * k < total - key)
+              tc::mma_ts(t_o, t_p + 8 * k, vd + (k * 2048 >> 4), kIdesc, i > 1 || k > 0);
           tc::mma_commit(&o_done[x]);
           tc::mma_commit(&v_empty[u]);
         }
         __syncwarp();
-        scores();
       }
-    }
-  } else if (warp == 3) {
-    // ---------------------------------------- values behind the cached keys
-    // Zeros behind the last node, for the product with zero probabilities. A
-    // node's infinite or NaN value becomes zero too, since that product would
-    // pass it on to the nodes that do not see it: the item's end adds it where
-    // it is seen.
-    for (Turn unit; ok && next_segment(p, list, st);) {
-      const int tiles = tiles_of(sg), total = sg.length + sg.count;
-      for (int i = 0; i < tiles && ok; ++i, unit.next(lay.units)) {
-        const int key = (sg.tile0 + i) * kTile, u = unit.at;
-        ok = wait(&v_full[u], unit.lap);
-        if (!ok) break;
-        if (key + kTile <= sg.length) {
-          if (lane == 0) mbar_arrive(&v_ready[u]);
-          continue;
-        }
-        uint8_t* values = smem + lay.values() + u * kUnitBytes;
-        const int row0 = max(sg.length - key, 0), nodes_end = min(total - key, kTile);
-        const int rows_end = min((nodes_end + 15) & ~15, kTile);
-        bool odd = false;
-#pragma unroll 4
-        for (int at = row0 * (D / 8) + lane; at < rows_end * (D / 8); at += 32) {
-          uint4* to = reinterpret_cast<uint4*>(values + tile_at(kTile, at / (D / 8), at % (D / 8)));
-          const bool node = at / (D / 8) < nodes_end;
-          uint4 v = *to;
-          uint32_t* words = &v.x;
-          bool fix = !node;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool low = (words[j] & 0x7f80u) == 0x7f80u;
-            const bool high = (words[j] & 0x7f800000u) == 0x7f800000u;
-            odd |= node && (low || high);
-            fix |= low || high;
-            words[j] = node ? words[j] & (low ? 0xffff0000u : ~0u) & (high ? 0xffffu : ~0u) : 0u;
-          }
-          if (fix) *to = v;
-        }
-        odd = __any_sync(0xffffffffu, odd);
-        tc::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) {
-          odd_unit[u] = odd;
-          mbar_arrive(&v_ready[u]);
-        }
-      }
+      // Every phase of o_free is waited for, or two in a row would look alike.
+      if (tiles == 0 && n > 0) ok = ok && wait(o_free, n - 1);
     }
   } else if (warp >= 4 && warp < 12 && (warp & 3) < row_warps) {
     // --------------------------------------------------------------- softmax
@@ -476,10 +454,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&state_full[x]);
       if (!ok) break;
     }
-  } else if (warp >= 12) {
+  } else if (warp >= 12 && (warp & 3) < row_warps) {
     // ---------------------------------------------------------- an item's end
     const int quarter = warp & 3, r = 32 * quarter + lane;
-    const bool has_rows = quarter < row_warps;
     const uint32_t t_o = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
     int g = 0;
     for (int n = 0; next_segment(p, list, st); ++n) {
@@ -487,90 +464,74 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool whole = sg.whole();
       const int row = sg.mblock * p.block_rows + r;
       float* part = Parts<D>::mine(p, st);
-      if (has_rows) {
-        ok = ok && wait(&state_full[0], n) && wait(&state_full[1], n);
-        const RowState a = states[r], b = states[128 + r];
-        const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
-        const float fa = fast_exp2(a.m - ref), fb = fast_exp2(b.m - ref);
-        const float l = a.l * fa + b.l * fb;
-        end_masks[r] = a.mask;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&state_empty[0]), mbar_arrive(&state_empty[1]);
-        // Each slot's last P V of the segment; a slot without a tile has none.
-        const bool used[2] = {tiles > 1 || (tiles == 1 && (g & 1) == 0),
-                              tiles > 1 || (tiles == 1 && (g & 1) == 1)};
+      ok = ok && wait(&state_full[0], n) && wait(&state_full[1], n);
+      const RowState a = states[r], b = states[128 + r];
+      const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
+      const float fa = fast_exp2(a.m - ref), fb = fast_exp2(b.m - ref);
+      const float l = a.l * fa + b.l * fb;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&state_empty[0]), mbar_arrive(&state_empty[1]);
+      // Each slot's last P V of the segment; a slot without a tile has none.
+      const bool used[2] = {tiles > 1 || (tiles == 1 && (g & 1) == 0),
+                            tiles > 1 || (tiles == 1 && (g & 1) == 1)};
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int last = ((end - 1) & 1) == x ? end - 1 : end - 2;
-          if (used[x] && ok) ok = wait(&o_done[x], last >> 1);
-        }
-        tc::tc_fence_after();
-        const bool odd = tiles > 0 && *odd_segment != 0;
-        const bool live = row < p.rows;
-        const float f = whole ? 1.f / l : 1.f;
-        const float f0 = fa * f, f1 = fb * f;
-        T* out = out_row<T>(p, sg, live ? row : 0);
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float o[32], o1[32];
-          tc::tmem_ld32(t_o + col_o(0) + c, o);
-          tc::tmem_ld32(t_o + col_o(1) + c, o1);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = (used[0] ? o[i] * f0 : 0.f) + (used[1] ? o1[i] * f1 : 0.f);
-          if (c == D - 32) {
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(o_free);
-          }
-          if (!live) continue;
-          if (odd) {
-            // The infinite and NaN values of the nodes that the row sees, among
-            // the segment's tiles.
-            for (int i = 0; i < sg.count; ++i) {
-              const int at = sg.length + i - sg.tile0 * kTile;
-              if ((a.mask >> i & 1) == 0 || at < 0 || at >= tiles * kTile) continue;
-              const T* v = static_cast<const T*>(p.value_cache) + sg.b * p.c_sb +
-                           (int64_t)(sg.length + i) * p.c_sp + sg.h * p.c_sh + c;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const float value = __bfloat162float(v[j]);
-                if (!(fabsf(value) < INFINITY)) o[j] += value;
-              }
-            }
-          }
-          if (whole) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 w = make_uint4(0u, 0u, 0u, 0u);
-              if (a.mask != 0)
-                w = make_uint4(tc::bf16x2(o[i], o[i + 1]), tc::bf16x2(o[i + 2], o[i + 3]),
-                               tc::bf16x2(o[i + 4], o[i + 5]), tc::bf16x2(o[i + 6], o[i + 7]));
-              *reinterpret_cast<uint4*>(out + c + i) = w;
-            }
-          } else {
-            float4* to = reinterpret_cast<float4*>(part + 2 * p.block_rows + r * D + c);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
-        }
-        if (live && whole && p.weights) write_lse(p, sg, row, a.mask == 0, m, l);
-        if (live && !whole) part[r] = m, part[p.block_rows + r] = l;
+      for (int x = 0; x < 2; ++x) {
+        const int last = ((end - 1) & 1) == x ? end - 1 : end - 2;
+        if (used[x] && ok) ok = wait(&o_done[x], last >> 1);
       }
+      tc::tc_fence_after();
+      const bool odd = tiles > 0 && *odd_segment != 0;
+      const bool live = row < p.rows;
+      const float f = whole ? 1.f / l : 1.f;
+      const float f0 = fa * f, f1 = fb * f;
+      T* out = out_row<T>(p, sg.b, sg.h, live ? row : 0);
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float o[32], o1[32];
+        tc::tmem_ld32(t_o + col_o(0) + c, o);
+        tc::tmem_ld32(t_o + col_o(1) + c, o1);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = (used[0] ? o[i] * f0 : 0.f) + (used[1] ? o1[i] * f1 : 0.f);
+        if (c == D - 32) {
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(o_free);
+        }
+        if (!live) continue;
+        if (odd) {
+          // The infinite and NaN values of the nodes that the row sees, among
+          // the segment's tiles.
+          for (int i = 0; i < sg.count; ++i) {
+            const int at = sg.length + i - sg.tile0 * kTile;
+            if ((a.mask >> i & 1) == 0 || at < 0 || at >= tiles * kTile) continue;
+            const T* v = static_cast<const T*>(p.value_cache) + sg.b * p.c_sb +
+                         (int64_t)(sg.length + i) * p.c_sp + sg.h * p.c_sh + c;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float value = __bfloat162float(v[j]);
+              if (!(fabsf(value) < INFINITY)) o[j] += value;
+            }
+          }
+        }
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (a.mask != 0)
+              w = make_uint4(tc::bf16x2(o[i], o[i + 1]), tc::bf16x2(o[i + 2], o[i + 3]),
+                             tc::bf16x2(o[i + 4], o[i + 5]), tc::bf16x2(o[i + 6], o[i + 7]));
+            *reinterpret_cast<uint4*>(out + c + i) = w;
+          }
+        } else {
+          float4* to = reinterpret_cast<float4*>(part + 2 * p.block_rows + r * D + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      if (live && whole && p.weights) write_lse(p, sg, row, m, l);
+      if (live && !whole) part[r] = m, part[p.block_rows + r] = l;
       g = end;
-      if (!whole) {
-        __threadfence();
-        named_sync(1, 128);
-        const Sharers by(st);
-        if (threadIdx.x == 32 * 12) *is_last = take_ticket(by, p.counters + sg.item);
-        named_sync(1, 128);
-        if (*is_last && ok) {
-          __threadfence();
-          merge_parts<D, 128, T>(p, sg, by, end_masks, end_m, end_m + 128, threadIdx.x - 32 * 12,
-                                 [] { named_sync(1, 128); });
-        }
-        named_sync(1, 128);  // the masks may be overwritten
-      }
     }
   }
   if (!ok && lane == 0 && p.status) atomicOr(p.status, ASRBACK_STATUS_TIMEOUT);

@@ -415,15 +415,11 @@ ASRBACK_API int asrback_draft_tree(
  * A row whose counts, lengths or positions are out of range gets zeros, writes
  * nothing else and sets ASRBACK_STATUS_POSITION.
  *
- * counters     asrback_tree_counter_bytes(...) bytes, zero before the first
- *              call; every call leaves them zero. Calls that may run at the
- *              same time (other streams, other graphs) need their own.
  * workspace    asrback_tree_workspace_bytes(...) bytes of scratch (rotary:
  *              q_norm_weight is given, with_weights: weights are), of any
- *              content; likewise not shared by calls that run at the same time.
+ *              content. Calls that may run at the same time (other streams,
+ *              other graphs) need their own.
  */
-ASRBACK_API size_t asrback_tree_counter_bytes(int dtype, int batch, int nodes, int heads,
-                                              int kv_heads);
 ASRBACK_API size_t asrback_tree_workspace_bytes(int dtype, int batch, int nodes, int heads,
                                                 int kv_heads, int head_dim, int cache_length,
                                                 int rotary, int with_weights);
@@ -440,8 +436,7 @@ ASRBACK_API int asrback_tree_attention(
     int64_t c_stride_batch, int64_t c_stride_position, int64_t c_stride_head,
     void* out, int64_t o_stride_batch, int64_t o_stride_node, int64_t o_stride_head,
     float* weights, int64_t w_stride_batch, int64_t w_stride_head,
-    float scale, void* counters, size_t counter_bytes, void* workspace, size_t workspace_bytes,
-    int32_t* status, void* stream);
+    float scale, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /*
  * Greedy acceptance of a draft tree, and the decode-state update of as many
@@ -513,12 +508,6 @@ ASRBACK_API int asrback_evict(
     float* weights, int64_t w_stride_layer, int64_t w_stride_batch, int64_t w_stride_head,
     const int64_t* lengths, int budget, int sink, int recent,
     int64_t* new_lengths, int32_t* kept, int32_t* status, void* stream);
-
-/*
- * The id of the CUDA graph capture that `stream` is in, 0 if it is in none:
- * for callers that keep zeroed counters per graph.
- */
-ASRBACK_API uint64_t asrback_stream_capture_id(void* stream);
 
 /*
  * Self-test of the kernels' bounded waits: one CTA waits on an mbarrier that
