@@ -220,9 +220,6 @@ int rows_per_block(int dtype, int rows) {
   return std::min((rows + 31) / 32 * 32, 128);
 }
 
-// Fewest tiles of a CTA: below, the merge of the parts takes longer than the
-// tiles it saves. (A float32 tile on the FMA pipes takes longer than a merge.)
-int min_tiles(int dtype) { return dtype == ASRBACK_F32 ? 1 : 4; }
 
 struct Plan {
   int block_rows, mblocks, ctas;
@@ -245,9 +242,9 @@ Plan plan_for(int dtype, int batch, int nodes, int heads, int kv_heads, int head
   // As many CTAs as are resident at once.
   const int per_sm = dtype == ASRBACK_BF16 ? 1 : head_dim == 128 ? 2 : 3;
   plan.ctas = static_cast<int>(std::min<int64_t>(tiles, (int64_t)per_sm * sm_count()));
-  // float32, bf16 as it comes, or (rotary) two bf16 parts; then the masks.
+  // float32, bf16 as it comes, or (rotary) two bf16 parts; masks and flags.
   const int row_bytes = head_dim * (dtype == ASRBACK_F32 || rotary ? 4 : 2) + 8;
-  plan.q_block_bytes = plan.block_rows * row_bytes;
+  plan.q_block_bytes = plan.block_rows * row_bytes + kMaxNodes;
   plan.q_bytes = up16((size_t)items * plan.q_block_bytes);
   plan.part_bytes = up16((size_t)2 * plan.ctas * plan.block_rows * (head_dim + 2) * sizeof(float));
   if (weights) {
@@ -365,7 +362,7 @@ extern "C" int asrback_tree_attention(
   p.batch = batch, p.nodes = nodes, p.kv_heads = kv_heads, p.group = heads / kv_heads;
   p.cache_length = cache_length, p.rows = rows;
   p.block_rows = plan.block_rows, p.mblocks = plan.mblocks;
-  p.ctas = plan.ctas, p.min_tiles = min_tiles(dtype);
+  p.ctas = plan.ctas, p.min_tiles = 1;
   uint8_t* at = static_cast<uint8_t*>(workspace);
   p.q_blocks = at;
   p.q_block_bytes = plan.q_block_bytes;

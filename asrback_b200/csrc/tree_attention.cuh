@@ -33,7 +33,8 @@ struct TreeParams {
   int rows, block_rows, mblocks;  // query rows per key/value head, in blocks
   int ctas, min_tiles;            // fewest tiles of a CTA's stretch
   // The prepared query rows, a block per item: [block rows][D] (bf16: laid out as
-  // the products read it, in two parts if rotated), then the rows' masks.
+  // the products read it, in two parts if rotated), the rows' masks (8 bytes),
+  // and kMaxNodes bytes, one per node: its value holds infinities or NaN.
   uint8_t* q_blocks;
   int q_block_bytes;
   float* parts;   // two per CTA: [block rows] m, l, [block rows][D] o

@@ -41,9 +41,20 @@ constexpr int kThreads = 512;
 constexpr int kTailKeys = 16;  // positions per copy of a row's last tile
 constexpr int kMaxUnits = 16;  // tiles of keys, and of values, in their rings
 constexpr float kMoveThreshold = 8.0f;
+// TMEM: four S buffers (P over a buffer's first half), so that the scores run up
+// to four tiles ahead; then the slots' O, for head_dim 64 twice, so that a
+// segment's products begin while the last one's output is read.
 constexpr int kTmemCols = 512;
-constexpr int col_s(int x) { return kTile * x; }  // P over its first half
-constexpr int col_o(int x) { return 2 * kTile + 128 * x; }
+constexpr int kScores = 4;
+constexpr int col_s(int i) { return kTile * i; }
+template <int D>
+struct Outputs {
+  static constexpr int kCopies = D == 64 ? 2 : 1;
+  // Column of slot x's O in a segment whose number is n modulo kCopies.
+  __device__ __forceinline__ static uint32_t at(uint32_t n, uint32_t x) {
+    return kScores * kTile + D * (2 * n + x);
+  }
+};
 
 // What a softmax warp hands to the item's end, per slot and row.
 struct RowState {
@@ -79,8 +90,9 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
 constexpr int kOffStates = 0;                                // [slot][128] RowState
 constexpr int kOffBars = kOffStates + 2 * 128 * 16;
 // full, empty per unit of keys and of values; q_full, q_empty per block; s_full,
-// p_full, o_done, state_full, state_empty per slot; o_free
-constexpr int kNumBars = 4 * kMaxUnits + 4 + 10 + 1;
+// p_full, s_free per S buffer; o_done, state_full, state_empty per slot; o_final,
+// o_free per copy
+constexpr int kNumBars = 4 * kMaxUnits + 4 + 12 + 6 + 4;
 constexpr int kOffInts = kOffBars + kNumBars * 8;            // scratch[16], odd_segment, tmem
 constexpr int kOffList = (kOffInts + 20 * 4 + 15) / 16 * 16;
 constexpr int rest_bytes(int batch) { return kOffList + list_bytes(batch); }
@@ -94,6 +106,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kUnitBytes = kTile * D * 2;
   constexpr int kHalves = D / 64;  // 128-byte column blocks
   constexpr int kParts = kSplit ? 2 : 1;
+  constexpr int kCopies = Outputs<D>::kCopies;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -105,15 +118,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v_empty = v_full + kMaxUnits;
   uint64_t* q_full = v_empty + kMaxUnits;  // [block buffer]
   uint64_t* q_empty = q_full + 2;
-  uint64_t* s_full = q_empty + 2;  // [slot] from here
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_done = p_full + 2;
+  uint64_t* s_full = q_empty + 2;  // [S buffer] from here
+  uint64_t* p_full = s_full + kScores;
+  uint64_t* s_free = p_full + kScores;
+  uint64_t* o_done = s_free + kScores;  // [slot] from here
   uint64_t* state_full = o_done + 2;
   uint64_t* state_empty = state_full + 2;
-  uint64_t* o_free = state_empty + 2;
+  uint64_t* o_final = state_empty + 2;  // [copy] from here
+  uint64_t* o_free = o_final + 2;
   int* scratch = reinterpret_cast<int*>(rest + kOffInts);  // [16]
-  int* odd_segment = scratch + 16;  // the segment's nodes hold infinite or NaN values
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(odd_segment + 1);
+  int* odd_segment = scratch + 16;  // [copy] the segment's nodes hold infinite or NaN values
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(odd_segment + 2);
   TileList list(rest + kOffList, p.batch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row_warps = p.block_rows / 32;
@@ -127,14 +142,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 1 + 2 * row_warps);  // the MMA warp, the softmax warps
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], row_warps);
+      // The MMA warps and the softmax warps.
+      mbar_init(&q_empty[s], 2 + 2 * row_warps);
       mbar_init(&o_done[s], 1);
       mbar_init(&state_full[s], row_warps);
       mbar_init(&state_empty[s], row_warps);
     }
-    mbar_init(o_free, row_warps);
+    for (int i = 0; i < kScores; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], row_warps);
+      mbar_init(&s_free[i], 1);
+    }
+    for (int i = 0; i < kCopies; ++i) {
+      mbar_init(&o_final[i], 1);
+      mbar_init(&o_free[i], row_warps);
+    }
     fence_barrier_init();
   }
   if (warp == 1) tc::tmem_alloc(tmem_slot, kTmemCols);
@@ -256,11 +278,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < tiles && ok; ++i, ++g, unit.next(lay.units)) {
         const int u = unit.at;
         ok = wait(&k_full[u], unit.lap);
-        // S_x holds P_x until the P V of two tiles before is done.
-        if (g >= 2) ok = ok && wait(&o_done[g & 1], (g >> 1) - 1);
+        const int s = g % kScores;
+        if (g >= kScores) ok = ok && wait(&s_free[s], g / kScores - 1);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint32_t t_s = tmem + uniform(g & 1) * kTile;
+        const uint32_t t_s = tmem + uniform(s) * kTile;
         const uint64_t qd = q_desc + uniform(slot * lay.slot_bytes >> 4);
         const uint64_t kd = k_desc + uniform(u * (kUnitBytes >> 4));
         if (leader) {
@@ -273,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::mma_ss(t_s, qd + (part * kHalves + c) * half_step + 2 * k,
                            kd + c * (kTile * 128 >> 4) + 2 * k, kIdesc,
                            part > 0 || c > 0 || k > 0);
-          tc::mma_commit(&s_full[g & 1]);
+          tc::mma_commit(&s_full[s]);
           tc::mma_commit(&k_empty[u]);
           if (i == tiles - 1) tc::mma_commit(&q_empty[slot]);
         }
@@ -285,83 +307,96 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool leader = tc::elect_one();
     constexpr uint32_t kIdesc = tc::idesc_bf16(128, D, true);
     const uint64_t v_desc = tc::sw128_desc(smem_addr(smem + lay.values()), kTile * 128, 1024);
-    Turn unit;
+    Turn unit, block, copy;
     int g = 0;
-    for (int n = 0; ok && next_segment(p, list, st); ++n) {
+    for (; ok && next_segment(p, list, st); block.next(lay.slots), copy.next(kCopies)) {
       const int tiles = tiles_of(sg), total = sg.length + sg.count;
-      bool odd_in_segment = false;
+      // The block ends with a flag per node: its value holds infinities or NaN.
+      ok = wait(&q_full[block.at], block.lap);
+      const uint8_t* flags = smem + block.at * lay.slot_bytes + p.q_block_bytes - kMaxNodes;
+      const bool odd = __any_sync(0xffffffffu, ok && ((lane < sg.count && flags[lane]) ||
+                                                      (lane + 32 < sg.count && flags[lane + 32])));
+      if (lane == 0) mbar_arrive(&q_empty[block.at]);
       for (int i = 0; i < tiles && ok; ++i, ++g, unit.next(lay.units)) {
-        const int x = g & 1, u = unit.at, key = (sg.tile0 + i) * kTile;
+        const int x = g & 1, u = unit.at, s = g % kScores, key = (sg.tile0 + i) * kTile;
         ok = wait(&v_full[u], unit.lap);
         if (!ok) break;
         if (key + kTile > sg.length) {
-          // Behind the last node: zeros, for the product with zero
-          // probabilities. A node's infinite or NaN value becomes zero too,
-          // since that product would pass it on to the nodes that do not see
-          // it: the item's end adds it where it is seen.
           uint8_t* values = smem + lay.values() + u * kUnitBytes;
-          const int row0 = max(sg.length - key, 0), nodes_end = min(total - key, kTile);
-          const int rows_end = min((nodes_end + 15) & ~15, kTile);
-          bool odd = false;
-#pragma unroll 4
-          for (int at = row0 * (D / 8) + lane; at < rows_end * (D / 8); at += 32) {
-            uint4* to = reinterpret_cast<uint4*>(values + tile_at(kTile, at / (D / 8), at % (D / 8)));
-            const bool node = at / (D / 8) < nodes_end;
-            uint4 v = *to;
-            uint32_t* words = &v.x;
-            bool fix = !node;
+          const int nodes_end = min(total - key, kTile), rows_end = min((nodes_end + 15) & ~15, kTile);
+          // Behind the last node: zeros, for the product with zero
+          // probabilities.
+          for (int at = nodes_end * (D / 8) + lane; at < rows_end * (D / 8); at += 32)
+            *reinterpret_cast<uint4*>(values + tile_at(kTile, at / (D / 8), at % (D / 8))) =
+                make_uint4(0u, 0u, 0u, 0u);
+          // An infinite or NaN value becomes zero too, since that product
+          // would pass it on to the nodes that do not see it: the item's end
+          // adds it where it is seen.
+          if (odd) {
+            const int row0 = max(sg.length - key, 0);
+            for (int at = row0 * (D / 8) + lane; at < nodes_end * (D / 8); at += 32) {
+              uint4* to = reinterpret_cast<uint4*>(values +
+                                                   tile_at(kTile, at / (D / 8), at % (D / 8)));
+              uint4 v = *to;
+              uint32_t* words = &v.x;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const bool low = (words[j] & 0x7f80u) == 0x7f80u;
-              const bool high = (words[j] & 0x7f800000u) == 0x7f800000u;
-              odd |= node && (low || high);
-              fix |= low || high;
-              words[j] = node ? words[j] & (low ? 0xffff0000u : ~0u) & (high ? 0xffffu : ~0u) : 0u;
+              for (int j = 0; j < 4; ++j) {
+                if ((words[j] & 0x7f80u) == 0x7f80u) words[j] &= 0xffff0000u;
+                if ((words[j] & 0x7f800000u) == 0x7f800000u) words[j] &= 0xffffu;
+              }
+              *to = v;
             }
-            if (fix) *to = v;
           }
-          odd_in_segment |= __any_sync(0xffffffffu, odd) != 0;
           tc::fence_proxy_async();
           __syncwarp();
         }
-        // The segment's first products overwrite the accumulators, once the
-        // last segment's have been read.
-        if (i == 0 && n > 0) ok = wait(o_free, n - 1);
-        ok = ok && wait(&p_full[x], g >> 1);
+        // The segment's first products overwrite an accumulator whose last
+        // segment has been read.
+        if (i == 0 && copy.lap > 0) ok = wait(&o_free[copy.at], copy.lap - 1);
+        ok = ok && wait(&p_full[s], g / kScores);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint32_t t_o = tmem + col_o(0) + uniform(x) * (col_o(1) - col_o(0));
-        const uint32_t t_p = tmem + uniform(x) * kTile;
+        const uint32_t t_o = tmem + Outputs<D>::at(uniform(copy.at), uniform(x));
+        const uint32_t t_p = tmem + uniform(s) * kTile;
         const uint64_t vd = v_desc + uniform(u * (kUnitBytes >> 4));
         if (leader) {
-          *odd_segment = odd_in_segment;
-          __threadfence_block();
+          if (i == 0) {
+            odd_segment[copy.at] = odd;
+            __threadfence_block();
+          }
 #pragma unroll
           for (int k = 0; k < kTile / 16; ++k)
             if (16 * k < total - key)
               tc::mma_ts(t_o, t_p + 8 * k, vd + (k * 2048 >> 4), kIdesc, i > 1 || k > 0);
           tc::mma_commit(&o_done[x]);
+          if (i == tiles - 1) tc::mma_commit(&o_final[copy.at]);
+          tc::mma_commit(&s_free[s]);
           tc::mma_commit(&v_empty[u]);
         }
         __syncwarp();
       }
-      // Every phase of o_free is waited for, or two in a row would look alike.
-      if (tiles == 0 && n > 0) ok = ok && wait(o_free, n - 1);
+      // A segment without tiles takes its turn all the same: two phases of a
+      // barrier in a row would look alike.
+      if (tiles == 0) {
+        if (copy.lap > 0) ok = ok && wait(&o_free[copy.at], copy.lap - 1);
+        if (leader) mbar_arrive(&o_final[copy.at]);
+      }
     }
   } else if (warp >= 4 && warp < 12 && (warp & 3) < row_warps) {
     // --------------------------------------------------------------- softmax
     const int x = (warp >> 2) - 1, quarter = warp & 3;
     const int r = 32 * quarter + lane;  // this thread's row of the block
     const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
-    const uint32_t t_s = tmem + lanes + col_s(x), t_o = tmem + lanes + col_o(x);
-    Turn block;
+    Turn block, copy;
     int g = 0;
-    for (int n = 0; next_segment(p, list, st); ++n, block.next(lay.slots)) {
+    for (int n = 0; next_segment(p, list, st); ++n, block.next(lay.slots), copy.next(kCopies)) {
+      const uint32_t t_o = tmem + lanes + Outputs<D>::at(copy.at, x);
       const int slot = block.at;
       if (ok) ok = wait(&q_full[slot], block.lap);
       const unsigned long long mask =
           ok ? reinterpret_cast<const unsigned long long*>(smem + slot * lay.slot_bytes +
-                                                           p.q_block_bytes)[r - p.block_rows]
+                                                           p.q_block_bytes - kMaxNodes)[r -
+                                                                                        p.block_rows]
              : 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[slot]);
@@ -369,8 +404,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int total = sg.length + sg.count, g0 = g, end = g + tiles_of(sg);
       // This slot's tiles: every second one of the CTA's.
       for (g += (g ^ x) & 1; g < end && ok; g += 2) {
-        const int tile = sg.tile0 + g - g0;
-        ok = wait(&s_full[x], g >> 1);
+        const int tile = sg.tile0 + g - g0, buffer = g % kScores;
+        const uint32_t t_s = tmem + lanes + buffer * kTile;
+        ok = wait(&s_full[buffer], g / kScores);
         if (!ok) break;
         tc::tc_fence_after();
         float s[kTile];
@@ -445,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_wait_st();
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
+        if (lane == 0) mbar_arrive(&p_full[buffer]);
       }
       g = end;
       if (n > 0 && ok) ok = wait(&state_empty[x], n - 1);
@@ -457,9 +493,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= 12 && (warp & 3) < row_warps) {
     // ---------------------------------------------------------- an item's end
     const int quarter = warp & 3, r = 32 * quarter + lane;
-    const uint32_t t_o = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+    const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
+    Turn copy;
     int g = 0;
-    for (int n = 0; next_segment(p, list, st); ++n) {
+    for (int n = 0; next_segment(p, list, st); ++n, copy.next(kCopies)) {
+      const uint32_t t_o0 = tmem + lanes + Outputs<D>::at(copy.at, 0), t_o1 = t_o0 + D;
       const int tiles = tiles_of(sg), end = g + tiles;
       const bool whole = sg.whole();
       const int row = sg.mblock * p.block_rows + r;
@@ -471,33 +509,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float l = a.l * fa + b.l * fb;
       __syncwarp();
       if (lane == 0) mbar_arrive(&state_empty[0]), mbar_arrive(&state_empty[1]);
-      // Each slot's last P V of the segment; a slot without a tile has none.
+      ok = ok && wait(&o_final[copy.at], copy.lap);
+      // A slot without a tile of the segment holds another's output.
       const bool used[2] = {tiles > 1 || (tiles == 1 && (g & 1) == 0),
                             tiles > 1 || (tiles == 1 && (g & 1) == 1)};
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int last = ((end - 1) & 1) == x ? end - 1 : end - 2;
-        if (used[x] && ok) ok = wait(&o_done[x], last >> 1);
-      }
       tc::tc_fence_after();
-      const bool odd = tiles > 0 && *odd_segment != 0;
+      const bool odd = tiles > 0 && odd_segment[copy.at] != 0;
       const bool live = row < p.rows;
       const float f = whole ? 1.f / l : 1.f;
       const float f0 = fa * f, f1 = fb * f;
       T* out = out_row<T>(p, sg.b, sg.h, live ? row : 0);
+      // 32 columns of the row, both slots' shares.
+      auto read = [&](int c, float (&o)[32]) {
+        float o1[32];
+        tc::tmem_ld32(t_o0 + c, o);
+        tc::tmem_ld32(t_o1 + c, o1);
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        float o[32], o1[32];
-        tc::tmem_ld32(t_o + col_o(0) + c, o);
-        tc::tmem_ld32(t_o + col_o(1) + c, o1);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = (used[0] ? o[i] * f0 : 0.f) + (used[1] ? o1[i] * f1 : 0.f);
-        if (c == D - 32) {
-          tc::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(o_free);
-        }
-        if (!live) continue;
+        for (int i = 0; i < 32; ++i)
+          o[i] = (used[0] ? o[i] * f0 : 0.f) + (used[1] ? o1[i] * f1 : 0.f);
         if (odd) {
           // The infinite and NaN values of the nodes that the row sees, among
           // the segment's tiles.
@@ -513,16 +542,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (whole) {
+      };
+      auto release = [&] {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[copy.at]);
+      };
+      if (whole) {
+        // All columns are read before the first is written, so that the
+        // accumulators are free as early as may be.
+        uint32_t w[D / 2];
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-            if (a.mask != 0)
-              w = make_uint4(tc::bf16x2(o[i], o[i + 1]), tc::bf16x2(o[i + 2], o[i + 3]),
-                             tc::bf16x2(o[i + 4], o[i + 5]), tc::bf16x2(o[i + 6], o[i + 7]));
-            *reinterpret_cast<uint4*>(out + c + i) = w;
-          }
-        } else {
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          read(c, o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            w[c / 2 + i] = a.mask == 0 ? 0u : tc::bf16x2(o[2 * i], o[2 * i + 1]);
+        }
+        release();
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < D / 2; i += 4)
+            *reinterpret_cast<uint4*>(out + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          read(c, o);
+          if (c == D - 32) release();
+          if (!live) continue;
           float4* to = reinterpret_cast<float4*>(part + 2 * p.block_rows + r * D + c);
 #pragma unroll
           for (int i = 0; i < 8; ++i)

@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(kThreads)
   }
   const RowSpan span = row_span(p, b);
   const auto* of_rows = reinterpret_cast<const unsigned long long*>(
-      p.q_blocks + (int64_t)(item + 1) * p.q_block_bytes) - p.block_rows;
+      p.q_blocks + (int64_t)(item + 1) * p.q_block_bytes - kMaxNodes) - p.block_rows;
   if (tid < rows) masks[tid] = of_rows[tid];
   before = __reduce_add_sync(0xffffffffu, before);
   total = __reduce_add_sync(0xffffffffu, total);

@@ -166,11 +166,24 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t to = b * p.c_sb + (int64_t)(span.length + node) * p.c_sp + h * p.c_sh;
     T* key = static_cast<T*>(p.key_cache) + to;
     T* value = static_cast<T*>(p.value_cache) + to;
+    bool odd = false;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       Octet<T>::store(key, half * (D / 2) + 8 * c, x + 8 * half);
       v_in.half[half].copy(value, half * (D / 2) + 8 * c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) odd |= !(fabsf(v_in.half[half][i]) < INFINITY);
     }
+    // Whether any lane of the row (lanes leave together) found one.
+    const unsigned mine = ((1u << (Slice::kLanes - 1)) * 2u - 1u)
+                          << ((threadIdx.x & 31) / Slice::kLanes * Slice::kLanes);
+    odd = __any_sync(mine, odd);
+    if (c < p.mblocks)  // the flag goes to each of the head's blocks
+      for (int i = c; i < p.mblocks; i += Slice::kLanes) {
+        uint8_t* out = p.q_blocks +
+                       ((int64_t)b * p.kv_heads * p.mblocks + h * p.mblocks + i) * p.q_block_bytes;
+        (out + p.q_block_bytes - kMaxNodes)[node] = odd;
+      }
     return;
   }
   if (mask == 0) {
@@ -179,7 +192,7 @@ __global__ void __launch_bounds__(kThreads)
   }
   uint8_t* out = p.q_blocks + ((int64_t)b * p.kv_heads * p.mblocks + block) * p.q_block_bytes;
   if (c == 0)
-    reinterpret_cast<unsigned long long*>(out + p.q_block_bytes)[r - block_rows] = mask;
+    reinterpret_cast<unsigned long long*>(out + p.q_block_bytes - kMaxNodes)[r - block_rows] = mask;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int e = half * (D / 2) + 8 * c;

@@ -186,6 +186,27 @@ def test_weights(family, tag, nodes, heads, kv_heads, dim):
     _check(x, _call(x), _want(x))
 
 
+@pytest.mark.parametrize("family,tag,heads,kv_heads,dim,nodes,weights", [
+    ("qwen3", "bf16", 16, 8, 128, 1, True), ("qwen3", "bf16", 16, 8, 128, 16, False),
+    ("qwen3", "bf16", 16, 4, 64, 5, False), ("qwen3", "bf16", 16, 8, 128, 60, False),
+    ("whisper", "bf16", 20, 20, 64, 7, False), ("whisper", "bf16", 20, 20, 64, 16, True),
+    ("qwen3", "f32", 16, 8, 128, 2, True)])
+def test_many_items_per_sm(family, tag, heads, kv_heads, dim, nodes, weights):
+    """Rows of one to many tiles, some empty, so that a CTA runs through many
+    items and pieces of items; twice, back to back, with the same results."""
+    rows = [700, 447 - nodes, 5, 64, 0, 128, 1, 63, 300, 190, 65, 2]
+    lengths = np.minimum(np.array(rows * 6), 704 if family == "qwen3" else 447 - nodes)
+    rng = np.random.default_rng(nodes)
+    counts = rng.integers(0, nodes + 1, len(lengths))
+    counts[::3] = nodes
+    x = _inputs(nodes, family, tag, len(lengths), nodes, 768, heads, kv_heads, dim, lengths, counts,
+                weights=weights)
+    got = [_call(x) for _ in range(4)]
+    _check(x, got[0], _want(x))
+    for again in got[1:]:
+        assert all(a is None or torch.equal(a, b) for a, b in zip(again, got[0]))
+
+
 def test_long_cache_splits_over_the_gpu():
     """One row, one head: every CTA takes a piece of one item."""
     x = _inputs(0, "qwen3", "bf16", 1, 3, 40000, 2, 1, 128, [39990], weights=True)
