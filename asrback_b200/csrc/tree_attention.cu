@@ -214,9 +214,10 @@ int launch_simt(const TreeParams& p, cudaStream_t stream) {
 }
 
 // Query rows that one CTA holds against a key tile, by dtype and rows per
-// key/value head: in bf16 whole warps of TMEM lanes.
+// key/value head: in bf16 16 for the mma.sync kernel, whole warps of TMEM lanes
+// for the tcgen05 kernel.
 int rows_per_block(int dtype, int rows) {
-  if (dtype == ASRBACK_F32) return 16;
+  if (dtype == ASRBACK_F32 || rows <= 16) return 16;
   return std::min((rows + 31) / 32 * 32, 128);
 }
 
@@ -240,7 +241,9 @@ Plan plan_for(int dtype, int batch, int nodes, int heads, int kv_heads, int head
   const int64_t items = (int64_t)batch * kv_heads * plan.mblocks;
   const int64_t tiles = items * ((cache_length + kTile - 1) / kTile);
   // As many CTAs as are resident at once.
-  const int per_sm = dtype == ASRBACK_BF16 ? 1 : head_dim == 128 ? 2 : 3;
+  const int per_sm = dtype == ASRBACK_F32 ? (head_dim == 128 ? 2 : 3)
+                     : plan.block_rows == 16 ? mma_ctas_per_sm(head_dim)
+                                             : 1;
   plan.ctas = static_cast<int>(std::min<int64_t>(tiles, (int64_t)per_sm * sm_count()));
   // float32, bf16 as it comes, or (rotary) two bf16 parts; masks and flags.
   const int row_bytes = head_dim * (dtype == ASRBACK_F32 || rotary ? 4 : 2) + 8;
@@ -379,7 +382,7 @@ extern "C" int asrback_tree_attention(
   int rc = launch_prepare(dtype, head_dim, p, s);
   if (rc) return rc;
   if (dtype == ASRBACK_BF16)
-    rc = launch_tc(head_dim, p, s);
+    rc = plan.block_rows == 16 ? launch_mma(head_dim, p, s) : launch_tc(head_dim, p, s);
   else
     rc = head_dim == 64 ? launch_simt<64>(p, s) : launch_simt<128>(p, s);
   if (!rc) rc = launch_finish(dtype, head_dim, p, s);

@@ -44,6 +44,14 @@ struct TreeParams {
   int32_t* status;
 };
 
+// A ring's or buffer's place and lap, counted on without divisions.
+struct Turn {
+  int at = 0, lap = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++at == size) at = 0, ++lap;
+  }
+};
+
 struct RowSpan {
   int length, count;  // cached keys, live nodes; 0, 0 for a row that is skipped
   bool bad;
@@ -246,7 +254,10 @@ __device__ __forceinline__ int tile_at(int rows, int row, int piece) {
 int launch_prepare(int dtype, int head_dim, const TreeParams& p, cudaStream_t stream);
 // tree_finish.cu: the merge of split items, the accumulated weights.
 int launch_finish(int dtype, int head_dim, const TreeParams& p, cudaStream_t stream);
-// tree_attention_tc.cu: bf16.
+// tree_attention_mma.cu: bf16, one block of 16 query rows.
+int mma_ctas_per_sm(int head_dim);
+int launch_mma(int head_dim, const TreeParams& p, cudaStream_t stream);
+// tree_attention_tc.cu: bf16, blocks of 32 to 128 query rows.
 int launch_tc(int head_dim, const TreeParams& p, cudaStream_t stream);
 
 }  // namespace tree

@@ -27,10 +27,8 @@
 //               more than 8 (base 2);
 //   warps 12-15 an item's end: merge of the slots, output or part.
 #include <algorithm>
-#include <type_traits>
 
-#include "tcgen05.cuh"
-#include "tree_attention.cuh"
+#include "tree_tma.cuh"
 
 namespace asrback {
 namespace {
@@ -38,7 +36,6 @@ namespace {
 using namespace tree;
 
 constexpr int kThreads = 512;
-constexpr int kTailKeys = 16;  // positions per copy of a row's last tile
 constexpr int kMaxUnits = 16;  // tiles of keys, and of values, in their rings
 constexpr float kMoveThreshold = 8.0f;
 // TMEM: four S buffers (P over a buffer's first half), so that the scores run up
@@ -72,21 +69,6 @@ struct Layout {
   __host__ __device__ int rest() const { return values() + units * unit_bytes; }
 };
 
-// Tensor maps of the cache: whole tiles (a box of 64 positions x D) and blocks
-// of kTailKeys positions x 64 columns.
-struct Maps {
-  CUtensorMap tile[2], tail[2];  // keys, values
-};
-
-__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int c0, int c1, int c2,
-                                            int c3, int c4, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4),
-      "r"(smem_addr(bar))
-      : "memory");
-}
 constexpr int kOffStates = 0;                                // [slot][128] RowState
 constexpr int kOffBars = kOffStates + 2 * 128 * 16;
 // full, empty per unit of keys and of values; q_full, q_empty per block; s_full,
@@ -98,7 +80,7 @@ constexpr int kOffList = (kOffInts + 20 * 4 + 15) / 16 * 16;
 constexpr int rest_bytes(int batch) { return kOffList + list_bytes(batch); }
 constexpr int kBudget = 227 * 1024 - 1024;  // less the alignment of the base
 
-template <int D, bool kSplit, bool kWeights>
+template <int D, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ TreeParams p,
                    const Layout lay) {
@@ -178,13 +160,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   // The same in every lane, and known to be: descriptors built from it are kept in
   // uniform registers, which the issue of an MMA reads.
   auto uniform = [](uint32_t x) { return __reduce_max_sync(0xffffffffu, x); };
-  // A ring's or buffer's place and lap, counted on without divisions.
-  struct Turn {
-    int at = 0, lap = 0;
-    __device__ __forceinline__ void next(int size) {
-      if (++at == size) at = 0, ++lap;
-    }
-  };
 
   if (warp == 0 || warp == 2) {
     // ------------------------------------------------------------------- TMA
@@ -233,22 +208,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!waited) griddep_wait();
           waited = true;
         }
-        uint64_t* bar = &full[unit.at];
         if (ok && unit.lap > 0) ok = wait(&empty[unit.at], unit.lap - 1);
         if (ok && leader) {
-          uint8_t* dst = ring + unit.at * kUnitBytes;
-          if (keys == kTile) {
-            mbar_arrive_expect_tx(bar, kUnitBytes);
-            tma_load_5d(dst, &maps.tile[which], 0, key, 0, sg.h, sg.b, bar);
-          } else {
-            const int blocks = (keys + kTailKeys - 1) / kTailKeys;
-            mbar_arrive_expect_tx(bar, blocks * kTailKeys * D * 2);
-            for (int k = 0; k < blocks * kTailKeys; k += kTailKeys)
-#pragma unroll
-              for (int c = 0; c < kHalves; ++c)
-                tc::tma_load_4d(dst + c * kTile * 128 + k * 128, &maps.tail[which], 64 * c, key + k,
-                                sg.h, sg.b, bar);
-          }
+          load_tile<D>(ring + unit.at * kUnitBytes, maps, which, key, keys, sg.h, sg.b,
+                       &full[unit.at]);
         }
         __syncwarp();
         if (ok) unit.next(lay.units);
@@ -425,16 +388,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < kTile; ++i)
             if ((seen >> i & 1) == 0) s[i] = -INFINITY;
         }
-        if constexpr (kWeights) {
-          if (r < p.rows) {
-            float4* to = reinterpret_cast<float4*>(
-                p.scores + (((int64_t)sg.b * p.kv_heads + sg.h) * p.rows + r) * p.score_stride +
-                tile * kTile);
-#pragma unroll
-            for (int i = 0; i < kTile; i += 4)
-              to[i / 4] = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
-          }
-        }
         float top[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) top[i] = fmaxf(s[i], s[i + 4]);
@@ -579,7 +532,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
-      if (live && whole && p.weights) write_lse(p, sg, row, m, l);
       if (live && !whole) part[r] = m, part[p.block_rows + r] = l;
       g = end;
     }
@@ -593,50 +545,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The cache as a map {64 columns, position, column block, head, row} with a box
-// of 64 positions of all column blocks, and as one {column, position, head, row}
-// with a box of 64 columns of kTailKeys positions.
-int make_maps(CUtensorMap* tile, CUtensorMap* tail, void* base, const TreeParams& p,
-              int head_dim) {
-  int rc = ASRBACK_OK;
-  auto encode = tc::tensor_map_encoder(&rc);
-  if (!encode) return rc;
-  // A dimension of one may have any stride; the encoder wants a plausible one.
-  const auto bytes = [&](int64_t stride, int64_t size) {
-    return static_cast<cuuint64_t>((size > 1 ? stride : head_dim) * 2);
-  };
-  const cuuint64_t position = bytes(p.c_sp, p.cache_length), head = bytes(p.c_sh, p.kv_heads),
-                   row = bytes(p.c_sb, p.batch);
-  const cuuint64_t length = p.cache_length, heads = p.kv_heads, rows = p.batch;
-  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
-  const auto make = [&](CUtensorMap* map, int rank, const cuuint64_t* dims,
-                        const cuuint64_t* strides, const cuuint32_t* box) {
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, base, dims, strides, box, ones,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  };
-  const cuuint64_t blocks = head_dim / 64;
-  const cuuint64_t dims5[5] = {64, length, blocks, heads, rows};
-  const cuuint64_t strides5[4] = {position, 128, head, row};
-  const cuuint32_t box5[5] = {64, kTile, (cuuint32_t)blocks, 1, 1};
-  const cuuint64_t dims4[4] = {(cuuint64_t)head_dim, length, heads, rows};
-  const cuuint64_t strides4[3] = {position, head, row};
-  const cuuint32_t box4[4] = {64, kTailKeys, 1, 1};
-  CUresult res = make(tile, 5, dims5, strides5, box5);
-  if (res == CUDA_SUCCESS) res = make(tail, 4, dims4, strides4, box4);
-  if (res != CUDA_SUCCESS)
-    return fail(ASRBACK_ERR_ARGUMENT,
-                "cuTensorMapEncodeTiled rejected the cache (error %d): strides (%lld, %lld, %lld)",
-                (int)res, (long long)p.c_sb, (long long)p.c_sp, (long long)p.c_sh);
-  return ASRBACK_OK;
-}
-
-template <int D, bool kSplit, bool kWeights>
+template <int D, bool kSplit>
 int launch(const TreeParams& p, cudaStream_t stream) {
-  auto kernel = tree_tc_kernel<D, kSplit, kWeights>;
+  auto kernel = tree_tc_kernel<D, kSplit>;
   Maps maps;
-  if (int rc = make_maps(&maps.tile[0], &maps.tail[0], p.key_cache, p, D)) return rc;
-  if (int rc = make_maps(&maps.tile[1], &maps.tail[1], p.value_cache, p, D)) return rc;
+  if (int rc = make_maps(&maps, p, D)) return rc;
   static thread_local int prepared_device = -1;
   int device = 0;
   if (int rc = check_cuda(cudaGetDevice(&device), "cudaGetDevice")) return rc;
@@ -662,17 +575,8 @@ int launch(const TreeParams& p, cudaStream_t stream) {
 namespace tree {
 
 int launch_tc(int head_dim, const TreeParams& p, cudaStream_t stream) {
-  auto pick = [&](auto dim, auto split) {
-    constexpr int D = decltype(dim)::value;
-    constexpr bool kSplit = decltype(split)::value;
-    return p.weights ? launch<D, kSplit, true>(p, stream) : launch<D, kSplit, false>(p, stream);
-  };
-  using std::integral_constant;
-  if (head_dim == 64)
-    return p.q_norm ? pick(integral_constant<int, 64>{}, std::true_type{})
-                    : pick(integral_constant<int, 64>{}, std::false_type{});
-  return p.q_norm ? pick(integral_constant<int, 128>{}, std::true_type{})
-                  : pick(integral_constant<int, 128>{}, std::false_type{});
+  if (head_dim == 64) return p.q_norm ? launch<64, true>(p, stream) : launch<64, false>(p, stream);
+  return p.q_norm ? launch<128, true>(p, stream) : launch<128, false>(p, stream);
 }
 
 }  // namespace tree
