@@ -31,12 +31,13 @@ struct TreeParams {
   float scale_log2;  // softmax scale times log2(e)
   int batch, nodes, kv_heads, group, cache_length;
   int rows, block_rows, mblocks;  // query rows per key/value head, in blocks
-  int ctas, min_tiles;            // fewest tiles of a CTA's stretch
+  int ctas;
   // The prepared query rows, a block per item: [block rows][D] (bf16: laid out as
   // the products read it, in two parts if rotated), the rows' masks (8 bytes),
   // and kMaxNodes bytes, one per node: its value holds infinities or NaN.
   uint8_t* q_blocks;
   int q_block_bytes;
+  int* place;     // tiles of rows 0..b, then the tiles per CTA: CTA 0 notes them
   float* parts;   // two per CTA: [block rows] m, l, [block rows][D] o
   float* lse;     // with weights: (batch, kv_heads, rows), base 2, of items in one part
   float* scores;  // with weights: (batch, kv_heads, rows, score_stride), base 2
@@ -111,10 +112,6 @@ struct Sharers {
   }
 };
 
-__device__ __forceinline__ int stretch_tiles(const TreeParams& p, int total) {
-  return max((total + p.ctas - 1) / p.ctas, p.min_tiles);
-}
-
 // Fills the tile list and finds the CTA's stretch. All kThreads threads of the
 // CTA call it; `scratch` holds kThreads / 32 ints.
 template <int kThreads>
@@ -150,7 +147,11 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, const Tile
   }
   Stretch st;
   const int total = carry;
-  st.per = stretch_tiles(p, total);
+  st.per = max(1, (total + p.ctas - 1) / p.ctas);
+  if (blockIdx.x == 0) {
+    for (int b = tid; b < p.batch; b += kThreads) p.place[b] = list.prefix[b];
+    if (tid == 0) p.place[p.batch] = st.per;
+  }
   st.lo = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * st.per, (int64_t)total));
   st.hi = min(st.lo + st.per, total);
   st.cur = st.lo;

@@ -115,11 +115,8 @@ __global__ void __launch_bounds__(kThreads)
   const int task = blockIdx.x * (kThreads / Slice::kLanes) + threadIdx.x / Slice::kLanes;
   const int block_rows = p.block_rows;
   const int q_rows = p.kv_heads * p.mblocks * block_rows;
-  const RowSpan span = row_span(p, b);
-  if (span.bad && blockIdx.x == 0 && threadIdx.x == 0 && p.status)
-    atomicOr(p.status, ASRBACK_STATUS_POSITION);
   const bool query = task < q_rows;
-  // A query row's block, place in it and node; or a key's head and node.
+  // A query row's block, row of the block and node; or a key's head and node.
   int block = 0, r = 0, h = 0, node = 0, head = 0;
   bool in = false;
   if (query) {
@@ -129,19 +126,21 @@ __global__ void __launch_bounds__(kThreads)
     const int row = block % p.mblocks * block_rows + r;
     node = row / p.group;
     head = h * p.group + row % p.group;
-    in = row < p.rows && node < span.count;
+    in = row < p.rows;
   } else {
     h = (task - q_rows) / p.nodes;
     node = (task - q_rows) % p.nodes;
-    in = h < p.kv_heads && node < span.count;
+    in = h < p.kv_heads;
   }
-  const unsigned long long live = span.count >= 64 ? ~0ull : (1ull << span.count) - 1;
+  // All loads that need nothing else go out together, whether or not the node
+  // turns out to be live; the angles follow the positions.
   unsigned long long mask = 0;
+  int depth = 0;
   Slice x_in, v_in, w, cs, sn;
   x_in.zero(), v_in.zero(), w.zero(), cs.zero(), sn.zero();
   if (in) {
     const int64_t at = (int64_t)b * p.nodes + node;
-    mask = static_cast<unsigned long long>(__ldg(p.ancestors + at)) & live;
+    mask = static_cast<unsigned long long>(__ldg(p.ancestors + at));
     if (query) {
       x_in.load(static_cast<const T*>(p.q) + b * p.q_sb + node * p.q_sn + head * p.q_sh, c);
     } else {
@@ -152,11 +151,18 @@ __global__ void __launch_bounds__(kThreads)
       w.load(query ? p.q_norm : p.k_norm, c);
       // A valid plan's depth is at most the node's index; any other stays in
       // the table.
-      const int depth = min(max(__ldg(p.depths + at), 0), node);
-      const int64_t place = __ldg(p.positions + b) + depth;
-      cs.load(static_cast<const T*>(p.cos) + place * p.table_stride, c);
-      sn.load(static_cast<const T*>(p.sin) + place * p.table_stride, c);
+      depth = min(max(__ldg(p.depths + at), 0), node);
     }
+  }
+  const RowSpan span = row_span(p, b);
+  if (span.bad && blockIdx.x == 0 && threadIdx.x == 0 && p.status)
+    atomicOr(p.status, ASRBACK_STATUS_POSITION);
+  in = in && node < span.count;
+  mask = in ? mask & (span.count >= 64 ? ~0ull : (1ull << span.count) - 1) : 0;
+  if (in && p.q_norm) {
+    const int64_t place = __ldg(p.positions + b) + depth;
+    cs.load(static_cast<const T*>(p.cos) + place * p.table_stride, c);
+    sn.load(static_cast<const T*>(p.sin) + place * p.table_stride, c);
   }
   float x[16];
   x_in.unpack(x);
@@ -178,12 +184,12 @@ __global__ void __launch_bounds__(kThreads)
     const unsigned mine = ((1u << (Slice::kLanes - 1)) * 2u - 1u)
                           << ((threadIdx.x & 31) / Slice::kLanes * Slice::kLanes);
     odd = __any_sync(mine, odd);
-    if (c < p.mblocks)  // the flag goes to each of the head's blocks
-      for (int i = c; i < p.mblocks; i += Slice::kLanes) {
-        uint8_t* out = p.q_blocks +
-                       ((int64_t)b * p.kv_heads * p.mblocks + h * p.mblocks + i) * p.q_block_bytes;
-        (out + p.q_block_bytes - kMaxNodes)[node] = odd;
-      }
+    // The flag goes to each of the head's blocks.
+    for (int i = c; i < p.mblocks; i += Slice::kLanes) {
+      uint8_t* next = p.q_blocks + (((int64_t)b * p.kv_heads + h) * p.mblocks + i + 1) *
+                                       p.q_block_bytes;
+      (next - kMaxNodes)[node] = odd;
+    }
     return;
   }
   if (mask == 0) {
