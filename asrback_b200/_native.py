@@ -232,7 +232,7 @@ def load() -> ctypes.CDLL:
 def call(name: str, *args) -> None:
     """Calls entry point ``name``; raises :class:`NativeError` with the
     library's message when it returns an error code."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != OK:
         message = lib.asrback_last_error().decode(errors="replace")

@@ -151,7 +151,11 @@ def _cache(t: Tensor, name: str) -> Tensor:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # What torch.cuda.current_stream(device).cuda_stream gives, without building
+    # a Stream object per call.
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if index is None else index)
 
 
 def reserve_workspace(device: torch.device | int | str, batch: int, heads: int, head_dim: int,
@@ -502,16 +506,19 @@ class DraftTree(NamedTuple):
     depths: Tensor
 
 
+_SAME_DEVICE = nullcontext()
+
+
 def _on(device: torch.device):
     """A context in which ``device`` is the current one."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _SAME_DEVICE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _int_rows(t: Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> Tensor:
-    if t.dtype != dtype or t.shape != shape or t.device != device:
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
         raise ValueError(f"asrback_b200: {name} must be {shape} {dtype} on {device}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
@@ -544,75 +551,64 @@ def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
     return DraftTree(parents, live, ancestors, depths)
 
 
-def _tree_call(q: Tensor, k: Tensor, v: Tensor, rotary: tuple | None, tree: DraftTree,
-               lengths: Tensor, keys: Tensor, values: Tensor, scale: float | None,
-               weights: Tensor | None) -> Tensor:
-    """``q`` (B, N, H, D), ``k``/``v`` (B, N, KVH, D) and the caches as
-    (B, L, KVH, D) views, whatever their memory order."""
-    batch, nodes, heads, head_dim = q.shape
-    kv_heads, length = keys.shape[2], keys.shape[1]
-    device = q.device
-    dtype = _dtype_code(q, k, v, keys, values)
-    if values.shape != keys.shape or values.stride() != keys.stride():
-        raise ValueError("asrback_b200: key and value caches differ in shape or strides")
-    if q.stride(3) != 1 or k.stride(3) != 1 or v.stride(3) != 1 or keys.stride(3) != 1:
-        raise ValueError("asrback_b200: head_dim must have unit stride")
-    for t in (k, v, keys, values):
-        if t.device != device:
-            raise ValueError("asrback_b200: tensors must be on one device")
+def _tree_call(dtype: int, q: tuple, k: tuple, v: tuple, sizes: tuple, rotary: tuple | None,
+               tree: DraftTree, lengths: Tensor, keys: Tensor, values: Tensor, strides: tuple,
+               like: Tensor, scale: float | None, weights: Tensor | None) -> Tensor:
+    """``q``, ``k``, ``v``: pointer and strides (row, node, head); ``sizes``:
+    batch, nodes, heads, kv_heads, head_dim, length; ``strides``: the caches'
+    (row, position, head). The tensors' own checks are the callers'."""
+    batch, nodes, heads, kv_heads, head_dim, length = sizes
+    device = like.device
     ancestors = _int_rows(tree.ancestors, "tree.ancestors", torch.int64, (batch, nodes), device)
     depths = _int_rows(tree.depths, "tree.depths", torch.int32, (batch, nodes), device)
     counts = _int_rows(tree.counts, "tree.counts", torch.int32, (batch,), device)
     lengths = _int_rows(lengths, "lengths", torch.int64, (batch,), device)
+    if keys.device != device or values.device != device:
+        raise ValueError("asrback_b200: tensors must be on one device")
     if weights is None:
         w_ptr, w_batch, w_head = None, 0, 0
     else:
-        if weights.dtype != torch.float32 or weights.shape != (batch, kv_heads, length) \
+        if weights.dtype is not torch.float32 or weights.shape != (batch, kv_heads, length) \
                 or weights.device != device or (length > 1 and weights.stride(2) != 1):
             raise ValueError(f"asrback_b200: weights must be {(batch, kv_heads, length)} float32 "
                              "with unit last stride, on the tensors' device")
-        w_ptr, w_batch, w_head = weights.data_ptr(), weights.stride(0), weights.stride(1)
+        w_ptr, (w_batch, w_head, _) = weights.data_ptr(), weights.stride()
     if rotary is None:
         qn = kn = cos = sin = positions = None
         eps, table_stride, table_length = 0.0, 0, 0
     else:
         qn, kn, eps, cos, sin, positions = rotary
-        _dtype_code(q, qn, kn, cos, sin)
-        for weight in (qn, kn):
-            if weight.shape != (head_dim,) or weight.stride(0) != 1 or weight.device != device:
-                raise ValueError("asrback_b200: norm weights must be contiguous (head_dim,)")
-        if cos.dim() != 2 or cos.shape[1] != head_dim or cos.shape != sin.shape \
+        _dtype_code(like, qn, kn, cos, sin)
+        table_length, table_stride = cos.shape[0] if cos.dim() == 2 else 0, cos.stride(0)
+        if cos.shape != (table_length, head_dim) or sin.shape != cos.shape \
                 or cos.stride(1) != 1 or cos.stride() != sin.stride() or cos.device != device \
                 or sin.device != device:
             raise ValueError("asrback_b200: cos and sin must be (table_length, head_dim) of one "
                              "layout")
-        positions = _int_rows(positions, "positions", torch.int64, (batch,), device)
-        qn, kn, table_stride, table_length = qn.data_ptr(), kn.data_ptr(), cos.stride(0), cos.shape[0]
+        for weight in (qn, kn):
+            if weight.shape != (head_dim,) or weight.stride(0) != 1 or weight.device != device:
+                raise ValueError("asrback_b200: norm weights must be contiguous (head_dim,)")
+        positions = _int_rows(positions, "positions", torch.int64, (batch,), device).data_ptr()
+        qn, kn, cos, sin = qn.data_ptr(), kn.data_ptr(), cos.data_ptr(), sin.data_ptr()
         if table_length == 1:
             table_stride = head_dim
-        cos, sin, positions = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
-    lib = _native.load()
+    width = heads * head_dim
+    ws_bytes = _native.load().asrback_tree_workspace_bytes(
+        dtype, batch, nodes, heads, kv_heads, head_dim, length, rotary is not None,
+        weights is not None)
     with _on(device):
-        stream = _stream(device)
-        out = torch.empty((batch, nodes, heads * head_dim), dtype=q.dtype, device=device)
-        ws_bytes = lib.asrback_tree_workspace_bytes(dtype, batch, nodes, heads, kv_heads, head_dim,
-                                                    length, 0 if rotary is None else 1,
-                                                    0 if weights is None else 1)
+        out = torch.empty((batch, nodes, width), dtype=like.dtype, device=device)
         status = _state(device).status
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
         _native.call(
             "asrback_tree_attention",
-            dtype, batch, nodes, heads, kv_heads, head_dim, length,
-            q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
-            k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-            v.data_ptr(), v.stride(0), v.stride(1), v.stride(2),
+            dtype, batch, nodes, heads, kv_heads, head_dim, length, *q, *k, *v,
             qn, kn, eps, cos, sin, table_stride, table_length, positions,
             ancestors.data_ptr(), depths.data_ptr(), counts.data_ptr(), lengths.data_ptr(),
-            keys.data_ptr(), values.data_ptr(), keys.stride(0), keys.stride(1), keys.stride(2),
-            out.data_ptr(), nodes * heads * head_dim, heads * head_dim, head_dim,
-            w_ptr, w_batch, w_head,
-            scale if scale is not None else 1.0 / math.sqrt(head_dim),
-            workspace.data_ptr(), ws_bytes, status.data_ptr(), stream,
+            keys.data_ptr(), values.data_ptr(), *strides,
+            out.data_ptr(), nodes * width, width, head_dim, w_ptr, w_batch, w_head,
+            head_dim ** -0.5 if scale is None else scale,
+            workspace.data_ptr(), ws_bytes, status.data_ptr(), _stream(device),
         )
     return out
 
@@ -640,16 +636,25 @@ def qwen3_attention_tree(qkv: Tensor, q_norm_weight: Tensor, k_norm_weight: Tens
     table gets zeros and sets ``_native.STATUS_POSITION``."""
     if qkv.dim() != 3 or qkv.stride(2) != 1:
         raise ValueError("asrback_b200: qkv must be (batch, nodes, width) with unit last stride")
-    if keys.dim() != 4 or keys.shape[0] != qkv.shape[0] or keys.shape[2] != kv_heads:
-        raise ValueError("asrback_b200: keys must be (batch, length, kv_heads, head_dim)")
     batch, nodes, width = qkv.shape
-    head_dim = keys.shape[3]
+    if keys.dim() != 4 or keys.shape[0] != batch or keys.shape[2] != kv_heads:
+        raise ValueError("asrback_b200: keys must be (batch, length, kv_heads, head_dim)")
+    dtype = _dtype_code(qkv, keys, values)
+    _, length, _, head_dim = keys.shape
     if width != (heads + 2 * kv_heads) * head_dim:
         raise ValueError("asrback_b200: qkv width or cache heads do not match heads/kv_heads")
-    x = qkv.unflatten(2, (heads + 2 * kv_heads, head_dim))
-    return _tree_call(x[:, :, :heads], x[:, :, heads:heads + kv_heads], x[:, :, heads + kv_heads:],
-                      (q_norm_weight, k_norm_weight, float(eps), cos, sin, positions), tree,
-                      positions if lengths is None else lengths, keys, values, scale, weights)
+    strides = keys.stride()
+    if values.shape != keys.shape or values.stride() != strides or strides[3] != 1:
+        raise ValueError("asrback_b200: key and value caches must share shape and strides, "
+                         "head_dim with unit stride")
+    row, node, _ = qkv.stride()
+    start, step = qkv.data_ptr(), head_dim * qkv.element_size()
+    return _tree_call(
+        dtype, (start, row, node, head_dim), (start + heads * step, row, node, head_dim),
+        (start + (heads + kv_heads) * step, row, node, head_dim),
+        (batch, nodes, heads, kv_heads, head_dim, length),
+        (q_norm_weight, k_norm_weight, float(eps), cos, sin, positions), tree,
+        positions if lengths is None else lengths, keys, values, strides[:3], qkv, scale, weights)
 
 
 def whisper_self_attention_tree(query: Tensor, key: Tensor, value: Tensor, key_cache: Tensor,
@@ -667,11 +672,23 @@ def whisper_self_attention_tree(query: Tensor, key: Tensor, value: Tensor, key_c
     if query.dim() != 4 or key.shape != query.shape or value.shape != query.shape:
         raise ValueError("asrback_b200: query, key and value must be (batch, heads, nodes, "
                          "head_dim) of one shape")
-    batch, heads, _, head_dim = query.shape
+    batch, heads, nodes, head_dim = query.shape
     if key_cache.dim() != 4 or key_cache.shape[:2] != (batch, heads) \
             or key_cache.shape[3] != head_dim:
         raise ValueError(f"asrback_b200: cache {tuple(key_cache.shape)} does not match query "
                          f"{tuple(query.shape)}")
-    query, key, value, key_cache, value_cache = (
-        t.transpose(1, 2) for t in (query, key, value, key_cache, value_cache))
-    return _tree_call(query, key, value, None, tree, lengths, key_cache, value_cache, scale, weights)
+    dtype = _dtype_code(query, key, value, key_cache, value_cache)
+    strides = key_cache.stride()
+    if value_cache.shape != key_cache.shape or value_cache.stride() != strides or strides[3] != 1:
+        raise ValueError("asrback_b200: key and value caches must share shape and strides, "
+                         "head_dim with unit stride")
+    inputs = []
+    for t in (query, key, value):
+        row, head, node, unit = t.stride()
+        if unit != 1 or t.device != query.device:
+            raise ValueError("asrback_b200: query, key and value must be on one device, head_dim "
+                             "with unit stride")
+        inputs.append((t.data_ptr(), row, node, head))
+    return _tree_call(dtype, *inputs, (batch, nodes, heads, heads, head_dim, key_cache.shape[2]),
+                      None, tree, lengths, key_cache, value_cache,
+                      (strides[0], strides[2], strides[1]), query, scale, weights)

@@ -17,90 +17,76 @@ from . import _native, attention, step
 __all__ = ["qwen3_commit_tree", "whisper_commit_tree", "qwen3_evict", "whisper_evict"]
 
 
-def _caches(keys: Tensor, values: Tensor, heads_first: bool) -> tuple[Tensor, Tensor]:
-    """The caches as ``(layers, B, L, H, D)`` views."""
-    if keys.dim() not in (4, 5) or values.shape != keys.shape or values.stride() != keys.stride():
+def _caches(keys: Tensor, values: Tensor, heads_first: bool) -> tuple[tuple, tuple, int]:
+    """The caches' sizes (layers, batch, heads, head_dim, length) and strides
+    (layer, row, position, head; a dimension of one has none), and their dtype."""
+    dtype = attention._dtype_code(keys, values)
+    size, stride = keys.shape, keys.stride()
+    if len(size) not in (4, 5) or values.shape != size or values.stride() != stride:
         raise ValueError("asrback_b200: keys and values must be caches of one shape and layout, "
                          "one layer's (4-D) or all layers' (5-D)")
-    if keys.stride(-1) != 1:
-        raise ValueError("asrback_b200: head_dim must have unit stride")
-    if values.device != keys.device:
-        raise ValueError("asrback_b200: keys and values must be on one device")
-    if keys.dim() == 4:
-        keys, values = keys[None], values[None]
+    if stride[-1] != 1 or values.device != keys.device:
+        raise ValueError("asrback_b200: the caches must be on one device, head_dim with unit stride")
+    if len(size) == 4:
+        size, stride = (1, *size), (0, *stride)
+    layers, batch, length, heads, head_dim = size
+    layer, row, position, head, _ = stride
     if heads_first:
-        keys, values = keys.transpose(2, 3), values.transpose(2, 3)
-    return keys, values
+        length, heads, position, head = heads, length, head, position
+    return ((layers, batch, heads, head_dim, length),
+            (layer if layers > 1 else 0, row if batch > 1 else 0,
+             position if length > 1 else head_dim, head if heads > 1 else head_dim), dtype)
 
 
-def _sizes(keys: Tensor) -> tuple:
-    layers, batch, length, heads, head_dim = keys.shape
-    return layers, batch, heads, head_dim, length
-
-
-def _strides(keys: Tensor) -> tuple:
-    """Layer, row, position and head strides (a dimension of one has none)."""
-    layer, batch, position, head, _ = keys.stride()
-    size = keys.shape
-    return (layer if size[0] > 1 else 0, batch if size[1] > 1 else 0,
-            position if size[2] > 1 else size[4], head if size[3] > 1 else size[4])
-
-
-def _weights(weights: Tensor, keys: Tensor, layered: bool) -> Tensor:
-    layers, batch, heads, _, length = _sizes(keys)
-    if not layered and weights.dim() == 3:
-        weights = weights[None]
-    if weights.dtype != torch.float32 or weights.shape != (layers, batch, heads, length) \
-            or weights.device != keys.device or (length > 1 and weights.stride(3) != 1):
+def _weights(weights: Tensor, keys: Tensor, sizes: tuple) -> tuple:
+    """Pointer and strides (layer, row, head) of the accumulated weights."""
+    layers, batch, heads, _, length = sizes
+    shape = (batch, heads, length) if keys.dim() == 4 else (layers, batch, heads, length)
+    if keys.dim() == 4 and weights.dim() == 4:
+        shape = (1, *shape)
+    if weights.dtype is not torch.float32 or weights.shape != shape \
+            or weights.device != keys.device or (length > 1 and weights.stride(-1) != 1):
         raise ValueError("asrback_b200: weights must be ([layers,] batch, heads, length) float32 "
                          "with unit last stride, on the caches' device")
-    return weights
+    stride = weights.stride()[:-1]
+    return (weights.data_ptr(), *(stride if len(stride) == 3 else (0, *stride)))
 
 
 def _commit(keys: Tensor, values: Tensor, accepted: step.AcceptedPath, weights: Tensor | None,
             heads_first: bool) -> None:
-    layered = keys.dim() == 5
-    keys, values = _caches(keys, values, heads_first)
-    dtype = attention._dtype_code(keys, values)
-    device, batch = keys.device, keys.shape[1]
-    nodes = accepted.path.shape[1]
+    sizes, strides, dtype = _caches(keys, values, heads_first)
+    layers, batch, heads, head_dim, length = sizes
+    device, nodes = keys.device, accepted.path.shape[1]
     path = attention._int_rows(accepted.path, "path", torch.int32, (batch, nodes), device)
     counts = attention._int_rows(accepted.counts, "counts", torch.int32, (batch,), device)
     start = attention._int_rows(accepted.start, "start", torch.int64, (batch,), device)
-    layers, batch, heads, head_dim, length = _sizes(keys)
-    if weights is None:
-        w = (None, 0, 0, 0)
-    else:
-        weights = _weights(weights, keys, layered)
-        w = (weights.data_ptr(), *weights.stride()[:3])
+    w = (None, 0, 0, 0) if weights is None else _weights(weights, keys, sizes)
     with attention._on(device):
         _native.call("asrback_commit_tree", dtype, layers, batch, nodes, heads, head_dim, length,
-                     keys.data_ptr(), values.data_ptr(), *_strides(keys), *w, path.data_ptr(),
+                     keys.data_ptr(), values.data_ptr(), *strides, *w, path.data_ptr(),
                      counts.data_ptr(), start.data_ptr(),
                      attention._state(device).status.data_ptr(), attention._stream(device))
 
 
 def _evict(keys: Tensor, values: Tensor, weights: Tensor, lengths: Tensor, budget: int, sink: int,
            recent: int, heads_first: bool) -> tuple[Tensor, Tensor]:
-    layered = keys.dim() == 5
-    keys, values = _caches(keys, values, heads_first)
-    dtype = attention._dtype_code(keys, values)
+    sizes, strides, dtype = _caches(keys, values, heads_first)
+    layers, batch, heads, head_dim, length = sizes
     device = keys.device
-    layers, batch, heads, head_dim, length = _sizes(keys)
-    weights = _weights(weights, keys, layered)
+    w = _weights(weights, keys, sizes)
     lengths = attention._int_rows(lengths, "lengths", torch.int64, (batch,), device)
     if not 1 <= budget <= length or sink < 0 or recent < 0 or sink + recent > budget:
         raise ValueError(f"asrback_b200: budget must be in [1, {length}] and hold sink + recent, "
                          f"got {budget}, {sink}, {recent}")
     with attention._on(device):
         new_lengths = torch.empty(batch, dtype=torch.int64, device=device)
-        kept = torch.empty((layers, batch, heads, budget), dtype=torch.int32, device=device)
+        shape = (batch, heads, budget) if keys.dim() == 4 else (layers, batch, heads, budget)
+        kept = torch.empty(shape, dtype=torch.int32, device=device)
         _native.call("asrback_evict", dtype, layers, batch, heads, head_dim, length,
-                     keys.data_ptr(), values.data_ptr(), *_strides(keys), weights.data_ptr(),
-                     *weights.stride()[:3], lengths.data_ptr(), budget, sink, recent,
-                     new_lengths.data_ptr(), kept.data_ptr(),
+                     keys.data_ptr(), values.data_ptr(), *strides, *w, lengths.data_ptr(), budget,
+                     sink, recent, new_lengths.data_ptr(), kept.data_ptr(),
                      attention._state(device).status.data_ptr(), attention._stream(device))
-    return new_lengths, kept if layered else kept[0]
+    return new_lengths, kept
 
 
 def qwen3_commit_tree(keys: Tensor, values: Tensor, accepted: step.AcceptedPath,

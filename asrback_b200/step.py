@@ -161,11 +161,13 @@ class AcceptedPath(NamedTuple):
     start: Tensor
 
 
-def _node_rows(t: Tensor, name: str, dtype: torch.dtype, shape: tuple, device) -> Tensor:
-    if t.dtype != dtype or t.shape != shape or t.device != device:
+def _node_rows(t: Tensor, name: str, dtype: torch.dtype, shape: tuple, device) -> tuple:
+    """The tensor (which keeps its memory alive) and its row stride."""
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
         raise ValueError(f"asrback_b200: {name} must be {shape} {dtype} on {device}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return t if t.stride(1) == 1 and t.stride(0) >= shape[1] else t.contiguous()
+    row, node = t.stride()
+    return (t, row) if node == 1 and row >= shape[1] else (t.contiguous(), shape[1])
 
 
 def accept_tree(tree: attention.DraftTree, drafts: Tensor, chosen: Tensor, logprob: Tensor,
@@ -184,24 +186,25 @@ def accept_tree(tree: attention.DraftTree, drafts: Tensor, chosen: Tensor, logpr
     with ``position``, for a cache whose slots are not its positions. The
     caches' rows are brought in order by :func:`asrback_b200.cache.qwen3_commit_tree`
     or :func:`~asrback_b200.cache.whisper_commit_tree` with the returned path."""
-    batch, nodes = tree.parents.shape
-    device = tree.parents.device
-    if not tree.parents.is_cuda or tree.parents.dtype != torch.int32:
-        raise ValueError("asrback_b200: tree must be a draft_tree() plan on a CUDA device")
     parents = tree.parents
-    if parents.stride(1) != 1 or 0 < parents.stride(0) < nodes:
-        parents = parents.contiguous()
+    batch, nodes = parents.shape
+    device = parents.device
+    if not parents.is_cuda or parents.dtype is not torch.int32:
+        raise ValueError("asrback_b200: tree must be a draft_tree() plan on a CUDA device")
+    parents_stride, unit = parents.stride()
+    if unit != 1 or 0 < parents_stride < nodes:
+        parents, parents_stride = parents.contiguous(), nodes
     counts = _vector(tree.counts, "tree.counts", torch.int32, batch)
-    drafts = _node_rows(drafts, "drafts", torch.int64, (batch, nodes), device)
-    chosen = _node_rows(chosen, "chosen", torch.int64, (batch, nodes), device)
-    logprob = _node_rows(logprob, "logprob", torch.float32, (batch, nodes), device)
-    if tokens.dtype != torch.int64 or tokens.shape[0] != batch or tokens.numel() != batch:
+    drafts, drafts_stride = _node_rows(drafts, "drafts", torch.int64, (batch, nodes), device)
+    chosen, chosen_stride = _node_rows(chosen, "chosen", torch.int64, (batch, nodes), device)
+    logprob, logprob_stride = _node_rows(logprob, "logprob", torch.float32, (batch, nodes), device)
+    if tokens.dtype is not torch.int64 or tokens.shape[0] != batch or tokens.numel() != batch:
         raise ValueError(f"asrback_b200: tokens must be ({batch},) or ({batch}, 1) int64")
     position = _vector(position, "position", torch.int64, batch)
     end = _vector(end, "end", torch.int64, batch)
     finished = _vector(finished, "finished", torch.bool, batch)
     sums = _vector(sum_logprobs, "sum_logprobs", torch.float32, batch)
-    if generated.dtype != torch.int64 or generated.dim() != 2 or generated.shape[0] != batch \
+    if generated.dtype is not torch.int64 or generated.dim() != 2 or generated.shape[0] != batch \
             or generated.stride(1) != 1:
         raise ValueError(f"asrback_b200: generated must be ({batch}, length) int64 with "
                          "contiguous rows")
@@ -216,13 +219,14 @@ def accept_tree(tree: attention.DraftTree, drafts: Tensor, chosen: Tensor, logpr
         path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
         accepted = torch.empty(batch, dtype=torch.int32, device=device)
         start = torch.empty(batch, dtype=torch.int64, device=device)
+        columns = generated.shape[1]
         _native.call(
-            "asrback_accept_tree", batch, nodes, parents.data_ptr(), parents.stride(0),
-            counts.data_ptr(), drafts.data_ptr(), drafts.stride(0), chosen.data_ptr(),
-            chosen.stride(0), logprob.data_ptr(), logprob.stride(0),
+            "asrback_accept_tree", batch, nodes, parents.data_ptr(), parents_stride,
+            counts.data_ptr(), drafts.data_ptr(), drafts_stride, chosen.data_ptr(), chosen_stride,
+            logprob.data_ptr(), logprob_stride,
             tokens.data_ptr(), tokens.stride(0) if batch > 1 else 1, position.data_ptr(),
             end.data_ptr(), finished.data_ptr(), sums.data_ptr(), generated.data_ptr(),
-            generated.stride(0) if batch > 1 else generated.shape[1], generated.shape[1],
+            generated.stride(0) if batch > 1 else columns, columns,
             None if lengths is None else lengths.data_ptr(), eos_host, len(eos),
             path.data_ptr(), accepted.data_ptr(), start.data_ptr(),
             attention._state(device).status.data_ptr(), attention._stream(device))
