@@ -18,144 +18,187 @@ namespace {
 using namespace tree;
 
 constexpr int kThreads = 128;
-constexpr int kRowsPer = 16;            // output rows of a CTA
+constexpr int kMaxRows = 16;            // rows of a CTA
 constexpr int kKeysPer = 4 * kThreads;  // keys of a CTA
 
-template <int D, typename T>
+// Shared memory of a CTA.
+struct Shared {
+  float part_m[kThreads], part_l[kThreads];  // [group of parts][row]
+  float row_m[kMaxRows], row_l[kMaxRows];    // the rows' references and sums
+  unsigned long long masks[kMaxRows];
+};
+
+// References and sums of the item's rows row0.. over its parts: a thread per row
+// and group of parts.
+template <int D, int kRows>
+__device__ __forceinline__ void join_sums(const TreeParams& p, const Sharers& by, int row0,
+                                          int rows, Shared& s) {
+  constexpr int kGroups = kThreads / kRows, kDeep = 4;
+  const int tid = threadIdx.x, r = tid % kRows, group = tid / kRows;
+  float m = -INFINITY, l = 0.f;
+  if (r < rows && by.count > 1) {
+    for (int c0 = group; c0 < by.count; c0 += kGroups * kDeep) {
+      float m2[kDeep], l2[kDeep];
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        const int c = c0 + u * kGroups;
+        const float* x = Parts<D>::of(p, by, min(c, by.count - 1)) + row0 + r;
+        m2[u] = c < by.count ? x[0] : -INFINITY;
+        l2[u] = c < by.count ? x[p.block_rows] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        const float now = fmaxf(m, m2[u]), ref = now == -INFINITY ? 0.f : now;
+        l = l * fast_exp2(m - ref) + l2[u] * fast_exp2(m2[u] - ref);
+        m = now;
+      }
+    }
+  }
+  s.part_m[tid] = m;
+  s.part_l[tid] = l;
+  __syncthreads();
+  if (tid < min(rows, kRows)) {
+    m = -INFINITY;
+#pragma unroll 8
+    for (int g = 0; g < kGroups; ++g) m = fmaxf(m, s.part_m[g * kRows + tid]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll 8
+    for (int g = 0; g < kGroups; ++g)
+      l += s.part_l[g * kRows + tid] * fast_exp2(s.part_m[g * kRows + tid] - ref);
+    s.row_m[tid] = ref;
+    s.row_l[tid] = l;
+  }
+  __syncthreads();
+}
+
+// kRows: output rows of a CTA that merges. 512 / D, where a thread has four
+// elements and the most parts in flight, for the blocks of few rows, which many
+// CTAs share; kMaxRows, for fewer CTAs, for the blocks of up to 128.
+template <int D, typename T, int kRows>
 __global__ void __launch_bounds__(kThreads)
     tree_finish_kernel(const __grid_constant__ TreeParams p) {
-  // [group of parts][row], then the rows' references and sums.
-  __shared__ float part_m[kThreads], part_l[kThreads];
-  __shared__ float row_m[kRowsPer], row_l[kRowsPer];
-  __shared__ unsigned long long masks[kRowsPer];
+  __shared__ Shared s;
   const int tid = threadIdx.x;
   const int b = blockIdx.z, index = blockIdx.y;
   const int h = index / p.mblocks, mblock = index - h * p.mblocks;
   const int item = (b * p.kv_heads + h) * p.mblocks + mblock;
-  // The CTA's rows. With weights there is one block of at most kRowsPer rows, of
-  // which every CTA needs the references, and the first writes the outputs.
-  const int row0 = p.weights ? 0 : blockIdx.x * kRowsPer;
-  const int rows = min(p.block_rows, p.rows - mblock * p.block_rows) - row0;
+  // The first CTAs of an item merge its rows; with weights (one block of at most
+  // kMaxRows rows) those behind them have each their keys, and all rows.
+  const int block = min(p.block_rows, p.rows - mblock * p.block_rows);
+  const int mergers = (min(p.block_rows, p.rows) + kRows - 1) / kRows;
+  const bool weighs = static_cast<int>(blockIdx.x) >= mergers;
+  const int row0 = weighs ? 0 : blockIdx.x * kRows, rows = block - row0;
+  const int j = (static_cast<int>(blockIdx.x) - mergers) * kKeysPer + 4 * tid;
   griddep_wait();
   griddep_launch_dependents();
+  // The scores of the first rows, wherever the row ends: they wait for nothing.
+  constexpr int kEarly = 8;
+  const float* scores = p.scores + ((int64_t)b * p.kv_heads + h) * p.rows * p.score_stride + j;
+  float4 early[kEarly];
+  if (weighs && j < p.score_stride) {
+#pragma unroll
+    for (int r = 0; r < kEarly; ++r)
+      if (r < rows) early[r] = *reinterpret_cast<const float4*>(scores + r * p.score_stride);
+  }
   const int before = b > 0 ? p.place[b - 1] : 0, upto = p.place[b], per = p.place[p.batch];
   const int length = static_cast<int>(p.lengths[b]), count = p.counts[b];
   const auto* of_rows = reinterpret_cast<const unsigned long long*>(
       p.q_blocks + (int64_t)(item + 1) * p.q_block_bytes - kMaxNodes) - p.block_rows + row0;
-  if (tid < min(rows, kRowsPer)) masks[tid] = of_rows[tid];
+  if (tid < min(rows, kMaxRows)) s.masks[tid] = of_rows[tid];
   const int tiles = (upto - before) / (p.kv_heads * p.mblocks);
   const Sharers by(before + index * tiles, tiles, per);
-  if (rows <= 0 || (by.count == 1 && !p.weights)) return;
-  {
-    // References and sums: a thread per row and eighth of the parts.
-    constexpr int kGroups = kThreads / kRowsPer, kDeep = 4;
-    const int r = tid % kRowsPer, group = tid / kRowsPer;
-    float m = -INFINITY, l = 0.f;
-    if (r < rows && by.count > 1) {
-      for (int c0 = group; c0 < by.count; c0 += kGroups * kDeep) {
-        float m2[kDeep], l2[kDeep];
-#pragma unroll
-        for (int u = 0; u < kDeep; ++u) {
-          const int c = c0 + u * kGroups;
-          const float* x = Parts<D>::of(p, by, min(c, by.count - 1)) + row0 + r;
-          m2[u] = c < by.count ? x[0] : -INFINITY;
-          l2[u] = c < by.count ? x[p.block_rows] : 0.f;
-        }
-#pragma unroll
-        for (int u = 0; u < kDeep; ++u) {
-          const float now = fmaxf(m, m2[u]), ref = now == -INFINITY ? 0.f : now;
-          l = l * fast_exp2(m - ref) + l2[u] * fast_exp2(m2[u] - ref);
-          m = now;
-        }
-      }
-    }
-    part_m[tid] = m;
-    part_l[tid] = l;
-    __syncthreads();
-    if (tid < min(rows, kRowsPer)) {
-      m = -INFINITY;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) m = fmaxf(m, part_m[g * kRowsPer + tid]);
-      const float ref = m == -INFINITY ? 0.f : m;
-      l = 0.f;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g)
-        l += part_l[g * kRowsPer + tid] * fast_exp2(part_m[g * kRowsPer + tid] - ref);
-      row_m[tid] = ref;
-      row_l[tid] = l;
-    }
-    __syncthreads();
-  }
-  if (by.count > 1 && (!p.weights || blockIdx.x == 0)) {
+  if (rows <= 0 || (by.count == 1 && !weighs)) return;
+  if (!weighs) {
+    join_sums<D, kRows>(p, by, row0, rows, s);
     // Outputs: a thread has pieces of four elements.
-    constexpr int kPieces = D / 4, kMine = kRowsPer * kPieces / kThreads;
+    constexpr int kPieces = D / 4, kMine = kRows * kPieces / kThreads, kDeep = 8 / kMine;
     float4 o[kMine];
     int piece[kMine];  // within the CTA's rows
 #pragma unroll
     for (int u = 0; u < kMine; ++u) {
       o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      piece[u] = min(tid + u * kThreads, min(rows, kRowsPer) * kPieces - 1);
+      piece[u] = min(tid + u * kThreads, min(rows, kRows) * kPieces - 1);
     }
-#pragma unroll 4
-    for (int c = 0; c < by.count; ++c) {
-      const float* x = Parts<D>::of(p, by, c);
-      const float4* y = reinterpret_cast<const float4*>(x + 2 * p.block_rows + row0 * D);
+    for (int c0 = 0; c0 < by.count; c0 += kDeep) {
+      float m[kDeep][kMine];
+      float4 v[kDeep][kMine];
 #pragma unroll
-      for (int u = 0; u < kMine; ++u) {
-        const int r = piece[u] / kPieces;
-        const float f = fast_exp2(x[row0 + r] - row_m[r]);
-        const float4 v = y[piece[u]];
-        o[u].x = fmaf(v.x, f, o[u].x), o[u].y = fmaf(v.y, f, o[u].y);
-        o[u].z = fmaf(v.z, f, o[u].z), o[u].w = fmaf(v.w, f, o[u].w);
+      for (int i = 0; i < kDeep; ++i) {
+        const float* x = Parts<D>::of(p, by, min(c0 + i, by.count - 1)) + row0;
+        const float4* y =
+            reinterpret_cast<const float4*>(x + 2 * p.block_rows + row0 * (D - 1));
+#pragma unroll
+        for (int u = 0; u < kMine; ++u) m[i][u] = x[piece[u] / kPieces], v[i][u] = y[piece[u]];
+      }
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) {
+#pragma unroll
+        for (int u = 0; u < kMine; ++u) {
+          const float f =
+              c0 + i < by.count ? fast_exp2(m[i][u] - s.row_m[piece[u] / kPieces]) : 0.f;
+          o[u].x = fmaf(v[i][u].x, f, o[u].x), o[u].y = fmaf(v[i][u].y, f, o[u].y);
+          o[u].z = fmaf(v[i][u].z, f, o[u].z), o[u].w = fmaf(v[i][u].w, f, o[u].w);
+        }
       }
     }
 #pragma unroll
     for (int u = 0; u < kMine; ++u) {
       const int r = (tid + u * kThreads) / kPieces, e = piece[u] % kPieces * 4;
-      if (r < rows)
-        write_four<T>(out_row<T>(p, b, h, mblock * p.block_rows + row0 + r) + e, masks[r] == 0,
-                      row_l[r], o[u]);
+      if (r < min(rows, kRows))
+        write_four<T>(out_row<T>(p, b, h, mblock * p.block_rows + row0 + r) + e, s.masks[r] == 0,
+                      s.row_l[r], o[u]);
     }
+    return;
   }
-  if (!p.weights) return;
+  join_sums<D, kMaxRows>(p, by, 0, rows, s);
   // A skipped row's nodes have masks of zero: no row of it has weights.
-  __syncthreads();
-  if (tid < rows) {
-    const float lse = by.count > 1 ? row_m[tid] + log2f(row_l[tid])
-                                   : p.lse[((int64_t)b * p.kv_heads + h) * p.rows + tid];
-    row_m[tid] = masks[tid] == 0 ? INFINITY : lse;
-  }
-  bool any = false;
-  for (int r = 0; r < rows; ++r) any |= masks[r] != 0;
-  __syncthreads();
-  const int n = length + count, j = blockIdx.x * kKeysPer + 4 * tid;
-  if (!any || j >= n) return;
-  const int64_t unit = (int64_t)b * p.kv_heads + h;
-  const float* scores = p.scores + unit * p.rows * p.score_stride + j;
+  const int n = length + count;
   float* w = p.weights + b * p.w_sb + h * p.w_sh + j;
   float old[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int u = 0; u < 4; ++u) old[u] = j + u < length ? w[u] : 0.f;
-#pragma unroll 8
-  for (int r = 0; r < rows; ++r) {
-    const float4 s = *reinterpret_cast<const float4*>(scores + r * p.score_stride);
-    const float lse = row_m[r];
+  for (int u = 0; u < 4; ++u) old[u] = j + u < min(length, p.cache_length) ? w[u] : 0.f;
+  if (tid < rows) {
+    const float lse = by.count > 1 ? s.row_m[tid] + log2f(s.row_l[tid])
+                                   : p.lse[((int64_t)b * p.kv_heads + h) * p.rows + tid];
+    s.row_m[tid] = s.masks[tid] == 0 ? INFINITY : lse;
+  }
+  bool any = false;
+  for (int r = 0; r < rows; ++r) any |= s.masks[r] != 0;
+  __syncthreads();
+  if (!any || j >= n) return;
+  const auto add = [&](const float4& s, float lse) {
     if (lse != INFINITY) {
       sum[0] += fast_exp2(s.x - lse), sum[1] += fast_exp2(s.y - lse);
       sum[2] += fast_exp2(s.z - lse), sum[3] += fast_exp2(s.w - lse);
     }
-  }
+  };
+#pragma unroll
+  for (int r = 0; r < kEarly; ++r)
+    if (r < rows) add(early[r], s.row_m[r]);
+#pragma unroll 8
+  for (int r = kEarly; r < rows; ++r)
+    add(*reinterpret_cast<const float4*>(scores + r * p.score_stride), s.row_m[r]);
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     if (j + u < n) w[u] = old[u] + sum[u];
 }
 
-template <int D, typename T>
+template <int D, typename T, int kRows>
 int launch(const TreeParams& p, cudaStream_t stream) {
-  unsigned x = (std::min(p.rows, p.block_rows) + kRowsPer - 1) / kRowsPer;
-  if (p.weights) x = std::max<unsigned>(x, (p.cache_length + kKeysPer - 1) / kKeysPer);
-  return launch_pdl(tree_finish_kernel<D, T>, dim3(x, p.kv_heads * p.mblocks, p.batch),
+  unsigned x = (std::min(p.rows, p.block_rows) + kRows - 1) / kRows;
+  if (p.weights) x += (p.cache_length + kKeysPer - 1) / kKeysPer;
+  return launch_pdl(tree_finish_kernel<D, T, kRows>, dim3(x, p.kv_heads * p.mblocks, p.batch),
                     dim3(kThreads), 0, stream, "tree finish launch", p);
+}
+
+template <int D>
+int launch(int dtype, const TreeParams& p, cudaStream_t stream) {
+  const bool few = p.block_rows <= kMaxRows;
+  if (dtype == ASRBACK_F32)
+    return few ? launch<D, float, 512 / D>(p, stream) : launch<D, float, kMaxRows>(p, stream);
+  return few ? launch<D, __nv_bfloat16, 512 / D>(p, stream)
+             : launch<D, __nv_bfloat16, kMaxRows>(p, stream);
 }
 
 }  // namespace
@@ -163,10 +206,7 @@ int launch(const TreeParams& p, cudaStream_t stream) {
 namespace tree {
 
 int launch_finish(int dtype, int head_dim, const TreeParams& p, cudaStream_t stream) {
-  if (dtype == ASRBACK_F32)
-    return head_dim == 64 ? launch<64, float>(p, stream) : launch<128, float>(p, stream);
-  return head_dim == 64 ? launch<64, __nv_bfloat16>(p, stream)
-                        : launch<128, __nv_bfloat16>(p, stream);
+  return head_dim == 64 ? launch<64>(dtype, p, stream) : launch<128>(dtype, p, stream);
 }
 
 }  // namespace tree
