@@ -134,14 +134,15 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // counting the keys at or above each candidate: the count ends early once it
 // is exactly the budget, which distinct weights do after some 10 to 20 bits.
 // Keys equal to the threshold are taken from the lowest slot up. A thread
-// holds V consecutive slots of a chunk in registers; a row of one chunk is
+// holds V slots of a chunk in registers, THREADS apart; a row of one chunk is
 // read once. The kept weights are compacted here, their slots go to `kept`.
 template <int THREADS, int V>
 __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__ SelectParams p) {
   constexpr int kChunk = THREADS * V;
   constexpr int kWarps = THREADS / 32;
-  __shared__ int counter[33];
-  __shared__ int scan[2][kWarps];
+  __shared__ int counts[2][kWarps];
+  __shared__ int scan[V * kWarps];  // keys above | equal << 16 of each 32 slots, in slot order
+  __shared__ int sums[V * kWarps / 32];
   griddep_wait();
   griddep_launch_dependents();
   const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
@@ -163,20 +164,30 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
     for (int k = tid; k < p.budget; k += THREADS) kept[k] = k < n ? k : -1;
     return;
   }
-  if (tid < 33) counter[tid] = 0;
-  __syncthreads();
   float* row = p.weights + layer * p.w_layer + b * p.w_batch + h * p.w_head;
   const int chunks = (n + kChunk - 1) / kChunk;
   const int tail = n - p.recent;
+  float raw[V];
   uint32_t key[V];
   // Slots past the row's end hold key 0, below every weight's.
   auto load = [&](int chunk) {
-    const int base = chunk * kChunk + tid * V;
+    const int base = chunk * kChunk + tid;
+#pragma unroll
+    for (int u = 0; u < V; ++u) raw[u] = row[min(base + u * THREADS, n - 1)];
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-      const int j = base + u;
-      key[u] = j >= n ? 0u : j < p.sink || j >= tail ? kProtected : weight_key(row[j]);
+      const int j = base + u * THREADS;
+      key[u] = j >= n ? 0u : j < p.sink || j >= tail ? kProtected : weight_key(raw[u]);
     }
+  };
+  int turn = 0;
+  // The CTA's sum of the threads' counts; a barrier for all.
+  auto total = [&](int count) {
+    turn ^= 1;
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (lane == 0) counts[turn][warp] = count;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, lane < kWarps ? counts[turn][lane] : 0);
   };
   load(0);
   uint32_t threshold = 0;
@@ -189,16 +200,13 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
 #pragma unroll
       for (int u = 0; u < V; ++u) count += key[u] >= candidate;
     }
-    count = __reduce_add_sync(0xffffffffu, count);
-    if (lane == 0 && count) atomicAdd(&counter[bit], count);
-    __syncthreads();
-    const int total = counter[bit];
-    if (total >= p.budget) threshold = candidate;
-    exact = total == p.budget;
+    count = total(count);
+    if (count >= p.budget) threshold = candidate;
+    exact = count == p.budget;
   }
   // Keys above the threshold (or, if exact, at it) are all kept; of the ones
   // equal to it the `ties` lowest slots.
-  int above_all = 0;
+  int ties = n;
   if (!exact) {
     int count = 0;
     for (int chunk = 0; chunk < chunks; ++chunk) {
@@ -206,50 +214,55 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
 #pragma unroll
       for (int u = 0; u < V; ++u) count += key[u] > threshold;
     }
-    count = __reduce_add_sync(0xffffffffu, count);
-    if (lane == 0 && count) atomicAdd(&counter[32], count);
-    __syncthreads();
-    above_all = counter[32];
+    ties = p.budget - total(count);
   }
-  const int ties = exact ? n : p.budget - above_all;
+  const uint32_t lower = (1u << lane) - 1;
   int above_before = 0, equal_before = 0;  // of the chunks before this one
   for (int chunk = 0; chunk < chunks; ++chunk) {
     if (chunks > 1) load(chunk);
-    const int base = chunk * kChunk + tid * V;
-    int above = 0, equal = 0;
-    float raw[V];
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-      raw[u] = base + u < n ? row[base + u] : 0.f;
-      above += key[u] > threshold;
-      equal += key[u] == threshold;
+      const uint32_t above = __ballot_sync(0xffffffffu, key[u] > threshold);
+      const uint32_t equal = __ballot_sync(0xffffffffu, key[u] == threshold);
+      if (lane == 0) scan[u * kWarps + warp] = __popc(above) | __popc(equal) << 16;
     }
-    int above_scan = above, equal_scan = equal;
+    __syncthreads();  // all counts are there; the chunk's raw weights have been read
+    int mine = 0, through = 0;
+    if (tid < V * kWarps) {
+      mine = through = scan[tid];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int a = __shfl_up_sync(0xffffffffu, above_scan, o);
-      const int e = __shfl_up_sync(0xffffffffu, equal_scan, o);
-      if (lane >= o) above_scan += a, equal_scan += e;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, through, o);
+        if (lane >= o) through += x;
+      }
+      if (lane == 31) sums[warp] = through;
     }
-    __syncthreads();  // the last chunk's sums have been read, the raw weights too
-    if (lane == 31) scan[0][warp] = above_scan, scan[1][warp] = equal_scan;
     __syncthreads();
-    int above_at = above_before + above_scan - above, equal_at = equal_before + equal_scan - equal;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) above_at += scan[0][w], equal_at += scan[1][w];
-      above_before += scan[0][w], equal_before += scan[1][w];
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < V * kWarps / 32; ++w) {
+      if (w < warp) through += sums[w];
+      all += sums[w];
     }
+    if (tid < V * kWarps) scan[tid] = through - mine;
+    __syncthreads();
 #pragma unroll
     for (int u = 0; u < V; ++u) {
       const bool over = key[u] > threshold, same = key[u] == threshold;
+      const uint32_t above = __ballot_sync(0xffffffffu, over);
+      const uint32_t equal = __ballot_sync(0xffffffffu, same);
+      const int at = scan[u * kWarps + warp];
+      const int above_at = above_before + (at & 0xffff) + __popc(above & lower);
+      const int equal_at = equal_before + (at >> 16) + __popc(equal & lower);
       if (over || (same && equal_at < ties)) {
         const int k = above_at + min(equal_at, ties);
-        kept[k] = base + u;
+        kept[k] = chunk * kChunk + u * THREADS + tid;
         row[k] = raw[u];
       }
-      above_at += over;
-      equal_at += same;
     }
+    above_before += all & 0xffff;
+    equal_before += all >> 16;
+    __syncthreads();  // `scan` and `sums` have been read
   }
 }
 
@@ -260,31 +273,34 @@ struct MoveParams {
   const int64_t* lengths;
   const int32_t* kept;
   int batch, heads, length, budget;
-  int vectors;  // 16-byte pieces of the part of a row that one CTA moves
+  int vectors;  // 16-byte pieces of a row
+  int cluster;  // CTAs that move one head's rows
 };
 
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnroll = 4;
 
-// A CTA moves one head's kept rows of the keys or of the values (or a part of
-// their columns, where the batch has few heads), kMoveUnroll rows per thread
-// and turn. A turn's loads come before its barrier and its stores after it;
-// the next turn's loads are issued in between, since its rows lie behind all
-// that this turn writes.
+// A cluster of CTAs moves one head's kept rows of the keys or of the values,
+// kMoveUnroll rows per thread and turn. A turn's loads come before its barrier
+// and its stores after it; the next turn's loads are issued in between, since
+// its rows lie behind all that this turn writes.
+template <bool kCluster>
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveParams p) {
   griddep_wait();
   griddep_launch_dependents();
+  const int cluster = kCluster ? p.cluster : 1;
+  const int h = blockIdx.x / cluster, rank = blockIdx.x - h * cluster;
   const int b = blockIdx.y % p.batch, layer = blockIdx.y / p.batch;
-  const int which = blockIdx.z & 1, part = blockIdx.z >> 1, h = blockIdx.x;
+  const int which = blockIdx.z;
   const int64_t given = p.lengths[b];
   if (given <= p.budget || given > p.length) return;
   const CacheView& c = p.cache[which];
   uint8_t* rows = c.base + layer * c.layer + b * c.batch + h * c.head +
-                  (part * p.vectors + threadIdx.x % p.vectors) * 16;
+                  (threadIdx.x % p.vectors) * 16;
   const int32_t* kept = p.kept + ((int64_t)blockIdx.y * p.heads + h) * p.budget;
   const int lanes = kMoveThreads / p.vectors;  // rows per pass of the CTA
-  const int turn = lanes * kMoveUnroll;
-  const int mine = threadIdx.x / p.vectors;
+  const int turn = lanes * kMoveUnroll * cluster;
+  const int mine = rank * lanes * kMoveUnroll + threadIdx.x / p.vectors;
   uint4 piece[2][kMoveUnroll];
   int from[2][kMoveUnroll];
   auto load = [&](int set, int k0) {
@@ -307,13 +323,17 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
       if (from[set][u] != k) *reinterpret_cast<uint4*>(rows + k * c.position) = piece[set][u];
     }
   };
+  auto barrier = [&]() {
+    if constexpr (kCluster) cluster_sync();
+    else __syncthreads();
+  };
   load(0, 0);
   for (int k0 = 0; k0 < p.budget; k0 += 2 * turn) {
     load(1, k0 + turn);
-    __syncthreads();
+    barrier();
     store(0, k0);
     load(0, k0 + 2 * turn);
-    __syncthreads();
+    barrier();
     store(1, k0 + turn);
   }
 }
@@ -451,15 +471,20 @@ extern "C" int asrback_evict(int dtype, int layers, int batch, int heads, int he
   m.heads = heads;
   m.length = length;
   m.budget = budget;
-  // A row is cut into column parts of at least 64 bytes until the launch has
-  // two CTAs per SM.
-  const int vectors = static_cast<int>(head_dim * esize / 16);
-  int parts = 1;
-  while (vectors / parts > 4 &&
-         static_cast<int64_t>(layers) * batch * heads * 2 * parts < 2 * sm_count())
-    parts *= 2;
-  m.vectors = vectors / parts;
-  rc = launch_pdl(move_kernel, dim3(heads, layers * batch, 2 * parts), dim3(kMoveThreads), 0, st,
-                  "evict move launch", m);
+  // A head's rows are split over a cluster until the launch has four CTAs per SM
+  // or a turn of the cluster holds all rows.
+  m.vectors = static_cast<int>(head_dim * esize / 16);
+  const int64_t moves = static_cast<int64_t>(layers) * batch * heads * 2;
+  const int rows_per_turn = kMoveThreads / m.vectors * kMoveUnroll;
+  m.cluster = 1;
+  while (m.cluster < 8 && moves * m.cluster < 4 * sm_count() && rows_per_turn * m.cluster < budget)
+    m.cluster *= 2;
+  const dim3 move_grid(heads * m.cluster, layers * batch, 2);
+  if (m.cluster == 1)
+    rc = launch_pdl(move_kernel<false>, move_grid, dim3(kMoveThreads), 0, st, "evict move launch",
+                    m);
+  else
+    rc = launch_pdl_cluster(move_kernel<true>, move_grid, dim3(kMoveThreads), 0, m.cluster, st,
+                            "evict move launch", m);
   return rc ? rc : ok();
 }
