@@ -130,19 +130,23 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // One CTA per (layer, row, head) finds the `budget` largest keys. The
-// threshold (the budget-th largest key) is built bit by bit from the top,
-// counting the keys at or above each candidate: the count ends early once it
-// is exactly the budget, which distinct weights do after some 10 to 20 bits.
-// Keys equal to the threshold are taken from the lowest slot up. A thread
-// holds V slots of a chunk in registers, THREADS apart; a row of one chunk is
-// read once. The kept weights are compacted here, their slots go to `kept`.
+// threshold (the budget-th largest key) is built digit by digit from the top:
+// the keys that share the digits so far are counted by their next one, and the
+// digit in which the budget-th lies is the threshold's. It ends early once the
+// keys down to that digit are exactly the budget. Keys equal to the threshold
+// are taken from the lowest slot up. A thread holds V slots of a chunk in
+// registers, THREADS apart; a row of one chunk is read once. The kept weights
+// are compacted here, their slots go to `kept`.
 template <int THREADS, int V>
 __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__ SelectParams p) {
   constexpr int kChunk = THREADS * V;
   constexpr int kWarps = THREADS / 32;
-  __shared__ int counts[2][kWarps];
+  constexpr int kBits = THREADS > 256 ? 11 : 8;  // of a digit, the last one's up to that
+  constexpr int kBins = 1 << kBits, kMine = kBins / THREADS;
+  __shared__ int bins[kBins];
+  __shared__ int found[3];  // the digit, the keys above it, its own
   __shared__ int scan[V * kWarps];  // keys above | equal << 16 of each 32 slots, in slot order
-  __shared__ int sums[V * kWarps / 32];
+  __shared__ int sums[kWarps];
   griddep_wait();
   griddep_launch_dependents();
   const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
@@ -180,42 +184,70 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
       key[u] = j >= n ? 0u : j < p.sink || j >= tail ? kProtected : weight_key(raw[u]);
     }
   };
-  int turn = 0;
-  // The CTA's sum of the threads' counts; a barrier for all.
-  auto total = [&](int count) {
-    turn ^= 1;
-    count = __reduce_add_sync(0xffffffffu, count);
-    if (lane == 0) counts[turn][warp] = count;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, lane < kWarps ? counts[turn][lane] : 0);
-  };
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) bins[tid * kMine + i] = 0;
   load(0);
+  __syncthreads();
   uint32_t threshold = 0;
+  int ties = p.budget;  // kept keys that share the threshold's digits so far
   bool exact = false;
-  for (int bit = 31; bit >= 0 && !exact; --bit) {
-    const uint32_t candidate = threshold | 1u << bit;
-    int count = 0;
+  for (int high = 32; high > 0 && !exact; high -= kBits) {
+    // Bits [low, high) of the keys that share the threshold's above them.
+    const int low = max(high - kBits, 0);
+    const uint32_t mask = (1u << (high - low)) - 1;
     for (int chunk = 0; chunk < chunks; ++chunk) {
       if (chunks > 1) load(chunk);
 #pragma unroll
-      for (int u = 0; u < V; ++u) count += key[u] >= candidate;
+      for (int u = 0; u < V; ++u) {
+        const bool in =
+            key[u] != 0u && static_cast<uint64_t>(key[u] ^ threshold) >> high == 0;
+        const int bin = key[u] >> low & mask;
+        // Many equal keys, as zeros are, count at once.
+        const uint32_t ins = __ballot_sync(0xffffffffu, in);
+        if (ins == 0) continue;
+        const int leader = __ffs(ins) - 1;
+        const int leaders = __shfl_sync(0xffffffffu, bin, leader);  // every lane takes part
+        const bool same = in && bin == leaders;
+        const uint32_t sames = __ballot_sync(0xffffffffu, same);
+        if (lane == leader) atomicAdd(&bins[bin], __popc(sames));
+        else if (in && !same) atomicAdd(&bins[bin], 1);
+      }
     }
-    count = total(count);
-    if (count >= p.budget) threshold = candidate;
-    exact = count == p.budget;
-  }
-  // Keys above the threshold (or, if exact, at it) are all kept; of the ones
-  // equal to it the `ties` lowest slots.
-  int ties = n;
-  if (!exact) {
-    int count = 0;
-    for (int chunk = 0; chunk < chunks; ++chunk) {
-      if (chunks > 1) load(chunk);
+    __syncthreads();
+    int own[kMine], mine = 0;
 #pragma unroll
-      for (int u = 0; u < V; ++u) count += key[u] > threshold;
+    for (int i = 0; i < kMine; ++i) {
+      own[i] = bins[kBins - 1 - tid * kMine - i];
+      bins[kBins - 1 - tid * kMine - i] = 0;
+      mine += own[i];
     }
-    ties = p.budget - total(count);
+    int through = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, through, o);
+      if (lane >= o) through += x;
+    }
+    if (lane == 31) sums[warp] = through;
+    __syncthreads();
+    int before = through - mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      if (w < warp) before += sums[w];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      if (before < ties && ties <= before + own[i]) {
+        found[0] = kBins - 1 - tid * kMine - i;
+        found[1] = before;
+        found[2] = own[i];
+      }
+      before += own[i];
+    }
+    __syncthreads();
+    threshold |= static_cast<uint32_t>(found[0]) << low;
+    ties -= found[1];
+    exact = ties == found[2];
   }
+  if (exact) ties = n;  // whatever shares the digits found is kept
   const uint32_t lower = (1u << lane) - 1;
   int above_before = 0, equal_before = 0;  // of the chunks before this one
   for (int chunk = 0; chunk < chunks; ++chunk) {
