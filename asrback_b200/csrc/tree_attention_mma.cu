@@ -484,7 +484,7 @@ int launch(const TreeParams& p, cudaStream_t stream) {
   using Sh = Shape<D, kSplit>;
   auto kernel = tree_mma_kernel<D, kSplit, kWeights>;
   Maps maps;
-  if (int rc = make_maps(&maps, p, D)) return rc;
+  if (int rc = make_maps(&maps, p, D, kTile)) return rc;
   static thread_local int prepared_device = -1;
   int device = 0;
   if (int rc = check_cuda(cudaGetDevice(&device), "cudaGetDevice")) return rc;

@@ -4,17 +4,18 @@
 // A block of query rows (the nodes of a row times the query heads of one
 // key/value head, up to 128) is one 128-row tcgen05 tile against the row's keys
 // in tiles of 64. The call is bound by streaming the cache, so the TMA warps run
-// ahead of everything through the CTA's whole stretch, across items. Tiles
-// alternate between two slots, each with its own scores, probabilities, output
-// accumulator and softmax state, so that one slot's softmax runs beside the
-// other's products; the two states of an item are merged when it ends, by warps
-// of their own, while the next item is under way. Roles:
-//   warp 0      TMA: a segment's query block, the tiles' keys;
+// ahead of everything through the CTA's whole stretch, across items. A segment's
+// tiles are taken in pairs, whose scores are one product of 128 columns (in
+// shared memory one of 64 reads the queries as long, for half the result); each
+// tile of a pair has a slot, with its own probabilities, output accumulator and
+// softmax state. Scores are a pair ahead, so that the softmax of one runs beside
+// the products of its neighbours; the two states of an item are merged when it
+// ends, by warps of their own, while the next item is under way. Roles:
+//   warp 0      TMA: a segment's query block, the pairs' keys;
 //   warp 2      TMA: the tiles' values. (Two warps, since one issues tiles more
-//               slowly than they arrive.) A full tile is one copy of 64
-//               positions x D, of the row's last one only the blocks of 16
-//               positions that hold keys;
-//   warp 1      TMEM allocation, S_x = Q K^T. A rotated query is two bf16 parts
+//               slowly than they arrive.) A full pair or tile is one copy, of
+//               others only the blocks of 16 positions that hold keys;
+//   warp 1      TMEM allocation, S = Q K^T. A rotated query is two bf16 parts
 //               (their sum has 2^-17 of rounding), whose products are added up
 //               in S;
 //   warp 3      O_x (+)= P_x V, and of the values behind the cached keys: zeros
@@ -36,20 +37,20 @@ namespace {
 using namespace tree;
 
 constexpr int kThreads = 512;
-constexpr int kMaxUnits = 16;  // tiles of keys, and of values, in their rings
+constexpr int kPair = 2 * kTile;  // keys whose scores are one product
+constexpr int kMaxUnits = 16;     // pairs of keys, and tiles of values, in their rings
 constexpr float kMoveThreshold = 8.0f;
-// TMEM: four S buffers (P over a buffer's first half), so that the scores run up
-// to four tiles ahead; then the slots' O, for head_dim 64 twice, so that a
-// segment's products begin while the last one's output is read.
+// TMEM: two S buffers of a pair (a tile's P over the first half of its S); then
+// the slots' O, for head_dim 64 twice, so that a segment's products begin while
+// the last one's output is read.
 constexpr int kTmemCols = 512;
-constexpr int kScores = 4;
-constexpr int col_s(int i) { return kTile * i; }
+constexpr int kScores = 2;
 template <int D>
 struct Outputs {
   static constexpr int kCopies = D == 64 ? 2 : 1;
   // Column of slot x's O in a segment whose number is n modulo kCopies.
   __device__ __forceinline__ static uint32_t at(uint32_t n, uint32_t x) {
-    return kScores * kTile + D * (2 * n + x);
+    return kScores * kPair + D * (2 * n + x);
   }
 };
 
@@ -63,18 +64,18 @@ struct RowState {
 // rest. The tensor core reads 128 rows from a block's start whatever its rows:
 // what follows are keys, as rows of no one.
 struct Layout {
-  int slots, slot_bytes, units, unit_bytes;
+  int slots, slot_bytes, pairs, tiles, tile_bytes;  // rings: pairs of keys, tiles of values
   __host__ __device__ int keys() const { return slots * slot_bytes; }
-  __host__ __device__ int values() const { return keys() + units * unit_bytes; }
-  __host__ __device__ int rest() const { return values() + units * unit_bytes; }
+  __host__ __device__ int values() const { return keys() + pairs * 2 * tile_bytes; }
+  __host__ __device__ int rest() const { return values() + tiles * tile_bytes; }
 };
 
 constexpr int kOffStates = 0;                                // [slot][128] RowState
 constexpr int kOffBars = kOffStates + 2 * 128 * 16;
 // full, empty per unit of keys and of values; q_full, q_empty per block; s_full,
-// p_full, s_free per S buffer; o_done, state_full, state_empty per slot; o_final,
-// o_free per copy
-constexpr int kNumBars = 4 * kMaxUnits + 4 + 12 + 6 + 4;
+// s_free per S buffer; p_full per buffer and slot; o_done, state_full,
+// state_empty per slot; o_final, o_free per copy
+constexpr int kNumBars = 4 * kMaxUnits + 4 + 8 + 6 + 4;
 constexpr int kOffInts = kOffBars + kNumBars * 8;            // scratch[16], odd_segment, tmem
 constexpr int kOffList = (kOffInts + 20 * 4 + 15) / 16 * 16;
 constexpr int rest_bytes(int batch) { return kOffList + list_bytes(batch); }
@@ -101,9 +102,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = v_empty + kMaxUnits;  // [block buffer]
   uint64_t* q_empty = q_full + 2;
   uint64_t* s_full = q_empty + 2;  // [S buffer] from here
-  uint64_t* p_full = s_full + kScores;
-  uint64_t* s_free = p_full + kScores;
-  uint64_t* o_done = s_free + kScores;  // [slot] from here
+  uint64_t* s_free = s_full + kScores;
+  uint64_t* p_full = s_free + kScores;      // [S buffer][slot]
+  uint64_t* o_done = p_full + 2 * kScores;  // [slot] from here
   uint64_t* state_full = o_done + 2;
   uint64_t* state_empty = state_full + 2;
   uint64_t* o_final = state_empty + 2;  // [copy] from here
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int row_warps = p.block_rows / 32;
 
   if (threadIdx.x == 0) {
-    for (int u = 0; u < lay.units; ++u) {
+    for (int u = 0; u < kMaxUnits; ++u) {
       mbar_init(&k_full[u], 1);
       mbar_init(&k_empty[u], 1);
       mbar_init(&v_full[u], 1);
@@ -132,8 +133,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kScores; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], row_warps);
       mbar_init(&s_free[i], 1);
+      for (int x = 0; x < 2; ++x) mbar_init(&p_full[2 * i + x], row_warps);
     }
     for (int i = 0; i < kCopies; ++i) {
       mbar_init(&o_final[i], 1);
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0 || warp == 2) {
     // ------------------------------------------------------------------- TMA
     const int which = warp >> 1;  // keys or values
+    const int units = which ? lay.tiles : lay.pairs, step = which ? kTile : kPair;
     uint64_t* full = which ? v_full : k_full;
     uint64_t* empty = which ? v_empty : k_empty;
     uint8_t* ring = smem + (which ? lay.values() : lay.keys());
@@ -198,56 +200,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       };
-      const int total = sg.length + sg.count, tiles = tiles_of(sg);
-      for (int i = 0; i < tiles && ok; ++i) {
-        const int key = (sg.tile0 + i) * kTile, keys = min(kTile, total - key);
-        load_q(i >= lay.units);
-        // A tile with nodes in it comes after the preparation.
-        if (!waited && key + kTile > sg.length) {
+      const int begin = sg.tile0 * kTile;
+      const int end = min(begin + tiles_of(sg) * kTile, sg.length + sg.count);
+      for (int i = 0, key = begin; key < end && ok; ++i, key += step) {
+        load_q(i >= units);
+        // What has nodes in it comes after the preparation.
+        if (!waited && min(key + step, end) > sg.length) {
           load_q(true);
           if (!waited) griddep_wait();
           waited = true;
         }
         if (ok && unit.lap > 0) ok = wait(&empty[unit.at], unit.lap - 1);
         if (ok && leader) {
-          load_tile<D>(ring + unit.at * kUnitBytes, maps, which, key, keys, sg.h, sg.b,
-                       &full[unit.at]);
+          uint8_t* to = ring + unit.at * step * D * 2;
+          if (which)
+            load_tile<D>(to, maps, 1, key, end - key, sg.h, sg.b, &full[unit.at]);
+          else
+            load_tile<D, kPair>(to, maps, 0, key, end - key, sg.h, sg.b, &full[unit.at]);
         }
         __syncwarp();
-        if (ok) unit.next(lay.units);
+        if (ok) unit.next(units);
       }
       if (ok) load_q(true);
     }
     // A wait gave up: the copies in flight still have to land before the CTA
     // may end.
     if (!ok)
-      for (int u = 0; u < lay.units; ++u) {
+      for (int u = 0; u < units; ++u) {
         const int laps = unit.lap + (u < unit.at ? 1 : 0);
         if (laps > 0) wait(&full[u], laps - 1);
       }
   } else if (warp == 1) {
     // ------------------------------------------------------------ S = Q K^T
     const bool leader = tc::elect_one();
-    constexpr uint32_t kIdesc = tc::idesc_bf16(128, kTile, false);
     const uint64_t q_desc = tc::sw128_desc(smem_addr(smem), 16, 1024);
     const uint64_t k_desc = tc::sw128_desc(smem_addr(smem + lay.keys()), 16, 1024);
     const uint32_t half_step = p.block_rows * 128 >> 4;
-    Turn unit, block;
-    int g = 0;
+    Turn unit, block, scores;
     for (; ok && next_segment(p, list, st); block.next(lay.slots)) {
       const int tiles = tiles_of(sg), slot = block.at;
       ok = wait(&q_full[slot], block.lap);
       if (tiles == 0 && leader) mbar_arrive(&q_empty[slot]);
-      for (int i = 0; i < tiles && ok; ++i, ++g, unit.next(lay.units)) {
-        const int u = unit.at;
+      for (int i = 0; i < tiles && ok; i += 2, unit.next(lay.pairs), scores.next(kScores)) {
+        const int u = unit.at, s = scores.at;
         ok = wait(&k_full[u], unit.lap);
-        const int s = g % kScores;
-        if (g >= kScores) ok = ok && wait(&s_free[s], g / kScores - 1);
+        if (scores.lap > 0) ok = ok && wait(&s_free[s], scores.lap - 1);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint32_t t_s = tmem + uniform(s) * kTile;
+        const uint32_t t_s = tmem + uniform(s) * kPair;
         const uint64_t qd = q_desc + uniform(slot * lay.slot_bytes >> 4);
-        const uint64_t kd = k_desc + uniform(u * (kUnitBytes >> 4));
+        const uint64_t kd = k_desc + uniform(u * (kPair * D * 2 >> 4));
+        const uint32_t idesc = uniform(i + 1 < tiles ? tc::idesc_bf16(128, kPair, false)
+                                                     : tc::idesc_bf16(128, kTile, false));
         if (leader) {
 #pragma unroll
           for (int part = 0; part < kParts; ++part)
@@ -256,11 +260,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 tc::mma_ss(t_s, qd + (part * kHalves + c) * half_step + 2 * k,
-                           kd + c * (kTile * 128 >> 4) + 2 * k, kIdesc,
+                           kd + c * (kPair * 128 >> 4) + 2 * k, idesc,
                            part > 0 || c > 0 || k > 0);
           tc::mma_commit(&s_full[s]);
           tc::mma_commit(&k_empty[u]);
-          if (i == tiles - 1) tc::mma_commit(&q_empty[slot]);
+          if (i + 2 >= tiles) tc::mma_commit(&q_empty[slot]);
         }
         __syncwarp();
       }
@@ -270,8 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool leader = tc::elect_one();
     constexpr uint32_t kIdesc = tc::idesc_bf16(128, D, true);
     const uint64_t v_desc = tc::sw128_desc(smem_addr(smem + lay.values()), kTile * 128, 1024);
-    Turn unit, block, copy;
-    int g = 0;
+    Turn unit, block, copy, scores;
     for (; ok && next_segment(p, list, st); block.next(lay.slots), copy.next(kCopies)) {
       const int tiles = tiles_of(sg), total = sg.length + sg.count;
       // The block ends with a flag per node: its value holds infinities or NaN.
@@ -280,8 +283,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool odd = __any_sync(0xffffffffu, ok && ((lane < sg.count && flags[lane]) ||
                                                       (lane + 32 < sg.count && flags[lane + 32])));
       if (lane == 0) mbar_arrive(&q_empty[block.at]);
-      for (int i = 0; i < tiles && ok; ++i, ++g, unit.next(lay.units)) {
-        const int x = g & 1, u = unit.at, s = g % kScores, key = (sg.tile0 + i) * kTile;
+      for (int i = 0; i < tiles && ok; ++i, unit.next(lay.tiles)) {
+        const int x = i & 1, u = unit.at, s = scores.at, key = (sg.tile0 + i) * kTile;
+        const bool last = i == tiles - 1;
         ok = wait(&v_full[u], unit.lap);
         if (!ok) break;
         if (key + kTile > sg.length) {
@@ -316,11 +320,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The segment's first products overwrite an accumulator whose last
         // segment has been read.
         if (i == 0 && copy.lap > 0) ok = wait(&o_free[copy.at], copy.lap - 1);
-        ok = ok && wait(&p_full[s], g / kScores);
+        ok = ok && wait(&p_full[2 * s + x], scores.lap);
         if (!ok) break;
         tc::tc_fence_after();
         const uint32_t t_o = tmem + Outputs<D>::at(uniform(copy.at), uniform(x));
-        const uint32_t t_p = tmem + uniform(s) * kTile;
+        const uint32_t t_p = tmem + uniform(s) * kPair + uniform(x) * kTile;
         const uint64_t vd = v_desc + uniform(u * (kUnitBytes >> 4));
         if (leader) {
           if (i == 0) {
@@ -332,11 +336,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (16 * k < total - key)
               tc::mma_ts(t_o, t_p + 8 * k, vd + (k * 2048 >> 4), kIdesc, i > 1 || k > 0);
           tc::mma_commit(&o_done[x]);
-          if (i == tiles - 1) tc::mma_commit(&o_final[copy.at]);
-          tc::mma_commit(&s_free[s]);
+          if (last) tc::mma_commit(&o_final[copy.at]);
+          // A pair's barriers go through a phase per pair, whether its second
+          // tile is there or not.
+          if (last && x == 0) tc::mma_commit(&o_done[1]);
+          if (last || x == 1) tc::mma_commit(&s_free[s]);
           tc::mma_commit(&v_empty[u]);
         }
         __syncwarp();
+        if (last && x == 0) ok = wait(&p_full[2 * s + 1], scores.lap);
+        if (last || x == 1) scores.next(kScores);
       }
       // A segment without tiles takes its turn all the same: two phases of a
       // barrier in a row would look alike.
@@ -350,8 +359,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x = (warp >> 2) - 1, quarter = warp & 3;
     const int r = 32 * quarter + lane;  // this thread's row of the block
     const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
-    Turn block, copy;
-    int g = 0;
+    Turn block, copy, scores;
+    int done = 0;  // pairs of the segments before
     for (int n = 0; next_segment(p, list, st); ++n, block.next(lay.slots), copy.next(kCopies)) {
       const uint32_t t_o = tmem + lanes + Outputs<D>::at(copy.at, x);
       const int slot = block.at;
@@ -364,13 +373,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[slot]);
       float m = -INFINITY, l = 0.f;
-      const int total = sg.length + sg.count, g0 = g, end = g + tiles_of(sg);
-      // This slot's tiles: every second one of the CTA's.
-      for (g += (g ^ x) & 1; g < end && ok; g += 2) {
-        const int tile = sg.tile0 + g - g0, buffer = g % kScores;
-        const uint32_t t_s = tmem + lanes + buffer * kTile;
-        ok = wait(&s_full[buffer], g / kScores);
+      const int tiles = tiles_of(sg);
+      for (int i = x; i < tiles + x && ok; i += 2, ++done, scores.next(kScores)) {
+        const int tile = sg.tile0 + i, buffer = scores.at;
+        const uint32_t t_s = tmem + lanes + buffer * kPair + x * kTile;
+        ok = wait(&s_full[buffer], scores.lap);
         if (!ok) break;
+        if (i >= tiles) {  // a pair of one tile
+          if (lane == 0) mbar_arrive(&p_full[2 * buffer + 1]);
+          continue;
+        }
         tc::tc_fence_after();
         float s[kTile];
         tc::tmem_ld64(t_s, s);
@@ -399,9 +411,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool moves = highest > m + kMoveThreshold;
         if (__any_sync(0xffffffffu, moves)) {
           const float now = moves ? highest : m;
-          if (g - g0 > 1) {
+          if (i > 1) {
             // The slot's O of this segment has to be at rest.
-            ok = wait(&o_done[x], (g >> 1) - 1);
+            ok = wait(&o_done[x], done - 1);
             if (!ok) break;
             tc::tc_fence_after();
             const float a = moves ? fast_exp2(m - now) : 1.f;
@@ -434,9 +446,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_wait_st();
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[buffer]);
+        if (lane == 0) mbar_arrive(&p_full[2 * buffer + x]);
       }
-      g = end;
       if (n > 0 && ok) ok = wait(&state_empty[x], n - 1);
       states[128 * x + r] = RowState{m, l, mask};
       __syncwarp();
@@ -448,10 +459,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3, r = 32 * quarter + lane;
     const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
     Turn copy;
-    int g = 0;
     for (int n = 0; next_segment(p, list, st); ++n, copy.next(kCopies)) {
       const uint32_t t_o0 = tmem + lanes + Outputs<D>::at(copy.at, 0), t_o1 = t_o0 + D;
-      const int tiles = tiles_of(sg), end = g + tiles;
+      const int tiles = tiles_of(sg);
       const bool whole = sg.whole();
       const int row = sg.mblock * p.block_rows + r;
       float* part = Parts<D>::mine(p, st);
@@ -464,8 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&state_empty[0]), mbar_arrive(&state_empty[1]);
       ok = ok && wait(&o_final[copy.at], copy.lap);
       // A slot without a tile of the segment holds another's output.
-      const bool used[2] = {tiles > 1 || (tiles == 1 && (g & 1) == 0),
-                            tiles > 1 || (tiles == 1 && (g & 1) == 1)};
+      const bool used[2] = {tiles > 0, tiles > 1};
       tc::tc_fence_after();
       const bool odd = tiles > 0 && odd_segment[copy.at] != 0;
       const bool live = row < p.rows;
@@ -533,7 +542,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (live && !whole) part[r] = m, part[p.block_rows + r] = l;
-      g = end;
     }
   }
   if (!ok && lane == 0 && p.status) atomicOr(p.status, ASRBACK_STATUS_TIMEOUT);
@@ -549,7 +557,7 @@ template <int D, bool kSplit>
 int launch(const TreeParams& p, cudaStream_t stream) {
   auto kernel = tree_tc_kernel<D, kSplit>;
   Maps maps;
-  if (int rc = make_maps(&maps, p, D)) return rc;
+  if (int rc = make_maps(&maps, p, D, kPair)) return rc;
   static thread_local int prepared_device = -1;
   int device = 0;
   if (int rc = check_cuda(cudaGetDevice(&device), "cudaGetDevice")) return rc;
@@ -564,8 +572,11 @@ int launch(const TreeParams& p, cudaStream_t stream) {
   Layout lay{};
   lay.slot_bytes = (p.q_block_bytes + 1023) / 1024 * 1024;
   lay.slots = lay.slot_bytes <= 40 * 1024 ? 2 : 1;
-  lay.unit_bytes = kTile * D * 2;
-  lay.units = std::min((kBudget - rest_bytes(p.batch) - lay.keys()) / lay.unit_bytes / 2, kMaxUnits);
+  lay.tile_bytes = kTile * D * 2;
+  // At least nine tiles' room: half of it, or the lesser part, for the keys.
+  const int room = (kBudget - rest_bytes(p.batch) - lay.keys()) / lay.tile_bytes;
+  lay.pairs = (room + 1) / 4;
+  lay.tiles = std::min(room - 2 * lay.pairs, kMaxUnits);
   return launch_pdl(kernel, dim3(p.ctas), dim3(kThreads), 1024 + lay.rest() + rest_bytes(p.batch),
                     stream, "tree attention launch", maps, p, lay);
 }

@@ -10,8 +10,8 @@ namespace tree {
 
 constexpr int kTailKeys = 16;  // positions per copy of a row's last tile
 
-// Tensor maps of the cache: whole tiles (a box of 64 positions x D) and blocks
-// of kTailKeys positions x 64 columns.
+// Tensor maps of the cache: ring units (a box of 64 or 128 positions x D) and
+// blocks of kTailKeys positions x 64 columns.
 struct Maps {
   CUtensorMap tile[2], tail[2];  // keys, values
 };
@@ -25,14 +25,14 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
       "r"(smem_addr(bar))
       : "memory");
 }
-// Loads the `keys` positions from `key` on of a row's head as one ring unit: a full
-// tile is one copy, of the row's last one only the blocks of kTailKeys positions
-// that hold keys. One thread calls it.
-template <int D>
+// Loads the `keys` positions from `key` on of a row's head as one ring unit of
+// kKeys positions, the box of `maps`: a full unit is one copy, of others only the
+// blocks of kTailKeys positions that hold keys. One thread calls it.
+template <int D, int kKeys = kTile>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const Maps& maps, int which, int key,
                                           int keys, int h, int b, uint64_t* bar) {
-  if (keys >= kTile) {
-    mbar_arrive_expect_tx(bar, kTile * D * 2);
+  if (keys >= kKeys) {
+    mbar_arrive_expect_tx(bar, kKeys * D * 2);
     tma_load_5d(dst, &maps.tile[which], 0, key, 0, h, b, bar);
     return;
   }
@@ -41,15 +41,15 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const Maps& maps, int wh
   for (int k = 0; k < blocks * kTailKeys; k += kTailKeys)
 #pragma unroll
     for (int c = 0; c < D / 64; ++c)
-      tc::tma_load_4d(dst + c * kTile * 128 + k * 128, &maps.tail[which], 64 * c, key + k, h, b,
+      tc::tma_load_4d(dst + c * kKeys * 128 + k * 128, &maps.tail[which], 64 * c, key + k, h, b,
                       bar);
 }
 
 // The cache as a map {64 columns, position, column block, head, row} with a box
-// of 64 positions of all column blocks, and as one {column, position, head, row}
+// of `unit` positions of all column blocks, and as one {column, position, head, row}
 // with a box of 64 columns of kTailKeys positions.
 inline int make_maps(CUtensorMap* tile, CUtensorMap* tail, void* base, const TreeParams& p,
-              int head_dim) {
+                     int head_dim, int unit) {
   int rc = ASRBACK_OK;
   auto encode = tc::tensor_map_encoder(&rc);
   if (!encode) return rc;
@@ -70,7 +70,7 @@ inline int make_maps(CUtensorMap* tile, CUtensorMap* tail, void* base, const Tre
   const cuuint64_t blocks = head_dim / 64;
   const cuuint64_t dims5[5] = {64, length, blocks, heads, rows};
   const cuuint64_t strides5[4] = {position, 128, head, row};
-  const cuuint32_t box5[5] = {64, kTile, (cuuint32_t)blocks, 1, 1};
+  const cuuint32_t box5[5] = {64, (cuuint32_t)unit, (cuuint32_t)blocks, 1, 1};
   const cuuint64_t dims4[4] = {(cuuint64_t)head_dim, length, heads, rows};
   const cuuint64_t strides4[3] = {position, head, row};
   const cuuint32_t box4[4] = {64, kTailKeys, 1, 1};
@@ -83,10 +83,11 @@ inline int make_maps(CUtensorMap* tile, CUtensorMap* tail, void* base, const Tre
   return ASRBACK_OK;
 }
 
-// Both caches' maps.
-inline int make_maps(Maps* maps, const TreeParams& p, int head_dim) {
-  if (int rc = make_maps(&maps->tile[0], &maps->tail[0], p.key_cache, p, head_dim)) return rc;
-  return make_maps(&maps->tile[1], &maps->tail[1], p.value_cache, p, head_dim);
+// Both caches' maps, the keys' with units of `key_unit` positions.
+inline int make_maps(Maps* maps, const TreeParams& p, int head_dim, int key_unit) {
+  if (int rc = make_maps(&maps->tile[0], &maps->tail[0], p.key_cache, p, head_dim, key_unit))
+    return rc;
+  return make_maps(&maps->tile[1], &maps->tail[1], p.value_cache, p, head_dim, kTile);
 }
 
 }  // namespace tree
