@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(kThreads)
     } else {
       float* part = Parts<D>::mine(p, st);
       for (int i = tid; i < kRows * kPieces; i += kThreads)
-        reinterpret_cast<float4*>(part + 2 * kRows)[i] = reinterpret_cast<const float4*>(os)[i];
+        *reinterpret_cast<float4*>(part + Parts<D>::at(p, i / kPieces, i % kPieces * 4)) =
+            reinterpret_cast<const float4*>(os)[i];
       if (tid < kRows) part[tid] = state_m[tid], part[kRows + tid] = state_l[tid];
     }
     __syncthreads();
@@ -225,9 +226,9 @@ int rows_per_block(int dtype, int rows) {
 struct Plan {
   int block_rows, mblocks, ctas;
   int q_block_bytes;
-  size_t q_bytes, place_bytes, part_bytes, lse_bytes, score_bytes;
+  size_t q_bytes, part_bytes, lse_bytes, score_bytes;
   int64_t score_stride;
-  size_t workspace() const { return q_bytes + place_bytes + part_bytes + lse_bytes + score_bytes; }
+  size_t workspace() const { return q_bytes + part_bytes + lse_bytes + score_bytes; }
 };
 
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
@@ -249,7 +250,6 @@ Plan plan_for(int dtype, int batch, int nodes, int heads, int kv_heads, int head
   const int row_bytes = head_dim * (dtype == ASRBACK_F32 || rotary ? 4 : 2) + 8;
   plan.q_block_bytes = plan.block_rows * row_bytes + kMaxNodes;
   plan.q_bytes = up16((size_t)items * plan.q_block_bytes);
-  plan.place_bytes = up16((size_t)(batch + 1) * sizeof(int));
   plan.part_bytes = up16((size_t)2 * plan.ctas * plan.block_rows * (head_dim + 2) * sizeof(float));
   if (weights) {
     plan.score_stride = (cache_length + kTile - 1) / kTile * kTile;
@@ -371,8 +371,6 @@ extern "C" int asrback_tree_attention(
   p.q_blocks = at;
   p.q_block_bytes = plan.q_block_bytes;
   at += plan.q_bytes;
-  p.place = reinterpret_cast<int*>(at);
-  at += plan.place_bytes;
   p.parts = reinterpret_cast<float*>(at);
   at += plan.part_bytes;
   p.lse = reinterpret_cast<float*>(at);

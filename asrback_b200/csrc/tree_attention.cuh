@@ -37,7 +37,6 @@ struct TreeParams {
   // and kMaxNodes bytes, one per node: its value holds infinities or NaN.
   uint8_t* q_blocks;
   int q_block_bytes;
-  int* place;     // tiles of rows 0..b, then the tiles per CTA: CTA 0 notes them
   float* parts;   // two per CTA: [block rows] m, l, [block rows][D] o
   float* lse;     // with weights: (batch, kv_heads, rows), base 2, of items in one part
   float* scores;  // with weights: (batch, kv_heads, rows, score_stride), base 2
@@ -148,10 +147,6 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, const Tile
   Stretch st;
   const int total = carry;
   st.per = max(1, (total + p.ctas - 1) / p.ctas);
-  if (blockIdx.x == 0) {
-    for (int b = tid; b < p.batch; b += kThreads) p.place[b] = list.prefix[b];
-    if (tid == 0) p.place[p.batch] = st.per;
-  }
   st.lo = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * st.per, (int64_t)total));
   st.hi = min(st.lo + st.per, total);
   st.cur = st.lo;
@@ -202,11 +197,16 @@ __device__ __forceinline__ float* score_row(const TreeParams& p, const Segment& 
 }
 
 // Where a segment's result goes, if other CTAs hold the rest of its item: m and l
-// of the block's rows, then their unnormalised outputs.
+// of the block's rows, then their unnormalised outputs, four columns of all rows
+// after the other: the threads of a warp, which have rows, write side by side.
 template <int D>
 struct Parts {
   __device__ __forceinline__ static int64_t floats(const TreeParams& p) {
     return (int64_t)p.block_rows * (D + 2);
+  }
+  // Element (row r, column c) of the outputs.
+  __device__ __forceinline__ static int at(const TreeParams& p, int r, int c) {
+    return 2 * p.block_rows + (c / 4 * p.block_rows + r) * 4 + c % 4;
   }
   // A CTA's first segment leaves part 0, a later one (its last) part 1.
   __device__ __forceinline__ static float* mine(const TreeParams& p, const Stretch& st) {

@@ -468,7 +468,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit>::kPerSm)
           if (warp == 0 && quad == 0) part[r] = m[half], part[kRows + r] = sum;
 #pragma unroll
           for (int c = 0; c < kCols / 8; ++c)
-            *reinterpret_cast<float2*>(part + 2 * kRows + r * D + warp * kCols + 8 * c + 2 * quad) =
+            *reinterpret_cast<float2*>(part +
+                                       Parts<D>::at(p, r, warp * kCols + 8 * c + 2 * quad)) =
                 make_float2(o[c][2 * half], o[c][2 * half + 1]);
         }
       }

@@ -78,8 +78,47 @@ constexpr int kOffBars = kOffStates + 2 * 128 * 16;
 constexpr int kNumBars = 4 * kMaxUnits + 4 + 8 + 6 + 4;
 constexpr int kOffInts = kOffBars + kNumBars * 8;            // scratch[16], odd_segment, tmem
 constexpr int kOffList = (kOffInts + 20 * 4 + 15) / 16 * 16;
+constexpr int kRead = 32;  // output columns that an item's end reads at a time
 constexpr int rest_bytes(int batch) { return kOffList + list_bytes(batch); }
 constexpr int kBudget = 227 * 1024 - 1024;  // less the alignment of the base
+
+// Two floats in one operation.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long x, y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(x), "l"(y));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
+  return a;
+}
+
+// kRead columns of two places of this thread's TMEM lane, waited for once: a load
+// of a few columns takes as long as one of many.
+__device__ __forceinline__ void load_both(uint32_t t0, uint32_t t1, float* v0, float* v1) {
+  uint32_t x[kRead], y[kRead];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+      "%28, %29, %30, %31}, [%64];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, "
+      "%41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, "
+      "%58, %59, %60, %61, %62, %63}, [%65];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]),
+        "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]),
+        "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
+        "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]),
+        "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31]), "=r"(y[0]), "=r"(y[1]), "=r"(y[2]),
+        "=r"(y[3]), "=r"(y[4]), "=r"(y[5]), "=r"(y[6]), "=r"(y[7]), "=r"(y[8]), "=r"(y[9]),
+        "=r"(y[10]), "=r"(y[11]), "=r"(y[12]), "=r"(y[13]), "=r"(y[14]), "=r"(y[15]), "=r"(y[16]),
+        "=r"(y[17]), "=r"(y[18]), "=r"(y[19]), "=r"(y[20]), "=r"(y[21]), "=r"(y[22]), "=r"(y[23]),
+        "=r"(y[24]), "=r"(y[25]), "=r"(y[26]), "=r"(y[27]), "=r"(y[28]), "=r"(y[29]), "=r"(y[30]),
+        "=r"(y[31])
+      : "r"(t0), "r"(t1)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < kRead; ++i) v0[i] = __uint_as_float(x[i]), v1[i] = __uint_as_float(y[i]);
+}
 
 template <int D, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -115,6 +154,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   TileList list(rest + kOffList, p.batch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row_warps = p.block_rows / 32;
+  // Of a query buffer: the rows, then their masks and the nodes' flags.
+  const int rows_bytes = kParts * kHalves * p.block_rows * 128;
 
   if (threadIdx.x == 0) {
     for (int u = 0; u < kMaxUnits; ++u) {
@@ -279,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tiles = tiles_of(sg), total = sg.length + sg.count;
       // The block ends with a flag per node: its value holds infinities or NaN.
       ok = wait(&q_full[block.at], block.lap);
-      const uint8_t* flags = smem + block.at * lay.slot_bytes + p.q_block_bytes - kMaxNodes;
+      const uint8_t* flags = smem + block.at * lay.slot_bytes + rows_bytes + 8 * p.block_rows;
       const bool odd = __any_sync(0xffffffffu, ok && ((lane < sg.count && flags[lane]) ||
                                                       (lane + 32 < sg.count && flags[lane + 32])));
       if (lane == 0) mbar_arrive(&q_empty[block.at]);
@@ -320,7 +361,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The segment's first products overwrite an accumulator whose last
         // segment has been read.
         if (i == 0 && copy.lap > 0) ok = wait(&o_free[copy.at], copy.lap - 1);
+        // A pair of one tile waits for its other slot too, which has seen the
+        // scores then: the buffer is not given on before.
         ok = ok && wait(&p_full[2 * s + x], scores.lap);
+        if (last && x == 0) ok = ok && wait(&p_full[2 * s + 1], scores.lap);
         if (!ok) break;
         tc::tc_fence_after();
         const uint32_t t_o = tmem + Outputs<D>::at(uniform(copy.at), uniform(x));
@@ -344,7 +388,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::mma_commit(&v_empty[u]);
         }
         __syncwarp();
-        if (last && x == 0) ok = wait(&p_full[2 * s + 1], scores.lap);
         if (last || x == 1) scores.next(kScores);
       }
       // A segment without tiles takes its turn all the same: two phases of a
@@ -367,8 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) ok = wait(&q_full[slot], block.lap);
       const unsigned long long mask =
           ok ? reinterpret_cast<const unsigned long long*>(smem + slot * lay.slot_bytes +
-                                                           p.q_block_bytes - kMaxNodes)[r -
-                                                                                        p.block_rows]
+                                                           rows_bytes)[r]
              : 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[slot]);
@@ -433,15 +475,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Probabilities are rounded to bf16 for the second product (2^-8 at
         // most, against an output in bf16 itself); their sum is not.
         const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t packed[kTile / 2];
 #pragma unroll
         for (int i = 0; i < kTile; i += 2) {
-          const float p0 = fast_exp2(s[i] - ref), p1 = fast_exp2(s[i + 1] - ref);
-          sum[(i >> 1) & 3] += p0 + p1;
-          packed[i / 2] = tc::bf16x2(p0, p1);
+          float2 e = add2(make_float2(s[i], s[i + 1]), make_float2(-ref, -ref));
+          e = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+          packed[i / 2] = tc::bf16x2(e.x, e.y);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc::tmem_st32u(t_s, packed);
         tc::tmem_wait_st();
         tc::tc_fence_before();
@@ -481,13 +524,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float f = whole ? 1.f / l : 1.f;
       const float f0 = fa * f, f1 = fb * f;
       T* out = out_row<T>(p, sg.b, sg.h, live ? row : 0);
-      // 32 columns of the row, both slots' shares.
-      auto read = [&](int c, float (&o)[32]) {
-        float o1[32];
-        tc::tmem_ld32(t_o0 + c, o);
-        tc::tmem_ld32(t_o1 + c, o1);
+      // kRead columns of the row, both slots' shares.
+      auto read = [&](int c, float (&o)[kRead]) {
+        float o1[kRead];
+        load_both(t_o0 + c, t_o1 + c, o, o1);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < kRead; ++i)
           o[i] = (used[0] ? o[i] * f0 : 0.f) + (used[1] ? o1[i] * f1 : 0.f);
         if (odd) {
           // The infinite and NaN values of the nodes that the row sees, among
@@ -498,47 +540,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             const T* v = static_cast<const T*>(p.value_cache) + sg.b * p.c_sb +
                          (int64_t)(sg.length + i) * p.c_sp + sg.h * p.c_sh + c;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
+            for (int j = 0; j < kRead; ++j) {
               const float value = __bfloat162float(v[j]);
               if (!(fabsf(value) < INFINITY)) o[j] += value;
             }
           }
         }
       };
-      auto release = [&] {
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free[copy.at]);
-      };
-      if (whole) {
-        // All columns are read before the first is written, so that the
-        // accumulators are free as early as may be.
-        uint32_t w[D / 2];
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float o[32];
-          read(c, o);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            w[c / 2 + i] = a.mask == 0 ? 0u : tc::bf16x2(o[2 * i], o[2 * i + 1]);
+      for (int c = 0; c < D; c += kRead) {
+        float o[kRead];
+        read(c, o);
+        if (c == D - kRead) {
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_free[copy.at]);
         }
-        release();
-        if (live) {
+        if (!live) continue;
+        if (whole) {
+          uint32_t w[kRead / 2];
 #pragma unroll
-          for (int i = 0; i < D / 2; i += 4)
-            *reinterpret_cast<uint4*>(out + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-        }
-      } else {
+          for (int i = 0; i < kRead / 2; ++i)
+            w[i] = a.mask == 0 ? 0u : tc::bf16x2(o[2 * i], o[2 * i + 1]);
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float o[32];
-          read(c, o);
-          if (c == D - 32) release();
-          if (!live) continue;
-          float4* to = reinterpret_cast<float4*>(part + 2 * p.block_rows + r * D + c);
+          for (int i = 0; i < kRead / 2; i += 4)
+            *reinterpret_cast<uint4*>(out + c + 2 * i) =
+                make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < kRead; i += 4)
+            *reinterpret_cast<float4*>(part + Parts<D>::at(p, r, c + i)) =
+                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
       if (live && !whole) part[r] = m, part[p.block_rows + r] = l;
@@ -573,7 +605,7 @@ int launch(const TreeParams& p, cudaStream_t stream) {
   lay.slot_bytes = (p.q_block_bytes + 1023) / 1024 * 1024;
   lay.slots = lay.slot_bytes <= 40 * 1024 ? 2 : 1;
   lay.tile_bytes = kTile * D * 2;
-  // At least nine tiles' room: half of it, or the lesser part, for the keys.
+  // At least eight tiles' room: half of it, or the lesser part, for the keys.
   const int room = (kBudget - rest_bytes(p.batch) - lay.keys()) / lay.tile_bytes;
   lay.pairs = (room + 1) / 4;
   lay.tiles = std::min(room - 2 * lay.pairs, kMaxUnits);

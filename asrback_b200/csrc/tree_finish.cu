@@ -5,8 +5,8 @@
 // A kernel of its own, so that the attention's CTAs end without waiting for one
 // another's parts and the merges run on the whole GPU at once. It moves the parts
 // once, 4 bytes per score and 8 per weight, but latency bounds it: a CTA has one
-// item, and each of its steps (the item's place in the tile list, the references
-// and sums over the parts, the outputs or the scores) loads all it needs at once.
+// item, finds its place in the tile list while the attention still runs, and then
+// loads all it needs (references, sums and outputs of the parts, scores) at once.
 #include "capi_internal.h"
 #include "tree_attention.cuh"
 
@@ -26,7 +26,29 @@ struct Shared {
   float part_m[kThreads], part_l[kThreads];  // [group of parts][row]
   float row_m[kMaxRows], row_l[kMaxRows];    // the rows' references and sums
   unsigned long long masks[kMaxRows];
+  int tiles[2][kThreads / 32];  // warps' shares: of the rows before the CTA's, of all
 };
+
+// The item's place in the list of all items' tiles.
+__device__ __forceinline__ Sharers find_place(const TreeParams& p, int b, int index, int tiles,
+                                              Shared& s) {
+  const int tid = threadIdx.x, per_row = p.kv_heads * p.mblocks;
+  int before = 0, all = 0;
+  for (int row = tid; row < p.batch; row += kThreads) {
+    const RowSpan span = row_span(p, row);
+    const int n = row_tiles(span.length + span.count) * per_row;
+    all += n;
+    before += row < b ? n : 0;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  all = __reduce_add_sync(0xffffffffu, all);
+  if (tid % 32 == 0) s.tiles[0][tid / 32] = before, s.tiles[1][tid / 32] = all;
+  __syncthreads();
+  before = all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) before += s.tiles[0][w], all += s.tiles[1][w];
+  return Sharers(before + index * tiles, tiles, max(1, (all + p.ctas - 1) / p.ctas));
+}
 
 // References and sums of the item's rows row0.. over its parts: a thread per row
 // and group of parts.
@@ -90,8 +112,14 @@ __global__ void __launch_bounds__(kThreads)
   const bool weighs = static_cast<int>(blockIdx.x) >= mergers;
   const int row0 = weighs ? 0 : blockIdx.x * kRows, rows = block - row0;
   const int j = (static_cast<int>(blockIdx.x) - mergers) * kKeysPer + 4 * tid;
+  // The lengths and counts are older than the call's first kernel, behind which
+  // all of its kernels begin.
+  const RowSpan span = row_span(p, b);
+  const int n = span.length + span.count, tiles = row_tiles(n);
+  const Sharers by = find_place(p, b, index, tiles, s);
   griddep_wait();
   griddep_launch_dependents();
+  if (rows <= 0 || (by.count == 1 && !weighs)) return;
   // The scores of the first rows, wherever the row ends: they wait for nothing.
   constexpr int kEarly = 8;
   const float* scores = p.scores + ((int64_t)b * p.kv_heads + h) * p.rows * p.score_stride + j;
@@ -101,63 +129,62 @@ __global__ void __launch_bounds__(kThreads)
     for (int r = 0; r < kEarly; ++r)
       if (r < rows) early[r] = *reinterpret_cast<const float4*>(scores + r * p.score_stride);
   }
-  const int before = b > 0 ? p.place[b - 1] : 0, upto = p.place[b], per = p.place[p.batch];
-  const int length = static_cast<int>(p.lengths[b]), count = p.counts[b];
   const auto* of_rows = reinterpret_cast<const unsigned long long*>(
       p.q_blocks + (int64_t)(item + 1) * p.q_block_bytes - kMaxNodes) - p.block_rows + row0;
   if (tid < min(rows, kMaxRows)) s.masks[tid] = of_rows[tid];
-  const int tiles = (upto - before) / (p.kv_heads * p.mblocks);
-  const Sharers by(before + index * tiles, tiles, per);
-  if (rows <= 0 || (by.count == 1 && !weighs)) return;
   if (!weighs) {
-    join_sums<D, kRows>(p, by, row0, rows, s);
-    // Outputs: a thread has pieces of four elements.
-    constexpr int kPieces = D / 4, kMine = kRows * kPieces / kThreads, kDeep = 8 / kMine;
+    // Outputs: a thread has pieces of four elements, neighbours those of the rows.
+    constexpr int kMine = kRows * D / 4 / kThreads, kDeep = 8 / kMine;
     float4 o[kMine];
-    int piece[kMine];  // within the CTA's rows
+    const int r = tid % kRows, safe_r = min(r, rows - 1);
+    int e[kMine];  // first column
 #pragma unroll
     for (int u = 0; u < kMine; ++u) {
       o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      piece[u] = min(tid + u * kThreads, min(rows, kRows) * kPieces - 1);
+      e[u] = (tid + u * kThreads) / kRows * 4;
     }
-    for (int c0 = 0; c0 < by.count; c0 += kDeep) {
-      float m[kDeep][kMine];
-      float4 v[kDeep][kMine];
+    float m[kDeep];
+    float4 v[kDeep][kMine];
+    auto load = [&](int c0) {
 #pragma unroll
       for (int i = 0; i < kDeep; ++i) {
-        const float* x = Parts<D>::of(p, by, min(c0 + i, by.count - 1)) + row0;
-        const float4* y =
-            reinterpret_cast<const float4*>(x + 2 * p.block_rows + row0 * (D - 1));
+        const float* x = Parts<D>::of(p, by, min(c0 + i, by.count - 1));
+        m[i] = x[row0 + safe_r];
 #pragma unroll
-        for (int u = 0; u < kMine; ++u) m[i][u] = x[piece[u] / kPieces], v[i][u] = y[piece[u]];
+        for (int u = 0; u < kMine; ++u)
+          v[i][u] =
+              *reinterpret_cast<const float4*>(x + Parts<D>::at(p, row0 + safe_r, e[u]));
       }
+    };
+    load(0);
+    join_sums<D, kRows>(p, by, row0, rows, s);
+    const float ref = s.row_m[safe_r];
+    for (int c0 = 0; c0 < by.count; c0 += kDeep) {
+      if (c0 > 0) load(c0);
 #pragma unroll
       for (int i = 0; i < kDeep; ++i) {
+        const float f = c0 + i < by.count ? fast_exp2(m[i] - ref) : 0.f;
 #pragma unroll
         for (int u = 0; u < kMine; ++u) {
-          const float f =
-              c0 + i < by.count ? fast_exp2(m[i][u] - s.row_m[piece[u] / kPieces]) : 0.f;
           o[u].x = fmaf(v[i][u].x, f, o[u].x), o[u].y = fmaf(v[i][u].y, f, o[u].y);
           o[u].z = fmaf(v[i][u].z, f, o[u].z), o[u].w = fmaf(v[i][u].w, f, o[u].w);
         }
       }
     }
+    if (r < rows) {
+      T* out = out_row<T>(p, b, h, mblock * p.block_rows + row0 + r);
 #pragma unroll
-    for (int u = 0; u < kMine; ++u) {
-      const int r = (tid + u * kThreads) / kPieces, e = piece[u] % kPieces * 4;
-      if (r < min(rows, kRows))
-        write_four<T>(out_row<T>(p, b, h, mblock * p.block_rows + row0 + r) + e, s.masks[r] == 0,
-                      s.row_l[r], o[u]);
+      for (int u = 0; u < kMine; ++u)
+        write_four<T>(out + e[u], s.masks[r] == 0, s.row_l[r], o[u]);
     }
     return;
   }
   join_sums<D, kMaxRows>(p, by, 0, rows, s);
   // A skipped row's nodes have masks of zero: no row of it has weights.
-  const int n = length + count;
   float* w = p.weights + b * p.w_sb + h * p.w_sh + j;
   float old[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int u = 0; u < 4; ++u) old[u] = j + u < min(length, p.cache_length) ? w[u] : 0.f;
+  for (int u = 0; u < 4; ++u) old[u] = j + u < span.length ? w[u] : 0.f;
   if (tid < rows) {
     const float lse = by.count > 1 ? s.row_m[tid] + log2f(s.row_l[tid])
                                    : p.lse[((int64_t)b * p.kv_heads + h) * p.rows + tid];
