@@ -543,7 +543,8 @@ def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
     with _on(device):
         ancestors = torch.empty((batch, nodes), dtype=torch.int64, device=device)
         depths = torch.empty((batch, nodes), dtype=torch.int32, device=device)
-        live = torch.empty(batch, dtype=torch.int32, device=device)
+        live = torch.empty(batch, dtype=torch.int32, device=device) if counts is None \
+            else torch.empty_like(counts)
         _native.call("asrback_draft_tree", batch, nodes, parents.data_ptr(), parents.stride(0),
                      None if counts is None else counts.data_ptr(), ancestors.data_ptr(),
                      depths.data_ptr(), live.data_ptr(), _state(device).status.data_ptr(),

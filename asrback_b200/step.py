@@ -24,6 +24,7 @@ the drafts were right, and :func:`greedy_tree_step` does the nodes' logits too.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from collections.abc import Sequence
 from typing import NamedTuple
@@ -161,6 +162,11 @@ class AcceptedPath(NamedTuple):
     start: Tensor
 
 
+@functools.lru_cache(maxsize=64)
+def _eos_array(eos_ids: tuple):
+    return (ctypes.c_int64 * len(eos_ids))(*map(int, eos_ids))
+
+
 def _node_rows(t: Tensor, name: str, dtype: torch.dtype, shape: tuple, device) -> tuple:
     """The tensor (which keeps its memory alive) and its row stride."""
     if t.dtype is not dtype or t.shape != shape or t.device != device:
@@ -213,12 +219,10 @@ def accept_tree(tree: attention.DraftTree, drafts: Tensor, chosen: Tensor, logpr
     for t in (counts, tokens, position, end, finished, sums, generated, lengths):
         if t is not None and t.device != device:
             raise ValueError("asrback_b200: the decode state must be on the tree's device")
-    eos = [int(e) for e in eos_ids]
-    eos_host = (ctypes.c_int64 * max(len(eos), 1))(*eos)
+    eos_host = _eos_array(tuple(eos_ids))
     with attention._on(device):
         path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
-        accepted = torch.empty(batch, dtype=torch.int32, device=device)
-        start = torch.empty(batch, dtype=torch.int64, device=device)
+        accepted, start = torch.empty_like(counts), torch.empty_like(position)
         columns = generated.shape[1]
         _native.call(
             "asrback_accept_tree", batch, nodes, parents.data_ptr(), parents_stride,
@@ -227,7 +231,7 @@ def accept_tree(tree: attention.DraftTree, drafts: Tensor, chosen: Tensor, logpr
             tokens.data_ptr(), tokens.stride(0) if batch > 1 else 1, position.data_ptr(),
             end.data_ptr(), finished.data_ptr(), sums.data_ptr(), generated.data_ptr(),
             generated.stride(0) if batch > 1 else columns, columns,
-            None if lengths is None else lengths.data_ptr(), eos_host, len(eos),
+            None if lengths is None else lengths.data_ptr(), eos_host, len(eos_host),
             path.data_ptr(), accepted.data_ptr(), start.data_ptr(),
             attention._state(device).status.data_ptr(), attention._stream(device))
     return AcceptedPath(path, accepted, start)
