@@ -36,10 +36,6 @@ constexpr int kWarps = 4;  // that compute
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr float kMoveThreshold = 8.0f;
 constexpr int kMaxUnits = 16;
-#ifndef TREE_AHEAD
-#define TREE_AHEAD 4
-#endif
-constexpr int kAhead = TREE_AHEAD;  // tiles that the L2 fetches ahead of the ring
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"

@@ -6,11 +6,12 @@
 // in tiles of 64. The call is bound by streaming the cache, so the TMA warps run
 // ahead of everything through the CTA's whole stretch, across items. A segment's
 // tiles are taken in pairs, whose scores are one product of 128 columns (in
-// shared memory one of 64 reads the queries as long, for half the result); each
-// tile of a pair has a slot, with its own probabilities, output accumulator and
-// softmax state. Scores are a pair ahead, so that the softmax of one runs beside
-// the products of its neighbours; the two states of an item are merged when it
-// ends, by warps of their own, while the next item is under way. Roles:
+// shared memory one of 64 reads the queries as long, for half the result); the
+// softmax of each tile of a pair has warps of its own, which share the rows'
+// references. The scores of the next pair are computed as soon as a pair's are
+// in registers, beside its softmax and the products with the values of the pair
+// before; an item's end is read by warps of its own, from one of two output
+// accumulators, while the next item is under way. Roles:
 //   warp 0      TMA: a segment's query block, the pairs' keys;
 //   warp 2      TMA: the tiles' values. (Two warps, since one issues tiles more
 //               slowly than they arrive.) A full pair or tile is one copy, of
@@ -18,15 +19,15 @@
 //   warp 1      TMEM allocation, S = Q K^T. A rotated query is two bf16 parts
 //               (their sum has 2^-17 of rounding), whose products are added up
 //               in S;
-//   warp 3      O_x (+)= P_x V, and of the values behind the cached keys: zeros
+//   warp 3      O (+)= P V, and of the values behind the cached keys: zeros
 //               behind the last node, nothing infinite or NaN. (Two warps issue
 //               MMAs, since the waits and descriptors of a tile take one of them
 //               longer than the tile's share of the stream.)
-//   warps 4-7   softmax of slot 0, warps 8-11 of slot 1: thread = TMEM lane =
-//               query row; only the warps that hold rows run. A row's reference
-//               moves, and its O is rescaled, only when a score passes it by
-//               more than 8 (base 2);
-//   warps 12-15 an item's end: merge of the slots, output or part.
+//   warps 4-7   softmax of a pair's first tile, warps 8-11 of its second: thread =
+//               TMEM lane = query row; only the warps that hold rows run. A row's
+//               reference moves, and its O is rescaled, only when a score passes
+//               it by more than 8 (base 2);
+//   warps 12-15 an item's end: output or part.
 #include <algorithm>
 
 #include "tree_tma.cuh"
@@ -40,21 +41,13 @@ constexpr int kThreads = 512;
 constexpr int kPair = 2 * kTile;  // keys whose scores are one product
 constexpr int kMaxUnits = 16;     // pairs of keys, and tiles of values, in their rings
 constexpr float kMoveThreshold = 8.0f;
-// TMEM: two S buffers of a pair (a tile's P over the first half of its S); then
-// the slots' O, for head_dim 64 twice, so that a segment's products begin while
-// the last one's output is read.
+// TMEM: a pair's S, two buffers of a pair's P, two O, so that a segment's products
+// begin while the last one's output is read.
 constexpr int kTmemCols = 512;
-constexpr int kScores = 2;
-template <int D>
-struct Outputs {
-  static constexpr int kCopies = D == 64 ? 2 : 1;
-  // Column of slot x's O in a segment whose number is n modulo kCopies.
-  __device__ __forceinline__ static uint32_t at(uint32_t n, uint32_t x) {
-    return kScores * kPair + D * (2 * n + x);
-  }
-};
+constexpr int kColP = kPair;
+constexpr int kColO = kColP + kPair;
 
-// What a softmax warp hands to the item's end, per slot and row.
+// What a softmax warp hands to the item's end, per tile of the pairs and row.
 struct RowState {
   float m, l;
   unsigned long long mask;
@@ -70,12 +63,13 @@ struct Layout {
   __host__ __device__ int rest() const { return values() + tiles * tile_bytes; }
 };
 
-constexpr int kOffStates = 0;                                // [slot][128] RowState
-constexpr int kOffBars = kOffStates + 2 * 128 * 16;
+constexpr int kOffStates = 0;                                // [tile of a pair][128] RowState
+constexpr int kOffTops = kOffStates + 2 * 128 * 16;          // [tile of a pair][128] float
+constexpr int kOffBars = kOffTops + 2 * 128 * 4;
 // full, empty per unit of keys and of values; q_full, q_empty per block; s_full,
-// s_free per S buffer; p_full per buffer and slot; o_done, state_full,
-// state_empty per slot; o_final, o_free per copy
-constexpr int kNumBars = 4 * kMaxUnits + 4 + 8 + 6 + 4;
+// s_free; p_full per P buffer and tile; p_free per P buffer; state_full,
+// state_empty per tile of a pair; o_final, o_free per O
+constexpr int kNumBars = 4 * kMaxUnits + 4 + 2 + 4 + 2 + 4 + 4;
 constexpr int kOffInts = kOffBars + kNumBars * 8;            // scratch[16], odd_segment, tmem
 constexpr int kOffList = (kOffInts + 20 * 4 + 15) / 16 * 16;
 constexpr int kRead = 32;  // output columns that an item's end reads at a time
@@ -92,32 +86,36 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return a;
 }
 
-// kRead columns of two places of this thread's TMEM lane, waited for once: a load
-// of a few columns takes as long as one of many.
-__device__ __forceinline__ void load_both(uint32_t t0, uint32_t t1, float* v0, float* v1) {
-  uint32_t x[kRead], y[kRead];
+// Eight columns of this thread's TMEM lane, multiplied by `a`.
+__device__ __forceinline__ void scale8(uint32_t at, float a) {
+  float v[8];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-      "%28, %29, %30, %31}, [%64];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, "
-      "%41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, "
-      "%58, %59, %60, %61, %62, %63}, [%65];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]),
-        "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]),
-        "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
-        "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]),
-        "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31]), "=r"(y[0]), "=r"(y[1]), "=r"(y[2]),
-        "=r"(y[3]), "=r"(y[4]), "=r"(y[5]), "=r"(y[6]), "=r"(y[7]), "=r"(y[8]), "=r"(y[9]),
-        "=r"(y[10]), "=r"(y[11]), "=r"(y[12]), "=r"(y[13]), "=r"(y[14]), "=r"(y[15]), "=r"(y[16]),
-        "=r"(y[17]), "=r"(y[18]), "=r"(y[19]), "=r"(y[20]), "=r"(y[21]), "=r"(y[22]), "=r"(y[23]),
-        "=r"(y[24]), "=r"(y[25]), "=r"(y[26]), "=r"(y[27]), "=r"(y[28]), "=r"(y[29]), "=r"(y[30]),
-        "=r"(y[31])
-      : "r"(t0), "r"(t1)
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7])
+      : "r"(at)
       : "memory");
 #pragma unroll
-  for (int i = 0; i < kRead; ++i) v0[i] = __uint_as_float(x[i]), v1[i] = __uint_as_float(y[i]);
+  for (int i = 0; i < 8; ++i) v[i] *= a;
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+      : "memory");
+}
+
+// Whether a predicate holds in any of the 64 threads that meet at barrier `id`.
+__device__ __forceinline__ bool any_of_64(int id, bool x) {
+  int any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.s32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, 64, p;\n\t"
+      "selp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<int>(x)), "r"(id)
+      : "memory");
+  return any != 0;
 }
 
 template <int D, bool kSplit>
@@ -128,28 +126,28 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kUnitBytes = kTile * D * 2;
   constexpr int kHalves = D / 64;  // 128-byte column blocks
   constexpr int kParts = kSplit ? 2 : 1;
-  constexpr int kCopies = Outputs<D>::kCopies;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* rest = smem + lay.rest();
   RowState* states = reinterpret_cast<RowState*>(rest + kOffStates);
+  float* tops = reinterpret_cast<float*>(rest + kOffTops);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(rest + kOffBars);  // [unit]
   uint64_t* k_empty = k_full + kMaxUnits;
   uint64_t* v_full = k_empty + kMaxUnits;
   uint64_t* v_empty = v_full + kMaxUnits;
   uint64_t* q_full = v_empty + kMaxUnits;  // [block buffer]
   uint64_t* q_empty = q_full + 2;
-  uint64_t* s_full = q_empty + 2;  // [S buffer] from here
-  uint64_t* s_free = s_full + kScores;
-  uint64_t* p_full = s_free + kScores;      // [S buffer][slot]
-  uint64_t* o_done = p_full + 2 * kScores;  // [slot] from here
-  uint64_t* state_full = o_done + 2;
+  uint64_t* s_full = q_empty + 2;
+  uint64_t* s_free = s_full + 1;
+  uint64_t* p_full = s_free + 1;  // [P buffer][tile]
+  uint64_t* p_free = p_full + 4;  // [P buffer]: its products are done
+  uint64_t* state_full = p_free + 2;  // [tile of a pair] from here
   uint64_t* state_empty = state_full + 2;
-  uint64_t* o_final = state_empty + 2;  // [copy] from here
+  uint64_t* o_final = state_empty + 2;  // [O] from here
   uint64_t* o_free = o_final + 2;
   int* scratch = reinterpret_cast<int*>(rest + kOffInts);  // [16]
-  int* odd_segment = scratch + 16;  // [copy] the segment's nodes hold infinite or NaN values
+  int* odd_segment = scratch + 16;  // [O] the segment's nodes hold infinite or NaN values
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(odd_segment + 2);
   TileList list(rest + kOffList, p.batch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -168,19 +166,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[s], 1);
       // The MMA warps and the softmax warps.
       mbar_init(&q_empty[s], 2 + 2 * row_warps);
-      mbar_init(&o_done[s], 1);
+      mbar_init(&p_full[s], row_warps);
+      mbar_init(&p_full[2 + s], row_warps);
+      mbar_init(&p_free[s], 1);
       mbar_init(&state_full[s], row_warps);
       mbar_init(&state_empty[s], row_warps);
+      mbar_init(&o_final[s], 1);
+      mbar_init(&o_free[s], row_warps);
     }
-    for (int i = 0; i < kScores; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 1);
-      for (int x = 0; x < 2; ++x) mbar_init(&p_full[2 * i + x], row_warps);
-    }
-    for (int i = 0; i < kCopies; ++i) {
-      mbar_init(&o_final[i], 1);
-      mbar_init(&o_free[i], row_warps);
-    }
+    mbar_init(s_full, 1);
+    mbar_init(s_free, 2 * row_warps);
     fence_barrier_init();
   }
   if (warp == 1) tc::tmem_alloc(tmem_slot, kTmemCols);
@@ -194,6 +189,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Segment& sg = st.seg;
   auto wait = [](uint64_t* bar, int parity) {
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity & 1)) != 0;
+  };
+  // Between the softmax and the products, where a suspended waiter wakes late.
+  auto spin = [](uint64_t* bar, int parity) {
+    return __all_sync(0xffffffffu, mbar_spin_bounded(bar, parity & 1)) != 0;
   };
   auto tiles_of = [](const Segment& s) {
     return s.length + s.count > 0 ? s.tile1 - s.tile0 : 0;  // a skipped row has none
@@ -277,18 +276,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t q_desc = tc::sw128_desc(smem_addr(smem), 16, 1024);
     const uint64_t k_desc = tc::sw128_desc(smem_addr(smem + lay.keys()), 16, 1024);
     const uint32_t half_step = p.block_rows * 128 >> 4;
-    Turn unit, block, scores;
+    Turn unit, block;
+    int pair = 0;
     for (; ok && next_segment(p, list, st); block.next(lay.slots)) {
       const int tiles = tiles_of(sg), slot = block.at;
       ok = wait(&q_full[slot], block.lap);
       if (tiles == 0 && leader) mbar_arrive(&q_empty[slot]);
-      for (int i = 0; i < tiles && ok; i += 2, unit.next(lay.pairs), scores.next(kScores)) {
-        const int u = unit.at, s = scores.at;
+      for (int i = 0; i < tiles && ok; i += 2, unit.next(lay.pairs), ++pair) {
+        const int u = unit.at;
         ok = wait(&k_full[u], unit.lap);
-        if (scores.lap > 0) ok = ok && wait(&s_free[s], scores.lap - 1);
+        if (pair > 0) ok = ok && spin(s_free, pair - 1);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint32_t t_s = tmem + uniform(s) * kPair;
+        const uint32_t t_s = uniform(tmem);
         const uint64_t qd = q_desc + uniform(slot * lay.slot_bytes >> 4);
         const uint64_t kd = k_desc + uniform(u * (kPair * D * 2 >> 4));
         const uint32_t idesc = uniform(i + 1 < tiles ? tc::idesc_bf16(128, kPair, false)
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::mma_ss(t_s, qd + (part * kHalves + c) * half_step + 2 * k,
                            kd + c * (kPair * 128 >> 4) + 2 * k, idesc,
                            part > 0 || c > 0 || k > 0);
-          tc::mma_commit(&s_full[s]);
+          tc::mma_commit(s_full);
           tc::mma_commit(&k_empty[u]);
           if (i + 2 >= tiles) tc::mma_commit(&q_empty[slot]);
         }
@@ -315,8 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool leader = tc::elect_one();
     constexpr uint32_t kIdesc = tc::idesc_bf16(128, D, true);
     const uint64_t v_desc = tc::sw128_desc(smem_addr(smem + lay.values()), kTile * 128, 1024);
-    Turn unit, block, copy, scores;
-    for (; ok && next_segment(p, list, st); block.next(lay.slots), copy.next(kCopies)) {
+    Turn unit, block, out, buffer;
+    for (; ok && next_segment(p, list, st); block.next(lay.slots), out.next(2)) {
       const int tiles = tiles_of(sg), total = sg.length + sg.count;
       // The block ends with a flag per node: its value holds infinities or NaN.
       ok = wait(&q_full[block.at], block.lap);
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                       (lane + 32 < sg.count && flags[lane + 32])));
       if (lane == 0) mbar_arrive(&q_empty[block.at]);
       for (int i = 0; i < tiles && ok; ++i, unit.next(lay.tiles)) {
-        const int x = i & 1, u = unit.at, s = scores.at, key = (sg.tile0 + i) * kTile;
+        const int x = i & 1, u = unit.at, s = buffer.at, key = (sg.tile0 + i) * kTile;
         const bool last = i == tiles - 1;
         ok = wait(&v_full[u], unit.lap);
         if (!ok) break;
@@ -360,41 +360,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // The segment's first products overwrite an accumulator whose last
         // segment has been read.
-        if (i == 0 && copy.lap > 0) ok = wait(&o_free[copy.at], copy.lap - 1);
-        // A pair of one tile waits for its other slot too, which has seen the
-        // scores then: the buffer is not given on before.
-        ok = ok && wait(&p_full[2 * s + x], scores.lap);
-        if (last && x == 0) ok = ok && wait(&p_full[2 * s + 1], scores.lap);
+        if (i == 0 && out.lap > 0) ok = wait(&o_free[out.at], out.lap - 1);
+        ok = ok && spin(&p_full[2 * s + x], buffer.lap);
+        // The second tile's softmax takes its turn in a pair of one tile too.
+        if (last && x == 0) ok = ok && wait(&p_full[2 * s + 1], buffer.lap);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint32_t t_o = tmem + Outputs<D>::at(uniform(copy.at), uniform(x));
-        const uint32_t t_p = tmem + uniform(s) * kPair + uniform(x) * kTile;
+        const uint32_t t_o = tmem + kColO + uniform(out.at) * D;
+        const uint32_t t_p = tmem + kColP + uniform(2 * s + x) * (kTile / 2);
         const uint64_t vd = v_desc + uniform(u * (kUnitBytes >> 4));
         if (leader) {
           if (i == 0) {
-            odd_segment[copy.at] = odd;
+            odd_segment[out.at] = odd;
             __threadfence_block();
           }
 #pragma unroll
           for (int k = 0; k < kTile / 16; ++k)
             if (16 * k < total - key)
-              tc::mma_ts(t_o, t_p + 8 * k, vd + (k * 2048 >> 4), kIdesc, i > 1 || k > 0);
-          tc::mma_commit(&o_done[x]);
-          if (last) tc::mma_commit(&o_final[copy.at]);
-          // A pair's barriers go through a phase per pair, whether its second
-          // tile is there or not.
-          if (last && x == 0) tc::mma_commit(&o_done[1]);
-          if (last || x == 1) tc::mma_commit(&s_free[s]);
+              tc::mma_ts(t_o, t_p + 8 * k, vd + (k * 2048 >> 4), kIdesc, i > 0 || k > 0);
+          if (last) tc::mma_commit(&o_final[out.at]);
+          if (last || x == 1) tc::mma_commit(&p_free[s]);
           tc::mma_commit(&v_empty[u]);
         }
         __syncwarp();
-        if (last || x == 1) scores.next(kScores);
+        if (last || x == 1) buffer.next(2);
       }
       // A segment without tiles takes its turn all the same: two phases of a
       // barrier in a row would look alike.
       if (tiles == 0) {
-        if (copy.lap > 0) ok = ok && wait(&o_free[copy.at], copy.lap - 1);
-        if (leader) mbar_arrive(&o_final[copy.at]);
+        if (out.lap > 0) ok = ok && wait(&o_free[out.at], out.lap - 1);
+        if (leader) mbar_arrive(&o_final[out.at]);
       }
     }
   } else if (warp >= 4 && warp < 12 && (warp & 3) < row_warps) {
@@ -402,10 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x = (warp >> 2) - 1, quarter = warp & 3;
     const int r = 32 * quarter + lane;  // this thread's row of the block
     const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
-    Turn block, copy, scores;
-    int done = 0;  // pairs of the segments before
-    for (int n = 0; next_segment(p, list, st); ++n, block.next(lay.slots), copy.next(kCopies)) {
-      const uint32_t t_o = tmem + lanes + Outputs<D>::at(copy.at, x);
+    Turn block, out, buffer;
+    int pair = 0;
+    for (int n = 0; next_segment(p, list, st); ++n, block.next(lay.slots), out.next(2)) {
       const int slot = block.at;
       if (ok) ok = wait(&q_full[slot], block.lap);
       const unsigned long long mask =
@@ -414,123 +408,133 @@ __global__ void __launch_bounds__(kThreads, 1)
              : 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[slot]);
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f;  // m: the same for both tiles of a pair
       const int tiles = tiles_of(sg);
-      for (int i = x; i < tiles + x && ok; i += 2, ++done, scores.next(kScores)) {
-        const int tile = sg.tile0 + i, buffer = scores.at;
-        const uint32_t t_s = tmem + lanes + buffer * kPair + x * kTile;
-        ok = wait(&s_full[buffer], scores.lap);
-        if (!ok) break;
-        if (i >= tiles) {  // a pair of one tile
-          if (lane == 0) mbar_arrive(&p_full[2 * buffer + 1]);
-          continue;
-        }
-        tc::tc_fence_after();
+      // A wait that gives up ends the work, but not the turns at the barriers that
+      // the two tiles' warps share.
+      for (int i = 0; i < tiles; i += 2, ++pair, buffer.next(2)) {
+        if (ok) ok = spin(s_full, pair);
+        // The second tile of a pair of one takes part in all but the work.
+        const bool here = ok && i + x < tiles;
         float s[kTile];
-        tc::tmem_ld64(t_s, s);
-        if constexpr (!kSplit) {
-#pragma unroll
-          for (int i = 0; i < kTile; ++i) s[i] *= p.scale_log2;
+        float highest = -INFINITY;
+        if (here) {
+          tc::tc_fence_after();
+          tc::tmem_ld64(tmem + lanes + x * kTile, s);
+          tc::tc_fence_before();
         }
-        const int cached = sg.length - tile * kTile;  // columns before the nodes
-        if (cached < kTile) {
-          // Behind the cached keys lie the nodes, behind them nothing (a mask
-          // has no bits there).
-          const unsigned long long older = cached > 0 ? (1ull << cached) - 1 : 0;
-          const unsigned long long seen = older | (cached >= 0 ? mask << cached : mask >> -cached);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+        if (here) {
+          if constexpr (!kSplit) {
 #pragma unroll
-          for (int i = 0; i < kTile; ++i)
-            if ((seen >> i & 1) == 0) s[i] = -INFINITY;
-        }
-        float top[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top[i] = fmaxf(s[i], s[i + 4]);
-#pragma unroll
-        for (int i = 8; i < kTile; i += 8)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top[j] = fmax3(top[j], s[i + j], s[i + j + 4]);
-        const float highest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        const bool moves = highest > m + kMoveThreshold;
-        if (__any_sync(0xffffffffu, moves)) {
-          const float now = moves ? highest : m;
-          if (i > 1) {
-            // The slot's O of this segment has to be at rest.
-            ok = wait(&o_done[x], done - 1);
-            if (!ok) break;
-            tc::tc_fence_after();
-            const float a = moves ? fast_exp2(m - now) : 1.f;
-#pragma unroll
-            for (int c = 0; c < D; c += 16) {
-              float o[16];
-              tc::tmem_ld16(t_o + c, o);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] *= a;
-              tc::tmem_st16f(t_o + c, o);
-            }
-            tc::tmem_wait_st();
-            l *= a;
+            for (int j = 0; j < kTile; ++j) s[j] *= p.scale_log2;
           }
+          const int cached = sg.length - (sg.tile0 + i + x) * kTile;  // columns before the nodes
+          if (cached < kTile) {
+            // Behind the cached keys lie the nodes, behind them nothing (a mask
+            // has no bits there).
+            const unsigned long long older = cached > 0 ? (1ull << cached) - 1 : 0;
+            const unsigned long long seen =
+                older | (cached >= 0 ? mask << cached : mask >> -cached);
+#pragma unroll
+            for (int j = 0; j < kTile; ++j)
+              if ((seen >> j & 1) == 0) s[j] = -INFINITY;
+          }
+          float top[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top[j] = fmaxf(s[j], s[j + 4]);
+#pragma unroll
+          for (int j = 8; j < kTile; j += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top[k] = fmax3(top[k], s[j + k], s[j + k + 4]);
+          highest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        }
+        // Both tiles' warps of the rows agree on the references.
+        if (any_of_64(2 + quarter, highest > m + kMoveThreshold)) {
+          tops[128 * x + r] = highest;
+          any_of_64(2 + quarter, false);
+          const float top = fmaxf(highest, tops[128 * (1 - x) + r]);
+          const float now = top > m + kMoveThreshold ? top : m;
+          const float a = now == m ? 1.f : fast_exp2(m - now);
+          if (i > 0 && x == 0) {
+            // The segment's O has to be at rest: its last pair's products are done.
+            const Turn before = buffer.at ? Turn{0, buffer.lap} : Turn{1, buffer.lap - 1};
+            if (ok) ok = wait(&p_free[before.at], before.lap);
+            tc::tc_fence_after();
+            const uint32_t t_o = tmem + lanes + kColO + out.at * D;
+#pragma unroll
+            for (int c = 0; c < D; c += 8) scale8(t_o + c, a);
+            tc::tmem_wait_st();
+          }
+          l *= a;
           m = now;
         }
-        // Probabilities are rounded to bf16 for the second product (2^-8 at
-        // most, against an output in bf16 itself); their sum is not.
-        const float ref = m == -INFINITY ? 0.f : m;
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t packed[kTile / 2];
+        // The buffer's products of two pairs before are done.
+        if (buffer.lap > 0) ok = ok && spin(&p_free[buffer.at], buffer.lap - 1);
+        if (here) {
+          // Probabilities are rounded to bf16 for the second product (2^-8 at
+          // most, against an output in bf16 itself); their sum is not.
+          const float ref = m == -INFINITY ? 0.f : m;
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          const uint32_t t_p = tmem + lanes + kColP + (2 * buffer.at + x) * (kTile / 2);
 #pragma unroll
-        for (int i = 0; i < kTile; i += 2) {
-          float2 e = add2(make_float2(s[i], s[i + 1]), make_float2(-ref, -ref));
-          e = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
-          packed[i / 2] = tc::bf16x2(e.x, e.y);
+          for (int part = 0; part < kTile; part += 32) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float2 e = add2(make_float2(s[part + j], s[part + j + 1]), make_float2(-ref, -ref));
+              e = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+              sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
+              packed[j / 2] = tc::bf16x2(e.x, e.y);
+            }
+            tc::tmem_st16(t_p + part / 2, packed);
+          }
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          tc::tmem_wait_st();
+          tc::tc_fence_before();
         }
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        tc::tmem_st32u(t_s, packed);
-        tc::tmem_wait_st();
-        tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * buffer + x]);
+        if (lane == 0) mbar_arrive(&p_full[2 * buffer.at + x]);
       }
       if (n > 0 && ok) ok = wait(&state_empty[x], n - 1);
       states[128 * x + r] = RowState{m, l, mask};
       __syncwarp();
       if (lane == 0) mbar_arrive(&state_full[x]);
-      if (!ok) break;
     }
   } else if (warp >= 12 && (warp & 3) < row_warps) {
     // ---------------------------------------------------------- an item's end
     const int quarter = warp & 3, r = 32 * quarter + lane;
     const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
-    Turn copy;
-    for (int n = 0; next_segment(p, list, st); ++n, copy.next(kCopies)) {
-      const uint32_t t_o0 = tmem + lanes + Outputs<D>::at(copy.at, 0), t_o1 = t_o0 + D;
+    Turn from;
+    for (int n = 0; next_segment(p, list, st); ++n, from.next(2)) {
+      const uint32_t t_o = tmem + lanes + kColO + from.at * D;
       const int tiles = tiles_of(sg);
       const bool whole = sg.whole();
       const int row = sg.mblock * p.block_rows + r;
       float* part = Parts<D>::mine(p, st);
       ok = ok && wait(&state_full[0], n) && wait(&state_full[1], n);
       const RowState a = states[r], b = states[128 + r];
-      const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
-      const float fa = fast_exp2(a.m - ref), fb = fast_exp2(b.m - ref);
-      const float l = a.l * fa + b.l * fb;
+      const float m = a.m, l = a.l + b.l;
       __syncwarp();
       if (lane == 0) mbar_arrive(&state_empty[0]), mbar_arrive(&state_empty[1]);
-      ok = ok && wait(&o_final[copy.at], copy.lap);
-      // A slot without a tile of the segment holds another's output.
-      const bool used[2] = {tiles > 0, tiles > 1};
+      ok = ok && wait(&o_final[from.at], from.lap);
       tc::tc_fence_after();
-      const bool odd = tiles > 0 && odd_segment[copy.at] != 0;
+      const bool odd = tiles > 0 && odd_segment[from.at] != 0;
       const bool live = row < p.rows;
       const float f = whole ? 1.f / l : 1.f;
-      const float f0 = fa * f, f1 = fb * f;
       T* out = out_row<T>(p, sg.b, sg.h, live ? row : 0);
-      // kRead columns of the row, both slots' shares.
-      auto read = [&](int c, float (&o)[kRead]) {
-        float o1[kRead];
-        load_both(t_o0 + c, t_o1 + c, o, o1);
 #pragma unroll
-        for (int i = 0; i < kRead; ++i)
-          o[i] = (used[0] ? o[i] * f0 : 0.f) + (used[1] ? o1[i] * f1 : 0.f);
+      for (int c = 0; c < D; c += kRead) {
+        float o[kRead];
+        tc::tmem_ld32(t_o + c, o);
+        if (c == D - kRead) {
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_free[from.at]);
+        }
+#pragma unroll
+        for (int i = 0; i < kRead; ++i) o[i] = tiles > 0 ? o[i] * f : 0.f;
         if (odd) {
           // The infinite and NaN values of the nodes that the row sees, among
           // the segment's tiles.
@@ -545,16 +549,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!(fabsf(value) < INFINITY)) o[j] += value;
             }
           }
-        }
-      };
-#pragma unroll
-      for (int c = 0; c < D; c += kRead) {
-        float o[kRead];
-        read(c, o);
-        if (c == D - kRead) {
-          tc::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&o_free[copy.at]);
         }
         if (!live) continue;
         if (whole) {
