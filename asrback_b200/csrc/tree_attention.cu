@@ -222,9 +222,8 @@ int rows_per_block(int dtype, int rows) {
   return std::min((rows + 31) / 32 * 32, 128);
 }
 
-
 struct Plan {
-  int block_rows, mblocks, ctas;
+  int block_rows, mblocks, ctas, lead;
   int q_block_bytes;
   size_t q_bytes, part_bytes, lse_bytes, score_bytes;
   int64_t score_stride;
@@ -246,6 +245,15 @@ Plan plan_for(int dtype, int batch, int nodes, int heads, int kv_heads, int head
                      : plan.block_rows == 16 ? mma_ctas_per_sm(head_dim)
                                              : 1;
   plan.ctas = static_cast<int>(std::min<int64_t>(tiles, (int64_t)per_sm * sm_count()));
+  // What an item's query block, first scores and end cost a CTA, in tiles, where
+  // items are of few tiles. Measured, without and with: 64 rows x 16 nodes of up
+  // to 1024 keys (tcgen05) 54.5 and 51.6 us; 64 rows x 8 nodes of up to 448 keys, 20
+  // heads of 64 (mma.sync) 32.2 and 30.3 us, but 64 rows x 1 node, 8 heads of
+  // 128, whose tiles are twice the bytes, 46.2 and 47.2 us.
+  plan.lead = dtype == ASRBACK_F32      ? 0
+              : plan.block_rows > 16    ? 2
+              : head_dim == 64          ? 1
+                                        : 0;
   // float32, bf16 as it comes, or (rotary) two bf16 parts; masks and flags.
   const int row_bytes = head_dim * (dtype == ASRBACK_F32 || rotary ? 4 : 2) + 8;
   plan.q_block_bytes = plan.block_rows * row_bytes + kMaxNodes;
@@ -339,7 +347,7 @@ extern "C" int asrback_tree_attention(
                 kMaxWeightRows, rows);
   const Plan plan = plan_for(dtype, batch, nodes, heads, kv_heads, head_dim, cache_length, rotary,
                              weights != nullptr);
-  if ((int64_t)batch * kv_heads * plan.mblocks * ((cache_length + kTile - 1) / kTile) >
+  if ((int64_t)batch * kv_heads * plan.mblocks * ((cache_length + kTile - 1) / kTile + plan.lead) >
           (int64_t)1 << 30 ||
       kv_heads * plan.mblocks > 65535)
     return fail(ASRBACK_ERR_ARGUMENT, "too many key tiles or heads for one call");
@@ -366,6 +374,8 @@ extern "C" int asrback_tree_attention(
   p.batch = batch, p.nodes = nodes, p.kv_heads = kv_heads, p.group = heads / kv_heads;
   p.cache_length = cache_length, p.rows = rows;
   p.block_rows = plan.block_rows, p.mblocks = plan.mblocks;
+  p.lead = plan.lead;
+  p.lead = plan.lead;
   p.ctas = plan.ctas;
   uint8_t* at = static_cast<uint8_t*>(workspace);
   p.q_blocks = at;

@@ -32,6 +32,7 @@ struct TreeParams {
   int batch, nodes, kv_heads, group, cache_length;
   int rows, block_rows, mblocks;  // query rows per key/value head, in blocks
   int ctas;
+  int lead;  // what an item costs a CTA besides its tiles, in tiles
   // The prepared query rows, a block per item: [block rows][D] (bf16: laid out as
   // the products read it, in two parts if rotated), the rows' masks (8 bytes),
   // and kMaxNodes bytes, one per node: its value holds infinities or NaN.
@@ -88,26 +89,38 @@ struct Segment {
   int length, count;
   int tiles;         // of the item
   int tile0, tile1;  // this segment's
-  int begin;         // tile0 in the list of all tiles
+  int begin;         // unit of the list where the CTA began it
   __device__ __forceinline__ bool whole() const { return tile1 - tile0 == tiles; }
 };
 
-// A CTA's stretch [cur, hi) of the list of all items' tiles, `per` tiles each
-// from `lo` on: `cur` is tile `tile` of item (row, h, mblock).
+// The list of all items' units: `lead` for the item, then one per tile. Every
+// CTA takes `per` units.
+struct Split {
+  int lead, per;
+  // With few tiles per CTA their number alone counts.
+  __device__ __forceinline__ Split(const TreeParams& p, int tiles) {
+    lead = tiles > 4 * p.ctas ? p.lead : 0;
+    per = max(1, (tiles + lead * p.batch * p.kv_heads * p.mblocks + p.ctas - 1) / p.ctas);
+  }
+};
+
+// A CTA's stretch [cur, hi) of the units, from `lo` on: `cur` is unit `unit` of
+// item (row, h, mblock). A stretch that ends in an item's lead has none of it.
 struct Stretch {
-  int lo, hi, cur, per;
-  int row, h, mblock, tile;
+  int lo, hi, cur, lead;
+  int row, h, mblock, unit;
   Segment seg;
 };
 
-// The CTAs that hold parts of an item of `tiles` tiles from `start` on in the list.
+// The CTAs that hold tiles of an item whose units begin at `start` in the list.
 struct Sharers {
   int first, count;
-  bool begins;  // the item begins the first one's stretch
-  __device__ __forceinline__ Sharers(int start, int tiles, int per) {
-    first = start / per;
-    count = (start + tiles - 1) / per - first + 1;
-    begins = start == first * per;
+  bool begins;  // the item is the first one's first
+  __device__ __forceinline__ Sharers(const Split& split, int start, int tiles) {
+    const int at = start + split.lead;
+    first = at / split.per;
+    count = (at + tiles - 1) / split.per - first + 1;
+    begins = start <= first * split.per;
   }
 };
 
@@ -145,21 +158,25 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, const Tile
     __syncthreads();
   }
   Stretch st;
-  const int total = carry;
-  st.per = max(1, (total + p.ctas - 1) / p.ctas);
-  st.lo = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * st.per, (int64_t)total));
-  st.hi = min(st.lo + st.per, total);
+  const Split split(p, carry);
+  const int per_row = p.kv_heads * p.mblocks;
+  const int total = carry + split.lead * p.batch * per_row;
+  st.lead = split.lead;
+  st.lo = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * split.per, (int64_t)total));
+  st.hi = min(st.lo + split.per, total);
   st.cur = st.lo;
-  int low = 0, high = p.batch - 1;  // the first row whose prefix lies past lo
+  int low = 0, high = p.batch - 1;  // the first row whose units end past lo
   while (low < high) {
     const int mid = (low + high) >> 1;
-    if (list.prefix[mid] > st.lo) high = mid;
+    if (list.prefix[mid] + split.lead * (mid + 1) * per_row > st.lo) high = mid;
     else low = mid + 1;
   }
   st.row = low;
-  const int tiles = row_tiles(static_cast<int>((list.span[low] >> 7) + (list.span[low] & 127u)));
-  const int off = st.lo - (low > 0 ? list.prefix[low - 1] : 0), index = off / tiles;
-  st.tile = off - index * tiles;
+  const int units =
+      row_tiles(static_cast<int>((list.span[low] >> 7) + (list.span[low] & 127u))) + split.lead;
+  const int off = st.lo - (low > 0 ? list.prefix[low - 1] + split.lead * low * per_row : 0);
+  const int index = off / units;
+  st.unit = off - index * units;
   st.h = index / p.mblocks;
   st.mblock = index - st.h * p.mblocks;
   return st;
@@ -168,7 +185,9 @@ __device__ __forceinline__ Stretch begin_stretch(const TreeParams& p, const Tile
 // The next (part of an) item of the stretch; false at its end.
 __device__ __forceinline__ bool next_segment(const TreeParams& p, const TileList& list,
                                              Stretch& st) {
-  if (st.cur >= st.hi) return false;
+  // The end lies `last` tiles into the item.
+  const int last = st.unit + st.hi - st.cur - st.lead;
+  if (st.cur >= st.hi || last <= 0) return false;
   Segment& s = st.seg;
   s.b = st.row;
   s.h = st.h;
@@ -177,11 +196,11 @@ __device__ __forceinline__ bool next_segment(const TreeParams& p, const TileList
   s.length = static_cast<int>(list.span[s.b] >> 7);
   s.count = static_cast<int>(list.span[s.b] & 127u);
   s.tiles = row_tiles(s.length + s.count);
-  s.tile0 = st.tile;
+  s.tile0 = max(st.unit - st.lead, 0);
   s.begin = st.cur;
-  s.tile1 = min(s.tiles, s.tile0 + st.hi - st.cur);
-  st.cur += s.tile1 - s.tile0;
-  st.tile = 0;
+  s.tile1 = min(s.tiles, last);
+  st.cur += s.tile1 + st.lead - st.unit;
+  st.unit = 0;
   if (++st.mblock == p.mblocks) {
     st.mblock = 0;
     if (++st.h == p.kv_heads) {

@@ -47,7 +47,8 @@ __device__ __forceinline__ Sharers find_place(const TreeParams& p, int b, int in
   before = all = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) before += s.tiles[0][w], all += s.tiles[1][w];
-  return Sharers(before + index * tiles, tiles, max(1, (all + p.ctas - 1) / p.ctas));
+  const Split split(p, all);
+  return Sharers(split, before + split.lead * b * per_row + index * (tiles + split.lead), tiles);
 }
 
 // References and sums of the item's rows row0.. over its parts: a thread per row
