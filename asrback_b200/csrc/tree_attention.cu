@@ -44,7 +44,10 @@ constexpr int kThreads = 128;
 //
 // float32 products run on the FMA pipes: a thread takes one key of a tile and
 // half the block's rows for the scores, then one column and all rows (head_dim
-// 128) or half of them (64) for the output.
+// 128) or half of them (64) for the output. Few calls have more tiles than the
+// GPU takes at once, so a tile's chain of loads and products is what bounds
+// them: loads are issued eight at a time, and both products read the operand
+// that a warp shares four elements at a time.
 
 template <int D>
 struct SimtShape {
@@ -83,9 +86,10 @@ __global__ void __launch_bounds__(kThreads)
   float* os = reinterpret_cast<float*>(smem + Sh::kOffO);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  griddep_wait();
   griddep_launch_dependents();
+  // The lengths and counts are older than the preparation kernel.
   Stretch st = begin_stretch<kThreads>(p, list, scratch);
+  griddep_wait();
   while (next_segment(p, list, st)) {
     const Segment& sg = st.seg;
     const uint8_t* block = p.q_blocks + (int64_t)sg.item * p.q_block_bytes;
@@ -94,6 +98,13 @@ __global__ void __launch_bounds__(kThreads)
     if (tid < kRows)
       masks[tid] = __ldcg(reinterpret_cast<const unsigned long long*>(block + kRows * D * 4) + tid);
     if (tid < kRows) state_m[tid] = -INFINITY, state_l[tid] = 0.f;
+    // A node whose value holds infinities or NaN: a byte per node, as four words.
+    const uint32_t flags =
+        __ldcg(reinterpret_cast<const uint32_t*>(block + p.q_block_bytes - kMaxNodes) + lane % 16);
+    const bool odd = __any_sync(0xffffffffu, [&] {
+      const int live = sg.count - 4 * (lane % 16);  // of the word's nodes
+      return live > 0 && (live >= 4 ? flags : flags & ((1u << 8 * live) - 1)) != 0;
+    }());
     float o[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) o[i] = 0.f;
@@ -104,16 +115,25 @@ __global__ void __launch_bounds__(kThreads)
       const int first_key = tile * kTile, keys = min(kTile, total - first_key);
       const bool edge = first_key + kTile > sg.length;  // nodes in the tile
       __syncthreads();
-      for (int i = tid; i < kTile * D / 4; i += kThreads) {
-        const int row = i / (D / 4), e = i % (D / 4) * 4;
-        float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-        if (row < keys) {
-          const int64_t at = (int64_t)(first_key + row) * p.c_sp + e;
-          k = *reinterpret_cast<const float4*>(kbase + at);
-          v = *reinterpret_cast<const float4*>(vbase + at);
+      constexpr int kBatch = 4, kStep = kThreads / (D / 4);  // rows of a pass
+      const int e0 = tid % (D / 4) * 4;
+      for (int base = tid / (D / 4); base < kTile; base += kBatch * kStep) {
+        float4 k[kBatch], v[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int64_t at =
+              (int64_t)(first_key + min(base + u * kStep, keys - 1)) * p.c_sp + e0;
+          k[u] = *reinterpret_cast<const float4*>(kbase + at);
+          v[u] = *reinterpret_cast<const float4*>(vbase + at);
         }
-        *reinterpret_cast<float4*>(ks + row * kPitch + e) = k;
-        *reinterpret_cast<float4*>(vs + row * D + e) = v;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int row = base + u * kStep;
+          // Behind the last key: zeros, for the product with zero probabilities.
+          if (row >= keys) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          *reinterpret_cast<float4*>(ks + row * kPitch + e0) = k[u];
+          *reinterpret_cast<float4*>(vs + row * D + e0) = v[u];
+        }
       }
       __syncthreads();
       {
@@ -141,7 +161,7 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
       __syncthreads();
-      for (int r = warp; r < kRows; r += kThreads / 32) {
+      for (int r = warp; r < min(kRows, p.rows - sg.mblock * kRows); r += kThreads / 32) {
         const float x0 = ss[r * kTile + lane], x1 = ss[r * kTile + lane + 32];
         float top = fmaxf(x0, x1);
 #pragma unroll
@@ -165,14 +185,27 @@ __global__ void __launch_bounds__(kThreads)
       const int column = tid % D, row0 = tid / D * kMine;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) o[i] *= state_a[row0 + i];
-      for (int key = 0; key < keys; ++key) {
-        const float v = vs[key * D + column];
+      if (!(edge && odd)) {
+        for (int key = 0; key < keys; key += 4) {
+          float v[4];
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const float w = ss[(row0 + i) * kTile + key];
-          // An unseen node's value may be infinite or NaN: no product with zero.
+          for (int u = 0; u < 4; ++u) v[u] = vs[(key + u) * D + column];
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            const float4 w = *reinterpret_cast<const float4*>(ss + (row0 + i) * kTile + key);
+            o[i] = fmaf(w.x, v[0], fmaf(w.y, v[1], fmaf(w.z, v[2], fmaf(w.w, v[3], o[i]))));
+          }
+        }
+      } else {
+        // An infinite or NaN value must not reach the nodes that do not see it, as
+        // a product with zero would let it.
+        for (int key = 0; key < keys; ++key) {
+          const float v = vs[key * D + column];
           const int age = first_key + key - sg.length;
-          if (!edge || age < 0 || (masks[row0 + i] >> age & 1) != 0) o[i] = fmaf(w, v, o[i]);
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+            if (age < 0 || (masks[row0 + i] >> age & 1) != 0)
+              o[i] = fmaf(ss[(row0 + i) * kTile + key], v, o[i]);
         }
       }
     }

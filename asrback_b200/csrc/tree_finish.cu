@@ -222,11 +222,9 @@ int launch(const TreeParams& p, cudaStream_t stream) {
 
 template <int D>
 int launch(int dtype, const TreeParams& p, cudaStream_t stream) {
-  const bool few = p.block_rows <= kMaxRows;
-  if (dtype == ASRBACK_F32)
-    return few ? launch<D, float, 512 / D>(p, stream) : launch<D, float, kMaxRows>(p, stream);
-  return few ? launch<D, __nv_bfloat16, 512 / D>(p, stream)
-             : launch<D, __nv_bfloat16, kMaxRows>(p, stream);
+  if (dtype == ASRBACK_F32) return launch<D, float, 512 / D>(p, stream);
+  return p.block_rows <= kMaxRows ? launch<D, __nv_bfloat16, 512 / D>(p, stream)
+                                  : launch<D, __nv_bfloat16, kMaxRows>(p, stream);
 }
 
 }  // namespace
