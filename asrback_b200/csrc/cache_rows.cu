@@ -115,8 +115,21 @@ struct SelectParams {
   int64_t* new_lengths;
   int32_t* kept;  // (layers, batch, heads, budget)
   int batch, heads, length, budget, sink, recent;
+  int cluster;  // CTAs that share a row
   int32_t* status;
 };
+
+constexpr int kSelectThreads = 256;
+
+// What lies at `at` in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ int load_remote(const int* at, int rank) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];"
+               : "=r"(v)
+               : "r"(cluster_map(smem_addr(at), rank))
+               : "memory");
+  return v;
+}
 
 // Order-preserving key of a weight: larger weight, larger key. Zeros of both
 // signs are equal, NaN counts as -inf. The protected slots' key is above every
@@ -129,79 +142,90 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// One CTA per (layer, row, head) finds the `budget` largest keys. The
-// threshold (the budget-th largest key) is built digit by digit from the top:
-// the keys that share the digits so far are counted by their next one, and the
-// digit in which the budget-th lies is the threshold's. It ends early once the
-// keys down to that digit are exactly the budget. Keys equal to the threshold
+// A cluster of CTAs per (layer, row, head) finds the `budget` largest keys, each
+// CTA in a contiguous share of the slots. The threshold (the budget-th largest
+// key) is built digit by digit from the top: the keys that share the digits so
+// far are counted by their next one, every CTA adds up the cluster's counts, and
+// the digit in which the budget-th lies is the threshold's. It ends early once
+// the keys down to that digit are exactly the budget. Keys equal to the threshold
 // are taken from the lowest slot up. A thread holds V slots of a chunk in
-// registers, THREADS apart; a row of one chunk is read once. The kept weights
-// are compacted here, their slots go to `kept`.
-template <int THREADS, int V>
-__global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__ SelectParams p) {
-  constexpr int kChunk = THREADS * V;
-  constexpr int kWarps = THREADS / 32;
-  constexpr int kBits = THREADS > 256 ? 11 : 8;  // of a digit, the last one's up to that
-  constexpr int kBins = 1 << kBits, kMine = kBins / THREADS;
-  __shared__ int bins[kBins];
-  __shared__ int found[3];  // the digit, the keys above it, its own
+// registers, kSelectThreads apart; a share of one chunk is read once. The kept
+// weights are compacted here, their slots go to `kept`.
+//
+// The counting's instructions bound it, not the bytes (one SM took 18 us for a
+// row of 16384 keys), hence the clusters.
+template <int V, bool kCluster>
+__global__ void __launch_bounds__(kSelectThreads)
+    select_kernel(const __grid_constant__ SelectParams p) {
+  constexpr int kChunk = kSelectThreads * V, kWarps = kSelectThreads / 32;
+  constexpr int kBits = 8, kDigits = 32 / kBits, kBins = 1 << kBits;
+  static_assert(kBins == kSelectThreads, "a thread per bin");
+  __shared__ int bins[kDigits][kBins];
+  __shared__ int found[3];          // the digit, the keys above it, its own
   __shared__ int scan[V * kWarps];  // keys above | equal << 16 of each 32 slots, in slot order
   __shared__ int sums[kWarps];
+  __shared__ int share[2];  // of this CTA: keys above, equal
   griddep_wait();
   griddep_launch_dependents();
-  const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
+  const int cluster = kCluster ? p.cluster : 1;
+  const int h = blockIdx.x / cluster, rank = blockIdx.x - h * cluster;
+  const int b = blockIdx.y, layer = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t given = p.lengths[b];
-  const bool first = h == 0 && layer == 0 && tid == 0;
+  const bool first = h == 0 && layer == 0 && rank == 0 && tid == 0;
   int32_t* kept = p.kept + (((int64_t)layer * p.batch + b) * p.heads + h) * p.budget;
+  const int every = cluster * kSelectThreads, mine = rank * kSelectThreads + tid;
   if (given < 0 || given > p.length) {
     if (first) {
       p.new_lengths[b] = given;
       if (p.status) atomicOr(p.status, ASRBACK_STATUS_POSITION);
     }
-    for (int k = tid; k < p.budget; k += THREADS) kept[k] = -1;
+    for (int k = mine; k < p.budget; k += every) kept[k] = -1;
     return;
   }
   const int n = static_cast<int>(given);
   if (first) p.new_lengths[b] = min(n, p.budget);
   if (n <= p.budget) {
-    for (int k = tid; k < p.budget; k += THREADS) kept[k] = k < n ? k : -1;
+    for (int k = mine; k < p.budget; k += every) kept[k] = k < n ? k : -1;
     return;
   }
   float* row = p.weights + layer * p.w_layer + b * p.w_batch + h * p.w_head;
-  const int chunks = (n + kChunk - 1) / kChunk;
-  const int tail = n - p.recent;
+  const int chunks = (n + cluster * kChunk - 1) / (cluster * kChunk);
+  const int start = rank * chunks * kChunk, tail = n - p.recent;
   float raw[V];
   uint32_t key[V];
   // Slots past the row's end hold key 0, below every weight's.
   auto load = [&](int chunk) {
-    const int base = chunk * kChunk + tid;
+    const int base = start + chunk * kChunk + tid;
 #pragma unroll
-    for (int u = 0; u < V; ++u) raw[u] = row[min(base + u * THREADS, n - 1)];
+    for (int u = 0; u < V; ++u) raw[u] = row[min(base + u * kSelectThreads, n - 1)];
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-      const int j = base + u * THREADS;
+      const int j = base + u * kSelectThreads;
       key[u] = j >= n ? 0u : j < p.sink || j >= tail ? kProtected : weight_key(raw[u]);
     }
   };
+  auto barrier = [&] {
+    if constexpr (kCluster) cluster_sync();
+    else __syncthreads();
+  };
 #pragma unroll
-  for (int i = 0; i < kMine; ++i) bins[tid * kMine + i] = 0;
+  for (int d = 0; d < kDigits; ++d) bins[d][tid] = 0;
   load(0);
   __syncthreads();
   uint32_t threshold = 0;
   int ties = p.budget;  // kept keys that share the threshold's digits so far
   bool exact = false;
-  for (int high = 32; high > 0 && !exact; high -= kBits) {
-    // Bits [low, high) of the keys that share the threshold's above them.
-    const int low = max(high - kBits, 0);
-    const uint32_t mask = (1u << (high - low)) - 1;
+  for (int d = 0; d < kDigits && !exact; ++d) {
+    // Bits [low, low + kBits) of the keys that share the threshold's above them.
+    const int low = 32 - (d + 1) * kBits;
     for (int chunk = 0; chunk < chunks; ++chunk) {
       if (chunks > 1) load(chunk);
 #pragma unroll
       for (int u = 0; u < V; ++u) {
         const bool in =
-            key[u] != 0u && static_cast<uint64_t>(key[u] ^ threshold) >> high == 0;
-        const int bin = key[u] >> low & mask;
+            key[u] != 0u && static_cast<uint64_t>(key[u] ^ threshold) >> (low + kBits) == 0;
+        const int bin = key[u] >> low & (kBins - 1);
         // Many equal keys, as zeros are, count at once.
         const uint32_t ins = __ballot_sync(0xffffffffu, in);
         if (ins == 0) continue;
@@ -209,19 +233,19 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
         const int leaders = __shfl_sync(0xffffffffu, bin, leader);  // every lane takes part
         const bool same = in && bin == leaders;
         const uint32_t sames = __ballot_sync(0xffffffffu, same);
-        if (lane == leader) atomicAdd(&bins[bin], __popc(sames));
-        else if (in && !same) atomicAdd(&bins[bin], 1);
+        if (lane == leader) atomicAdd(&bins[d][bin], __popc(sames));
+        else if (in && !same) atomicAdd(&bins[d][bin], 1);
       }
     }
-    __syncthreads();
-    int own[kMine], mine = 0;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      own[i] = bins[kBins - 1 - tid * kMine - i];
-      bins[kBins - 1 - tid * kMine - i] = 0;
-      mine += own[i];
+    barrier();
+    const int mine_bin = kBins - 1 - tid;
+    int own = 0;
+    if constexpr (kCluster) {
+      for (int r = 0; r < cluster; ++r) own += load_remote(&bins[d][mine_bin], r);
+    } else {
+      own = bins[d][mine_bin];
     }
-    int through = mine;
+    int through = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, through, o);
@@ -229,29 +253,20 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
     }
     if (lane == 31) sums[warp] = through;
     __syncthreads();
-    int before = through - mine;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
-      if (w < warp) before += sums[w];
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      if (before < ties && ties <= before + own[i]) {
-        found[0] = kBins - 1 - tid * kMine - i;
-        found[1] = before;
-        found[2] = own[i];
-      }
-      before += own[i];
-    }
+      if (w < warp) through += sums[w];
+    if (through - own < ties && ties <= through)
+      found[0] = mine_bin, found[1] = through - own, found[2] = own;
     __syncthreads();
     threshold |= static_cast<uint32_t>(found[0]) << low;
     ties -= found[1];
     exact = ties == found[2];
   }
   if (exact) ties = n;  // whatever shares the digits found is kept
-  const uint32_t lower = (1u << lane) - 1;
-  int above_before = 0, equal_before = 0;  // of the chunks before this one
-  for (int chunk = 0; chunk < chunks; ++chunk) {
-    if (chunks > 1) load(chunk);
+  // Each 32 slots' keys above and equal, and what lies before them in the chunk;
+  // returns the chunk's.
+  auto count = [&] {
 #pragma unroll
     for (int u = 0; u < V; ++u) {
       const uint32_t above = __ballot_sync(0xffffffffu, key[u] > threshold);
@@ -259,9 +274,9 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
       if (lane == 0) scan[u * kWarps + warp] = __popc(above) | __popc(equal) << 16;
     }
     __syncthreads();  // all counts are there; the chunk's raw weights have been read
-    int mine = 0, through = 0;
+    int own = 0, through = 0;
     if (tid < V * kWarps) {
-      mine = through = scan[tid];
+      own = through = scan[tid];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, through, o);
@@ -276,8 +291,27 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
       if (w < warp) through += sums[w];
       all += sums[w];
     }
-    if (tid < V * kWarps) scan[tid] = through - mine;
+    if (tid < V * kWarps) scan[tid] = through - own;
     __syncthreads();
+    return all;
+  };
+  int above_before = 0, equal_before = 0;  // of the slots before the chunk
+  if constexpr (kCluster) {
+    int above = 0, equal = 0;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+      if (chunks > 1) load(chunk);
+      const int all = count();
+      above += all & 0xffff, equal += all >> 16;
+    }
+    if (tid == 0) share[0] = above, share[1] = equal;
+    barrier();
+    for (int r = 0; r < rank; ++r)
+      above_before += load_remote(&share[0], r), equal_before += load_remote(&share[1], r);
+  }
+  const uint32_t lower = (1u << lane) - 1;
+  for (int chunk = 0; chunk < chunks; ++chunk) {
+    if (chunks > 1) load(chunk);
+    const int all = kCluster && chunks == 1 ? 0 : count();
 #pragma unroll
     for (int u = 0; u < V; ++u) {
       const bool over = key[u] > threshold, same = key[u] == threshold;
@@ -288,14 +322,27 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
       const int equal_at = equal_before + (at >> 16) + __popc(equal & lower);
       if (over || (same && equal_at < ties)) {
         const int k = above_at + min(equal_at, ties);
-        kept[k] = chunk * kChunk + u * THREADS + tid;
-        row[k] = raw[u];
+        kept[k] = start + chunk * kChunk + u * kSelectThreads + tid;
+        // All CTAs have read the row, if it is of one chunk each.
+        if (chunks == 1) row[k] = raw[u];
       }
     }
     above_before += all & 0xffff;
     equal_before += all >> 16;
     __syncthreads();  // `scan` and `sums` have been read
   }
+  if (chunks > 1) {
+    // In turns from the front, whose loads come before their stores: what a turn
+    // writes lies before all that later turns read.
+    barrier();
+    for (int k0 = 0; k0 < p.budget; k0 += every) {
+      const int k = k0 + mine;
+      const float w = k < p.budget ? row[kept[k]] : 0.f;
+      barrier();
+      if (k < p.budget) row[k] = w;
+    }
+  }
+  if constexpr (kCluster) cluster_sync();  // the others have read this CTA's counts
 }
 
 // -------------------------------------------------------- eviction: the moves
@@ -488,14 +535,17 @@ extern "C" int asrback_evict(int dtype, int layers, int batch, int heads, int he
   s.recent = recent;
   s.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(heads, batch, layers);
   int rc;
-  if (length <= 1024)
-    rc = launch_pdl(select_kernel<256, 4>, grid, dim3(256), 0, st, "evict selection launch", s);
-  else if (length <= 4096)
-    rc = launch_pdl(select_kernel<1024, 4>, grid, dim3(1024), 0, st, "evict selection launch", s);
-  else
-    rc = launch_pdl(select_kernel<1024, 16>, grid, dim3(1024), 0, st, "evict selection launch", s);
+  if (length <= 4 * kSelectThreads) {
+    rc = launch_pdl(select_kernel<4, false>, dim3(heads, batch, layers), dim3(kSelectThreads), 0, st,
+                    "evict selection launch", s);
+  } else {
+    // As many CTAs as hold a row's slots in registers, up to 8.
+    s.cluster = 2;
+    while (s.cluster < 8 && s.cluster * 8 * kSelectThreads < length) s.cluster *= 2;
+    rc = launch_pdl_cluster(select_kernel<8, true>, dim3(heads * s.cluster, batch, layers),
+                            dim3(kSelectThreads), 0, s.cluster, st, "evict selection launch", s);
+  }
   if (rc) return rc;
   m.lengths = lengths;
   m.kept = kept;
