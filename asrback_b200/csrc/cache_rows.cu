@@ -417,15 +417,24 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
   }
 }
 
+// Rows of weights that are written: no two of them may be one.
+int check_weights(int layers, int batch, int heads, int length, int64_t layer, int64_t row,
+                  int64_t head) {
+  if ((layers > 1 && layer < length) || (batch > 1 && row < length) || (heads > 1 && head < length))
+    return fail(ASRBACK_ERR_ARGUMENT, "weights strides do not hold rows of the cache's length");
+  return ASRBACK_OK;
+}
+
 // Checks a cache's shape and fills `view` (strides in bytes); an ABI code.
-int cache_view(CacheView* view, const char* name, void* base, int64_t esize, int head_dim,
-               int64_t layer, int64_t batch, int64_t position, int64_t head) {
+int cache_view(CacheView* view, const char* name, void* base, int64_t esize, int layers, int rows,
+               int head_dim, int64_t layer, int64_t batch, int64_t position, int64_t head) {
   if (!base) return fail(ASRBACK_ERR_ARGUMENT, "null %s pointer", name);
   if (!aligned16(base) || (layer * esize) % 16 || (batch * esize) % 16 ||
       (position * esize) % 16 || (head * esize) % 16)
     return fail(ASRBACK_ERR_ARGUMENT,
                 "%s rows must start on 16-byte boundaries (pointer and strides)", name);
-  if (position < head_dim || head < head_dim || layer < 0 || batch < 0)
+  if (position < head_dim || head < head_dim || (layers > 1 && layer < head_dim) ||
+      (rows > 1 && batch < head_dim))
     return fail(ASRBACK_ERR_ARGUMENT, "%s strides do not hold rows of head_dim elements", name);
   *view = {static_cast<uint8_t*>(base), layer * esize, batch * esize, position * esize,
            head * esize};
@@ -463,13 +472,17 @@ extern "C" int asrback_commit_tree(int dtype, int layers, int batch, int nodes, 
                 layers);
   if (!path || !counts || !start)
     return fail(ASRBACK_ERR_ARGUMENT, "null path, counts or start pointer");
+  if (weights)
+    if (int rc = check_weights(layers, batch, heads, length, w_stride_layer, w_stride_batch,
+                               w_stride_head))
+      return rc;
   const int64_t esize = dtype == ASRBACK_BF16 ? 2 : 4;
   CommitParams p{};
-  if (int rc = cache_view(&p.cache[0], "key_cache", key_cache, esize, head_dim, c_stride_layer,
-                          c_stride_batch, c_stride_position, c_stride_head))
+  if (int rc = cache_view(&p.cache[0], "key_cache", key_cache, esize, layers, batch, head_dim,
+                          c_stride_layer, c_stride_batch, c_stride_position, c_stride_head))
     return rc;
-  if (int rc = cache_view(&p.cache[1], "value_cache", value_cache, esize, head_dim, c_stride_layer,
-                          c_stride_batch, c_stride_position, c_stride_head))
+  if (int rc = cache_view(&p.cache[1], "value_cache", value_cache, esize, layers, batch, head_dim,
+                          c_stride_layer, c_stride_batch, c_stride_position, c_stride_head))
     return rc;
   p.layers = layers;
   p.batch = batch;
@@ -511,13 +524,16 @@ extern "C" int asrback_evict(int dtype, int layers, int batch, int heads, int he
                 batch);
   if (!weights || !lengths || !new_lengths || !kept)
     return fail(ASRBACK_ERR_ARGUMENT, "null weights, lengths, new_lengths or kept pointer");
+  if (int rc = check_weights(layers, batch, heads, length, w_stride_layer, w_stride_batch,
+                             w_stride_head))
+    return rc;
   const int64_t esize = dtype == ASRBACK_BF16 ? 2 : 4;
   MoveParams m{};
-  if (int rc = cache_view(&m.cache[0], "key_cache", key_cache, esize, head_dim, c_stride_layer,
-                          c_stride_batch, c_stride_position, c_stride_head))
+  if (int rc = cache_view(&m.cache[0], "key_cache", key_cache, esize, layers, batch, head_dim,
+                          c_stride_layer, c_stride_batch, c_stride_position, c_stride_head))
     return rc;
-  if (int rc = cache_view(&m.cache[1], "value_cache", value_cache, esize, head_dim, c_stride_layer,
-                          c_stride_batch, c_stride_position, c_stride_head))
+  if (int rc = cache_view(&m.cache[1], "value_cache", value_cache, esize, layers, batch, head_dim,
+                          c_stride_layer, c_stride_batch, c_stride_position, c_stride_head))
     return rc;
   SelectParams s{};
   s.weights = weights;

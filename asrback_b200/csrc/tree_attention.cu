@@ -369,9 +369,14 @@ extern "C" int asrback_tree_attention(
                             k_norm_weight, cos, sin};
   for (const void* ptr : pointers)
     if (!aligned16(ptr)) return fail(ASRBACK_ERR_ARGUMENT, "pointers must be 16-byte aligned");
+  // The cache and the weights are written: no two of their rows may be one.
   if (c_stride_position < head_dim || (kv_heads > 1 && c_stride_head < head_dim) ||
+      (batch > 1 && c_stride_batch < head_dim) || (batch > 1 && o_stride_batch < head_dim) ||
       (heads > 1 && o_stride_head < head_dim) || (nodes > 1 && o_stride_node < head_dim))
     return fail(ASRBACK_ERR_ARGUMENT, "cache or output strides do not hold rows of head_dim");
+  if (weights && ((batch > 1 && w_stride_batch < cache_length) ||
+                  (kv_heads > 1 && w_stride_head < cache_length)))
+    return fail(ASRBACK_ERR_ARGUMENT, "weights strides do not hold rows of the cache's length");
   const int rows = nodes * (heads / kv_heads);
   if (weights && rows > kMaxWeightRows)
     return fail(ASRBACK_ERR_ARGUMENT,
@@ -407,7 +412,6 @@ extern "C" int asrback_tree_attention(
   p.batch = batch, p.nodes = nodes, p.kv_heads = kv_heads, p.group = heads / kv_heads;
   p.cache_length = cache_length, p.rows = rows;
   p.block_rows = plan.block_rows, p.mblocks = plan.mblocks;
-  p.lead = plan.lead;
   p.lead = plan.lead;
   p.ctas = plan.ctas;
   uint8_t* at = static_cast<uint8_t*>(workspace);

@@ -460,6 +460,51 @@ def test_evict(tag, heads_first, layers, heads, dim, length, budget, sink, recen
     assert attention.read_status() == 0
 
 
+@pytest.mark.parametrize("length,budget,sink,recent", [
+    (1025, 1000, 3, 9), (2049, 64, 0, 64), (4096, 2048, 0, 0), (4097, 4000, 100, 100),
+    (16384, 4096, 8, 1024), (16385, 1, 0, 0), (33000, 20000, 4, 0)])
+@pytest.mark.parametrize("distinct", [0, 2, 7])
+def test_evict_long_rows(length, budget, sink, recent, distinct):
+    """Rows that several CTAs share, some of them with slots of few distinct
+    weights, some that end in the first CTA's."""
+    rng = np.random.default_rng(length + distinct)
+    lengths = np.array([length, budget + 1, (length + budget) // 2, length - 1])
+    weights = rng.random((1, 4, 2, length)).astype(np.float32)
+    if distinct:
+        weights = np.floor(weights ** 3 * distinct).astype(np.float32)
+    keys = torch.arange(length, device=DEV, dtype=torch.float32)[None, :, None, None].expand(
+        4, length, 2, 64).contiguous()
+    values, w = -keys, torch.from_numpy(weights[0].copy()).to(DEV)
+    n, kept = cache.qwen3_evict(keys, values, w, _gpu(lengths, torch.int64), budget, sink, recent)
+    want = oracle.evict(weights, lengths, budget, sink, recent)[0]
+    np.testing.assert_array_equal(n.cpu(), budget)
+    np.testing.assert_array_equal(kept.cpu(), want)
+    np.testing.assert_array_equal(keys[:, :budget, :, 0].cpu(), want.transpose(0, 2, 1))
+    np.testing.assert_array_equal(values[:, :budget, :, 63].cpu(), -want.transpose(0, 2, 1))
+    np.testing.assert_array_equal(w[:, :, :budget].cpu(), np.take_along_axis(weights[0], want, -1))
+    np.testing.assert_array_equal(w[:, :, budget:].cpu(), weights[0, :, :, budget:])
+    assert attention.read_status() == 0
+
+
+@pytest.mark.parametrize("family,heads,kv_heads,dim,nodes", [
+    ("qwen3", 16, 8, 128, 4), ("qwen3", 16, 8, 128, 16), ("whisper", 4, 4, 64, 40)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_score_that_is_not_finite_stays_in_its_row(family, heads, kv_heads, dim, nodes, bad):
+    """A cached key that makes scores NaN or infinite (of either sign): only the
+    batch row's outputs of that head change, and a NaN is seen in all of them."""
+    x = _inputs(3, family, "bf16", 3, nodes, 400, heads, kv_heads, dim, [300, 300, 300])
+    good = _call(x)[0]
+    position = (1, 70, 1, 5) if family == "qwen3" else (1, 1, 70, 5)
+    x["keys"][position] = bad
+    out = _call(x)[0].view(3, nodes, heads, dim)
+    group = heads // kv_heads
+    if np.isnan(bad):
+        assert torch.isnan(out[1, :, group:2 * group]).all()
+    good = good.view(3, nodes, heads, dim)
+    for b, first, last in ((0, 0, heads), (2, 0, heads), (1, 0, group), (1, 2 * group, heads)):
+        assert torch.equal(out[b, :, first:last], good[b, :, first:last])
+
+
 def test_evict_skips_rows_out_of_range():
     keys, values = torch.randn((2, 3, 50, 2, 64), device=DEV)
     before, weights = keys.clone(), torch.rand((3, 2, 50), device=DEV)
