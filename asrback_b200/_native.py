@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -190,6 +191,14 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "asrback_selftest_bounded_wait": ([_c_i64, _c_p, _c_p], _c_int),
 }
 
+# Entry points that also take their arguments as one array of 64-bit words.
+_PACKED = {}
+for _name in ("asrback_draft_tree", "asrback_tree_attention", "asrback_accept_tree",
+              "asrback_commit_tree", "asrback_evict"):
+    _PACKED[_name] = struct.Struct("=" + "".join(
+        "d" if t is _c_f else "q" for t in SIGNATURES[_name][0])).pack
+    SIGNATURES[_name + "_packed"] = ([ctypes.c_char_p], _c_int)
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -235,7 +244,20 @@ def call(name: str, *args) -> None:
     lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != OK:
-        message = lib.asrback_last_error().decode(errors="replace")
-        kind = {ERR_ARGUMENT: "invalid argument", ERR_CUDA: "CUDA error",
-                ERR_WORKSPACE: "workspace too small"}.get(rc, f"error {rc}")
-        raise NativeError(f"{name}: {kind}: {message}")
+        _raise(lib, name, rc)
+
+
+def call_packed(name: str, *args) -> None:
+    """:func:`call` for an entry point of many arguments (null pointers as 0),
+    converted all at once."""
+    lib = _lib or load()
+    rc = getattr(lib, name + "_packed")(_PACKED[name](*args))
+    if rc != OK:
+        _raise(lib, name, rc)
+
+
+def _raise(lib: ctypes.CDLL, name: str, rc: int) -> None:
+    message = lib.asrback_last_error().decode(errors="replace")
+    kind = {ERR_ARGUMENT: "invalid argument", ERR_CUDA: "CUDA error",
+            ERR_WORKSPACE: "workspace too small"}.get(rc, f"error {rc}")
+    raise NativeError(f"{name}: {kind}: {message}")

@@ -32,6 +32,7 @@ that every key gathers (:mod:`asrback_b200.cache` evicts by it).
 
 from __future__ import annotations
 
+import functools
 import math
 import threading
 from contextlib import nullcontext
@@ -545,11 +546,17 @@ def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
         depths = torch.empty((batch, nodes), dtype=torch.int32, device=device)
         live = torch.empty(batch, dtype=torch.int32, device=device) if counts is None \
             else torch.empty_like(counts)
-        _native.call("asrback_draft_tree", batch, nodes, parents.data_ptr(), parents.stride(0),
-                     None if counts is None else counts.data_ptr(), ancestors.data_ptr(),
-                     depths.data_ptr(), live.data_ptr(), _state(device).status.data_ptr(),
-                     _stream(device))
+        _native.call_packed(
+            "asrback_draft_tree", batch, nodes, parents.data_ptr(), parents.stride(0),
+            0 if counts is None else counts.data_ptr(), ancestors.data_ptr(), depths.data_ptr(),
+            live.data_ptr(), _state(device).status.data_ptr(), _stream(device))
     return DraftTree(parents, live, ancestors, depths)
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_workspace(device: int, *sizes: int) -> int:
+    """The workspace's bytes on the current device, ``device``."""
+    return _native.load().asrback_tree_workspace_bytes(*sizes)
 
 
 def _tree_call(dtype: int, q: tuple, k: tuple, v: tuple, sizes: tuple, rotary: tuple | None,
@@ -567,7 +574,7 @@ def _tree_call(dtype: int, q: tuple, k: tuple, v: tuple, sizes: tuple, rotary: t
     if keys.device != device or values.device != device:
         raise ValueError("asrback_b200: tensors must be on one device")
     if weights is None:
-        w_ptr, w_batch, w_head = None, 0, 0
+        w_ptr, w_batch, w_head = 0, 0, 0
     else:
         if weights.dtype is not torch.float32 or weights.shape != (batch, kv_heads, length) \
                 or weights.device != device or (length > 1 and weights.stride(2) != 1):
@@ -575,7 +582,7 @@ def _tree_call(dtype: int, q: tuple, k: tuple, v: tuple, sizes: tuple, rotary: t
                              "with unit last stride, on the tensors' device")
         w_ptr, (w_batch, w_head, _) = weights.data_ptr(), weights.stride()
     if rotary is None:
-        qn = kn = cos = sin = positions = None
+        qn = kn = cos = sin = positions = 0
         eps, table_stride, table_length = 0.0, 0, 0
     else:
         qn, kn, eps, cos, sin, positions = rotary
@@ -594,16 +601,14 @@ def _tree_call(dtype: int, q: tuple, k: tuple, v: tuple, sizes: tuple, rotary: t
         if table_length == 1:
             table_stride = head_dim
     width = heads * head_dim
-    ws_bytes = _native.load().asrback_tree_workspace_bytes(
-        dtype, batch, nodes, heads, kv_heads, head_dim, length, rotary is not None,
-        weights is not None)
     with _on(device):
+        ws_bytes = _tree_workspace(torch._C._cuda_getDevice(), dtype, *sizes, rotary is not None,
+                                   weights is not None)
         out = torch.empty((batch, nodes, width), dtype=like.dtype, device=device)
         status = _state(device).status
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-        _native.call(
-            "asrback_tree_attention",
-            dtype, batch, nodes, heads, kv_heads, head_dim, length, *q, *k, *v,
+        _native.call_packed(
+            "asrback_tree_attention", dtype, *sizes, *q, *k, *v,
             qn, kn, eps, cos, sin, table_stride, table_length, positions,
             ancestors.data_ptr(), depths.data_ptr(), counts.data_ptr(), lengths.data_ptr(),
             keys.data_ptr(), values.data_ptr(), *strides,

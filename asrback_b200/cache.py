@@ -60,12 +60,13 @@ def _commit(keys: Tensor, values: Tensor, accepted: step.AcceptedPath, weights: 
     path = attention._int_rows(accepted.path, "path", torch.int32, (batch, nodes), device)
     counts = attention._int_rows(accepted.counts, "counts", torch.int32, (batch,), device)
     start = attention._int_rows(accepted.start, "start", torch.int64, (batch,), device)
-    w = (None, 0, 0, 0) if weights is None else _weights(weights, keys, sizes)
+    w = (0, 0, 0, 0) if weights is None else _weights(weights, keys, sizes)
     with attention._on(device):
-        _native.call("asrback_commit_tree", dtype, layers, batch, nodes, heads, head_dim, length,
-                     keys.data_ptr(), values.data_ptr(), *strides, *w, path.data_ptr(),
-                     counts.data_ptr(), start.data_ptr(),
-                     attention._state(device).status.data_ptr(), attention._stream(device))
+        _native.call_packed(
+            "asrback_commit_tree", dtype, layers, batch, nodes, heads, head_dim, length,
+            keys.data_ptr(), values.data_ptr(), *strides, *w, path.data_ptr(), counts.data_ptr(),
+            start.data_ptr(), attention._state(device).status.data_ptr(),
+            attention._stream(device))
 
 
 def _evict(keys: Tensor, values: Tensor, weights: Tensor, lengths: Tensor, budget: int, sink: int,
@@ -82,10 +83,11 @@ def _evict(keys: Tensor, values: Tensor, weights: Tensor, lengths: Tensor, budge
         new_lengths = torch.empty(batch, dtype=torch.int64, device=device)
         shape = (batch, heads, budget) if keys.dim() == 4 else (layers, batch, heads, budget)
         kept = torch.empty(shape, dtype=torch.int32, device=device)
-        _native.call("asrback_evict", dtype, layers, batch, heads, head_dim, length,
-                     keys.data_ptr(), values.data_ptr(), *strides, *w, lengths.data_ptr(), budget,
-                     sink, recent, new_lengths.data_ptr(), kept.data_ptr(),
-                     attention._state(device).status.data_ptr(), attention._stream(device))
+        _native.call_packed(
+            "asrback_evict", dtype, layers, batch, heads, head_dim, length, keys.data_ptr(),
+            values.data_ptr(), *strides, *w, lengths.data_ptr(), budget, sink, recent,
+            new_lengths.data_ptr(), kept.data_ptr(), attention._state(device).status.data_ptr(),
+            attention._stream(device))
     return new_lengths, kept
 
 

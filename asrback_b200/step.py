@@ -224,15 +224,15 @@ def accept_tree(tree: attention.DraftTree, drafts: Tensor, chosen: Tensor, logpr
         path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
         accepted, start = torch.empty_like(counts), torch.empty_like(position)
         columns = generated.shape[1]
-        _native.call(
+        _native.call_packed(
             "asrback_accept_tree", batch, nodes, parents.data_ptr(), parents_stride,
             counts.data_ptr(), drafts.data_ptr(), drafts_stride, chosen.data_ptr(), chosen_stride,
             logprob.data_ptr(), logprob_stride,
             tokens.data_ptr(), tokens.stride(0) if batch > 1 else 1, position.data_ptr(),
             end.data_ptr(), finished.data_ptr(), sums.data_ptr(), generated.data_ptr(),
             generated.stride(0) if batch > 1 else columns, columns,
-            None if lengths is None else lengths.data_ptr(), eos_host, len(eos_host),
-            path.data_ptr(), accepted.data_ptr(), start.data_ptr(),
+            0 if lengths is None else lengths.data_ptr(), ctypes.addressof(eos_host),
+            len(eos_host), path.data_ptr(), accepted.data_ptr(), start.data_ptr(),
             attention._state(device).status.data_ptr(), attention._stream(device))
     return AcceptedPath(path, accepted, start)
 

@@ -510,6 +510,18 @@ ASRBACK_API int asrback_evict(
     int64_t* new_lengths, int32_t* kept, int32_t* status, void* stream);
 
 /*
+ * The entry points for draft trees and eviction with their arguments as one array
+ * of 64-bit words, in the order of the parameters: integers, sizes and pointers
+ * (null: 0) by value, floats as the bits of a double. For bindings that pay per
+ * argument; same checks, same results.
+ */
+ASRBACK_API int asrback_draft_tree_packed(const int64_t* args);
+ASRBACK_API int asrback_tree_attention_packed(const int64_t* args);
+ASRBACK_API int asrback_accept_tree_packed(const int64_t* args);
+ASRBACK_API int asrback_commit_tree_packed(const int64_t* args);
+ASRBACK_API int asrback_evict_packed(const int64_t* args);
+
+/*
  * Self-test of the kernels' bounded waits: one CTA waits on an mbarrier that
  * nothing completes, gives up after budget_ns (at most 1 s) of %globaltimer,
  * sets ASRBACK_STATUS_TIMEOUT in `status` and exits; the context stays usable.

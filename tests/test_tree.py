@@ -18,7 +18,15 @@ P = 1 << 20  # a pointer that no refused call reads
 
 def _status(name: str, args: dict, **changes) -> int:
     assert set(changes) <= set(args), changes
-    return getattr(_native.load(), name)(*{**args, **changes}.values())
+    values = {**args, **changes}.values()
+    rc = getattr(_native.load(), name)(*values)
+    error = _native.load().asrback_last_error()
+    # The arguments as one array of words: the same answer.
+    words = [0 if x is None else ctypes.addressof(x) if isinstance(x, ctypes.Array) else x
+             for x in values]
+    assert getattr(_native.load(), name + "_packed")(_native._PACKED[name](*words)) == rc
+    assert _native.load().asrback_last_error() == error
+    return rc
 
 
 PLAN = dict(batch=2, nodes=5, parents=P, parents_stride=5, counts=None, ancestors=P, depths=P,
