@@ -301,10 +301,16 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit>::kPerSm)
           }
         }
         if constexpr (kWeights) {
+          // Rows of scores end with a tile: what lies behind the last key is
+          // written too, and not read.
+          float* to = score_row(p, sg, row0) + key0 + 2 * quad;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = row0 + 8 * ((i >> 1) & 1), key = key0 + 8 * (i >> 2) + 2 * quad + (i & 1);
-            if (r < p.rows && key < total) score_row(p, sg, r)[key] = s[i];
+          for (int half = 0; half < 2; ++half) {
+            if (row0 + 8 * half < p.rows) {
+              *reinterpret_cast<float2*>(to) = make_float2(s[2 * half], s[2 * half + 1]);
+              *reinterpret_cast<float2*>(to + 8) = make_float2(s[4 + 2 * half], s[5 + 2 * half]);
+            }
+            to += 8 * p.score_stride;
           }
         }
         const float limit0 = m[0] + kMoveThreshold, limit1 = m[1] + kMoveThreshold;
