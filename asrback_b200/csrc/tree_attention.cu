@@ -247,15 +247,26 @@ int launch_simt(const TreeParams& p, cudaStream_t stream) {
                     "tree attention (f32) launch", p);
 }
 
-// Query rows that one CTA holds against a key tile, by dtype and rows per
-// key/value head: in bf16 16 for the mma.sync kernel, whole warps of TMEM lanes
-// for the tcgen05 kernel.
+// Query rows that one CTA holds against a key tile: blocks of 16 in float32 and for
+// the mma.sync kernel, whole warps of TMEM lanes for the tcgen05 kernel.
 int rows_per_block(int dtype, int rows) {
   if (dtype == ASRBACK_F32 || rows <= 16) return 16;
   return std::min((rows + 31) / 32 * 32, 128);
 }
 
+// In bf16, up to 16 rows per key/value head go to the mma.sync kernel, in head_dim
+// 64 up to 32: the tcgen05 kernel's tile has 128 rows whatever it is given, but
+// its products cost no registers. Measured, mma.sync and tcgen05: 64 rows of up to
+// 1024 keys, 8 heads of 128, 2 query rows 39.6 and 45.3 us, 16 query rows 46.4 and
+// 47.5, 32 query rows 60.0 and 51.5 (two parts of 32 queries no longer fit beside
+// the outputs); 64 rows of up to 448 keys, 20 heads of 64, 8 query rows 29.3 and
+// 53.1 us, 24 query rows 47.3 and 57.2.
+bool takes_mma(int dtype, int rows, int head_dim) {
+  return dtype == ASRBACK_BF16 && rows <= (head_dim == 64 ? 32 : 16);
+}
+
 struct Plan {
+  bool mma;
   int block_rows, mblocks, ctas, lead;
   int q_block_bytes;
   size_t q_bytes, part_bytes, lse_bytes, score_bytes;
@@ -269,24 +280,22 @@ Plan plan_for(int dtype, int batch, int nodes, int heads, int kv_heads, int head
               int cache_length, bool rotary, bool weights) {
   Plan plan{};
   const int rows = nodes * (heads / kv_heads);
+  plan.mma = takes_mma(dtype, rows, head_dim);
   plan.block_rows = rows_per_block(dtype, rows);
   plan.mblocks = (rows + plan.block_rows - 1) / plan.block_rows;
   const int64_t items = (int64_t)batch * kv_heads * plan.mblocks;
   const int64_t tiles = items * ((cache_length + kTile - 1) / kTile);
   // As many CTAs as are resident at once.
   const int per_sm = dtype == ASRBACK_F32 ? (head_dim == 128 ? 2 : 3)
-                     : plan.block_rows == 16 ? mma_ctas_per_sm(head_dim)
-                                             : 1;
+                     : plan.mma ? mma_ctas_per_sm(head_dim, plan.block_rows)
+                                : 1;
   plan.ctas = static_cast<int>(std::min<int64_t>(tiles, (int64_t)per_sm * sm_count()));
   // What an item's query block, first scores and end cost a CTA, in tiles, where
   // items are of few tiles. Measured, without and with: 64 rows x 16 nodes of up
   // to 1024 keys (tcgen05) 54.5 and 51.6 us; 64 rows x 8 nodes of up to 448 keys, 20
   // heads of 64 (mma.sync) 32.2 and 30.3 us, but 64 rows x 1 node, 8 heads of
   // 128, whose tiles are twice the bytes, 46.2 and 47.2 us.
-  plan.lead = dtype == ASRBACK_F32      ? 0
-              : plan.block_rows > 16    ? 2
-              : head_dim == 64          ? 1
-                                        : 0;
+  plan.lead = dtype == ASRBACK_F32 ? 0 : !plan.mma ? 2 : head_dim == 64 ? 1 : 0;
   // float32, bf16 as it comes, or (rotary) two bf16 parts; masks and flags.
   const int row_bytes = head_dim * (dtype == ASRBACK_F32 || rotary ? 4 : 2) + 8;
   plan.q_block_bytes = plan.block_rows * row_bytes + kMaxNodes;
@@ -430,7 +439,7 @@ extern "C" int asrback_tree_attention(
   int rc = launch_prepare(dtype, head_dim, p, s);
   if (rc) return rc;
   if (dtype == ASRBACK_BF16)
-    rc = plan.block_rows == 16 ? launch_mma(head_dim, p, s) : launch_tc(head_dim, p, s);
+    rc = plan.mma ? launch_mma(head_dim, p, s) : launch_tc(head_dim, p, s);
   else
     rc = head_dim == 64 ? launch_simt<64>(p, s) : launch_simt<128>(p, s);
   if (!rc) rc = launch_finish(dtype, head_dim, p, s);

@@ -274,8 +274,8 @@ __device__ __forceinline__ int tile_at(int rows, int row, int piece) {
 int launch_prepare(int dtype, int head_dim, const TreeParams& p, cudaStream_t stream);
 // tree_finish.cu: the merge of split items, the accumulated weights.
 int launch_finish(int dtype, int head_dim, const TreeParams& p, cudaStream_t stream);
-// tree_attention_mma.cu: bf16, one block of 16 query rows.
-int mma_ctas_per_sm(int head_dim);
+// tree_attention_mma.cu: bf16, one block of 16 query rows, or (head_dim 64) of 32.
+int mma_ctas_per_sm(int head_dim, int block_rows);
 int launch_mma(int head_dim, const TreeParams& p, cudaStream_t stream);
 // tree_attention_tc.cu: bf16, blocks of 32 to 128 query rows.
 int launch_tc(int head_dim, const TreeParams& p, cudaStream_t stream);

@@ -22,8 +22,6 @@
 // here, and their products issue as fast as the cache arrives (measured: one
 // m16n8k16 in 2.05 cycles per SM). 64 rows x 8 nodes, 20 heads of 64, 448
 // positions: see the measurements at the launch.
-#include <type_traits>
-
 #include "tree_tma.cuh"
 
 namespace asrback {
@@ -31,7 +29,6 @@ namespace {
 
 using namespace tree;
 
-constexpr int kRows = 16;
 constexpr int kWarps = 4;  // that compute
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr float kMoveThreshold = 8.0f;
@@ -76,11 +73,15 @@ __device__ __forceinline__ void sync_warps() { named_sync(1, 32 * kWarps); }
 // CTAs per SM: as many as registers and shared memory allow, since a tile's
 // chain of products, barrier and exponentials and an item's end are latencies
 // that only other CTAs' work fills.
-constexpr int ctas_per_sm(int head_dim) { return head_dim == 64 ? 4 : 3; }
+constexpr int ctas_per_sm(int head_dim, int rows) {
+  return head_dim == 64 && rows == 16 ? 4 : 3;
+}
 
-template <int D, bool kSplit>
+// kBlocks: of 16 query rows.
+template <int D, bool kSplit, int kBlocks>
 struct Shape {
-  static constexpr int kPerSm = ctas_per_sm(D);
+  static constexpr int kRows = 16 * kBlocks;
+  static constexpr int kPerSm = ctas_per_sm(D, kRows);
   static constexpr int kUnitBytes = kTile * D * 2;  // keys or values of a tile
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kBlockBytes = (kSplit ? 2 : 1) * kQBytes + kRows * 8 + kMaxNodes;
@@ -105,12 +106,13 @@ struct Shape {
   static_assert(units(kMaxBatch) >= 3, "the ring is too short");
 };
 
-template <int D, bool kSplit, bool kWeights>
-__global__ void __launch_bounds__(kThreads, Shape<D, kSplit>::kPerSm)
+template <int D, bool kSplit, int kBlocks, bool kWeights>
+__global__ void __launch_bounds__(kThreads, Shape<D, kSplit, kBlocks>::kPerSm)
     tree_mma_kernel(const __grid_constant__ Maps maps, const __grid_constant__ TreeParams p,
                     const int units) {
-  using Sh = Shape<D, kSplit>;
+  using Sh = Shape<D, kSplit, kBlocks>;
   using T = __nv_bfloat16;
+  constexpr int kRows = Sh::kRows;
   constexpr int kQSlots = Sh::kQSlots;
   constexpr int kCols = D / kWarps;  // output columns of a warp
   extern __shared__ uint8_t smem_raw[];
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit>::kPerSm)
       }
   } else {
     // -------------------------------------------------------------- products
-    const int quad = lane & 3, row0 = lane >> 2;  // rows row0 and row0 + 8
+    const int quad = lane & 3, row0 = lane >> 2;  // of each block rows row0 and row0 + 8
     const uint32_t base = smem_addr(smem);
     const uint32_t ring = base + Sh::kOffRing;
     // ldmatrix: lane l gives the address of row l % 8 of matrix l / 8. Tiles start
@@ -235,130 +237,168 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit>::kPerSm)
       const uint8_t* flags = smem + block.at * Sh::kSlotBytes + Sh::kBlockBytes - kMaxNodes;
       const auto* masks = reinterpret_cast<const unsigned long long*>(flags) - kRows;
       if (ok) ok = wait(&q_full[block.at], block.lap);
-      const unsigned long long mask[2] = {ok ? masks[row0] : 0, ok ? masks[row0 + 8] : 0};
+      unsigned long long mask[kBlocks][2];
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          mask[i][half] = ok ? masks[16 * i + row0 + 8 * half] : 0;
       // A node (at most kRows here) whose value holds infinities or NaN.
       const bool odd = __any_sync(0xffffffffu, ok && lane < sg.count && lane < kRows && flags[lane]);
-      // Part `part` of the query rows, columns 16 ks ...
-      auto load_q = [&](uint32_t (&a)[4], int part, int ks) {
-        ldsm4(a, ((q_at + q_lane) ^ (32 * (ks & 3))) + part * Sh::kQBytes + (ks >> 2) * kRows * 128);
+      // Part `part` of a block's query rows, columns 16 ks ...
+      auto load_q = [&](uint32_t (&a)[4], int i, int part, int ks) {
+        ldsm4(a, ((q_at + q_lane) ^ (32 * (ks & 3))) + part * Sh::kQBytes + i * 16 * 128 +
+                     (ks >> 2) * kRows * 128);
       };
-      uint32_t qa[D / 16][4];
+      // The first part stays in registers where they hold it.
+      constexpr bool kKeepQ = kBlocks == 1 || !kSplit;
+      uint32_t qa[kBlocks][kKeepQ ? D / 16 : 1][4];
+      if constexpr (kKeepQ) {
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) load_q(qa[ks], 0, ks);
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) load_q(qa[i][ks], i, 0, ks);
+      }
 
-      float o[kCols / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      float o[kBlocks][kCols / 8][4], m[kBlocks][2], l[kBlocks][2];
 #pragma unroll
-      for (int c = 0; c < kCols / 8; ++c)
+      for (int i = 0; i < kBlocks; ++i) {
+        m[i][0] = m[i][1] = -INFINITY, l[i][0] = l[i][1] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[c][j] = 0.f;
+        for (int c = 0; c < kCols / 8; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][c][j] = 0.f;
+      }
 
-      // This warp's 16 keys of a tile: scaled scores (base 2) of rows row0,
+      // This warp's 16 keys of a tile: scaled scores (base 2) of a block's rows row0,
       // row0 + 8 in s[0..3] (keys 2 quad, + 1) and s[4..7] (keys 8 + 2 quad, + 1),
       // -inf where unseen. Frees the keys; returns whether a reference has to
       // move.
       const int total = sg.length + sg.count;
-      auto scores = [&](int tile, float (&s)[8]) {
+      auto scores = [&](int tile, float (&s)[kBlocks][8]) {
         const int key0 = tile * kTile + 16 * warp;  // the warp's first
         const int ku = unit.at;
         if (ok) ok = wait(&full[ku], unit.lap);
         unit.next(units);
-        float high[2][4], low[2][4];
+        float high[kBlocks][2][4], low[kBlocks][2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) high[h][j] = low[h][j] = 0.f;
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) high[i][h][j] = low[i][h][j] = 0.f;
         if (ok && key0 < total) {
           const uint32_t kt = ring + ku * Sh::kUnitBytes + k_lane;
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             uint32_t kb[4];
             ldsm4(kb, (kt ^ (32 * (ks & 3))) + (ks >> 2) * kTile * 128);
-            mma16816(high[0], qa[ks], kb[0], kb[1]);
-            mma16816(high[1], qa[ks], kb[2], kb[3]);
-            if constexpr (kSplit) {
-              uint32_t a[4];
-              load_q(a, 1, ks);
-              mma16816(low[0], a, kb[0], kb[1]);
-              mma16816(low[1], a, kb[2], kb[3]);
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) {
+              if constexpr (!kKeepQ) load_q(qa[i][0], i, 0, ks);
+              mma16816(high[i][0], qa[i][kKeepQ ? ks : 0], kb[0], kb[1]);
+              mma16816(high[i][1], qa[i][kKeepQ ? ks : 0], kb[2], kb[3]);
+              if constexpr (kSplit) {
+                uint32_t a[4];
+                load_q(a, i, 1, ks);
+                mma16816(low[i][0], a, kb[0], kb[1]);
+                mma16816(low[i][1], a, kb[2], kb[3]);
+              }
             }
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[ku]);
+        bool moves = false;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < kBlocks; ++i) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            s[4 * h + j] = kSplit ? high[h][j] + low[h][j] : high[h][j] * p.scale_log2;
-        if ((tile + 1) * kTile > sg.length) {
-          // Behind the cached keys lie the nodes, behind them nothing.
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = key0 + 8 * (i >> 2) + 2 * quad + (i & 1);
-            const int age = key - sg.length;
-            if (age >= 0 && (age >= sg.count || (mask[(i >> 1) & 1] >> age & 1) == 0))
-              s[i] = -INFINITY;
-          }
-        }
-        if constexpr (kWeights) {
-          // Rows of scores end with a tile: what lies behind the last key is
-          // written too, and not read.
-          float* to = score_row(p, sg, row0) + key0 + 2 * quad;
+            for (int j = 0; j < 4; ++j)
+              s[i][4 * h + j] =
+                  kSplit ? high[i][h][j] + low[i][h][j] : high[i][h][j] * p.scale_log2;
+          if ((tile + 1) * kTile > sg.length) {
+            // Behind the cached keys lie the nodes, behind them nothing.
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (row0 + 8 * half < p.rows) {
-              *reinterpret_cast<float2*>(to) = make_float2(s[2 * half], s[2 * half + 1]);
-              *reinterpret_cast<float2*>(to + 8) = make_float2(s[4 + 2 * half], s[5 + 2 * half]);
+            for (int j = 0; j < 8; ++j) {
+              const int age = key0 + 8 * (j >> 2) + 2 * quad + (j & 1) - sg.length;
+              if (age >= 0 && (age >= sg.count || (mask[i][(j >> 1) & 1] >> age & 1) == 0))
+                s[i][j] = -INFINITY;
             }
-            to += 8 * p.score_stride;
           }
+          if constexpr (kWeights) {
+            // Rows of scores end with a tile: what lies behind the last key is
+            // written too, and not read.
+            float* to = score_row(p, sg, row0) + key0 + 2 * quad;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (row0 + 8 * half < p.rows) {
+                *reinterpret_cast<float2*>(to) = make_float2(s[i][2 * half], s[i][2 * half + 1]);
+                *reinterpret_cast<float2*>(to + 8) =
+                    make_float2(s[i][4 + 2 * half], s[i][5 + 2 * half]);
+              }
+              to += 8 * p.score_stride;
+            }
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            moves |= fmaxf(fmaxf(s[i][2 * half], s[i][2 * half + 1]),
+                           fmaxf(s[i][4 + 2 * half], s[i][5 + 2 * half])) >
+                     m[i][half] + kMoveThreshold;
         }
-        const float limit0 = m[0] + kMoveThreshold, limit1 = m[1] + kMoveThreshold;
-        return fmaxf(fmaxf(s[0], s[1]), fmaxf(s[4], s[5])) > limit0 ||
-               fmaxf(fmaxf(s[2], s[3]), fmaxf(s[6], s[7])) > limit1;
+        return moves;
       };
       // The references move to the rows' largest scores so far.
-      auto move = [&](const float (&s)[8]) {
+      auto move = [&](const float (&s)[kBlocks][8]) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float top = fmaxf(fmaxf(s[2 * half], s[2 * half + 1]),
-                            fmaxf(s[4 + 2 * half], s[5 + 2 * half]));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          if (quad == 0) row_top[warp * kRows + row0 + 8 * half] = top;
-        }
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float top = fmaxf(fmaxf(s[i][2 * half], s[i][2 * half + 1]),
+                              fmaxf(s[i][4 + 2 * half], s[i][5 + 2 * half]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (quad == 0) row_top[warp * kRows + 16 * i + row0 + 8 * half] = top;
+          }
         sync_warps();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float now = m[half];
+        for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w)
-            now = fmaxf(now, row_top[w * kRows + row0 + 8 * half]);
-          const float a = now == m[half] ? 1.f : fast_exp2(m[half] - now);
-          m[half] = now;
-          l[half] *= a;
+          for (int half = 0; half < 2; ++half) {
+            float now = m[i][half];
 #pragma unroll
-          for (int c = 0; c < kCols / 8; ++c) {
-            o[c][2 * half] *= a;
-            o[c][2 * half + 1] *= a;
+            for (int w = 0; w < kWarps; ++w)
+              now = fmaxf(now, row_top[w * kRows + 16 * i + row0 + 8 * half]);
+            const float a = now == m[i][half] ? 1.f : fast_exp2(m[i][half] - now);
+            m[i][half] = now;
+            l[i][half] *= a;
+#pragma unroll
+            for (int c = 0; c < kCols / 8; ++c) {
+              o[i][c][2 * half] *= a;
+              o[i][c][2 * half + 1] *= a;
+            }
           }
-        }
       };
       // Probabilities are rounded to bf16 for the second product (2^-8 at most,
       // against an output in bf16 itself); their sum is not.
-      auto publish = [&](const float (&s)[8]) {
+      auto publish = [&](const float (&s)[kBlocks][8]) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float ref = m[half] == -INFINITY ? 0.f : m[half];
-          const float x0 = fast_exp2(s[2 * half] - ref), x1 = fast_exp2(s[2 * half + 1] - ref);
-          const float x2 = fast_exp2(s[4 + 2 * half] - ref), x3 = fast_exp2(s[5 + 2 * half] - ref);
-          l[half] += (x0 + x1) + (x2 + x3);
-          uint8_t* row = smem + Sh::kOffP + parity * Sh::kPBytes + half * 1024;
-          *reinterpret_cast<uint32_t*>(row + p_store) = tc::bf16x2(x0, x1);
-          *reinterpret_cast<uint32_t*>(row + (p_store ^ 16)) = tc::bf16x2(x2, x3);
-        }
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float ref = m[i][half] == -INFINITY ? 0.f : m[i][half];
+            const float x0 = fast_exp2(s[i][2 * half] - ref);
+            const float x1 = fast_exp2(s[i][2 * half + 1] - ref);
+            const float x2 = fast_exp2(s[i][4 + 2 * half] - ref);
+            const float x3 = fast_exp2(s[i][5 + 2 * half] - ref);
+            l[i][half] += (x0 + x1) + (x2 + x3);
+            uint8_t* row = smem + Sh::kOffP + parity * Sh::kPBytes + (2 * i + half) * 1024;
+            *reinterpret_cast<uint32_t*>(row + p_store) = tc::bf16x2(x0, x1);
+            *reinterpret_cast<uint32_t*>(row + (p_store ^ 16)) = tc::bf16x2(x2, x3);
+          }
       };
-      float s[8];
+      float s[kBlocks][8];
       if (total > 0) {
         const bool vote = scores(sg.tile0, s);
         if (sync_any(vote)) move(s);
@@ -389,14 +429,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit>::kPerSm)
           const uint32_t vt = ring + values.at * Sh::kUnitBytes;
           const uint32_t pt = base + Sh::kOffP + parity * Sh::kPBytes;
           auto weigh = [&](int ks) {  // 16 keys' probabilities and values
-            uint32_t pa[4];
-            ldsm4(pa, (pt + q_lane) ^ (32 * ks));
+            uint32_t pa[kBlocks][4];
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i)
+              ldsm4(pa[i], ((pt + q_lane) ^ (32 * ks)) + i * 16 * 128);
 #pragma unroll
             for (int c = 0; c < kCols / 16; ++c) {
               uint32_t vb[4];
               ldsm4_t(vb, vt + v_lane[c] + ks * 16 * 128);
-              mma16816(o[2 * c], pa, vb[0], vb[1]);
-              mma16816(o[2 * c + 1], pa, vb[2], vb[3]);
+#pragma unroll
+              for (int i = 0; i < kBlocks; ++i) {
+                mma16816(o[i][2 * c], pa[i], vb[0], vb[1]);
+                mma16816(o[i][2 * c + 1], pa[i], vb[2], vb[3]);
+              }
             }
           };
           if (keys == kTile && !(edge && odd)) {
@@ -409,20 +454,20 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit>::kPerSm)
             // not see it, as a product with zero would let it: key by key,
             // added only where it is visible.
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int r = row0 + 8 * half;
+            for (int j = 0; j < 2 * kBlocks; ++j) {
+              const int i = j / 2, half = j % 2, r = 16 * i + row0 + 8 * half;
               for (int k = 0; k < keys; ++k) {
                 const int age = key0 + k - sg.length;
-                if (age >= 0 && (mask[half] >> age & 1) == 0) continue;
+                if (age >= 0 && (mask[i][half] >> age & 1) == 0) continue;
                 const float w = __bfloat162float(*reinterpret_cast<const T*>(
                     smem + (pt - base) + r * 128 + (((k >> 3) ^ (r & 7)) << 4) + (k & 7) * 2));
 #pragma unroll
                 for (int c = 0; c < kCols / 8; ++c) {
                   const uint32_t v = *reinterpret_cast<const uint32_t*>(
                       smem + (vt - base) + tile_at(kTile, k, warp * (kCols / 8) + c) + 4 * quad);
-                  o[c][2 * half] = fmaf(w, __uint_as_float(v << 16), o[c][2 * half]);
-                  o[c][2 * half + 1] =
-                      fmaf(w, __uint_as_float(v & 0xffff0000u), o[c][2 * half + 1]);
+                  o[i][c][2 * half] = fmaf(w, __uint_as_float(v << 16), o[i][c][2 * half]);
+                  o[i][c][2 * half + 1] =
+                      fmaf(w, __uint_as_float(v & 0xffff0000u), o[i][c][2 * half + 1]);
                 }
               }
             }
@@ -442,37 +487,40 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit>::kPerSm)
       // only this one barrier.)
       float* row_sum = row_sums + (n & 1) * kWarps * kRows;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float sum = l[half];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (quad == 0) row_sum[warp * kRows + row0 + 8 * half] = sum;
-      }
+      for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float sum = l[i][half];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          if (quad == 0) row_sum[warp * kRows + 16 * i + row0 + 8 * half] = sum;
+        }
       sync_warps();
       const bool whole = sg.whole();
       float* part = Parts<D>::mine(p, st);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = row0 + 8 * half;  // the only block's
+      for (int j = 0; j < 2 * kBlocks; ++j) {
+        const int i = j / 2, half = j % 2, r = 16 * i + row0 + 8 * half;
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) sum += row_sum[w * kRows + r];
         if (r >= p.rows) continue;
         if (whole) {
           const float f = 1.f / sum;
-          if (p.weights && warp == 0 && quad == 0) write_lse(p, sg, r, m[half], sum);
+          if (kWeights && warp == 0 && quad == 0) write_lse(p, sg, r, m[i][half], sum);
           T* out = out_row<T>(p, sg.b, sg.h, r) + warp * kCols + 2 * quad;
 #pragma unroll
           for (int c = 0; c < kCols / 8; ++c)
             *reinterpret_cast<uint32_t*>(out + 8 * c) =
-                mask[half] == 0 ? 0u : tc::bf16x2(o[c][2 * half] * f, o[c][2 * half + 1] * f);
+                mask[i][half] == 0 ? 0u
+                                   : tc::bf16x2(o[i][c][2 * half] * f, o[i][c][2 * half + 1] * f);
         } else {
-          if (warp == 0 && quad == 0) part[r] = m[half], part[kRows + r] = sum;
+          if (warp == 0 && quad == 0) part[r] = m[i][half], part[kRows + r] = sum;
 #pragma unroll
           for (int c = 0; c < kCols / 8; ++c)
             *reinterpret_cast<float2*>(part +
                                        Parts<D>::at(p, r, warp * kCols + 8 * c + 2 * quad)) =
-                make_float2(o[c][2 * half], o[c][2 * half + 1]);
+                make_float2(o[i][c][2 * half], o[i][c][2 * half + 1]);
         }
       }
       __syncwarp();
@@ -482,10 +530,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit>::kPerSm)
   if (!ok && lane == 0 && p.status) atomicOr(p.status, ASRBACK_STATUS_TIMEOUT);
 }
 
-template <int D, bool kSplit, bool kWeights>
+template <int D, bool kSplit, int kBlocks, bool kWeights>
 int launch(const TreeParams& p, cudaStream_t stream) {
-  using Sh = Shape<D, kSplit>;
-  auto kernel = tree_mma_kernel<D, kSplit, kWeights>;
+  using Sh = Shape<D, kSplit, kBlocks>;
+  auto kernel = tree_mma_kernel<D, kSplit, kBlocks, kWeights>;
   Maps maps;
   if (int rc = make_maps(&maps, p, D, kTile)) return rc;
   static thread_local int prepared_device = -1;
@@ -503,24 +551,24 @@ int launch(const TreeParams& p, cudaStream_t stream) {
                     "tree attention launch", maps, p, units);
 }
 
+template <int D, bool kSplit>
+int launch(const TreeParams& p, cudaStream_t stream) {
+  static_assert(kMaxWeightRows == 16, "weights come from one block");
+  if constexpr (D == 64)
+    if (p.block_rows == 32) return launch<D, kSplit, 2, false>(p, stream);
+  return p.weights ? launch<D, kSplit, 1, true>(p, stream)
+                   : launch<D, kSplit, 1, false>(p, stream);
+}
+
 }  // namespace
 
 namespace tree {
 
-int mma_ctas_per_sm(int head_dim) { return ctas_per_sm(head_dim); }
+int mma_ctas_per_sm(int head_dim, int block_rows) { return ctas_per_sm(head_dim, block_rows); }
 
 int launch_mma(int head_dim, const TreeParams& p, cudaStream_t stream) {
-  auto pick = [&](auto dim, auto split) {
-    constexpr int D = decltype(dim)::value;
-    constexpr bool kSplit = decltype(split)::value;
-    return p.weights ? launch<D, kSplit, true>(p, stream) : launch<D, kSplit, false>(p, stream);
-  };
-  using std::integral_constant;
-  if (head_dim == 64)
-    return p.q_norm ? pick(integral_constant<int, 64>{}, std::true_type{})
-                    : pick(integral_constant<int, 64>{}, std::false_type{});
-  return p.q_norm ? pick(integral_constant<int, 128>{}, std::true_type{})
-                  : pick(integral_constant<int, 128>{}, std::false_type{});
+  if (head_dim == 64) return p.q_norm ? launch<64, true>(p, stream) : launch<64, false>(p, stream);
+  return p.q_norm ? launch<128, true>(p, stream) : launch<128, false>(p, stream);
 }
 
 }  // namespace tree
