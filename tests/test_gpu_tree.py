@@ -190,6 +190,7 @@ def test_weights(family, tag, nodes, heads, kv_heads, dim):
     ("qwen3", "bf16", 16, 8, 128, 1, True), ("qwen3", "bf16", 16, 8, 128, 16, False),
     ("qwen3", "bf16", 16, 4, 64, 5, False), ("qwen3", "bf16", 16, 8, 128, 60, False),
     ("whisper", "bf16", 20, 20, 64, 7, False), ("whisper", "bf16", 20, 20, 64, 16, True),
+    ("whisper", "bf16", 20, 20, 64, 25, False), ("whisper", "bf16", 20, 20, 64, 40, False),
     ("qwen3", "f32", 16, 8, 128, 2, True)])
 def test_many_items_per_sm(family, tag, heads, kv_heads, dim, nodes, weights):
     """Rows of one to many tiles, some empty, so that a CTA runs through many
@@ -281,6 +282,34 @@ def test_masked_places_do_not_matter(tag):
     # The products are summed in another order, with the same roundings.
     mass = _want(x)["mass"][0][~sees].reshape(d.shape)
     assert (d.abs().cpu().numpy() <= mass * 2.0 ** (-8 if tag == "bf16" else -20)).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,nodes", [
+    (4, 2, 64, 16), (16, 8, 128, 8), (2, 2, 64, 7), (8, 1, 128, 16), (6, 2, 64, 21)])
+def test_an_unseen_value_does_not_matter(heads, kv_heads, dim, nodes):
+    """The last two nodes' values are infinite and NaN: whoever does not see them
+    is as without."""
+    x = _inputs(dim + nodes, "qwen3", "bf16", 2, nodes, 300, heads, kv_heads, dim, [190, 0])
+    clean, mass = _call(x)[0], _want(x)["mass"]
+    dirty = dict(x, qkv=x["qkv"].clone())
+    dirty["qkv"][:, nodes - 1, -dim * kv_heads:] = float("inf")
+    dirty["qkv"][:, nodes - 2, -dim * kv_heads:] = float("nan")
+    got = _call(dirty)[0]
+    above, _ = oracle.plan(x["parents"], x["counts"])
+    sees = above[:, :, nodes - 1] | above[:, :, nodes - 2]
+    assert not torch.isfinite(got[torch.from_numpy(sees)]).any()
+    d = (got.float() - clean.float())[torch.from_numpy(~sees)].abs().cpu().numpy()
+    # The products are summed in another order, with the same roundings.
+    assert (d <= mass[~sees].reshape(d.shape) * 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("family,heads,kv_heads,dim", [
+    ("whisper", 3, 3, 64), ("qwen3", 4, 2, 64), ("qwen3", 2, 2, 128)])
+@pytest.mark.parametrize("nodes", [9, 15, 16, 17, 31, 32, 33, 49])
+def test_blocks_of_every_size(family, heads, kv_heads, dim, nodes):
+    x = _inputs(nodes, family, "bf16", 3, nodes, 200, heads, kv_heads, dim, [128, 200 - nodes, 3],
+                [nodes, nodes, nodes - 2])
+    _check(x, _call(x), _want(x))
 
 
 def test_rows_that_do_not_fit_are_skipped():
