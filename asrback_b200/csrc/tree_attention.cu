@@ -17,15 +17,15 @@
 //
 // Split. The work is the list of 64-key tiles of every (row, key/value head,
 // block of query rows); each CTA takes an equal stretch of that list, whatever
-// the rows' lengths, so all CTAs stream the same number of bytes. A stretch
+// the rows' lengths, so all CTAs stream nearly the same number of bytes. A stretch
 // that covers only part of an item leaves its unnormalised result (m, l, o) in
 // the workspace. Three launches: tree_prepare.cu writes the nodes' keys and
 // values to the cache and the prepared query rows to the workspace (the nodes
 // then are an item's last keys, masked by the rows' ancestors), the attention
-// (tree_attention_tc.cu in bf16, below in float32), and tree_finish.cu, which
+// (tree_attention_mma.cu or tree_attention_tc.cu in bf16, by the number of query
+// rows; below in float32), and tree_finish.cu, which
 // merges the parts in list order. Each launch begins while the one before it
 // ends; no CTA waits for another, and results do not depend on their order.
-//
 #include "../../include/asrback_attn.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -47,7 +47,9 @@ constexpr int kThreads = 128;
 // 128) or half of them (64) for the output. Few calls have more tiles than the
 // GPU takes at once, so a tile's chain of loads and products is what bounds
 // them: loads are issued eight at a time, and both products read the operand
-// that a warp shares four elements at a time.
+// that a warp shares four elements at a time. Measured: 7 rows x 5 nodes of up to
+// 448 keys, 6 heads of 64 (one tile per CTA) 13.4 us with what comes before and
+// behind, 9.5 of them here.
 
 template <int D>
 struct SimtShape {

@@ -1,6 +1,6 @@
-// Draft-tree attention in bf16 for up to 16 query rows per key/value head
-// (nodes x heads / kv_heads): mma.sync with a TMA warp, sm_100a. The split of the
-// work is tree_attention.cu's.
+// Draft-tree attention in bf16 for up to 16 query rows per key/value head (nodes x
+// heads / kv_heads), with head_dim 64 up to 32: mma.sync with a TMA warp, sm_100a.
+// The split of the work is tree_attention.cu's.
 //
 // The call is bound by streaming the cache, so the TMA warp runs ahead of the
 // products through the CTA's whole stretch, across items, and waits for nothing
@@ -17,11 +17,17 @@
 // votes on whether a row of tile t + 1 passes its softmax reference by more than
 // 8 (base 2); only then the references move.
 //
-// mma.sync instead of tcgen05: 16 rows leave seven eighths of a 128-row tcgen05
-// tile empty, whose softmax would run in half of one warp. Four warps share it
+// mma.sync instead of tcgen05: 16 rows would leave seven eighths of a 128-row tcgen05
+// tile empty, and its softmax to half of one warp. Four warps share it
 // here, and their products issue as fast as the cache arrives (measured: one
-// m16n8k16 in 2.05 cycles per SM). 64 rows x 8 nodes, 20 heads of 64, 448
-// positions: see the measurements at the launch.
+// m16n8k16 in 2.05 cycles per SM). Bound: HBM's stream, for items of few tiles
+// an item's fixed cost too. Measured, with the preparation before and the merge
+// behind: 64 rows x 1 node of up to 1024 keys, 8 heads of 128, with weights (171
+// MB) 45 us, of which this kernel's 32 are 5.3 TB/s; 3 rows x 4 nodes of up to
+// 16384 keys, with weights (128 MB) 39 us; 64 rows x 8 nodes of up to 448 keys, 20
+// heads of 64 (98 MB) 30 us, of which this kernel's 21 are 4.6 TB/s; 1 row x 6
+// nodes of 256 keys 8.5 us. With head_dim 64 a second block of 16 rows shares the
+// fragments of keys and values.
 #include "tree_tma.cuh"
 
 namespace asrback {

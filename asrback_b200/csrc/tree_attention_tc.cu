@@ -28,6 +28,18 @@
 //               reference moves, and its O is rescaled, only when a score passes
 //               it by more than 8 (base 2);
 //   warps 12-15 an item's end: output or part.
+//
+// Bound: HBM's stream, with the tensor pipe close behind: a pair of 64 KB takes
+// 1480 ns of a GPU's share of it, its products 1530 cycles (16 of 128 x 128 x 16
+// for the scores in two parts, 8 for the output), whose operands keep shared
+// memory's port busy, so that a spilled register costs more than an exponential.
+// Measured, with the preparation before and the merge behind: 8 rows x 64 nodes
+// of up to 8192 keys, 8 heads of 128 (175 MB) 48 us, of which this kernel's 33 are
+// 5.3 TB/s; 64 rows x 16 nodes of up to 1024 keys (183 MB) 51.5 us. Steps on the
+// way for the two: scores of 64 columns and an accumulator per tile of a pair 61
+// and 63 us; one per pair, no spills 48.6 and 53; an item's fixed cost in the split
+// 48 and 51.5. Without effect: exponentials on the FMA pipe (49 and 55), the rows
+// laid out twice over the schedulers (69 for the second), other ring lengths.
 #include <algorithm>
 
 #include "tree_tma.cuh"

@@ -7,6 +7,9 @@
 // once, 4 bytes per score and 8 per weight, but latency bounds it: a CTA has one
 // item, finds its place in the tile list while the attention still runs, and then
 // loads all it needs (references, sums and outputs of the parts, scores) at once.
+// Measured, behind the attention: 3 us for 1 row x 6 nodes, 5 for 64 rows x 16
+// nodes, 7.5 for 8 rows x 64 nodes (13 MB of parts) and for 64 rows x 1 node with
+// weights (1536 CTAs).
 #include "capi_internal.h"
 #include "tree_attention.cuh"
 
