@@ -582,7 +582,7 @@ def _tree_call(dtype: int, q: tuple, k: tuple, v: tuple, sizes: tuple, rotary: t
                              "with unit last stride, on the tensors' device")
         w_ptr, (w_batch, w_head, _) = weights.data_ptr(), weights.stride()
     if rotary is None:
-        qn = kn = cos = sin = positions = 0
+        qn = kn = cos = sin = at = 0
         eps, table_stride, table_length = 0.0, 0, 0
     else:
         qn, kn, eps, cos, sin, positions = rotary
@@ -596,7 +596,8 @@ def _tree_call(dtype: int, q: tuple, k: tuple, v: tuple, sizes: tuple, rotary: t
         for weight in (qn, kn):
             if weight.shape != (head_dim,) or weight.stride(0) != 1 or weight.device != device:
                 raise ValueError("asrback_b200: norm weights must be contiguous (head_dim,)")
-        positions = _int_rows(positions, "positions", torch.int64, (batch,), device).data_ptr()
+        positions = _int_rows(positions, "positions", torch.int64, (batch,), device)
+        at = positions.data_ptr()
         qn, kn, cos, sin = qn.data_ptr(), kn.data_ptr(), cos.data_ptr(), sin.data_ptr()
         if table_length == 1:
             table_stride = head_dim
@@ -609,7 +610,7 @@ def _tree_call(dtype: int, q: tuple, k: tuple, v: tuple, sizes: tuple, rotary: t
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
         _native.call_packed(
             "asrback_tree_attention", dtype, *sizes, *q, *k, *v,
-            qn, kn, eps, cos, sin, table_stride, table_length, positions,
+            qn, kn, eps, cos, sin, table_stride, table_length, at,
             ancestors.data_ptr(), depths.data_ptr(), counts.data_ptr(), lengths.data_ptr(),
             keys.data_ptr(), values.data_ptr(), *strides,
             out.data_ptr(), nodes * width, width, head_dim, w_ptr, w_batch, w_head,

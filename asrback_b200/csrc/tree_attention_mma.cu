@@ -169,6 +169,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit, kBlocks>::kPerSm)
     __syncwarp();
     const uint64_t policy = l2_evict_first_policy();
     bool waited = false;
+    int loads = 0;  // of query blocks
     Turn unit, block;
     for (; ok && next_segment(p, list, st); block.next(kQSlots)) {
       // The query block is loaded as soon as its buffer is free, and at the
@@ -185,6 +186,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit, kBlocks>::kPerSm)
           ok = wait(bar, block.lap - 1);
         }
         q_due = false;
+        if (ok) ++loads;
         if (ok && leader) {
           mbar_arrive_expect_tx(&q_full[block.at], Sh::kBlockBytes);
           bulk_g2s(smem + block.at * Sh::kSlotBytes,
@@ -213,11 +215,16 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit, kBlocks>::kPerSm)
     }
     // A wait gave up: the copies in flight still have to land before the CTA
     // may end.
-    if (!ok)
+    if (!ok) {
       for (int u = 0; u < units; ++u) {
         const int laps = unit.lap + (u < unit.at ? 1 : 0);
         if (laps > 0) wait(&full[u], laps - 1);
       }
+      for (int s = 0; s < kQSlots; ++s) {
+        const int laps = (loads + kQSlots - 1 - s) / kQSlots;
+        if (laps > 0) wait(&q_full[s], laps - 1);
+      }
+    }
   } else {
     // -------------------------------------------------------------- products
     const int quad = lane & 3, row0 = lane >> 2;  // of each block rows row0 and row0 + 8

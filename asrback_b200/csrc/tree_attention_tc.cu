@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     const uint64_t policy = l2_evict_first_policy();
     bool waited = false;
+    int loads = 0;  // of query blocks
     Turn unit, block;
     for (; ok && next_segment(p, list, st); block.next(lay.slots)) {
       // The query block is loaded as soon as its buffer is free, and at the
@@ -245,6 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = wait(&q_empty[slot], q_lap - 1);
         }
         q_due = false;
+        if (ok) ++loads;
         if (ok && leader) {
           mbar_arrive_expect_tx(&q_full[slot], p.q_block_bytes);
           bulk_g2s(smem + slot * lay.slot_bytes, p.q_blocks + (int64_t)sg.item * p.q_block_bytes,
@@ -277,11 +279,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // A wait gave up: the copies in flight still have to land before the CTA
     // may end.
-    if (!ok)
+    if (!ok) {
       for (int u = 0; u < units; ++u) {
         const int laps = unit.lap + (u < unit.at ? 1 : 0);
         if (laps > 0) wait(&full[u], laps - 1);
       }
+      for (int s = 0; s < lay.slots; ++s) {
+        const int laps = (loads + lay.slots - 1 - s) / lay.slots;
+        if (laps > 0) wait(&q_full[s], laps - 1);
+      }
+    }
   } else if (warp == 1) {
     // ------------------------------------------------------------ S = Q K^T
     const bool leader = tc::elect_one();

@@ -760,6 +760,66 @@ def test_calls_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_strided_vectors():
+    """Lengths, positions and counts that are columns of wider tensors (their
+    copies have to outlive the call), and a fragmented allocator."""
+    x = _inputs(21, "qwen3", "bf16", 40, 3, 300, 16, 8, 128, list(range(0, 240, 6)), ahead=5)
+    want = _call(x)
+    tree = _tree(x["parents"], x["counts"])
+    wide = torch.empty((40, 7), dtype=torch.int64, device=DEV).fill_(1 << 40)
+    wide[:, 2], wide[:, 5] = _gpu(x["lengths"], torch.int64), _gpu(x["positions"], torch.int64)
+    counts = torch.zeros((40, 2), dtype=torch.int32, device=DEV)
+    counts[:, 1] = tree.counts
+    for _ in range(20):
+        held = [torch.empty(n, dtype=torch.uint8, device=DEV) for n in (512, 1024, 512, 40960)]
+        del held[::2]
+        keys, values = x["keys"].clone(), x["values"].clone()
+        out = attention.qwen3_attention_tree(
+            x["qkv"], x["wq"], x["wk"], 1e-6, x["cos"], x["sin"], wide[:, 5],
+            tree._replace(counts=counts[:, 1]), keys, values, 16, 8, lengths=wide[:, 2])
+        assert torch.equal(out, want[0]) and torch.equal(keys, want[1])
+    assert attention.read_status() == 0
+
+
+@pytest.mark.parametrize("length,nodes,heads,kv_heads", [
+    (1, 1, 2, 2), (17, 17, 4, 2), (40, 40, 2, 2), (64, 64, 2, 1), (70, 33, 4, 2), (127, 50, 2, 2)])
+def test_caches_shorter_than_a_tile(length, nodes, heads, kv_heads):
+    x = _inputs(length, "qwen3", "bf16", 2, nodes, length, heads, kv_heads, 128,
+                [0, length - nodes])
+    _check(x, _call(x), _want(x))
+
+
+def test_a_captured_eviction_replays():
+    """Rows that a cluster shares, captured with the commit before it."""
+    keys = torch.randn((2, 5000, 2, 64), device=DEV)
+    weights, lengths = torch.rand((2, 2, 5000), device=DEV), torch.tensor([5000, 4100], device=DEV)
+    accepted = step.AcceptedPath(torch.tensor([[0, 2, -1], [0, 1, 2]], device=DEV).int(),
+                                 torch.tensor([2, 3], device=DEV).int(),
+                                 torch.tensor([4990, 7], device=DEV))
+    first = [t.clone() for t in (keys, -keys, weights)]
+
+    def run(k, v, w):
+        cache.qwen3_commit_tree(k, v, accepted, weights=w)
+        return (k, v, w, *cache.qwen3_evict(k, v, w, lengths, 1000, sink=3, recent=30))
+
+    want = [t.clone() for t in run(*(t.clone() for t in first))]
+    state = [t.clone() for t in first]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(*(t.clone() for t in first))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(*state)
+    for _ in range(3):
+        for t, start in zip(state, first):
+            t.copy_(start)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert attention.read_status() == 0
+
+
 # ----------------------------------------------------------------- refusals
 
 
