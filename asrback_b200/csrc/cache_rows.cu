@@ -9,8 +9,7 @@
 // read once and written once. Measured: the commit of 64 rows x 16 nodes over 28
 // layers of 8 heads of 128 6 us; an eviction of 64 rows from 1024 slots to 512, 8
 // heads of 128, 57 us, of which the moves' 50 are 5.4 TB/s; of 2 rows from 16384
-// slots to 4096 34 us, 12 for the selection and 20 for the moves, which have 8
-// heads' rows each in turn.
+// slots to 4096 29 us, 12 for the selection and 16 for the moves.
 #include "../../include/asrback_attn.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -356,15 +355,15 @@ struct MoveParams {
   const int64_t* lengths;
   const int32_t* kept;
   int batch, heads, length, budget;
-  int vectors;  // 16-byte pieces of a row
+  int vectors;  // 16-byte pieces of the part of a row that one CTA moves
   int cluster;  // CTAs that move one head's rows
 };
 
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnroll = 4;
 
-// A cluster of CTAs moves one head's kept rows of the keys or of the values,
-// kMoveUnroll rows per thread and turn. A turn's loads come before its barrier
+// A cluster of CTAs moves one head's kept rows of the keys or of the values (or a
+// part of their columns), kMoveUnroll rows per thread and turn. A turn's loads come before its barrier
 // and its stores after it; the next turn's loads are issued in between, since
 // its rows lie behind all that this turn writes.
 template <bool kCluster>
@@ -374,12 +373,12 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
   const int cluster = kCluster ? p.cluster : 1;
   const int h = blockIdx.x / cluster, rank = blockIdx.x - h * cluster;
   const int b = blockIdx.y % p.batch, layer = blockIdx.y / p.batch;
-  const int which = blockIdx.z;
+  const int which = blockIdx.z & 1, part = blockIdx.z >> 1;
   const int64_t given = p.lengths[b];
   if (given <= p.budget || given > p.length) return;
   const CacheView& c = p.cache[which];
   uint8_t* rows = c.base + layer * c.layer + b * c.batch + h * c.head +
-                  (threadIdx.x % p.vectors) * 16;
+                  (part * p.vectors + threadIdx.x % p.vectors) * 16;
   const int32_t* kept = p.kept + ((int64_t)blockIdx.y * p.heads + h) * p.budget;
   const int lanes = kMoveThreads / p.vectors;  // rows per pass of the CTA
   const int turn = lanes * kMoveUnroll * cluster;
@@ -574,14 +573,20 @@ extern "C" int asrback_evict(int dtype, int layers, int batch, int heads, int he
   m.length = length;
   m.budget = budget;
   // A head's rows are split over a cluster until the launch has four CTAs per SM
-  // or a turn of the cluster holds all rows.
+  // or a turn of the cluster holds all rows; then their columns, in parts of at
+  // least 64 bytes, until it has two. (2 rows from 16384 slots to 4096: 43 us
+  // with neither, 36 with clusters, 31.5 with both.)
   m.vectors = static_cast<int>(head_dim * esize / 16);
   const int64_t moves = static_cast<int64_t>(layers) * batch * heads * 2;
-  const int rows_per_turn = kMoveThreads / m.vectors * kMoveUnroll;
+  int rows_per_turn = kMoveThreads / m.vectors * kMoveUnroll;
   m.cluster = 1;
   while (m.cluster < 8 && moves * m.cluster < 4 * sm_count() && rows_per_turn * m.cluster < budget)
     m.cluster *= 2;
-  const dim3 move_grid(heads * m.cluster, layers * batch, 2);
+  int parts = 1;
+  while (m.vectors > 4 && moves * m.cluster * parts < 2 * sm_count() &&
+         rows_per_turn * m.cluster < budget)
+    m.vectors /= 2, parts *= 2, rows_per_turn *= 2;
+  const dim3 move_grid(heads * m.cluster, layers * batch, 2 * parts);
   if (m.cluster == 1)
     rc = launch_pdl(move_kernel<false>, move_grid, dim3(kMoveThreads), 0, st, "evict move launch",
                     m);
