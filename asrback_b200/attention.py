@@ -542,10 +542,9 @@ def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
     if counts is not None:
         counts = _int_rows(counts, "counts", torch.int32, (batch,), device)
     with _on(device):
-        ancestors = torch.empty((batch, nodes), dtype=torch.int64, device=device)
-        depths = torch.empty((batch, nodes), dtype=torch.int32, device=device)
-        live = torch.empty(batch, dtype=torch.int32, device=device) if counts is None \
-            else torch.empty_like(counts)
+        ancestors = parents.new_empty((batch, nodes), dtype=torch.int64)
+        depths = parents.new_empty((batch, nodes))
+        live = parents.new_empty(batch) if counts is None else torch.empty_like(counts)
         _native.call_packed(
             "asrback_draft_tree", batch, nodes, parents.data_ptr(), parents.stride(0),
             0 if counts is None else counts.data_ptr(), ancestors.data_ptr(), depths.data_ptr(),
@@ -605,7 +604,7 @@ def _tree_call(dtype: int, q: tuple, k: tuple, v: tuple, sizes: tuple, rotary: t
     with _on(device):
         ws_bytes = _tree_workspace(torch._C._cuda_getDevice(), dtype, *sizes, rotary is not None,
                                    weights is not None)
-        out = torch.empty((batch, nodes, width), dtype=like.dtype, device=device)
+        out = like.new_empty((batch, nodes, width))
         status = _state(device).status
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
         _native.call_packed(

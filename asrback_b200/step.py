@@ -163,8 +163,8 @@ class AcceptedPath(NamedTuple):
 
 
 @functools.lru_cache(maxsize=64)
-def _eos_array(eos_ids: tuple):
-    return (ctypes.c_int64 * len(eos_ids))(*map(int, eos_ids))
+def _eos_array(eos_ids: tuple[int, ...]) -> ctypes.Array:
+    return (ctypes.c_int64 * len(eos_ids))(*eos_ids)
 
 
 def _node_rows(t: Tensor, name: str, dtype: torch.dtype, shape: tuple, device) -> tuple:
@@ -219,9 +219,9 @@ def accept_tree(tree: attention.DraftTree, drafts: Tensor, chosen: Tensor, logpr
     for t in (counts, tokens, position, end, finished, sums, generated, lengths):
         if t is not None and t.device != device:
             raise ValueError("asrback_b200: the decode state must be on the tree's device")
-    eos_host = _eos_array(tuple(eos_ids))
+    eos_host = _eos_array(tuple(map(int, eos_ids)))
     with attention._on(device):
-        path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
+        path = parents.new_empty((batch, nodes))
         accepted, start = torch.empty_like(counts), torch.empty_like(position)
         columns = generated.shape[1]
         _native.call_packed(
