@@ -527,6 +527,8 @@ extern "C" int asrback_evict(int dtype, int layers, int batch, int heads, int he
                 batch);
   if (!weights || !lengths || !new_lengths || !kept)
     return fail(ASRBACK_ERR_ARGUMENT, "null weights, lengths, new_lengths or kept pointer");
+  if (new_lengths == lengths)
+    return fail(ASRBACK_ERR_ARGUMENT, "new_lengths must not be lengths, which is read meanwhile");
   if (int rc = check_weights(layers, batch, heads, length, w_stride_layer, w_stride_batch,
                              w_stride_head))
     return rc;

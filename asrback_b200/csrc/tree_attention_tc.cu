@@ -38,8 +38,9 @@
 // 5.3 TB/s; 64 rows x 16 nodes of up to 1024 keys (183 MB) 51.5 us. Steps on the
 // way for the two: scores of 64 columns and an accumulator per tile of a pair 61
 // and 63 us; one per pair, no spills 48.6 and 53; an item's fixed cost in the split
-// 48 and 51.5. Without effect: exponentials on the FMA pipe (49 and 55), the rows
-// laid out twice over the schedulers (69 for the second), other ring lengths.
+// 48 and 51.5. No gain: exponentials on the FMA pipe (49 and 55), blocks of up to
+// 64 rows laid out twice, for the softmax to use more schedulers (53.5 for the
+// second), other ring lengths.
 #include <algorithm>
 
 #include "tree_tma.cuh"

@@ -410,8 +410,10 @@ ASRBACK_API int asrback_draft_tree(
  *              heads, are added to the cached keys' entries and assigned to
  *              the new slots'. At most 16 query rows per key/value head
  *              (nodes * heads / kv_heads).
- * head_dim 64 or 128; nodes <= 64; batch <= 1024; dtype ASRBACK_BF16 or
- * ASRBACK_F32; rows and pointers 16-byte aligned.
+ * head_dim 64 or 128; nodes <= 64; batch <= 1024; cache_length <= 2^24; dtype
+ * ASRBACK_BF16 or ASRBACK_F32; rows and pointers 16-byte aligned. Rows of the
+ * caches, of out and of weights must not overlap. With weights the workspace
+ * holds 4 bytes per query row and cache position.
  * A row whose counts, lengths or positions are out of range gets zeros, writes
  * nothing else and sets ASRBACK_STATUS_POSITION.
  *
@@ -496,7 +498,7 @@ ASRBACK_API int asrback_commit_tree(
  * caches, weights  as in asrback_commit_tree
  * lengths      (batch,) int64: keys per row; outside [0, length] the row is
  *              left alone and sets ASRBACK_STATUS_POSITION
- * new_lengths  (batch,) int64, out: min(lengths, budget)
+ * new_lengths  (batch,) int64, out, not lengths itself: min(lengths, budget)
  * kept         (layers, batch, heads, budget) int32, out: the old slots of the
  *              kept keys, ascending, then -1
  */

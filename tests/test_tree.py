@@ -55,7 +55,7 @@ COMMIT = dict(
 EVICT = dict(
     dtype=_native.BF16, layers=2, batch=2, heads=8, head_dim=128, length=64, key_cache=P,
     value_cache=P, c_l=2 * 64 * 1024, c_b=64 * 1024, c_p=1024, c_h=128, weights=P, w_l=2 * 8 * 64,
-    w_b=8 * 64, w_h=64, lengths=P, budget=32, sink=4, recent=8, new_lengths=P, kept=P, status=None,
+    w_b=8 * 64, w_h=64, lengths=P + 64, budget=32, sink=4, recent=8, new_lengths=P, kept=P, status=None,
     stream=None)
 
 _ODD = P + 8  # not on a 16-byte boundary
@@ -96,7 +96,7 @@ REFUSED = {
         dict(sink=25), dict(recent=29), dict(layers=256, batch=256), dict(key_cache=None),
         dict(value_cache=_ODD), dict(c_l=0), dict(c_b=0), dict(c_p=64), dict(c_h=0), dict(w_l=0),
         dict(w_b=32), dict(w_h=0), dict(weights=None), dict(lengths=None),
-        dict(new_lengths=None), dict(kept=None)]),
+        dict(new_lengths=None), dict(kept=None), dict(new_lengths=P + 64)]),
 }
 
 
