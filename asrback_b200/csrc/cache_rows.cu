@@ -8,8 +8,8 @@
 // its stores, with no copy of the cache. Both are bound by HBM: a moved row is
 // read once and written once. Measured: the commit of 64 rows x 16 nodes over 28
 // layers of 8 heads of 128 6 us; an eviction of 64 rows from 1024 slots to 512, 8
-// heads of 128, 57 us, of which the moves' 50 are 5.4 TB/s; of 2 rows from 16384
-// slots to 4096 29 us, 12 for the selection and 16 for the moves.
+// heads of 128 (273 MB), 52 us, 5.2 TB/s; of 2 rows from 16384 slots to 4096 29 us,
+// 12 for the selection and 16 for the moves.
 #include "../../include/asrback_attn.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -123,6 +123,7 @@ struct SelectParams {
 };
 
 constexpr int kSelectThreads = 256;
+constexpr int kShortRow = 4 * kSelectThreads;  // slots that one CTA holds in registers
 
 // What lies at `at` in the shared memory of the cluster's CTA `rank`.
 __device__ __forceinline__ int load_remote(const int* at, int rank) {
@@ -157,9 +158,12 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 //
 // The counting's instructions bound it, not the bytes (one SM took 18 us for a
 // row of 16384 keys), hence the clusters.
-template <int V, bool kCluster>
-__global__ void __launch_bounds__(kSelectThreads)
-    select_kernel(const __grid_constant__ SelectParams p) {
+//
+// kMoves: two CTAs (a cluster) select for a row of one chunk, each for itself; the
+// slots also go to `own_kept`, in shared memory, and only the first one writes.
+// Returns whether the row is cut.
+template <int V, bool kCluster, bool kMoves>
+__device__ __forceinline__ bool select_row(const SelectParams& p, int* own_kept) {
   constexpr int kChunk = kSelectThreads * V, kWarps = kSelectThreads / 32;
   constexpr int kBits = 8, kDigits = 32 / kBits, kBins = 1 << kBits;
   static_assert(kBins == kSelectThreads, "a thread per bin");
@@ -168,14 +172,13 @@ __global__ void __launch_bounds__(kSelectThreads)
   __shared__ int scan[V * kWarps];  // keys above | equal << 16 of each 32 slots, in slot order
   __shared__ int sums[kWarps];
   __shared__ int share[2];  // of this CTA: keys above, equal
-  griddep_wait();
-  griddep_launch_dependents();
-  const int cluster = kCluster ? p.cluster : 1;
-  const int h = blockIdx.x / cluster, rank = blockIdx.x - h * cluster;
+  const int cluster = kCluster ? p.cluster : 1, ctas = kMoves ? 2 : cluster;
+  const int h = blockIdx.x / ctas, rank = kMoves ? 0 : blockIdx.x - h * ctas;
+  const bool writes = !kMoves || blockIdx.x % 2 == 0;
   const int b = blockIdx.y, layer = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t given = p.lengths[b];
-  const bool first = h == 0 && layer == 0 && rank == 0 && tid == 0;
+  const bool first = h == 0 && layer == 0 && rank == 0 && tid == 0 && writes;
   int32_t* kept = p.kept + (((int64_t)layer * p.batch + b) * p.heads + h) * p.budget;
   const int every = cluster * kSelectThreads, mine = rank * kSelectThreads + tid;
   if (given < 0 || given > p.length) {
@@ -183,14 +186,14 @@ __global__ void __launch_bounds__(kSelectThreads)
       p.new_lengths[b] = given;
       if (p.status) atomicOr(p.status, ASRBACK_STATUS_POSITION);
     }
-    for (int k = mine; k < p.budget; k += every) kept[k] = -1;
-    return;
+    for (int k = mine; k < p.budget && writes; k += every) kept[k] = -1;
+    return false;
   }
   const int n = static_cast<int>(given);
   if (first) p.new_lengths[b] = min(n, p.budget);
   if (n <= p.budget) {
-    for (int k = mine; k < p.budget; k += every) kept[k] = k < n ? k : -1;
-    return;
+    for (int k = mine; k < p.budget && writes; k += every) kept[k] = k < n ? k : -1;
+    return false;
   }
   float* row = p.weights + layer * p.w_layer + b * p.w_batch + h * p.w_head;
   const int chunks = (n + cluster * kChunk - 1) / (cluster * kChunk);
@@ -315,6 +318,7 @@ __global__ void __launch_bounds__(kSelectThreads)
   for (int chunk = 0; chunk < chunks; ++chunk) {
     if (chunks > 1) load(chunk);
     const int all = kCluster && chunks == 1 ? 0 : count();
+    if constexpr (kMoves) cluster_sync();  // both CTAs have read the weights
 #pragma unroll
     for (int u = 0; u < V; ++u) {
       const bool over = key[u] > threshold, same = key[u] == threshold;
@@ -325,9 +329,11 @@ __global__ void __launch_bounds__(kSelectThreads)
       const int equal_at = equal_before + (at >> 16) + __popc(equal & lower);
       if (over || (same && equal_at < ties)) {
         const int k = above_at + min(equal_at, ties);
-        kept[k] = start + chunk * kChunk + u * kSelectThreads + tid;
+        const int slot = start + chunk * kChunk + u * kSelectThreads + tid;
+        if constexpr (kMoves) own_kept[k] = slot;
+        if (writes) kept[k] = slot;
         // All CTAs have read the row, if it is of one chunk each.
-        if (chunks == 1) row[k] = raw[u];
+        if (writes && chunks == 1) row[k] = raw[u];
       }
     }
     above_before += all & 0xffff;
@@ -346,6 +352,15 @@ __global__ void __launch_bounds__(kSelectThreads)
     }
   }
   if constexpr (kCluster) cluster_sync();  // the others have read this CTA's counts
+  return true;
+}
+
+template <int V, bool kCluster>
+__global__ void __launch_bounds__(kSelectThreads)
+    select_kernel(const __grid_constant__ SelectParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  select_row<V, kCluster, false>(p, nullptr);
 }
 
 // -------------------------------------------------------- eviction: the moves
@@ -362,10 +377,52 @@ struct MoveParams {
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnroll = 4;
 
+// Moves the part of one head's kept rows that lies at `rows`, kMoveUnroll rows per
+// thread and turn of `cluster` CTAs. A turn's loads come before its barrier and
+// its stores after it; the next turn's loads are issued in between, since its
+// rows lie behind all that this turn writes.
+template <typename Barrier>
+__device__ __forceinline__ void move_rows(uint8_t* rows, int64_t position, const int32_t* kept,
+                                          int budget, int vectors, int rank, int cluster,
+                                          Barrier barrier) {
+  const int lanes = kMoveThreads / vectors;  // rows per pass of the CTA
+  const int turn = lanes * kMoveUnroll * cluster;
+  const int mine = rank * lanes * kMoveUnroll + threadIdx.x / vectors;
+  uint4 piece[2][kMoveUnroll];
+  int from[2][kMoveUnroll];
+  auto load = [&](int set, int k0) {
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int k = k0 + u * lanes + mine;
+      from[set][u] = k < budget ? kept[k] : k;
+    }
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int k = k0 + u * lanes + mine;
+      if (from[set][u] != k)
+        piece[set][u] = *reinterpret_cast<const uint4*>(rows + from[set][u] * position);
+    }
+  };
+  auto store = [&](int set, int k0) {
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int k = k0 + u * lanes + mine;
+      if (from[set][u] != k) *reinterpret_cast<uint4*>(rows + k * position) = piece[set][u];
+    }
+  };
+  load(0, 0);
+  for (int k0 = 0; k0 < budget; k0 += 2 * turn) {
+    load(1, k0 + turn);
+    barrier();
+    store(0, k0);
+    load(0, k0 + 2 * turn);
+    barrier();
+    store(1, k0 + turn);
+  }
+}
+
 // A cluster of CTAs moves one head's kept rows of the keys or of the values (or a
-// part of their columns), kMoveUnroll rows per thread and turn. A turn's loads come before its barrier
-// and its stores after it; the next turn's loads are issued in between, since
-// its rows lie behind all that this turn writes.
+// part of their columns).
 template <bool kCluster>
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveParams p) {
   griddep_wait();
@@ -380,44 +437,27 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
   uint8_t* rows = c.base + layer * c.layer + b * c.batch + h * c.head +
                   (part * p.vectors + threadIdx.x % p.vectors) * 16;
   const int32_t* kept = p.kept + ((int64_t)blockIdx.y * p.heads + h) * p.budget;
-  const int lanes = kMoveThreads / p.vectors;  // rows per pass of the CTA
-  const int turn = lanes * kMoveUnroll * cluster;
-  const int mine = rank * lanes * kMoveUnroll + threadIdx.x / p.vectors;
-  uint4 piece[2][kMoveUnroll];
-  int from[2][kMoveUnroll];
-  auto load = [&](int set, int k0) {
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      const int k = k0 + u * lanes + mine;
-      from[set][u] = k < p.budget ? kept[k] : k;
-    }
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      const int k = k0 + u * lanes + mine;
-      if (from[set][u] != k)
-        piece[set][u] = *reinterpret_cast<const uint4*>(rows + from[set][u] * c.position);
-    }
-  };
-  auto store = [&](int set, int k0) {
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      const int k = k0 + u * lanes + mine;
-      if (from[set][u] != k) *reinterpret_cast<uint4*>(rows + k * c.position) = piece[set][u];
-    }
-  };
-  auto barrier = [&]() {
+  move_rows(rows, c.position, kept, p.budget, p.vectors, rank, cluster, [] {
     if constexpr (kCluster) cluster_sync();
     else __syncthreads();
-  };
-  load(0, 0);
-  for (int k0 = 0; k0 < p.budget; k0 += 2 * turn) {
-    load(1, k0 + turn);
-    barrier();
-    store(0, k0);
-    load(0, k0 + 2 * turn);
-    barrier();
-    store(1, k0 + turn);
-  }
+  });
+}
+
+// Selection and moves in one, for many short rows: a cluster of two CTAs per
+// (layer, row, head), one for the keys and one for the values, so that some rows'
+// counting runs beside others' moves.
+__global__ void __launch_bounds__(kMoveThreads)
+    evict_kernel(const __grid_constant__ SelectParams p, const __grid_constant__ MoveParams m) {
+  static_assert(kMoveThreads == kSelectThreads);
+  __shared__ int kept[kShortRow];
+  griddep_wait();
+  griddep_launch_dependents();
+  if (!select_row<kShortRow / kSelectThreads, false, true>(p, kept)) return;
+  __syncthreads();
+  const CacheView& c = m.cache[blockIdx.x % 2];
+  uint8_t* rows = c.base + blockIdx.z * c.layer + blockIdx.y * c.batch +
+                  (blockIdx.x / 2) * c.head + threadIdx.x % m.vectors * 16;
+  move_rows(rows, c.position, kept, m.budget, m.vectors, 0, 1, [] { __syncthreads(); });
 }
 
 // Rows of weights that are written: no two of them may be one.
@@ -556,8 +596,23 @@ extern "C" int asrback_evict(int dtype, int layers, int batch, int heads, int he
   s.recent = recent;
   s.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  m.lengths = lengths;
+  m.kept = kept;
+  m.batch = batch;
+  m.heads = heads;
+  m.length = length;
+  m.budget = budget;
+  m.vectors = static_cast<int>(head_dim * esize / 16);
+  const int64_t moves = static_cast<int64_t>(layers) * batch * heads * 2;
   int rc;
-  if (length <= 4 * kSelectThreads) {
+  // One launch where two CTAs per row fill the GPU: 64 rows of 8 heads from 1024
+  // slots to 512 54 us, 59 in two launches. Fewer rows want more CTAs each.
+  if (length <= kShortRow && moves >= 2 * sm_count()) {
+    rc = launch_pdl_cluster(evict_kernel, dim3(heads * 2, batch, layers), dim3(kMoveThreads), 0, 2,
+                            st, "evict launch", s, m);
+    return rc ? rc : ok();
+  }
+  if (length <= kShortRow) {
     rc = launch_pdl(select_kernel<4, false>, dim3(heads, batch, layers), dim3(kSelectThreads), 0, st,
                     "evict selection launch", s);
   } else {
@@ -568,18 +623,10 @@ extern "C" int asrback_evict(int dtype, int layers, int batch, int heads, int he
                             dim3(kSelectThreads), 0, s.cluster, st, "evict selection launch", s);
   }
   if (rc) return rc;
-  m.lengths = lengths;
-  m.kept = kept;
-  m.batch = batch;
-  m.heads = heads;
-  m.length = length;
-  m.budget = budget;
   // A head's rows are split over a cluster until the launch has four CTAs per SM
   // or a turn of the cluster holds all rows; then their columns, in parts of at
   // least 64 bytes, until it has two. (2 rows from 16384 slots to 4096: 43 us
   // with neither, 36 with clusters, 31.5 with both.)
-  m.vectors = static_cast<int>(head_dim * esize / 16);
-  const int64_t moves = static_cast<int64_t>(layers) * batch * heads * 2;
   int rows_per_turn = kMoveThreads / m.vectors * kMoveUnroll;
   m.cluster = 1;
   while (m.cluster < 8 && moves * m.cluster < 4 * sm_count() && rows_per_turn * m.cluster < budget)

@@ -453,7 +453,8 @@ def test_commit_skips_invalid_paths():
 @pytest.mark.parametrize("heads_first,layers,heads,dim,length,budget,sink,recent", [
     (False, 1, 8, 128, 1024, 512, 4, 64), (False, 2, 2, 64, 100, 33, 0, 0),
     (True, 1, 6, 64, 448, 200, 3, 197), (False, 1, 1, 128, 5000, 4999, 0, 1),
-    (False, 1, 2, 64, 20000, 777, 5, 70), (True, 1, 3, 64, 300, 1, 0, 0)])
+    (False, 1, 2, 64, 20000, 777, 5, 70), (True, 1, 3, 64, 300, 1, 0, 0),
+    (True, 3, 20, 64, 448, 200, 3, 7), (False, 2, 16, 128, 1024, 1000, 1, 1)])
 @pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
 def test_evict(tag, heads_first, layers, heads, dim, length, budget, sink, recent, kind):
     rng = np.random.default_rng(length)
