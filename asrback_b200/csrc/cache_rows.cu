@@ -196,7 +196,8 @@ __device__ __forceinline__ bool select_row(const SelectParams& p, int* own_kept)
     return false;
   }
   float* row = p.weights + layer * p.w_layer + b * p.w_batch + h * p.w_head;
-  const int chunks = (n + cluster * kChunk - 1) / (cluster * kChunk);
+  // Rows of more than one chunk per CTA come to clusters only.
+  const int chunks = kCluster ? (n + cluster * kChunk - 1) / (cluster * kChunk) : 1;
   const int start = rank * chunks * kChunk, tail = n - p.recent;
   float raw[V];
   uint32_t key[V];
