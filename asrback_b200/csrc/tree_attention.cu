@@ -240,13 +240,21 @@ __global__ void __launch_bounds__(kThreads)
 
 template <int D>
 int launch_simt(const TreeParams& p, cudaStream_t stream) {
-  const int smem = SimtShape<D>::bytes(p.batch);
-  if (int rc = check_cuda(cudaFuncSetAttribute(tree_simt_kernel<D>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                          "cudaFuncSetAttribute(tree attention f32)"))
-    return rc;
-  return launch_pdl(tree_simt_kernel<D>, dim3(p.ctas), dim3(kThreads), smem, stream,
-                    "tree attention (f32) launch", p);
+  // The limit is the largest batch's, set once: one set per call would be another
+  // thread's between its set and its launch.
+  static thread_local int prepared_device = -1;
+  int device = 0;
+  if (int rc = check_cuda(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+  if (prepared_device != device) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(tree_simt_kernel<D>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 SimtShape<D>::bytes(kMaxBatch)),
+                            "cudaFuncSetAttribute(tree attention f32)"))
+      return rc;
+    prepared_device = device;
+  }
+  return launch_pdl(tree_simt_kernel<D>, dim3(p.ctas), dim3(kThreads),
+                    SimtShape<D>::bytes(p.batch), stream, "tree attention (f32) launch", p);
 }
 
 // Query rows that one CTA holds against a key tile: blocks of 16 in float32 and for

@@ -1,0 +1,95 @@
+"""Calls of the draft-tree operators that other tests do not make: from several
+threads and streams, on views, at the edges of the cache."""
+
+from __future__ import annotations
+
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+from asrback_b200 import _native, attention
+from tests.test_gpu_tree import DEV, _gpu, _inputs, _tree
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def clean_status():
+    attention.read_status()
+    yield
+
+
+def _recorded(monkeypatch, name, call):
+    """A function that makes ``call``'s call of entry point ``name`` over again,
+    on the same buffers, with no work in Python; and ``call``'s result."""
+    made, held, empty = [], [], torch.empty
+
+    def record(entry, *args):
+        if entry == name:
+            made.append(args)
+        return real(entry, *args)
+
+    def hold(*args, **kwargs):
+        held.append(empty(*args, **kwargs))
+        return held[-1]
+
+    packed = name in _native._PACKED
+    real = _native.call_packed if packed else _native.call
+    with monkeypatch.context() as m:
+        m.setattr(_native, real.__name__, record)
+        m.setattr(torch, "empty", hold)
+        result = call()
+    (args,), lib = made, _native.load()
+    if packed:
+        entry, args = getattr(lib, name + "_packed"), (_native._PACKED[name](*args),)
+    else:
+        entry = getattr(lib, name)
+
+    def again(held=held):
+        if entry(*args) != _native.OK:
+            raise _native.NativeError(lib.asrback_last_error().decode())
+
+    return again, result
+
+
+def _in_threads(calls, times):
+    """Every call ``times`` times in a thread of its own, all at once; raises
+    what one of them raised."""
+    errors, start = [], threading.Barrier(len(calls))
+
+    def work(call):
+        start.wait()
+        try:
+            for _ in range(times):
+                call()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(call,)) for call in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    if errors:
+        raise errors[0]
+
+
+def test_float32_attention_from_two_threads(monkeypatch):
+    """Calls of few and of many rows, whose kernels ask for less and for more
+    shared memory."""
+    calls, outs = [], []
+    for batch in (1, 1024):
+        x = _inputs(batch, "whisper", "f32", batch, 1, 64, 2, 2, 64, np.arange(batch) % 64)
+        tree, at = _tree(x["parents"], x["counts"]), _gpu(x["lengths"], torch.int64)
+        again, out = _recorded(
+            monkeypatch, "asrback_tree_attention",
+            lambda x=x, tree=tree, at=at: attention.whisper_self_attention_tree(
+                x["q"], x["k"], x["v"], x["keys"], x["values"], at, tree))
+        calls.append(again)
+        outs.append((out, out.clone(), x, tree, at))  # what the call reads stays alive
+    _in_threads(calls, 5000)
+    assert all(torch.equal(out, want) for out, want, *_ in outs)
+    assert attention.read_status() == 0
