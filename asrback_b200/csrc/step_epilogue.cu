@@ -45,6 +45,7 @@ constexpr int kMaxEos = 8;
 constexpr int kNoIndex = 0x7fffffff;
 constexpr int kSimtWarps = 8;
 constexpr int kSimtMaxBatch = 64;
+constexpr int kSimtMaxSmem = 200 * 1024;  // the hidden states of a call
 // Workspace: a 256-byte header of tickets (the final one, then one per group
 // of CTAs in the tensor-core kernel), then the partials: one per (CTA, row),
 // then (tensor-core kernel) one per (group, row).
@@ -594,7 +595,7 @@ extern "C" int asrback_greedy_step(int dtype, int batch, int vocab, int hidden_d
       return fail(ASRBACK_ERR_ARGUMENT,
                   "bf16 rows must start on 16-byte boundaries: hidden_dim and strides multiples "
                   "of 8, pointers 16-byte aligned");
-  } else if (static_cast<size_t>(batch) * hidden_dim * 4 > 200 * 1024) {
+  } else if (static_cast<size_t>(batch) * hidden_dim * 4 > kSimtMaxSmem) {
     return fail(ASRBACK_ERR_ARGUMENT, "float32: batch x hidden_dim must fit 200 KB of shared memory");
   }
   if (n_eos < 0 || n_eos > kMaxEos || (n_eos > 0 && !eos_ids))
@@ -640,11 +641,19 @@ extern "C" int asrback_greedy_step(int dtype, int batch, int vocab, int hidden_d
   }
   const int ctas = std::min((vocab + kSimtWarps - 1) / kSimtWarps, 2 * sm_count());
   const size_t smem = static_cast<size_t>(batch) * hidden_dim * 4;
-  if (int rc = check_cuda(cudaFuncSetAttribute(greedy_step_simt_kernel,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem)),
-                          "cudaFuncSetAttribute(greedy step f32)"))
-    return rc;
+  // The limit is the largest call's, set once: one set per call would be another
+  // thread's between its set and its launch.
+  static thread_local int prepared_device = -1;
+  int device = 0;
+  if (int rc = check_cuda(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+  if (prepared_device != device) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(greedy_step_simt_kernel,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kSimtMaxSmem),
+                            "cudaFuncSetAttribute(greedy step f32)"))
+      return rc;
+    prepared_device = device;
+  }
   greedy_step_simt_kernel<<<ctas, kSimtWarps * 32, smem, s>>>(
       static_cast<const float*>(weight), weight_stride, static_cast<const float*>(hidden),
       hidden_stride, hidden_dim, p);

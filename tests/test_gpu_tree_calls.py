@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from asrback_b200 import _native, attention
+from asrback_b200 import _native, attention, step
 from tests.test_gpu_tree import DEV, _gpu, _inputs, _tree
 
 pytestmark = pytest.mark.gpu
@@ -92,4 +92,21 @@ def test_float32_attention_from_two_threads(monkeypatch):
         outs.append((out, out.clone(), x, tree, at))  # what the call reads stays alive
     _in_threads(calls, 5000)
     assert all(torch.equal(out, want) for out, want, *_ in outs)
+    assert attention.read_status() == 0
+
+
+def test_float32_choice_from_two_threads(monkeypatch):
+    """As above, for the step's choice of tokens: few and many hidden elements."""
+    calls, outs = [], []
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    for batch, width in ((1, 64), (50, 1024)):
+        hidden = torch.randn((batch, width), generator=gen, device=DEV)
+        weight = torch.randn((500, width), generator=gen, device=DEV)
+        again, out = _recorded(monkeypatch, "asrback_greedy_step",
+                               lambda hidden=hidden, weight=weight: step.greedy_choose(hidden, weight))
+        calls.append(again)
+        outs.append((*out, out[0].clone(), out[1].clone(), hidden, weight))
+    _in_threads(calls, 5000)
+    for token, logprob, want_token, want_logprob, *_ in outs:
+        assert torch.equal(token, want_token) and torch.equal(logprob, want_logprob)
     assert attention.read_status() == 0
