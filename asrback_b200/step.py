@@ -75,7 +75,8 @@ def _vector(t: Tensor, name: str, dtype: torch.dtype, batch: int) -> Tensor:
 
 
 def _launch(hidden: Tensor, weight: Tensor, suppress: Tensor | None, out_token, out_logprob,
-            state: dict | None, eos_ids: Sequence[int]) -> None:
+            state: dict | None, eos_ids: Sequence[int], workspace: Tensor | None = None) -> None:
+    """``workspace``: a zero-filled one of the call's own; by default the device's."""
     hidden = _rows(hidden, "hidden")
     weight = _rows(weight, "weight")
     dtype = attention._dtype_code(hidden, weight)
@@ -92,7 +93,8 @@ def _launch(hidden: Tensor, weight: Tensor, suppress: Tensor | None, out_token, 
     eos = [int(e) for e in eos_ids]
     eos_host = (ctypes.c_int64 * max(len(eos), 1))(*eos)
     device = hidden.device
-    workspace = _workspace(device)
+    if workspace is None:
+        workspace = _workspace(device)
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     if state is None:
         tokens = position = end = finished = sums = generated = None
@@ -131,7 +133,9 @@ def _launch(hidden: Tensor, weight: Tensor, suppress: Tensor | None, out_token, 
 def greedy_choose(hidden: Tensor, weight: Tensor,
                   suppress: Tensor | None = None) -> tuple[Tensor, Tensor]:
     """Greedy ``_choose`` of ``hidden (batch, d) @ weight (vocab, d).T``:
-    ``(token int64, logprob float32)``, each ``(batch,)``."""
+    ``(token int64, logprob float32)``, each ``(batch,)``. Like
+    :func:`greedy_step`, it uses the device's one workspace: not for calls, or
+    replays of captured ones, that may run at the same time on several streams."""
     batch = hidden.shape[0]
     token = torch.empty(batch, dtype=torch.int64, device=hidden.device)
     logprob = torch.empty(batch, dtype=torch.float32, device=hidden.device)
@@ -145,7 +149,9 @@ def greedy_step(hidden: Tensor, weight: Tensor, tokens: Tensor, position: Tensor
     """One greedy ``_step`` after the decoder, updating the decode state in
     place: ``tokens`` ``(batch,)`` or ``(batch, 1)``, ``position``, ``end``
     (int64), ``finished`` (bool), ``sum_logprobs`` (float32), ``generated``
-    ``(batch, length)`` (int64); ``eos_ids`` are host ints (at most 8)."""
+    ``(batch, length)`` (int64); ``eos_ids`` are host ints (at most 8). All calls
+    on a device share one workspace, so that steps (and captured ones' replays)
+    have to follow one another on it; :func:`greedy_tree_step` has its own."""
     state = dict(tokens=tokens, position=position, end=end, finished=finished,
                  sum_logprobs=sum_logprobs, generated=generated)
     _launch(hidden, weight, suppress, None, None, state, eos_ids)
@@ -244,18 +250,24 @@ def greedy_tree_step(hidden: Tensor, weight: Tensor, tree: attention.DraftTree, 
     """A greedy step after the decoder has run a tree of drafted tokens per
     row: every node's logits and choice from ``hidden`` ``(B, N, d)`` (as
     :func:`greedy_choose`, ``MAX_BATCH`` rows per launch), then
-    :func:`accept_tree`."""
+    :func:`accept_tree`. The call has a workspace of its own: calls on several
+    streams and captured ones replayed side by side do not meet in it."""
     if hidden.dim() != 3 or hidden.shape[:2] != tree.parents.shape:
         raise ValueError(f"asrback_b200: hidden must be (batch, nodes, width) for trees of "
                          f"{tuple(tree.parents.shape)}, got {tuple(hidden.shape)}")
+    attention._dtype_code(hidden, weight)
     batch, nodes, width = hidden.shape
     rows = hidden.flatten(0, 1)
     # float32 takes 64 rows, and as many as 200 KB of shared memory hold.
     limit = MAX_BATCH if hidden.dtype == torch.bfloat16 else max(1, min(64, 51200 // width))
     token = torch.empty(batch * nodes, dtype=torch.int64, device=hidden.device)
     logprob = torch.empty(batch * nodes, dtype=torch.float32, device=hidden.device)
+    with attention._on(hidden.device):
+        nbytes = _native.load().asrback_greedy_step_workspace_bytes(min(limit, batch * nodes))
+    # The kernel's tickets begin at zero; the launches of a call follow one another.
+    workspace = torch.zeros(nbytes, dtype=torch.uint8, device=hidden.device)
     for first in range(0, batch * nodes, limit):
         part = slice(first, first + limit)
-        _launch(rows[part], weight, suppress, token[part], logprob[part], None, ())
+        _launch(rows[part], weight, suppress, token[part], logprob[part], None, (), workspace)
     return accept_tree(tree, drafts, token.view(batch, nodes), logprob.view(batch, nodes), tokens,
                        position, end, finished, sum_logprobs, generated, eos_ids, lengths)

@@ -10,7 +10,8 @@ import pytest
 import torch
 
 from asrback_b200 import _native, attention, step
-from tests.test_gpu_tree import DEV, _gpu, _inputs, _tree
+from asrback_b200.transcription import CapturedGraph
+from tests.test_gpu_tree import DEV, _accept_case, _device_state, _gpu, _inputs, _tree
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +111,66 @@ def test_float32_choice_from_two_threads(monkeypatch):
     for token, logprob, want_token, want_logprob, *_ in outs:
         assert torch.equal(token, want_token) and torch.equal(logprob, want_logprob)
     assert attention.read_status() == 0
+
+
+def _step_case(seed, batch, nodes, vocab, width):
+    """A step over trees from the nodes' hidden states: a function that starts
+    from the same state every time, and the tensors that it writes."""
+    parents, counts, drafts, _, _, state = _accept_case(seed, batch, nodes)
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    hidden = torch.randn((batch, nodes, width), generator=gen, device=DEV).bfloat16()
+    weight = torch.randn((vocab, width), generator=gen, device=DEV).bfloat16()
+    tree, drafts = _tree(parents, counts), _gpu(drafts, torch.int64)
+    start = _device_state(state)
+    dev = {n: v.clone() for n, v in start.items()}
+    written = []
+
+    def run():
+        for n, v in dev.items():
+            v.copy_(start[n])
+        accepted = step.greedy_tree_step(hidden, weight, tree, drafts, *dev.values(), [5])
+        written[:] = [*accepted, *dev.values()]
+
+    return run, written
+
+
+def test_tree_steps_run_side_by_side():
+    """Steps on two streams at once, called and replayed: none meets the other's
+    partial results."""
+    cases = [_step_case(2, 16, 16, 30000, 512), _step_case(4, 9, 7, 50000, 256)]
+    wants = []
+    for run, written in cases:
+        run()
+        wants.append([t.clone() for t in written])
+    streams = [torch.cuda.Stream() for _ in cases]
+    graphs = []
+    torch.cuda.synchronize()
+    for kind in ("called", "replayed"):
+        if kind == "replayed":
+            graphs = [CapturedGraph(run) for run, _ in cases]
+            torch.cuda.synchronize()
+        for _ in range(100):
+            for i, stream in enumerate(streams):
+                with torch.cuda.stream(stream):
+                    graphs[i].replay() if graphs else cases[i][0]()
+        torch.cuda.synchronize()
+        for (_, written), want in zip(cases, wants):
+            assert all(torch.equal(a, b) for a, b in zip(written, want)), kind
+    assert attention.read_status() == 0
+
+
+def test_tree_steps_of_two_streams_have_two_workspaces(monkeypatch):
+    run, _ = _step_case(2, 2, 3, 1000, 64)
+    used, real = [], _native.call
+
+    def record(name, *args):
+        used.append(args[-4])
+        return real(name, *args)
+
+    monkeypatch.setattr(_native, "call", record)
+    for stream in (torch.cuda.Stream(), torch.cuda.Stream()):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            run()
+        torch.cuda.synchronize()
+    assert len(set(used)) == 2
