@@ -85,6 +85,8 @@ def _launch(hidden: Tensor, weight: Tensor, suppress: Tensor | None, out_token, 
     if weight.shape[1] != width:
         raise ValueError(f"asrback_b200: weight {tuple(weight.shape)} does not match hidden "
                          f"width {width}")
+    if weight.device != hidden.device:
+        raise ValueError("asrback_b200: weight must be on the hidden states' device")
     if suppress is not None:
         if suppress.shape != (vocab,) or suppress.dtype not in (torch.bool, torch.uint8) \
                 or suppress.stride(0) != 1 or suppress.device != hidden.device:
