@@ -537,8 +537,9 @@ def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
         raise ValueError(f"asrback_b200: a batch of trees of 1 to {MAX_NODES} nodes is needed, got "
                          f"{tuple(parents.shape)}")
     device = parents.device
-    if parents.stride(1) != 1 or 0 < parents.stride(0) < nodes:
-        parents = parents.contiguous()
+    row, unit = parents.stride()
+    if unit != 1 or 0 < row < nodes:  # one row may have any stride, contiguous or not
+        parents, row = parents.contiguous(), nodes
     if counts is not None:
         counts = _int_rows(counts, "counts", torch.int32, (batch,), device)
     with _on(device):
@@ -546,7 +547,7 @@ def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
         depths = parents.new_empty((batch, nodes))
         live = parents.new_empty(batch) if counts is None else torch.empty_like(counts)
         _native.call_packed(
-            "asrback_draft_tree", batch, nodes, parents.data_ptr(), parents.stride(0),
+            "asrback_draft_tree", batch, nodes, parents.data_ptr(), row,
             0 if counts is None else counts.data_ptr(), ancestors.data_ptr(), depths.data_ptr(),
             live.data_ptr(), _state(device).status.data_ptr(), _stream(device))
     return DraftTree(parents, live, ancestors, depths)

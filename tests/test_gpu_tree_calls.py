@@ -174,3 +174,13 @@ def test_tree_steps_of_two_streams_have_two_workspaces(monkeypatch):
             run()
         torch.cuda.synchronize()
     assert len(set(used)) == 2
+
+
+def test_a_plan_of_one_transposed_row():
+    """A view whose rows are one element apart, which matters to no one: there
+    is one row."""
+    parents = torch.tensor([[-1], [0], [0], [1]], dtype=torch.int32, device=DEV).t()
+    assert parents.shape == (1, 4) and parents.stride() == (1, 1)
+    tree = attention.draft_tree(parents)
+    assert tree.ancestors.tolist() == [[1, 3, 5, 11]] and tree.depths.tolist() == [[0, 1, 1, 2]]
+    assert attention.read_status() == 0
