@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kCommitThreads)
       if (k < count && k < p.nodes) {
         const int before = k > 0 ? path[k - 1] : -1;
         bad |= node[u] <= before || node[u] >= p.nodes || start < 0 ||
-               start + node[u] >= p.length;
+               start >= p.length - node[u];  // no sum that could pass 63 bits
       }
       moves |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, k < count && node[u] != k))
                << (32 * u);

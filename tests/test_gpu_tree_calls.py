@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from asrback_b200 import _native, attention, step
+from asrback_b200 import _native, attention, cache, step
 from asrback_b200.transcription import CapturedGraph
 from tests.test_gpu_tree import DEV, _accept_case, _device_state, _gpu, _inputs, _tree
 
@@ -184,3 +184,17 @@ def test_a_plan_of_one_transposed_row():
     tree = attention.draft_tree(parents)
     assert tree.ancestors.tolist() == [[1, 3, 5, 11]] and tree.depths.tolist() == [[0, 1, 1, 2]]
     assert attention.read_status() == 0
+
+
+@pytest.mark.parametrize("start", [(1 << 63) - 1, (1 << 63) - 2, 1 << 62, 1 << 32, 40, 39, -1])
+def test_commit_skips_starts_out_of_range(start):
+    """Starts up to the largest integer, whose sum with a node would pass it."""
+    keys = torch.randn((1, 1, 40, 2, 64), device=DEV)
+    before, weights = keys.clone(), torch.rand((1, 1, 2, 40), device=DEV)
+    old = weights.clone()
+    accepted = step.AcceptedPath(torch.tensor([[1, 2, -1]], device=DEV).int(),
+                                 torch.tensor([2], device=DEV).int(),
+                                 torch.tensor([start], device=DEV))
+    cache.qwen3_commit_tree(keys, keys.clone(), accepted, weights=weights)
+    assert attention.read_status() == _native.STATUS_POSITION
+    assert torch.equal(keys, before) and torch.equal(weights, old)
