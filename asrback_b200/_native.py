@@ -142,6 +142,10 @@ SIGNATURES: dict[str, tuple[list, object]] = {
         [_c_int, _c_int, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
         _c_int,
     ),
+    "asrback_draft_tree_in_cache": (
+        [_c_int, _c_int, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p],
+        _c_int,
+    ),
     "asrback_tree_workspace_bytes": ([_c_int] * 9, _c_size),
     "asrback_tree_attention": (
         [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
@@ -193,7 +197,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
 
 # Entry points that also take their arguments as one array of 64-bit words.
 _PACKED = {}
-for _name in ("asrback_draft_tree", "asrback_tree_attention", "asrback_accept_tree",
+for _name in ("asrback_draft_tree", "asrback_draft_tree_in_cache", "asrback_tree_attention", "asrback_accept_tree",
               "asrback_commit_tree", "asrback_evict"):
     _PACKED[_name] = struct.Struct("=" + "".join(
         "d" if t is _c_f else "q" for t in SIGNATURES[_name][0])).pack

@@ -522,14 +522,22 @@ def _int_rows(t: Tensor, name: str, dtype: torch.dtype, shape: tuple, device: to
     return t if t.is_contiguous() else t.contiguous()
 
 
-def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
+def draft_tree(parents: Tensor, counts: Tensor | None = None, lengths: Tensor | None = None,
+               capacity: int | None = None) -> DraftTree:
     """Plans the draft trees of a step, once for all layers. ``parents``
     ``(B, N)`` int32 on the device: node ``i``'s parent, below ``i``, or -1 for
     a root (``N <= 64``; an expanded ``(1, N)`` serves one tree for every row).
     ``counts`` ``(B,)`` int32: the row's first nodes that are live, the others
     being padding (default: all). Node 0 holds the row's current token, the
     others drafts of what follows it. A row with invalid parents or count gets
-    no nodes and sets ``_native.STATUS_TREE``."""
+    no nodes and sets ``_native.STATUS_TREE``.
+
+    ``lengths`` ``(B,)`` int64 and ``capacity``, the keys in a row's cache and its
+    slots: nodes behind the last free slot become padding, so that a row decodes
+    on until its cache is full. (For a rotary table that ends before the cache, a
+    second plan of the first one's counts, with the positions and the table's
+    length.) A row that wants nodes and has room for none gets none and sets
+    ``_native.STATUS_POSITION``."""
     if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_cuda:
         raise ValueError("asrback_b200: parents must be (batch, nodes) int32 on a CUDA device")
     batch, nodes = parents.shape
@@ -542,14 +550,21 @@ def draft_tree(parents: Tensor, counts: Tensor | None = None) -> DraftTree:
         parents, row = parents.contiguous(), nodes
     if counts is not None:
         counts = _int_rows(counts, "counts", torch.int32, (batch,), device)
+    if (lengths is None) != (capacity is None):
+        raise ValueError("asrback_b200: lengths and capacity go together")
+    if lengths is not None:
+        lengths = _int_rows(lengths, "lengths", torch.int64, (batch,), device)
+        if capacity < 1:
+            raise ValueError(f"asrback_b200: capacity must be positive, got {capacity}")
     with _on(device):
         ancestors = parents.new_empty((batch, nodes), dtype=torch.int64)
         depths = parents.new_empty((batch, nodes))
         live = parents.new_empty(batch) if counts is None else torch.empty_like(counts)
         _native.call_packed(
-            "asrback_draft_tree", batch, nodes, parents.data_ptr(), row,
-            0 if counts is None else counts.data_ptr(), ancestors.data_ptr(), depths.data_ptr(),
-            live.data_ptr(), _state(device).status.data_ptr(), _stream(device))
+            "asrback_draft_tree_in_cache", batch, nodes, parents.data_ptr(), row,
+            0 if counts is None else counts.data_ptr(),
+            0 if lengths is None else lengths.data_ptr(), capacity or 0, ancestors.data_ptr(),
+            depths.data_ptr(), live.data_ptr(), _state(device).status.data_ptr(), _stream(device))
     return DraftTree(parents, live, ancestors, depths)
 
 
@@ -639,8 +654,9 @@ def qwen3_attention_tree(qkv: Tensor, q_norm_weight: Tensor, k_norm_weight: Tens
     slots (at most ``MAX_WEIGHT_ROWS`` query rows, ``N * heads / kv_heads``).
 
     ``N = 1`` is the decode step, a chain a prompt pass of up to 64 tokens.
-    ``head_dim`` 64 or 128. A row whose nodes do not fit the cache or the RoPE
-    table gets zeros and sets ``_native.STATUS_POSITION``."""
+    ``head_dim`` 64 or 128. A row whose nodes do not all fit the cache or the
+    RoPE table gets zeros and sets ``_native.STATUS_POSITION``: plan those that
+    fit with :func:`draft_tree`'s ``lengths`` and ``capacity``."""
     if qkv.dim() != 3 or qkv.stride(2) != 1:
         raise ValueError("asrback_b200: qkv must be (batch, nodes, width) with unit last stride")
     batch, nodes, width = qkv.shape

@@ -26,6 +26,7 @@ constexpr int kWarps = 4;  // rows per CTA: 1 to 64 rows spread over the SMs
 __global__ void __launch_bounds__(kWarps * 32)
     draft_tree_kernel(int batch, int nodes, const int32_t* __restrict__ parents,
                       int64_t parents_stride, const int32_t* __restrict__ counts,
+                      const int64_t* __restrict__ lengths, int64_t capacity,
                       int64_t* __restrict__ ancestors, int32_t* __restrict__ depths,
                       int32_t* __restrict__ live_counts, int32_t* status) {
   __shared__ unsigned long long mask[kWarps][kMaxNodes];
@@ -36,6 +37,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   griddep_launch_dependents();
   if (b >= batch) return;
   int count = counts ? counts[b] : nodes;
+  const int64_t length = lengths ? lengths[b] : 0;
   int parent[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -51,6 +53,12 @@ __global__ void __launch_bounds__(kWarps * 32)
   if (__any_sync(0xffffffffu, bad)) {
     count = 0;
     if (lane == 0 && status) atomicOr(status, ASRBACK_STATUS_TREE);
+  }
+  // The first nodes are a tree by themselves, since parents come before children.
+  if (lengths && count > 0) {
+    const int64_t room = length < 0 || length >= capacity ? 0 : capacity - length;
+    if (room == 0 && lane == 0 && status) atomicOr(status, ASRBACK_STATUS_POSITION);
+    count = room < count ? static_cast<int>(room) : count;
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -226,10 +234,11 @@ __global__ void __launch_bounds__(kWarps * 32)
 
 using namespace asrback;
 
-extern "C" int asrback_draft_tree(int batch, int nodes, const int32_t* parents,
-                                  int64_t parents_stride, const int32_t* counts,
-                                  int64_t* ancestors, int32_t* depths, int32_t* live_counts,
-                                  int32_t* status, void* stream) {
+extern "C" int asrback_draft_tree_in_cache(int batch, int nodes, const int32_t* parents,
+                                           int64_t parents_stride, const int32_t* counts,
+                                           const int64_t* lengths, int64_t capacity,
+                                           int64_t* ancestors, int32_t* depths,
+                                           int32_t* live_counts, int32_t* status, void* stream) {
   if (batch < 1 || nodes < 1 || nodes > kMaxNodes)
     return fail(ASRBACK_ERR_ARGUMENT, "batch must be positive and nodes in [1, %d], got %d and %d",
                 kMaxNodes, batch, nodes);
@@ -238,11 +247,22 @@ extern "C" int asrback_draft_tree(int batch, int nodes, const int32_t* parents,
   if (parents_stride < 0 || (parents_stride > 0 && parents_stride < nodes))
     return fail(ASRBACK_ERR_ARGUMENT,
                 "parents_stride must be 0 (one tree for every row) or at least nodes");
+  if (lengths && capacity < 1)
+    return fail(ASRBACK_ERR_ARGUMENT, "capacity must be positive where lengths are given");
   if (int rc = launch_pdl(draft_tree_kernel, dim3((batch + kWarps - 1) / kWarps), dim3(kWarps * 32),
                           0, static_cast<cudaStream_t>(stream), "draft tree launch", batch, nodes,
-                          parents, parents_stride, counts, ancestors, depths, live_counts, status))
+                          parents, parents_stride, counts, lengths, capacity, ancestors, depths,
+                          live_counts, status))
     return rc;
   return ok();
+}
+
+extern "C" int asrback_draft_tree(int batch, int nodes, const int32_t* parents,
+                                  int64_t parents_stride, const int32_t* counts,
+                                  int64_t* ancestors, int32_t* depths, int32_t* live_counts,
+                                  int32_t* status, void* stream) {
+  return asrback_draft_tree_in_cache(batch, nodes, parents, parents_stride, counts, nullptr, 0,
+                                     ancestors, depths, live_counts, status, stream);
 }
 
 extern "C" int asrback_accept_tree(

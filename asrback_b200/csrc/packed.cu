@@ -42,6 +42,9 @@ using asrback::apply;
 extern "C" int asrback_draft_tree_packed(const int64_t* args) {
   return apply(asrback_draft_tree, args);
 }
+extern "C" int asrback_draft_tree_in_cache_packed(const int64_t* args) {
+  return apply(asrback_draft_tree_in_cache, args);
+}
 extern "C" int asrback_tree_attention_packed(const int64_t* args) {
   return apply(asrback_tree_attention, args);
 }

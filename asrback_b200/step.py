@@ -192,7 +192,9 @@ def accept_tree(tree: attention.DraftTree, drafts: Tensor, chosen: Tensor, logpr
     emitted, and the walk goes on to the lowest child whose draft it is. It ends
     when no child holds it or the row is finished (EOS, or its position at
     ``end``). Every emitted token updates the decode state as
-    :func:`greedy_step` does; finished rows stay as they are.
+    :func:`greedy_step` does; finished rows, and rows without nodes, stay as they
+    are. (A row that the attention skipped has to be one of these: its nodes chose
+    from zeros.)
 
     ``drafts`` ``(B, N)`` int64: the nodes' tokens; ``chosen`` int64 and
     ``logprob`` float32 ``(B, N)``: what :func:`greedy_choose` says of each

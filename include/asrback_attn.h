@@ -382,6 +382,20 @@ ASRBACK_API int asrback_draft_tree(
     int64_t* ancestors, int32_t* depths, int32_t* live_counts, int32_t* status, void* stream);
 
 /*
+ * As asrback_draft_tree, each row's nodes cut to those that fit its cache: the
+ * first capacity - lengths[b] of them at most. A row that wants nodes and has
+ * room for none sets ASRBACK_STATUS_POSITION.
+ *
+ * lengths      null (nothing is cut), or (batch,) int64: keys in the cache
+ * capacity     slots of a row of the cache (or, with positions for lengths, of
+ *              the rotary table)
+ */
+ASRBACK_API int asrback_draft_tree_in_cache(
+    int batch, int nodes, const int32_t* parents, int64_t parents_stride, const int32_t* counts,
+    const int64_t* lengths, int64_t capacity,
+    int64_t* ancestors, int32_t* depths, int32_t* live_counts, int32_t* status, void* stream);
+
+/*
  * Attention of a draft tree's nodes over a row's cache. Node i's key and value
  * are written to cache slot lengths[b] + i; it attends to the cache's first
  * lengths[b] keys and to the slots of the nodes in ancestors[b][i]. A node
@@ -415,7 +429,8 @@ ASRBACK_API int asrback_draft_tree(
  * caches, of out and of weights must not overlap. With weights the workspace
  * holds 4 bytes per query row and cache position.
  * A row whose counts, lengths or positions are out of range gets zeros, writes
- * nothing else and sets ASRBACK_STATUS_POSITION.
+ * nothing else and sets ASRBACK_STATUS_POSITION: a row whose nodes do not all
+ * fit its cache too (asrback_draft_tree_in_cache plans those that do).
  *
  * workspace    asrback_tree_workspace_bytes(...) bytes of scratch (rotary:
  *              q_norm_weight is given, with_weights: weights are), of any
@@ -447,7 +462,8 @@ ASRBACK_API int asrback_tree_attention(
  * the lowest child whose drafted token equals it, and ends when there is none
  * or the row is finished (EOS, or its position reaches end). Each emitted
  * token updates the state as asrback_greedy_step does. A finished row, and one
- * without nodes, stays as it is.
+ * without nodes, stays as it is. What the walk takes is what the nodes chose: a
+ * row that the attention skipped has to come with a count of 0.
  *
  * parents, counts  as in asrback_draft_tree (counts: its live_counts)
  * drafts       (batch, nodes) int64: the nodes' tokens (node 0's is not read)
@@ -518,6 +534,7 @@ ASRBACK_API int asrback_evict(
  * argument; same checks, same results.
  */
 ASRBACK_API int asrback_draft_tree_packed(const int64_t* args);
+ASRBACK_API int asrback_draft_tree_in_cache_packed(const int64_t* args);
 ASRBACK_API int asrback_tree_attention_packed(const int64_t* args);
 ASRBACK_API int asrback_accept_tree_packed(const int64_t* args);
 ASRBACK_API int asrback_commit_tree_packed(const int64_t* args);

@@ -11,7 +11,8 @@ import torch
 
 from asrback_b200 import _native, attention, cache, step
 from asrback_b200.transcription import CapturedGraph
-from tests.test_gpu_tree import DEV, _accept_case, _device_state, _gpu, _inputs, _tree
+from tests.test_gpu_tree import (DEV, _accept_case, _Decoder, _device_state, _fresh_state, _gpu,
+                                 _inputs, _parents, _tree)
 
 pytestmark = pytest.mark.gpu
 
@@ -198,3 +199,73 @@ def test_commit_skips_starts_out_of_range(start):
     cache.qwen3_commit_tree(keys, keys.clone(), accepted, weights=weights)
     assert attention.read_status() == _native.STATUS_POSITION
     assert torch.equal(keys, before) and torch.equal(weights, old)
+
+
+def test_a_plan_is_cut_to_the_room_in_the_cache():
+    nodes, capacity = 6, 40
+    parents = _parents(np.random.default_rng(0), 9, nodes, "tree")
+    counts = np.array([6, 6, 6, 6, 6, 6, 2, 4, 0])
+    lengths = np.array([0, 34, 35, 39, 12, 38, 37, 37, 40])
+    fits = np.array([6, 6, 5, 1, 6, 2, 2, 3, 0])
+    tree = attention.draft_tree(_gpu(parents, torch.int32), _gpu(counts, torch.int32),
+                                _gpu(lengths, torch.int64), capacity)
+    assert attention.read_status() == 0  # the last row is full and wants nothing
+    want = _tree(parents, fits)
+    assert tree.counts.tolist() == fits.tolist()
+    assert all(torch.equal(a, b) for a, b in zip(tree[1:], want[1:]))
+    for length in (40, 41, -1, 1 << 62, -(1 << 63)):
+        tree = attention.draft_tree(_gpu(parents[:2], torch.int32), None,
+                                    torch.tensor([5, length], device=DEV), capacity)
+        assert attention.read_status() == _native.STATUS_POSITION
+        assert tree.counts.tolist() == [6, 0] and not tree.ancestors[1].any()
+    two, at = _gpu(parents[:2], torch.int32), torch.tensor([5, 6], device=DEV)
+    for lengths, slots in ((at, None), (None, 40), (at, 0), (at.int(), 40), (at[:1], 40), (at.cpu(), 40)):
+        with pytest.raises(ValueError):
+            attention.draft_tree(two, None, lengths, slots)
+
+
+class _Varied(_Decoder):
+    """A decoder whose tokens follow from what it attends to."""
+
+    def __init__(self, batch, length):
+        super().__init__(batch, length)
+        gen = torch.Generator(device=DEV).manual_seed(1)
+        self.out = [8 * w for w in self.out]
+        self.head = torch.randn((50, 128), generator=gen, device=DEV)
+
+
+def test_speculative_decoding_up_to_a_full_cache():
+    """The documented loop: rows decode to the last slot, with drafts right and
+    wrong, and give the tokens of single steps."""
+    batch, length, nodes = 5, 40, 7
+    first = torch.arange(batch, device=DEV)
+    plain, state = _Varied(batch, length), _fresh_state(batch, length + 1, first)
+    fast, got = _Varied(batch, length), _fresh_state(batch, length + 1, first)
+    state["end"].fill_(length)
+    got["end"].fill_(length)
+    single = attention.draft_tree(torch.full((batch, 1), -1, dtype=torch.int32, device=DEV))
+    for _ in range(length):
+        hidden = plain(state["tokens"][:, None], single, state["position"], None)
+        step.greedy_step(hidden[:, 0], plain.head, *state.values(), [])
+    assert state["generated"][:, 1:].unique().numel() > 20  # they do vary
+    rng = np.random.default_rng(0)
+    steps = 0
+    while not got["finished"].all():
+        assert steps < length
+        counts = torch.where(got["finished"], 0, nodes).int()
+        parents = _gpu(_parents(rng, batch, nodes, "chain" if steps % 2 else "tree"), torch.int32)
+        tree = attention.draft_tree(parents, counts, got["position"], length)
+        at = (got["position"][:, None] + tree.depths).clamp(max=length)
+        drafts = state["generated"].gather(1, at)
+        wrong = torch.from_numpy(rng.random((batch, nodes)) < 0.2).to(DEV)
+        drafts = torch.where(wrong, (drafts + 1) % 50, drafts)
+        drafts[:, 0] = got["tokens"]
+        hidden = fast(drafts, tree, got["position"].clone(), None)
+        accepted = step.greedy_tree_step(hidden, fast.head, tree, drafts, *got.values(), [])
+        cache.qwen3_commit_tree(fast.keys, fast.values, accepted)
+        steps += 1
+    assert steps < length and attention.read_status() == 0
+    for name in ("tokens", "position", "finished", "generated"):
+        assert torch.equal(got[name], state[name]), name
+    for c, d in ((fast.keys, plain.keys), (fast.values, plain.values)):
+        torch.testing.assert_close(c, d, rtol=1e-3, atol=1e-3)
