@@ -211,8 +211,12 @@ __global__ void __launch_bounds__(kThreads)
   for (int r = kEarly; r < rows; ++r)
     add(*reinterpret_cast<const float4*>(scores + r * p.score_stride), s.row_m[r]);
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (j + u < n) w[u] = old[u] + sum[u];
+  for (int u = 0; u < 4; ++u) {
+    // A new slot is the node's whose row the first of its query heads is; one
+    // without a bit has written none.
+    const int node = j + u - span.length;
+    if (j + u < n && (node < 0 || s.masks[node * p.group] != 0)) w[u] = old[u] + sum[u];
+  }
 }
 
 template <int D, typename T, int kRows>

@@ -171,16 +171,19 @@ __global__ void __launch_bounds__(kThreads)
   if (p.q_norm) norm_rotate<D, T>(p.eps, w, cs, sn, x);
   if (!query) {
     if (!in) return;
-    const int64_t to = b * p.c_sb + (int64_t)(span.length + node) * p.c_sp + h * p.c_sh;
-    T* key = static_cast<T*>(p.key_cache) + to;
-    T* value = static_cast<T*>(p.value_cache) + to;
-    bool odd = false;
+    // A node without a bit writes nothing; what lies in its slot may be anything.
+    bool odd = mask == 0;
+    if (mask != 0) {
+      const int64_t to = b * p.c_sb + (int64_t)(span.length + node) * p.c_sp + h * p.c_sh;
+      T* key = static_cast<T*>(p.key_cache) + to;
+      T* value = static_cast<T*>(p.value_cache) + to;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      Octet<T>::store(key, half * (D / 2) + 8 * c, x + 8 * half);
-      v_in.half[half].copy(value, half * (D / 2) + 8 * c);
+      for (int half = 0; half < 2; ++half) {
+        Octet<T>::store(key, half * (D / 2) + 8 * c, x + 8 * half);
+        v_in.half[half].copy(value, half * (D / 2) + 8 * c);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) odd |= !(fabsf(v_in.half[half][i]) < INFINITY);
+        for (int i = 0; i < 8; ++i) odd |= !(fabsf(v_in.half[half][i]) < INFINITY);
+      }
     }
     // Whether any lane of the row (lanes leave together) found one.
     const unsigned mine = ((1u << (Slice::kLanes - 1)) * 2u - 1u)

@@ -11,8 +11,9 @@ import torch
 
 from asrback_b200 import _native, attention, cache, step
 from asrback_b200.transcription import CapturedGraph
-from tests.test_gpu_tree import (DEV, _accept_case, _Decoder, _device_state, _fresh_state, _gpu,
-                                 _inputs, _parents, _tree)
+from oracle import tree as oracle
+from tests.test_gpu_tree import (DEV, _accept_case, _call, _Decoder, _device_state, _fresh_state, _gpu,
+                                 _inputs, _np, _parents, _tree, _want)
 
 pytestmark = pytest.mark.gpu
 
@@ -269,3 +270,59 @@ def test_speculative_decoding_up_to_a_full_cache():
         assert torch.equal(got[name], state[name]), name
     for c, d in ((fast.keys, plain.keys), (fast.values, plain.values)):
         torch.testing.assert_close(c, d, rtol=1e-3, atol=1e-3)
+
+
+@pytest.mark.parametrize("family,tag,heads,kv_heads,dim,nodes,weights", [
+    ("whisper", "bf16", 6, 6, 64, 5, True), ("whisper", "f32", 6, 6, 64, 5, True),
+    ("qwen3", "bf16", 4, 2, 128, 8, True), ("qwen3", "f32", 4, 2, 128, 20, False),
+    ("whisper", "bf16", 2, 2, 64, 30, False), ("qwen3", "bf16", 4, 2, 128, 40, False)])
+@pytest.mark.parametrize("old", [0.25, float("nan")])
+def test_a_node_without_a_bit_writes_nothing(family, tag, heads, kv_heads, dim, nodes, weights, old):
+    """A caller's own plan, whose node 3 sees nothing: zeros, its slot and the
+    slot's weight as they were, whatever lies there; the others as without it."""
+    lengths = [70, 3]
+    x = _inputs(nodes, family, tag, 2, nodes, 100 + nodes, heads, kv_heads, dim, lengths,
+                shape="star", weights=weights)
+    tree = _tree(x["parents"], x["counts"])
+    tree.ancestors[:, 3] = 0
+    caches = [x[n].transpose(1, 2) if family == "whisper" else x[n] for n in ("keys", "values")]
+    for b, m in enumerate(lengths):
+        for c in caches:
+            c[b, m + 3] = old
+    out, keys, values, w = _call(x, tree)
+    want = _want(x)  # of node 0's children node 3 is no one's ancestor
+    others = [i for i in range(nodes) if i != 3]
+    assert not out[:, 3].any()
+    # The tolerance for the others: scores as in the draft-tree tests' module, one
+    # rounding of the probabilities and one of the output.
+    full, top = want["reach"][..., 0], want["reach"][..., 1]
+    bf16, rotated = tag == "bf16", family == "qwen3"
+    d = dim * 2.0 ** -24 * full + 2.0 ** -22 * (1 + full)
+    if bf16 and rotated:
+        d = d + 2 * 2.0 ** -7 * top + 2.0 ** -17 * full
+    shift = np.expm1(2 * d)
+    tol = (2.0 ** -8 if bf16 else 2.0 ** -24) * np.abs(want["out"]) + want["mass"] * (
+        (2.0 ** -8 if bf16 else 0) + shift[..., None] + 200 * 2.0 ** -24)
+    off = np.abs(_np(out).reshape(want["out"].shape) - want["out"])
+    assert (off[:, others] <= tol[:, others]).all()
+    for b, m in enumerate(lengths):
+        for got, before in zip((keys, values), caches):
+            torch.testing.assert_close(got[b, m + 3], before[b, m + 3], rtol=0, atol=0,
+                                       equal_nan=True)
+        if weights:
+            assert torch.equal(w[b, :, m + 3], x["weights"][b, :, m + 3])
+    if weights and not rotated:  # scores good to d: each weight to its share of what it gained
+        above, _ = oracle.plan(x["parents"], x["counts"])
+        above[:, 3] = False
+        q, k, v = (_np(x[n]).transpose(0, 2, 1, 3) for n in "qkv")
+        all_keys, all_values = (np.nan_to_num(_np(c)) for c in caches)
+        start = _np(x["weights"])
+        full_want = oracle.tree_attention(q, k, v, all_keys, all_values, x["lengths"], above,
+                                          x["counts"], dim ** -0.5, start)["weights"]
+        slots = np.ones(start.shape, bool)
+        for b, m in enumerate(lengths):
+            slots[b, :, m + 3] = False
+        gained = full_want - start
+        tol = (shift.max() + 2.0 ** -20) * np.abs(gained) + 2.0 ** -22 * (1 + np.abs(full_want))
+        assert (np.abs(_np(w) - full_want)[slots] <= tol[slots]).all()
+    assert attention.read_status() == 0
