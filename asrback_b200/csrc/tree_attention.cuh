@@ -58,15 +58,16 @@ struct RowSpan {
   bool bad;
 };
 
-// The row's cached keys and live nodes. A row without nodes reads nothing; a
-// row whose nodes do not fit the cache or the rotary table is skipped.
+// The row's cached keys and live nodes. A row without nodes reads nothing,
+// wherever it stands; a row whose nodes do not fit the cache or the rotary table
+// is skipped.
 __device__ __forceinline__ RowSpan row_span(const TreeParams& p, int b) {
   const int64_t length = p.lengths[b];
   const int count = p.counts[b];
   const int64_t position = p.q_norm ? p.positions[b] : 0;
   bool bad = count < 0 || count > p.nodes || length < 0 || length > p.cache_length - count;
   if (p.q_norm) bad |= position < 0 || position > p.table_length - count;
-  if (bad || count == 0) return {0, 0, bad};
+  if (bad || count == 0) return {0, 0, bad && count != 0};
   return {static_cast<int>(length), count, false};
 }
 

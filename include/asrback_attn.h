@@ -428,8 +428,8 @@ ASRBACK_API int asrback_draft_tree_in_cache(
  * ASRBACK_BF16 or ASRBACK_F32; rows and pointers 16-byte aligned. Rows of the
  * caches, of out and of weights must not overlap. With weights the workspace
  * holds 4 bytes per query row and cache position.
- * A row whose counts, lengths or positions are out of range gets zeros, writes
- * nothing else and sets ASRBACK_STATUS_POSITION: a row whose nodes do not all
+ * A row with nodes whose counts, lengths or positions are out of range gets zeros,
+ * writes nothing else and sets ASRBACK_STATUS_POSITION: a row whose nodes do not all
  * fit its cache too (asrback_draft_tree_in_cache plans those that do).
  *
  * workspace    asrback_tree_workspace_bytes(...) bytes of scratch (rotary:

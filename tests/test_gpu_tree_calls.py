@@ -326,3 +326,18 @@ def test_a_node_without_a_bit_writes_nothing(family, tag, heads, kv_heads, dim, 
         tol = (shift.max() + 2.0 ** -20) * np.abs(gained) + 2.0 ** -22 * (1 + np.abs(full_want))
         assert (np.abs(_np(w) - full_want)[slots] <= tol[slots]).all()
     assert attention.read_status() == 0
+
+
+@pytest.mark.parametrize("tag,nodes", [("bf16", 4), ("bf16", 40), ("f32", 4)])
+def test_rows_without_nodes_may_stand_anywhere(tag, nodes):
+    """Lengths and positions of rows without nodes are not looked at."""
+    lengths, counts = [50, 101, -1, 1 << 40, 7], [nodes, 0, 0, 0, 3]
+    x = _inputs(nodes, "qwen3", tag, 5, nodes, 100, 16, 8, 128, lengths, counts)
+    x["positions"] = np.array([50, 1 << 40, 3, -5, 7])
+    got = _call(x)
+    assert attention.read_status() == 0
+    near = dict(x, lengths=np.array([50, 0, 0, 0, 7]), positions=np.array([50, 0, 0, 0, 7]))
+    assert all(torch.equal(a, b) for a, b in zip(got[:3], _call(near)[:3]))
+    x["counts"] = np.array([nodes, 1, 0, 0, 3])  # one that has a node is flagged
+    _call(x)
+    assert attention.read_status() == _native.STATUS_POSITION
