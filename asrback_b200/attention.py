@@ -652,6 +652,8 @@ def qwen3_attention_tree(qkv: Tensor, q_norm_weight: Tensor, k_norm_weight: Tens
     weight that every key gets, summed over the row's live nodes and the query
     heads of its key/value head: added for cached keys, assigned for the new
     slots (at most ``MAX_WEIGHT_ROWS`` query rows, ``N * heads / kv_heads``).
+    Live nodes count whether or not they are accepted later: weights to evict by
+    come from single tokens, prompts and accepted paths run as chains.
 
     ``N = 1`` is the decode step, a chain a prompt pass of up to 64 tokens.
     ``head_dim`` 64 or 128. A row whose nodes do not all fit the cache or the

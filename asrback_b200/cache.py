@@ -96,7 +96,8 @@ def qwen3_commit_tree(keys: Tensor, values: Tensor, accepted: step.AcceptedPath,
     """Brings the accepted nodes' rows of Qwen3 caches ``([layers,] B, L,
     kv_heads, D)`` in order, in place: row ``start + path[k]`` moves to ``start
     + k`` (``accepted`` from :func:`asrback_b200.step.accept_tree`). ``weights``
-    ``([layers,] B, kv_heads, L)`` float32 move along."""
+    ``([layers,] B, kv_heads, L)`` float32 move along, with all that a call over
+    the tree put in them: rejected nodes' shares too."""
     _commit(keys, values, accepted, weights, False)
 
 
@@ -120,7 +121,8 @@ def qwen3_evict(keys: Tensor, values: Tensor, weights: Tensor, lengths: Tensor, 
     shorter row's.
 
     The weights come from :func:`asrback_b200.attention.qwen3_attention_tree`,
-    which then takes the new lengths beside the unchanged positions."""
+    which then takes the new lengths beside the unchanged positions. (From calls
+    over accepted nodes: single tokens, prompts, accepted paths.)"""
     return _evict(keys, values, weights, lengths, budget, sink, recent, False)
 
 

@@ -423,7 +423,10 @@ ASRBACK_API int asrback_draft_tree_in_cache(
  *              that key p got, summed over the live nodes and the head's query
  *              heads, are added to the cached keys' entries and assigned to
  *              the new slots'. At most 16 query rows per key/value head
- *              (nodes * heads / kv_heads).
+ *              (nodes * heads / kv_heads). Live nodes count whether or not an
+ *              acceptance takes them later: weights to evict by, as single
+ *              steps would gather them, come from calls over accepted nodes
+ *              (single tokens, prompts, a walk's path as a chain).
  * head_dim 64 or 128; nodes <= 64; batch <= 1024; cache_length <= 2^24; dtype
  * ASRBACK_BF16 or ASRBACK_F32; rows and pointers 16-byte aligned. Rows of the
  * caches, of out and of weights must not overlap. With weights the workspace
@@ -491,7 +494,8 @@ ASRBACK_API int asrback_accept_tree(
  * to row start[b] + k for k < counts[b] (path ascending, as asrback_accept_tree
  * returns it). Caches at [layer*c_stride_layer + b*c_stride_batch +
  * p*c_stride_position + h*c_stride_head + d]; weights null or (layers, batch,
- * heads, length) float, whose entries move along. Rows with an invalid path or
+ * heads, length) float, whose entries move along (what rejected nodes gave them
+ * or the cached keys stays in them). Rows with an invalid path or
  * start stay as they are and set ASRBACK_STATUS_POSITION.
  */
 ASRBACK_API int asrback_commit_tree(

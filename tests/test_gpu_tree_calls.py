@@ -341,3 +341,79 @@ def test_rows_without_nodes_may_stand_anywhere(tag, nodes):
     x["counts"] = np.array([nodes, 1, 0, 0, 3])  # one that has a node is flagged
     _call(x)
     assert attention.read_status() == _native.STATUS_POSITION
+
+
+class _Recorded(_Varied):
+    """Keeps each layer's qkv, and runs its attention over an accepted path."""
+
+    def __call__(self, tokens, tree, positions, lengths, keep_weights=False):
+        self.kept = []
+        x = self.embed[tokens]
+        for layer in range(2):
+            self.kept.append(x @ self.qkv[layer])
+            a = self.attend(layer, self.kept[-1], positions, tree, lengths, keep_weights)
+            x = x + a @ self.out[layer]
+        return x
+
+    def attend(self, layer, qkv, positions, tree, lengths, keep_weights):
+        return attention.qwen3_attention_tree(
+            qkv, self.norms, self.norms, 1e-6, self.cos, self.sin, positions, tree,
+            self.keys[layer], self.values[layer], 4, 2, lengths=lengths,
+            weights=self.weights[layer] if keep_weights else None)
+
+    def gather(self, accepted, before):
+        """The documented recipe: the path as a chain, in parts of 8 nodes."""
+        part = attention.MAX_WEIGHT_ROWS // 2
+        for first in range(0, accepted.path.shape[1], part):
+            at = accepted.path[:, first:first + part].long().clamp(min=0)
+            chain = attention.draft_tree(
+                torch.arange(-1, at.shape[1] - 1, dtype=torch.int32, device=DEV).expand(len(at), -1),
+                (accepted.counts - first).clamp(0, at.shape[1]))
+            for layer, qkv in enumerate(self.kept):
+                self.attend(layer, qkv.gather(1, at[..., None].expand(-1, -1, qkv.shape[2])),
+                            before + first, chain, accepted.start + first, True)
+
+
+def test_accepted_paths_gather_the_weights_of_single_steps():
+    """Speculative decoding that gathers weights, with drafts rejected on the way,
+    and an eviction by them: as single steps."""
+    batch, length, nodes = 4, 64, 12
+    first = torch.arange(batch, device=DEV)
+    plain, state = _Recorded(batch, length), _fresh_state(batch, length, first)
+    fast, got = _Recorded(batch, length), _fresh_state(batch, length, first)
+    state["end"].fill_(60)
+    got["end"].fill_(60)
+    single = attention.draft_tree(torch.full((batch, 1), -1, dtype=torch.int32, device=DEV))
+    for _ in range(60):
+        hidden = plain(state["tokens"][:, None], single, state["position"], None, True)
+        step.greedy_step(hidden[:, 0], plain.head, *state.values(), [])
+    rng, steps, longest = np.random.default_rng(0), 0, 0
+    while not got["finished"].all():
+        assert steps < 60
+        counts = torch.where(got["finished"], 0, nodes).int()
+        parents = _parents(rng, batch, nodes, "chain" if steps % 3 else "tree")
+        tree = attention.draft_tree(_gpu(parents, torch.int32), counts, got["position"], length)
+        at = (got["position"][:, None] + tree.depths).clamp(max=length - 1)
+        drafts = state["generated"].gather(1, at)
+        wrong = torch.from_numpy(rng.random((batch, nodes)) < 0.1).to(DEV)
+        drafts = torch.where(wrong, (drafts + 1) % 50, drafts)
+        drafts[:, 0] = got["tokens"]
+        before = got["position"].clone()
+        hidden = fast(drafts, tree, before, None)
+        accepted = step.greedy_tree_step(hidden, fast.head, tree, drafts, *got.values(), [])
+        fast.gather(accepted, before)
+        steps += 1
+        longest = max(longest, int(accepted.counts.max()))
+    assert steps < 50 and longest > 8 and attention.read_status() == 0
+    assert torch.equal(got["generated"], state["generated"])
+    ends = torch.full((batch,), 60, device=DEV)
+    for layer in range(2):
+        # float32 sums of some hundred terms of order one to ten, in another order,
+        # through two layers: some 1e-5; a rejected node's share is of order 1e-2.
+        for a, b in ((fast.keys[layer][:, :60], plain.keys[layer][:, :60]),
+                     (fast.values[layer][:, :60], plain.values[layer][:, :60]),
+                     (fast.weights[layer][..., :60], plain.weights[layer][..., :60])):
+            torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4)
+        kept = [cache.qwen3_evict(d.keys[layer], d.values[layer], d.weights[layer], ends, 30, 2, 4)[1]
+                for d in (fast, plain)]
+        assert torch.equal(*kept)
