@@ -374,12 +374,15 @@ extern "C" int asrback_tree_attention(
   if (!rotary && (k_norm_weight || cos || sin))
     return fail(ASRBACK_ERR_ARGUMENT, "k_norm_weight, cos and sin need q_norm_weight");
   const int64_t esize = dtype == ASRBACK_BF16 ? 2 : 4;
-  const int64_t strides[] = {q_stride_batch, q_stride_node, q_stride_head,  k_stride_batch,
-                             k_stride_node,  k_stride_head, v_stride_batch, v_stride_node,
-                             v_stride_head,  c_stride_batch, c_stride_position, c_stride_head,
-                             o_stride_batch, o_stride_node, o_stride_head};
-  for (int64_t s : strides)
-    if (s < 0 || (s * esize) % 16 != 0)
+  // Of a dimension of one the stride may be anything: no one reads it.
+  const struct { int64_t stride; int size; } strides[] = {
+      {q_stride_batch, batch}, {q_stride_node, nodes}, {q_stride_head, heads},
+      {k_stride_batch, batch}, {k_stride_node, nodes}, {k_stride_head, kv_heads},
+      {v_stride_batch, batch}, {v_stride_node, nodes}, {v_stride_head, kv_heads},
+      {c_stride_batch, batch}, {c_stride_position, cache_length}, {c_stride_head, kv_heads},
+      {o_stride_batch, batch}, {o_stride_node, nodes}, {o_stride_head, heads}};
+  for (const auto& s : strides)
+    if (s.size > 1 && (s.stride < 0 || (s.stride * esize) % 16 != 0))
       return fail(ASRBACK_ERR_ARGUMENT,
                   "strides must not be negative and rows must start on 16-byte boundaries");
   if (rotary && (table_stride * esize) % 16 != 0)
@@ -389,7 +392,7 @@ extern "C" int asrback_tree_attention(
   for (const void* ptr : pointers)
     if (!aligned16(ptr)) return fail(ASRBACK_ERR_ARGUMENT, "pointers must be 16-byte aligned");
   // The cache and the weights are written: no two of their rows may be one.
-  if (c_stride_position < head_dim || (kv_heads > 1 && c_stride_head < head_dim) ||
+  if ((cache_length > 1 && c_stride_position < head_dim) || (kv_heads > 1 && c_stride_head < head_dim) ||
       (batch > 1 && c_stride_batch < head_dim) || (batch > 1 && o_stride_batch < head_dim) ||
       (heads > 1 && o_stride_head < head_dim) || (nodes > 1 && o_stride_node < head_dim))
     return fail(ASRBACK_ERR_ARGUMENT, "cache or output strides do not hold rows of head_dim");

@@ -417,3 +417,33 @@ def test_accepted_paths_gather_the_weights_of_single_steps():
         kept = [cache.qwen3_evict(d.keys[layer], d.values[layer], d.weights[layer], ends, 30, 2, 4)[1]
                 for d in (fast, plain)]
         assert torch.equal(*kept)
+
+
+@pytest.mark.parametrize("family,tag,heads,nodes,weights", [
+    ("qwen3", "bf16", 2, 1, True), ("qwen3", "bf16", 2, 40, False), ("qwen3", "f32", 2, 1, True),
+    ("whisper", "bf16", 1, 1, False), ("whisper", "f32", 1, 1, False)])
+def test_dimensions_of_one_with_any_stride(family, tag, heads, nodes, weights):
+    """One row, one node, one key/value head, a cache of one slot: their strides,
+    which a view may leave at anything, are not read."""
+    length = 1 if nodes == 1 else 100
+    x = _inputs(nodes, family, tag, 1, nodes, length, heads, 1, 128 if family == "qwen3" else 64,
+                [length - nodes], weights=weights)
+    want = _call(x)
+    tree, at = _tree(x["parents"], x["counts"]), _gpu(x["lengths"], torch.int64)
+
+    def odd(t):
+        t = t.clone(memory_format=torch.contiguous_format)
+        return t.as_strided(t.shape, [3 if n == 1 else s for n, s in zip(t.shape, t.stride())])
+
+    keys, values = odd(x["keys"]), odd(x["values"])
+    w = odd(x["weights"]) if weights else None
+    if family == "whisper":
+        out = attention.whisper_self_attention_tree(odd(x["q"]), odd(x["k"]), odd(x["v"]), keys,
+                                                    values, at, tree)
+        keys, values = keys.transpose(1, 2), values.transpose(1, 2)
+    else:
+        out = attention.qwen3_attention_tree(odd(x["qkv"]), x["wq"], x["wk"], 1e-6, x["cos"],
+                                             x["sin"], at, tree, keys, values, heads, 1, weights=w)
+    for got, expected in zip((out, keys, values, w), want):
+        assert got is expected is None or torch.equal(got, expected)
+    assert attention.read_status() == 0
