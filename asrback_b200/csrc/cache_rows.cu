@@ -5,11 +5,14 @@
 // Both move cache row source[k] to row target + k with source ascending and
 // source[k] >= k, in place. A move then never overwrites a row that a later
 // move reads, so rows are moved in ascending order, a batch of loads before
-// its stores, with no copy of the cache. Both are bound by HBM: a moved row is
-// read once and written once. Measured: the commit of 64 rows x 16 nodes over 28
-// layers of 8 heads of 128 6 us; an eviction of 64 rows from 1024 slots to 512, 8
-// heads of 128 (273 MB), 52 us, 5.2 TB/s; of 2 rows from 16384 slots to 4096 29 us,
-// 12 for the selection and 16 for the moves.
+// its stores, with no copy of the cache. A moved row is read once and written
+// once. Measured: the commit of 64 rows x 16 nodes over 28 layers of 8 heads of 128
+// 6 us, which launch and load latency bound (its 14 MB keep DRAM 9 % busy); an
+// eviction of 64 rows from 1024 slots to 512, 8 heads of 128, 52 us, near HBM's
+// stream: 273 MB to read and write at 5.2 TB/s, of which part stays in L2 (cold and
+// profiled 216 MB in 49 us, DRAM 54 % busy); of 2 rows from 16384 slots to 4096 29
+// us, 12 for the selection and 16 for the moves, bound by their barriers and
+// latencies (DRAM 1 and 24 % busy).
 #include "../../include/asrback_attn.h"
 #include "capi_internal.h"
 #include "common.cuh"

@@ -495,8 +495,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kSplit, kBlocks>::kPerSm)
         }
       }
 
-      // The rows' sums, and the result: out, or to the workspace for the
-      // item's last CTA to merge. (Two buffers: a segment without keys has
+      // The rows' sums, and the result: out, or to the workspace, whose parts
+      // tree_finish.cu merges. (Two buffers: a segment without keys has
       // only this one barrier.)
       float* row_sum = row_sums + (n & 1) * kWarps * kRows;
 #pragma unroll

@@ -37,7 +37,8 @@
 // of up to 8192 keys, 8 heads of 128 (175 MB) 48 us, of which this kernel's 33 are
 // 5.3 TB/s; 64 rows x 16 nodes of up to 1024 keys (183 MB) 51.5 us. Steps on the
 // way for the two: scores of 64 columns and an accumulator per tile of a pair 61
-// and 63 us; one per pair, no spills 48.6 and 53; an item's fixed cost in the split
+// and 63 us; one per pair, few spills (16 to 20 bytes of a thread's are left; 112 to
+// 144 took 53.7 and 60) 48.6 and 53; an item's fixed cost in the split
 // 48 and 51.5. No gain: exponentials on the FMA pipe (49 and 55), blocks of up to
 // 64 rows laid out twice, for the softmax to use more schedulers (53.5 for the
 // second), other ring lengths.
