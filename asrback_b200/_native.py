@@ -197,8 +197,8 @@ SIGNATURES: dict[str, tuple[list, object]] = {
 
 # Entry points that also take their arguments as one array of 64-bit words.
 _PACKED = {}
-for _name in ("asrback_draft_tree", "asrback_draft_tree_in_cache", "asrback_tree_attention", "asrback_accept_tree",
-              "asrback_commit_tree", "asrback_evict"):
+for _name in ("asrback_draft_tree", "asrback_draft_tree_in_cache", "asrback_tree_attention",
+              "asrback_accept_tree", "asrback_commit_tree", "asrback_evict"):
     _PACKED[_name] = struct.Struct("=" + "".join(
         "d" if t is _c_f else "q" for t in SIGNATURES[_name][0])).pack
     SIGNATURES[_name + "_packed"] = ([ctypes.c_char_p], _c_int)

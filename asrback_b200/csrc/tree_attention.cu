@@ -392,7 +392,8 @@ extern "C" int asrback_tree_attention(
   for (const void* ptr : pointers)
     if (!aligned16(ptr)) return fail(ASRBACK_ERR_ARGUMENT, "pointers must be 16-byte aligned");
   // The cache and the weights are written: no two of their rows may be one.
-  if ((cache_length > 1 && c_stride_position < head_dim) || (kv_heads > 1 && c_stride_head < head_dim) ||
+  if ((cache_length > 1 && c_stride_position < head_dim) ||
+      (kv_heads > 1 && c_stride_head < head_dim) ||
       (batch > 1 && c_stride_batch < head_dim) || (batch > 1 && o_stride_batch < head_dim) ||
       (heads > 1 && o_stride_head < head_dim) || (nodes > 1 && o_stride_node < head_dim))
     return fail(ASRBACK_ERR_ARGUMENT, "cache or output strides do not hold rows of head_dim");
